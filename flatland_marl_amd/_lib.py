@@ -15,6 +15,7 @@ AGENT_ERRORS = {2: IndexError, 3: KeyError, 4: AssertionError, 5: OverflowError}
 GRAPH_ERR_NODES, GRAPH_ERR_RAILS, GRAPH_ERR_CELLS, GRAPH_ERR_STATES = 1, 2, 4, 8
 MAX_NODES = 2048
 ABI_VERSION = 4
+GROUPS_MAX, ADAPTER_MAX_RANK, GRAD_MAX_TENSORS, GRAD_WORKSPACE = 2047, 128, 65536, 2048
 DQN_MAX_ACTIONS = 16                                       # FLM_DQN_MAX_ACTIONS of include/flmarl.h
 
 _p = C.c_void_p
@@ -86,10 +87,22 @@ _SIGNATURES = {
     "flm_dqn_soft_update": [_p, _p, C.c_long, C.c_double, _p],
     "flm_dqn_adam_soft_update": [_p, _p, _p, _p, _p, C.c_long, C.c_double, C.c_double, C.c_double, C.c_double, _i,
                                  C.c_double, _p],
+    "flm_group_rows_ints": [_i, _i],
+    "flm_group_rows_workspace": [_i, _i],
+    "flm_group_rows": [_p, _i, _i, _i, _p, _p, _p],
+    "flm_adapter_workspace": [_i] * 5,
+    "flm_adapter_linear": [_p, C.c_long, _p, C.c_long, _p, _p, _p, _p, _p, C.c_float, _i, _i, _i, _i, _i, _i, _p, _p, C.c_long,
+                           _p, _p],
+    "flm_adapter_backward_workspace": [_i] * 7,
+    "flm_adapter_linear_backward": [_p, C.c_long, _p, C.c_long, _p, C.c_long, _p, _p, _p, _p, C.c_float, _p, _i, _i, _i, _i, _i,
+                                    _i, _p, _p, C.c_long, _p, _p, _p],
+    "flm_grad_clip": [_p, _p, _p, _p, _i, C.c_double, _i, _p, _p, _p],
+    "flm_dqn_grad_clip": [_p, _i, _i, _i, _i, _i, _p, C.c_double, _i, _p, _p, _p],
 }
 
 _LONG_RESULT = {"flm_paths_columns_lds_bytes", "flm_paths_columns_workspace", "flm_dqn_param_count", "flm_dqn_grad_split", "flm_dqn_learn_rails", "flm_dqn_learn_rails_rcb_offset", "flm_replay_store_slots_workspace", "flm_dqn_forward_workspace", "flm_dqn_learn_workspace",
-                "flm_dqn_learn_workspace_u8"}
+                "flm_dqn_learn_workspace_u8", "flm_group_rows_ints", "flm_group_rows_workspace", "flm_adapter_workspace",
+                "flm_adapter_backward_workspace"}
 _lib = None
 
 

@@ -1,0 +1,298 @@
+// Global gradient norm over many tensors, and clipping, on gfx950.
+//
+//   norm = sqrt(sum over every element of every tensor of g^2)   (or max |g|)
+//   g   *= min(1, max_norm / (norm + 1e-6))
+//
+// Two launches: every workgroup sums (or maximises) its share of the tensors into one partial result; then every
+// workgroup folds all partial results itself, in the same order, and scales its share.  Sums are kept in 64 bits: the
+// square of an fp32 number then neither overflows nor vanishes (1e-30 and 1e30 are ordinary gradients to this kernel),
+// and 64-bit multiply-adds run at a rate that a stream of memory does not notice.  Nothing depends on the order in which
+// workgroups finish.
+// The tensors' addresses travel in the launch's arguments, FLM_GRAD_LIST tensors a launch: no table in device memory has to be
+// kept or refreshed by the caller.
+#include "flm_common.h"
+
+namespace flm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+#define FLM_GRAD_LIST 112                // tensors per launch: 32 bytes each of the 4 KiB a launch's arguments may take
+#define GRAD_CHUNK 8192                  // elements a workgroup takes at a time
+#define GRAD_PARTS FLM_GRAD_WORKSPACE    // partial results at most
+
+struct GradItem {
+  const void* src;
+  void* dst;                             // nullptr: the tensor only counts in the norm
+  long numel;
+  int first;                             // number of chunks of the list before this tensor
+  int dtype;
+};
+struct GradList {
+  GradItem item[FLM_GRAD_LIST];
+  int count, chunks;
+};
+// What the gradient holds beside the listed tensors: `times` copies of the outer products g_i (x) r, r [64], over the
+// 512 + 512 values of two vectors (the first dense layer's gradient under empty rows, formed by the optimizer pass).
+struct GradOuter {
+  const float *r, *g0, *g1;
+  double times;
+};
+
+template <typename T> struct Pack8;
+template <> struct Pack8<float> { struct __attribute__((packed, aligned(4))) V { float v[8]; }; };
+template <> struct Pack8<__bf16> { struct __attribute__((packed, aligned(2))) V { __bf16 v[8]; }; };
+template <> struct Pack8<_Float16> { struct __attribute__((packed, aligned(2))) V { _Float16 v[8]; }; };
+
+__device__ __forceinline__ double larger(double m, double v) { return (m == m && !(v <= m)) ? v : m; }   // NaN stays
+
+// f(value array, count) over one chunk of a tensor, eight elements a thread and step
+template <typename T>
+__device__ __forceinline__ void grad_norm_chunk(const T* p, int n, int tid, int threads, bool inf_norm, double (&acc)[4]) {
+  typedef typename Pack8<T>::V V;
+  const int whole = n >> 3;
+  auto take = [&](const V& v) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const double g = (double)(float)v.v[j];
+      if (inf_norm) acc[j & 3] = larger(acc[j & 3], __builtin_fabs(g));
+      else acc[j & 3] = __builtin_fma(g, g, acc[j & 3]);
+    }
+  };
+  int i = tid;
+  for (; i + 3 * threads < whole; i += 4 * threads) {
+    V v[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) v[u] = reinterpret_cast<const V*>(p)[i + u * threads];
+#pragma unroll
+    for (int u = 0; u < 4; u++) take(v[u]);
+  }
+  for (; i < whole; i += threads) take(reinterpret_cast<const V*>(p)[i]);
+  if (tid < (n & 7)) {
+    const double g = (double)(float)p[(whole << 3) + tid];
+    acc[0] = inf_norm ? larger(acc[0], __builtin_fabs(g)) : __builtin_fma(g, g, acc[0]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void grad_scale_chunk(const T* p, T* q, int n, int tid, int threads, double coef) {
+  typedef typename Pack8<T>::V V;
+  const int whole = n >> 3;
+  auto scaled = [&](const V& v) {
+    V o;
+#pragma unroll
+    for (int j = 0; j < 8; j++) o.v[j] = (T)(float)((double)(float)v.v[j] * coef);
+    return o;
+  };
+  int i = tid;
+  for (; i + 3 * threads < whole; i += 4 * threads) {
+    V v[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) v[u] = reinterpret_cast<const V*>(p)[i + u * threads];
+#pragma unroll
+    for (int u = 0; u < 4; u++) reinterpret_cast<V*>(q)[i + u * threads] = scaled(v[u]);
+  }
+  for (; i < whole; i += threads) reinterpret_cast<V*>(q)[i] = scaled(reinterpret_cast<const V*>(p)[i]);
+  if (tid < (n & 7)) {
+    const int j = (whole << 3) + tid;
+    q[j] = (T)(float)((double)(float)p[j] * coef);
+  }
+}
+
+// the workgroup's total of one value per thread, in a fixed order; every thread gets it.  red: 16 doubles of LDS
+__device__ __forceinline__ double grad_fold(double v, bool inf_norm, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const double w = __shfl_xor(v, o);
+    v = inf_norm ? larger(larger(0.0, v), w) : v + w;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double t = red[0];
+  for (int i = 1; i < (int)(blockDim.x >> 6); i++) t = inf_norm ? larger(t, red[i]) : t + red[i];
+  return t;
+}
+
+// walks the chunks first, first + stride, ... of the list
+template <typename F>
+__device__ __forceinline__ void grad_chunks(const GradList& list, int first, int stride, F&& f) {
+  int t = 0;
+  for (int c = first; c < list.chunks; c += stride) {
+    while (t + 1 < list.count && list.item[t + 1].first <= c) t++;
+    const GradItem& it = list.item[t];
+    const long off = (long)(c - it.first) * GRAD_CHUNK;
+    const long left = it.numel - off;
+    f(it, off, (int)(left < GRAD_CHUNK ? left : GRAD_CHUNK));
+  }
+}
+
+__device__ __forceinline__ double grad_norm_share(const GradList& list, int first, int stride, bool inf_norm, double* red) {
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  const int tid = threadIdx.x, threads = blockDim.x;
+  grad_chunks(list, first, stride, [&](const GradItem& it, long off, int n) {
+    if (it.dtype == FLM_F32) grad_norm_chunk((const float*)it.src + off, n, tid, threads, inf_norm, acc);
+    else if (it.dtype == FLM_BF16) grad_norm_chunk((const __bf16*)it.src + off, n, tid, threads, inf_norm, acc);
+    else grad_norm_chunk((const _Float16*)it.src + off, n, tid, threads, inf_norm, acc);
+  });
+  const double v = inf_norm ? larger(larger(acc[0], acc[1]), larger(acc[2], acc[3])) : (acc[0] + acc[1]) + (acc[2] + acc[3]);
+  return grad_fold(v, inf_norm, red);
+}
+
+__device__ __forceinline__ void grad_scale_share(const GradList& list, int first, int stride, double coef) {
+  const int tid = threadIdx.x, threads = blockDim.x;
+  grad_chunks(list, first, stride, [&](const GradItem& it, long off, int n) {
+    if (!it.dst || (it.dst == it.src && coef == 1.0)) return;
+    if (it.dtype == FLM_F32) grad_scale_chunk((const float*)it.src + off, (float*)it.dst + off, n, tid, threads, coef);
+    else if (it.dtype == FLM_BF16) grad_scale_chunk((const __bf16*)it.src + off, (__bf16*)it.dst + off, n, tid, threads, coef);
+    else grad_scale_chunk((const _Float16*)it.src + off, (_Float16*)it.dst + off, n, tid, threads, coef);
+  });
+}
+
+// a NaN norm gives a NaN factor (NaN gradients), an infinite one the factor 0, as the formula does
+__device__ __forceinline__ double grad_factor(double norm, double max_norm) {
+  const double c = max_norm / (norm + 1e-6);
+  return c >= 1.0 ? 1.0 : c;
+}
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(GradList list, GradOuter outer, int inf_norm, double* __restrict__ part) {
+  __shared__ double red[16];
+  const bool inf = inf_norm != 0;
+  double v = grad_norm_share(list, blockIdx.x, gridDim.x, inf, red);
+  if (outer.r && blockIdx.x == gridDim.x - 1) {          // the implicit part: a product of two short sums
+    double sr = 0.0, sg = 0.0;
+    auto add = [&](double s, double g) { return inf ? larger(s, __builtin_fabs(g)) : __builtin_fma(g, g, s); };
+    for (int i = threadIdx.x; i < 512; i += 256) { sg = add(sg, outer.g0[i]); sg = add(sg, outer.g1[i]); }
+    if (threadIdx.x < 64) sr = add(sr, outer.r[threadIdx.x]);
+    sr = grad_fold(sr, inf, red);
+    sg = grad_fold(sg, inf, red);
+    v = inf ? larger(v, sr * sg) : v + outer.times * sr * sg;
+  }
+  if (threadIdx.x == 0) part[blockIdx.x] = v;
+}
+
+__global__ __launch_bounds__(256) void grad_clip_kernel(GradList list, int inf_norm, const double* __restrict__ part, int n_part,
+                                                        double max_norm, float* __restrict__ norm_out) {
+  __shared__ double red[16];
+  const bool inf = inf_norm != 0;
+  double v = 0.0;
+  for (int i = threadIdx.x; i < n_part; i += 256) v = inf ? larger(v, part[i]) : v + part[i];
+  v = grad_fold(v, inf, red);
+  const double norm = inf ? v : __builtin_sqrt(v);
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  if (list.chunks) grad_scale_share(list, blockIdx.x, gridDim.x, grad_factor(norm, max_norm));
+}
+
+// short lists: one workgroup sums, then scales what it has just read
+__global__ __launch_bounds__(1024) void grad_clip_small_kernel(GradList list, int inf_norm, double max_norm,
+                                                               float* __restrict__ norm_out) {
+  __shared__ double red[16];
+  const double v = grad_norm_share(list, 0, 1, inf_norm != 0, red);
+  const double norm = inf_norm ? v : __builtin_sqrt(v);
+  if (threadIdx.x == 0) *norm_out = (float)norm;
+  grad_scale_share(list, 0, 1, grad_factor(norm, max_norm));
+}
+
+// tensors [lo, lo + count) of the caller's arrays as one launch's list
+static bool grad_list(GradList& list, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype,
+                      int lo, int count) {
+  long chunks = 0;
+  list.count = 0;
+  for (int i = lo; i < lo + count; i++) {
+    if (numel[i] < 0 || (numel[i] > 0 && !src[i]) || dtype[i] < FLM_F32 || dtype[i] > FLM_F16) return false;
+    if (numel[i] == 0) continue;
+    GradItem& it = list.item[list.count++];
+    it.src = src[i];
+    it.dst = dst ? dst[i] : nullptr;
+    it.numel = numel[i];
+    it.dtype = dtype[i];
+    it.first = (int)chunks;
+    chunks += (numel[i] + GRAD_CHUNK - 1) / GRAD_CHUNK;
+    if (chunks >= (1L << 30)) return false;
+  }
+  list.chunks = (int)chunks;
+  return true;
+}
+
+// A list that one workgroup handles alone: up to this many elements in all.
+#define GRAD_SMALL 65536
+
+static int grad_clip_run(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count,
+                         const GradOuter& outer, double max_norm, int inf_norm, double* workspace, float* norm_out,
+                         hipStream_t stream) {
+  GradList list;
+  long total = 0;
+  for (int lo = 0; lo < count; lo += FLM_GRAD_LIST) {       // every tensor is checked before anything is launched
+    if (!grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST)) return FLM_E_ARG;
+    for (int i = 0; i < list.count; i++) total += list.item[i].numel;
+  }
+  if (count <= FLM_GRAD_LIST && total <= GRAD_SMALL && !outer.r) {
+    hipLaunchKernelGGL(grad_clip_small_kernel, dim3(1), dim3(1024), 0, stream, list, inf_norm, max_norm, norm_out);
+    FLM_CHECK_LAUNCH();
+    return FLM_OK;
+  }
+  // partial results are dealt to the launches in proportion to their chunks, at least one each
+  const int launches = (count + FLM_GRAD_LIST - 1) / FLM_GRAD_LIST;
+  const long all_chunks = total / GRAD_CHUNK + count;
+  const int parts_max = GRAD_PARTS - launches;             // (at most 586 launches)
+  int n_part = 0;
+  for (int lo = 0; lo < count; lo += FLM_GRAD_LIST) {
+    grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST);
+    long blocks = all_chunks <= parts_max ? list.chunks : (long)((double)list.chunks / all_chunks * parts_max);
+    if (blocks < 1) blocks = 1;
+    GradOuter o = outer;
+    if (lo != 0) o.r = nullptr;
+    hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, list, o, inf_norm, workspace + n_part);
+    FLM_CHECK_LAUNCH();
+    n_part += (int)blocks;
+  }
+  for (int lo = 0; lo < count; lo += FLM_GRAD_LIST) {
+    grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST);
+    if (!dst) list.chunks = 0;                              // the norm alone
+    const int blocks = list.chunks < 1 ? 1 : (list.chunks < GRAD_PARTS ? list.chunks : GRAD_PARTS);
+    hipLaunchKernelGGL(grad_clip_kernel, dim3(blocks), dim3(256), 0, stream, list, inf_norm, workspace, n_part, max_norm,
+                       lo == 0 ? norm_out : (float*)nullptr);
+    FLM_CHECK_LAUNCH();
+    if (!dst) break;
+  }
+  return FLM_OK;
+}
+
+}  // namespace flm
+
+extern "C" int flm_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count,
+                             double max_norm, int inf_norm, double* workspace, float* norm_out, void* stream) {
+  if (!src || !numel || !dtype || count <= 0 || count > FLM_GRAD_MAX_TENSORS || !workspace || !norm_out ||
+      !(max_norm >= 0.0))
+    return FLM_E_ARG;
+  return flm::grad_clip_run(src, dst, numel, dtype, count, flm::GradOuter{}, max_norm, inf_norm, workspace, norm_out,
+                            (hipStream_t)stream);
+}
+
+extern "C" int flm_dqn_grad_clip(float* grads, int Rp, int T1, int NA, int rails4, int packed, const float* rcb,
+                                 double max_norm, int inf_norm, double* workspace, float* norm_out, void* stream) {
+  if (!grads || Rp <= 0 || T1 <= 0 || rails4 < 0 || rails4 > Rp || (rails4 > 0 && !rcb) || (packed && rails4 <= 0) ||
+      !workspace || !norm_out || !(max_norm >= 0.0))
+    return FLM_E_ARG;
+  const long n = flm_dqn_param_count(3 * Rp, T1, NA);
+  if (n <= 0) return FLM_E_ARG;
+  const long a1_w = 64L * T1 + 64, block = 512L * 64 * 3 * Rp, v1_w = a1_w + block + 512;
+  if (!packed) {
+    // the used rails lie scattered among rows that were left unwritten: only whole gradients or packed ones are taken
+    if (rails4 > 0) return FLM_E_ARG;
+    const void* src[1] = {grads};
+    void* dst[1] = {grads};
+    const int64_t numel[1] = {n};
+    const int32_t dtype[1] = {FLM_F32};
+    return flm::grad_clip_run(src, dst, numel, dtype, 1, flm::GradOuter{}, max_norm, inf_norm, workspace, norm_out,
+                              (hipStream_t)stream);
+  }
+  const long used = 512L * 64 * 3 * rails4;
+  float* piece[3] = {grads, grads + a1_w + block, grads + v1_w + block};
+  const int64_t numel[3] = {a1_w + used, 512 + used, n - (v1_w + block)};
+  const void* src[3] = {piece[0], piece[1], piece[2]};
+  void* dst[3] = {piece[0], piece[1], piece[2]};
+  const int32_t dtype[3] = {FLM_F32, FLM_F32, FLM_F32};
+  const flm::GradOuter outer{rcb, grads + a1_w + block, grads + v1_w + block, 3.0 * (Rp - rails4)};
+  return flm::grad_clip_run(src, dst, numel, dtype, 3, outer, max_norm, inf_norm, workspace, norm_out, (hipStream_t)stream);
+}

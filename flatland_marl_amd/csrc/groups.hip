@@ -1,0 +1,301 @@
+// Rows sorted by the group (here: the low-rank adapter) each of them uses: a stable counting sort on the device, and the
+// table of row tiles the adapter kernels run over.  Ids outside 0..E-1 mean "no group" and sort behind all others.
+//
+// A wave owns a run of consecutive rows.  It counts them per group, the counts are turned into first positions (groups
+// slowest, runs within a group in row order), and the wave then walks its rows again, 64 at a time: a lane's place is the
+// group's next position plus the number of lower lanes with the same group, which log2(E) ballots give.  Nothing depends
+// on the order in which waves run.
+// Up to GROUP_SMALL rows one workgroup does all of it in LDS; beyond that the three steps are three launches.
+#include "flm_adapters.h"
+
+namespace flm {
+
+#define GROUP_SMALL 8192
+#define GROUP_RUN 1024                   // rows of a wave (at least) in the large form
+#define GROUP_RUNS_MAX 4096
+
+__device__ __forceinline__ int row_key(const void* ids, int ids64, long i, int E) {
+  if (ids64) {
+    const int64_t v = reinterpret_cast<const int64_t*>(ids)[i];
+    return v >= 0 && v < E ? (int)v : E;
+  }
+  const int v = reinterpret_cast<const int32_t*>(ids)[i];
+  return (unsigned)v < (unsigned)E ? v : E;
+}
+
+// lanes of the wave that hold the same key (all 64 lanes take part; bits: bits of a key)
+__device__ __forceinline__ unsigned long long same_key(int key, int bits) {
+  unsigned long long m = ~0ull;
+  for (int b = 0; b < bits; b++) {
+    const bool one = (key >> b) & 1;
+    const unsigned long long v = __ballot(one);
+    m &= one ? v : ~v;
+  }
+  return m;
+}
+
+// exclusive prefix over the workgroup of one int per thread; total to all.  scratch: 17 ints
+__device__ __forceinline__ int block_scan(int v, int* scratch, int* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(inc, o);
+    if (lane >= o) inc += t;
+  }
+  __syncthreads();
+  if (lane == 63) scratch[w] = inc;
+  __syncthreads();
+  int base = 0, tot = 0;
+  for (int i = 0; i < nw; i++) {
+    const int c = scratch[i];
+    if (i < w) base += c;
+    tot += c;
+  }
+  *total = tot;
+  return base + inc - v;
+}
+
+// places rows [lo, hi) of a wave; next [E+1]: the wave's next position per group
+__device__ __forceinline__ void place_rows(const void* ids, int ids64, int lo, int hi, int E, int bits, int* next, int* order,
+                                           int* keys) {
+  const int lane = threadIdx.x & 63;
+  for (int i0 = lo; i0 < hi; i0 += 64) {
+    const int i = i0 + lane;
+    const bool in = i < hi;
+    const int key = in ? row_key(ids, ids64, i, E) : E;
+    const unsigned long long same = same_key(key, bits) & __ballot(in);
+    const int rank = __popcll(same & lanemask_lt());
+    int pos = 0;
+    if (in) pos = next[key] + rank;
+    // (all lanes have read before one lane a group writes, and that write is there before the next 64 rows read)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (in && rank == 0) next[key] += __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (in) {
+      order[pos] = i;
+      keys[pos] = key;
+    }
+  }
+}
+
+// Writes tiles [first, cap) in steps of stride.  off [E+1] and tstart [E+1] (number of tiles before a group) in LDS.
+__device__ __forceinline__ void write_tiles(const int* off, const int* tstart, int E, int cap, int first, int stride, int2* tiles) {
+  for (int t = first; t < cap; t += stride) {
+    int2 out = make_int2(0, 0);
+    if (t < tstart[E]) {
+      int lo = 0, hi = E - 1;                    // the last group whose first tile is at or before t
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tstart[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const int pos = off[lo] + (t - tstart[lo]) * FLM_ROW_TILE;
+      out = make_int2(pos, lo | (min(FLM_ROW_TILE, off[lo + 1] - pos) << 16));
+    }
+    tiles[t] = out;
+  }
+}
+
+// off [E+1] (counts in, first positions out; off[E] = rows with a group), tstart [E+1] out.  All threads; E + 1 <= 2048.
+__device__ __forceinline__ void scan_groups(int* off, int* tstart, int E, int* scratch) {
+  const int per = (E + 1 + blockDim.x - 1) / blockDim.x;          // consecutive groups per thread
+  const int g0 = threadIdx.x * per;
+  int rows = 0, tl = 0;
+  for (int j = 0; j < per; j++)
+    if (g0 + j < E) {
+      rows += off[g0 + j];
+      tl += (off[g0 + j] + FLM_ROW_TILE - 1) / FLM_ROW_TILE;
+    }
+  int total_rows, total_tiles;
+  int r = block_scan(rows, scratch, &total_rows);
+  int t = block_scan(tl, scratch, &total_tiles);
+  __syncthreads();
+  for (int j = 0; j < per; j++)
+    if (g0 + j < E) {
+      const int c = off[g0 + j];
+      off[g0 + j] = r;
+      tstart[g0 + j] = t;
+      r += c;
+      t += (c + FLM_ROW_TILE - 1) / FLM_ROW_TILE;
+    }
+  if (threadIdx.x == 0) {
+    off[E] = total_rows;
+    tstart[E] = total_tiles;
+  }
+  __syncthreads();
+}
+
+// LDS: cnt [waves][E+1], off [E+1], tstart [E+1], scratch [17]
+__global__ __launch_bounds__(1024) void group_small_kernel(const void* ids, int ids64, int n, int E, int bits, int* order, int* keys,
+                                                           int* offsets, int2* tiles, int cap) {
+  extern __shared__ int lds[];
+  const int nw = blockDim.x >> 6, w = threadIdx.x >> 6, lane = threadIdx.x & 63, E1 = E + 1;
+  int* cnt = lds;
+  int* off = cnt + nw * E1;
+  int* tstart = off + E1;
+  int* scratch = tstart + E1;
+  for (int i = threadIdx.x; i < nw * E1; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  const int run = ((n + nw - 1) / nw + 63) & ~63;
+  const int lo = min(n, w * run), hi = min(n, lo + run);
+  for (int i = lo + lane; i < hi; i += 64) atomicAdd(&cnt[w * E1 + row_key(ids, ids64, i, E)], 1);
+  __syncthreads();
+  // per group: counts of the waves -> rows before each wave; the group's total to off
+  for (int g = threadIdx.x; g < E1; g += blockDim.x) {
+    int s = 0;
+    for (int k = 0; k < nw; k++) {
+      const int c = cnt[k * E1 + g];
+      cnt[k * E1 + g] = s;
+      s += c;
+    }
+    off[g] = s;
+  }
+  __syncthreads();
+  scan_groups(off, tstart, E, scratch);
+  for (int i = threadIdx.x; i < nw * E1; i += blockDim.x) cnt[i] += off[i % E1];
+  for (int g = threadIdx.x; g < E1; g += blockDim.x) offsets[g] = off[g];
+  __syncthreads();
+  place_rows(ids, ids64, lo, hi, E, bits, cnt + w * E1, order, keys);
+  write_tiles(off, tstart, E, cap, threadIdx.x, blockDim.x, tiles);
+}
+
+// counts[run][E+1]; one wave per run
+__global__ __launch_bounds__(64) void group_count_kernel(const void* ids, int ids64, int n, int run, int E, int* counts) {
+  extern __shared__ int lds[];
+  const int E1 = E + 1;
+  for (int i = threadIdx.x; i < E1; i += 64) lds[i] = 0;
+  __syncthreads();
+  const long lo = (long)blockIdx.x * run, hi = min((long)n, lo + run);
+  for (long i = lo + threadIdx.x; i < hi; i += 64) atomicAdd(&lds[row_key(ids, ids64, i, E)], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i < E1; i += 64) counts[(long)blockIdx.x * E1 + i] = lds[i];
+}
+
+// Per group the rows before each run, in place, and the group's total.  64 groups a workgroup, one per lane; the 16 waves
+// take a sixteenth of the runs each.
+__global__ __launch_bounds__(1024) void group_scan_kernel(int* counts, int runs, int E, int* totals) {
+  __shared__ int part[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, E1 = E + 1, g = blockIdx.x * 64 + lane;
+  const int per = (runs + 15) / 16, lo = min(runs, w * per), hi = min(runs, lo + per);
+  int s = 0;
+  if (g < E1) {
+    int k = lo;
+    for (; k + 8 <= hi; k += 8) {
+      int c[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) c[u] = counts[(long)(k + u) * E1 + g];
+#pragma unroll
+      for (int u = 0; u < 8; u++) s += c[u];
+    }
+    for (; k < hi; k++) s += counts[(long)k * E1 + g];
+  }
+  part[w][lane] = s;
+  __syncthreads();
+  int base = 0, total = 0;
+#pragma unroll
+  for (int k = 0; k < 16; k++) {
+    if (k < w) base += part[k][lane];
+    total += part[k][lane];
+  }
+  if (g >= E1) return;
+  int k = lo;
+  for (; k + 8 <= hi; k += 8) {
+    int c[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) c[u] = counts[(long)(k + u) * E1 + g];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      counts[(long)(k + u) * E1 + g] = base;
+      base += c[u];
+    }
+  }
+  for (; k < hi; k++) {
+    const int c = counts[(long)k * E1 + g];
+    counts[(long)k * E1 + g] = base;
+    base += c;
+  }
+  if (w == 0) totals[g] = total;
+}
+
+// four runs a workgroup.  LDS: next [4][E+1], off [E+1], tstart [E+1], scratch [17]
+__global__ __launch_bounds__(256) void group_place_kernel(const void* ids, int ids64, int n, int run, int runs, int E, int bits,
+                                                          const int* counts, const int* totals, int* order, int* keys,
+                                                          int* offsets, int2* tiles, int cap) {
+  extern __shared__ int lds[];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, E1 = E + 1;
+  int* next = lds;
+  int* off = next + 4 * E1;
+  int* tstart = off + E1;
+  int* scratch = tstart + E1;
+  for (int g = threadIdx.x; g < E1; g += 256) off[g] = totals[g];
+  __syncthreads();
+  scan_groups(off, tstart, E, scratch);
+  const int r = blockIdx.x * 4 + w;
+  if (r < runs)
+    for (int g = lane; g < E1; g += 64) next[w * E1 + g] = off[g] + counts[(long)r * E1 + g];
+  if (blockIdx.x == 0)
+    for (int g = threadIdx.x; g < E1; g += 256) offsets[g] = off[g];
+  __syncthreads();
+  if (r < runs) {
+    const long lo = (long)r * run;
+    place_rows(ids, ids64, (int)lo, (int)min((long)n, lo + run), E, bits, next + w * E1, order, keys);
+  }
+  write_tiles(off, tstart, E, cap, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, tiles);
+}
+
+}  // namespace flm
+
+using namespace flm;
+
+static int group_run_rows(int n) {
+  long run = GROUP_RUN;
+  while ((n + run - 1) / run > GROUP_RUNS_MAX) run *= 2;
+  return (int)run;
+}
+
+extern "C" long flm_group_rows_ints(int n, int n_groups) {
+  return n > 0 && n_groups > 0 ? row_groups_ints(n, n_groups) : 0;
+}
+
+extern "C" long flm_group_rows_workspace(int n, int n_groups) {
+  if (n <= GROUP_SMALL || n_groups <= 0) return 0;
+  const int run = group_run_rows(n);
+  return ((long)(n + run - 1) / run + 1) * (n_groups + 1);
+}
+
+extern "C" int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* groups, int32_t* workspace, void* stream) {
+  if (!ids || !groups || n <= 0 || n > (1 << 30) || n_groups <= 0 || n_groups > FLM_GROUPS_MAX) return FLM_E_ARG;
+  const int E = n_groups, E1 = E + 1;
+  const RowGroups g = row_groups(groups, n, E);
+  int* order = const_cast<int*>(g.order);
+  int* keys = const_cast<int*>(g.key);
+  int* offsets = const_cast<int*>(g.offsets);
+  int2* tiles = const_cast<int2*>(g.tiles);
+  int bits = 0;
+  while ((1 << bits) <= E) bits++;
+  hipStream_t st = (hipStream_t)stream;
+  if (n <= GROUP_SMALL) {
+    int waves = (n + 63) / 64;
+    waves = waves < 4 ? 4 : (waves > 16 ? 16 : waves);
+    const size_t lds = sizeof(int) * ((size_t)(waves + 2) * E1 + 17);
+    if (lds > 64 * 1024) FLM_RAISE_LDS_ONCE(group_small_kernel);
+    hipLaunchKernelGGL(group_small_kernel, dim3(1), dim3(64 * waves), lds, st, ids, ids64, n, E, bits, order, keys, offsets,
+                       tiles, g.cap);
+    FLM_CHECK_LAUNCH();
+    return FLM_OK;
+  }
+  if (!workspace) return FLM_E_ARG;
+  const int run = group_run_rows(n), runs = (n + run - 1) / run;
+  int* totals = workspace + (long)runs * E1;
+  hipLaunchKernelGGL(group_count_kernel, dim3(runs), dim3(64), sizeof(int) * E1, st, ids, ids64, n, run, E, workspace);
+  FLM_CHECK_LAUNCH();
+  hipLaunchKernelGGL(group_scan_kernel, dim3((E1 + 63) / 64), dim3(1024), 0, st, workspace, runs, E, totals);
+  FLM_CHECK_LAUNCH();
+  hipLaunchKernelGGL(group_place_kernel, dim3((runs + 3) / 4), dim3(256), sizeof(int) * (6 * E1 + 17), st, ids, ids64, n, run,
+                     runs, E, bits, workspace, totals, order, keys, offsets, tiles, g.cap);
+  FLM_CHECK_LAUNCH();
+  return FLM_OK;
+}

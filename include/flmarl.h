@@ -617,6 +617,73 @@ int flm_dqn_adam_soft_update(float* params, const float* grads, float* m, float*
 /* target <- tau*local + (1-tau)*target, src/agent.py:120-131. */
 int flm_dqn_soft_update(float* target, const float* local, long n, double tau, void* stream);
 
+/* ---- Operators beside the network: adapters of many requests, gradient clipping --------------------------------------
+ * No counterpart in the reference, whose one network has one set of weights and whose optimizer never clips
+ * (src/agent.py:38, 111-116). */
+#define FLM_F32 0                 /* element types */
+#define FLM_BF16 1
+#define FLM_F16 2
+#define FLM_GROUPS_MAX 2047
+#define FLM_ADAPTER_MAX_RANK 128
+#define FLM_GRAD_MAX_TENSORS 65536
+
+/* Rows sorted by the group each belongs to (stable; the plan of the adapter calls).
+ *   ids [n] int32 (ids64 = 0) or int64 (ids64 = 1): 0..n_groups-1; any other value = the row has no group
+ *   groups [flm_group_rows_ints(n, n_groups)] int32 out, 16-byte aligned: order [n] (row numbers by group, rows without a
+ *     group last), key [n] (the group of order[i], n_groups for none), offsets [n_groups+1] (first position of each group;
+ *     offsets[n_groups] = rows that have one) and a table of row tiles.  key starts at the next multiple of four ints
+ *     behind order, offsets at the next one behind key
+ *   workspace [flm_group_rows_workspace(n, n_groups)] int32 (0: may be NULL)
+ * n <= 2^30, n_groups <= FLM_GROUPS_MAX. */
+long flm_group_rows_ints(int n, int n_groups);
+long flm_group_rows_workspace(int n, int n_groups);
+int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* groups, int32_t* workspace, void* stream);
+
+/* A shared projection with low-rank adapters: y_i = W x_i + bias + s_e B_e (A_e x_i) for the adapter e of row i, the
+ * projection alone for rows without one.
+ *   x [n,K], w [N,K], bias [N] (or NULL), y [n,N]: rows ldx / ldw / ldy elements apart, each row contiguous;
+ *   a [E,r,K], b [E,N,r] contiguous; all of type dtype (FLM_F32 / FLM_BF16 / FLM_F16)
+ *   groups: flm_group_rows(ids, ., n, E, ...); scale [E] float or NULL (then scale_all for every adapter)
+ *   low [n,r] float out (or NULL): A_e x_i, not scaled, zeros for rows without an adapter: what the backward pass takes
+ *   workspace: flm_adapter_workspace(n, K, N, r, E) bytes, 16-byte aligned; one per call in flight
+ * Sums are fp32, rounded once.  fp32 operands are multiplied as three bf16 terms each (fp32 accuracy; a row that meets an
+ * infinity or NaN becomes NaN, other rows do not).  An adapter's values reach the rows of that adapter only.
+ * n, K, N <= 2^20, r <= FLM_ADAPTER_MAX_RANK, E <= FLM_GROUPS_MAX.  y must not overlap an input. */
+long flm_adapter_workspace(int n, int K, int N, int r, int E);
+int flm_adapter_linear(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* a, const void* b,
+                       const int32_t* groups, const float* scale, float scale_all, int n, int K, int N, int r, int E,
+                       int dtype, void* workspace, void* y, long ldy, float* low, void* stream);
+
+/* Its backward pass for the gradient dy [n,N] of y; the projection itself (w, bias) is held fixed.
+ *   u_i = s_e B_e^T dy_i;  da_e = sum_{i of e} u_i x_i^T [E,r,K];  db_e = s_e sum_{i of e} dy_i low_i^T [E,N,r];
+ *   dx_i = W^T dy_i + A_e^T u_i [n,K] (dx = NULL: not computed, w and a may then be NULL)
+ * da and db are written whole: zeros for adapters without rows.  Sums have a fixed order.
+ * workspace: flm_adapter_backward_workspace(n, K, N, r, E, dtype, dx != NULL) bytes, 16-byte aligned. */
+long flm_adapter_backward_workspace(int n, int K, int N, int r, int E, int dtype, int need_dx);
+int flm_adapter_linear_backward(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* a,
+                                const void* b, const int32_t* groups, const float* scale, float scale_all, const float* low,
+                                int n, int K, int N, int r, int E, int dtype, void* workspace, void* dx, long lddx, void* da,
+                                void* db, void* stream);
+
+/* Global norm of many gradient tensors and clipping: norm = sqrt(sum of all squares) (inf_norm != 0: the largest
+ * absolute value), dst = src * min(1, max_norm / (norm + 1e-6)).
+ *   src, dst, numel, dtype: HOST arrays of count device pointers, element counts and FLM_F32 / FLM_BF16 / FLM_F16;
+ *   dst[i] == src[i] clips in place, dst[i] == NULL only counts in the norm, dst == NULL: the norm alone.  A dst overlaps no
+ *   src but its own, and no other dst
+ *   workspace [FLM_GRAD_WORKSPACE] double; norm_out [1] float
+ * Sums are kept in 64 bits and have a fixed order.  A NaN norm makes every gradient NaN, an infinite one makes the finite
+ * ones zero, as the formula does.  count <= FLM_GRAD_MAX_TENSORS, max_norm >= 0. */
+#define FLM_GRAD_WORKSPACE 2048
+int flm_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count,
+                  double max_norm, int inf_norm, double* workspace, float* norm_out, void* stream);
+
+/* The same for the network's flat gradient, in place.  packed = 0: all flm_dqn_param_count(3*Rp, T1, NA) floats (rails4 = 0,
+ * rcb may be NULL).  packed = 1: the form flm_dqn_learn_grads_u8_rails leaves with fill_padding = 2 (rails4 and rcb as
+ * there): the pieces that are there, and in the norm also the gradient under the empty rows, which the optimizer pass
+ * forms from the (then clipped) bias gradient and rcb. */
+int flm_dqn_grad_clip(float* grads, int Rp, int T1, int NA, int rails4, int packed, const float* rcb, double max_norm,
+                      int inf_norm, double* workspace, float* norm_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,281 @@
+"""Rows sorted by group, the shared projection with low-rank adapters and its backward pass, against plain 64-bit forms.
+Needs an MI355X."""
+import numpy as np
+import pytest
+import torch
+
+from tests import adapter_ref as ref
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+# rows, inputs, outputs, rank, adapters, skewed
+SIZES = [
+    (1, 64, 32, 16, 1, False),
+    (1, 1000, 130, 4, 20, False),
+    (2, 7, 5, 1, 3, False),
+    (16, 515, 96, 5, 4, False),
+    (17, 256, 64, 16, 3, False),
+    (37, 1024, 512, 16, 24, False),
+    (64, 192, 128, 32, 200, False),
+    (65, 320, 129, 33, 5, True),
+    (130, 129, 131, 17, 2, False),
+    (300, 512, 256, 64, 9, True),
+    (517, 264, 384, 128, 6, False),
+    (1031, 200, 72, 8, 1, False),
+]
+
+
+def _check(got, exact, absolute, terms, kind):
+    tol = ref.bound(exact, absolute, terms, kind)
+    err = (got.cpu().double() - exact).abs()
+    assert torch.isfinite(got).all()
+    worst = (err / tol).max().item() if err.numel() else 0.0
+    assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("e", [1, 7, 64, 255, 2047])
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 317, 8191, 8192, 8193, 100003])
+def test_rows_sorted(n, e):
+    from flatland_marl_amd.adapters import group_rows
+    rng = np.random.default_rng(n * 31 + e)
+    ids = rng.integers(-1 if n % 2 else 0, e + (2 if n % 3 == 0 else 0), n)
+    g = group_rows(torch.from_numpy(ids.astype(np.int32 if n % 5 else np.int64)).cuda(), e)
+    key = np.where((ids >= 0) & (ids < e), ids, e)
+    order = np.argsort(key, kind="stable")
+    offsets = np.searchsorted(key[order], np.arange(e + 1))
+    assert np.array_equal(g.order.cpu().numpy(), order)
+    assert np.array_equal(g.keys.cpu().numpy(), key[order])
+    assert np.array_equal(g.offsets.cpu().numpy(), offsets)
+    # the tile table covers every row that has a group once, tiles inside one group
+    at = (n + 3) // 4 * 8 + (e + 4) // 4 * 4
+    tiles = g.buf[at:].cpu().numpy().reshape(-1, 2)
+    want = [(lo + i, grp, min(32, hi - lo - i)) for grp, (lo, hi) in enumerate(zip(offsets[:-1], offsets[1:]))
+            for i in range(0, hi - lo, 32)]
+    got = [(p, y & 0xffff, y >> 16) for p, y in tiles.tolist()]
+    assert got[:len(want)] == want and all(t[2] == 0 for t in got[len(want):])
+
+
+def test_rows_sorted_ids_of_any_value():
+    from flatland_marl_amd.adapters import group_rows
+    ids = torch.tensor([5, -2 ** 31, 2 ** 31 - 1, 0, 7, -1, 3, 8], dtype=torch.int32)
+    g = group_rows(ids.cuda(), 8)
+    assert g.order.tolist() == [3, 6, 0, 4, 1, 2, 5, 7] and g.keys.tolist() == [0, 3, 5, 7, 8, 8, 8, 8]
+    wide = torch.tensor([2 ** 32 + 1, 1, -2 ** 63, 0], dtype=torch.int64)       # not the group 1 that its low half names
+    assert group_rows(wide.cuda(), 2).order.tolist() == [3, 1, 0, 2]
+    none = group_rows(torch.zeros(0, dtype=torch.int32).cuda(), 3)
+    assert none.order.numel() == 0 and none.offsets.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("n,k,n_out,r,e,skew", SIZES)
+def test_forward(n, k, n_out, r, e, skew, kind):
+    from flatland_marl_amd.adapters import adapter_linear, group_rows
+    c = ref.case(n + k, n, k, n_out, r, e, kind, skew=skew)
+    d = ref.to_gpu(c)
+    y, low = adapter_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], group_rows(d["ids"], e), scale=d["scale"],
+                            keep_low=True)
+    want, want_low = ref.forward(c)
+    size, size_low = ref.forward(c, absolute=True)
+    _check(low, want_low, size_low, k, torch.float32)
+    _check(y, want, size, k + r, kind)
+    assert (low.cpu()[c["ids"] < 0] == 0).all()
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("n,k,n_out,r,e,skew", SIZES)
+def test_backward(n, k, n_out, r, e, skew, kind):
+    from flatland_marl_amd.adapters import adapter_linear_backward, group_rows
+    c = ref.case(n + k + 50, n, k, n_out, r, e, kind, skew=skew)
+    low = ref.forward(c)[1].float()
+    d = ref.to_gpu(c)
+    g = group_rows(d["ids"], e)
+    dx, da, db = adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low.cuda(), scale=d["scale"])
+    want, size = ref.backward(c, low), ref.backward(c, low, absolute=True)
+    _check(dx, want[0], size[0], n_out + r, kind)
+    _check(da, want[1], size[1], n_out + n, kind)
+    _check(db, want[2], size[2], n, kind)
+    # the gradients of the adapters alone: the same bits, into buffers that held something else
+    da2, db2 = torch.full_like(da, float("nan")), torch.full_like(db, float("nan"))
+    none, da3, db3 = adapter_linear_backward(d["dy"], d["x"], None, d["a"], d["b"], g, low.cuda(), scale=d["scale"],
+                                             need_dx=False, da=da2, db=db2)
+    assert none is None and da3 is da2 and db3 is db2
+    assert torch.equal(da, da2) and torch.equal(db, db2)
+
+
+def test_gradients_against_differences():
+    """The gradients of sum(dy * y) along random directions against central differences of the 64-bit formula."""
+    from flatland_marl_amd.adapters import adapter_linear_backward, group_rows
+    c = ref.case(3, 70, 90, 50, 6, 4, torch.float32)
+    low = ref.forward(c)[1].float()
+    d = ref.to_gpu(c)
+    got = dict(zip("xab", adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], group_rows(d["ids"], 4),
+                                                  low.cuda(), scale=d["scale"])))
+    for i, name in enumerate("xab"):
+        step = ref.rand(200 + i, *c[name].shape)
+        h = 1e-4
+        loss = []
+        for sign in (h, -h):
+            moved = dict(c)
+            moved[name] = c[name].double() + sign * step
+            loss.append((c["dy"].double() * ref.forward(moved)[0]).sum().item())
+        slope = (loss[0] - loss[1]) / (2 * h)
+        mine = (got[name].cpu().double() * step).sum().item()
+        # the loss is linear in each of the three; what is left is the kernels' rounding of every element
+        size = dict(zip("xab", ref.backward(c, low, absolute=True)))[name]
+        assert abs(mine - slope) <= (ref.bound(size, size, 160, torch.float32) * step.abs()).sum().item() + 1e-9
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("n", [40, 200])
+def test_bare_rows_and_one_adapter_for_all(n, kind):
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    for which in (-1, 2):
+        c = ref.case(9, n, 96, 80, 12, 5, kind)
+        c["ids"].fill_(which)
+        d = ref.to_gpu(c)
+        g = group_rows(d["ids"], 5)
+        y, low = adapter_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], g, scale=d["scale"], keep_low=True)
+        _check(y, ref.forward(c)[0], ref.forward(c, True)[0], 96 + 12, kind)
+        dx, da, db = adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low, scale=d["scale"])
+        for got, want, size, terms in zip((dx, da, db), ref.backward(c, low.cpu()), ref.backward(c, low.cpu(), True),
+                                          (92, 80 + n, n)):
+            _check(got, want, size, terms, kind)
+        others = [e for e in range(5) if e != which]
+        assert (da[others] == 0).all() and (db[others] == 0).all()
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("n", [24, 150])
+def test_bad_values_stay_where_they_are(n, kind):
+    """An adapter full of infinities and NaN reaches its own rows only, a row with one only itself, and neither reaches the
+    gradients of other adapters."""
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    c = ref.case(21, n, 72, 56, 9, 4, kind)
+    c["ids"][:4] = torch.tensor([0, 1, 2, 3])
+    clean = ref.forward(c)
+    size = ref.forward(c, True)
+    bad = {name: t.clone() for name, t in c.items()}
+    bad["a"][1] = float("nan")
+    bad["b"][1] = float("inf")
+    bad["x"][2, 5] = float("inf")                       # a row of adapter 2
+    bad["dy"][2, 7] = float("nan")
+    d = ref.to_gpu(bad)
+    g = group_rows(d["ids"], 4)
+    y, low = adapter_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], g, scale=d["scale"], keep_low=True)
+    hit = (c["ids"] == 1) | (torch.arange(n) == 2)
+    assert not torch.isfinite(y.cpu()[hit]).all(dim=1).any()
+    keep = ~hit
+    _check(y[keep.cuda()], clean[0][keep], size[0][keep], 72 + 9, kind)
+    low0 = clean[1].float()
+    dx, da, db = adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low0.cuda(), scale=d["scale"])
+    want, sizes = ref.backward(c, low0), ref.backward(c, low0, True)
+    _check(dx[keep.cuda()], want[0][keep], sizes[0][keep], 56 + 9, kind)
+    for e in (0, 3):
+        _check(da[e], want[1][e], sizes[1][e], 56 + n, kind)
+        _check(db[e], want[2][e], sizes[2][e], n, kind)
+    assert not torch.isfinite(da[2]).all() and not torch.isfinite(db[2]).all()
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("n", [5, 100])
+def test_strided_rows(n, kind):
+    """Operands that are columns of wider matrices, starting at odd elements, and an expanded row."""
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    c = ref.case(33, n, 64, 48, 8, 3, kind)
+
+    def wide(t, pad):
+        w = torch.full((t.shape[0], t.shape[1] + 2 * pad), float("nan"), dtype=t.dtype, device="cuda")
+        w[:, pad:-pad] = t.cuda()
+        return w[:, pad:-pad]
+
+    d = ref.to_gpu(c)
+    g = group_rows(d["ids"], 3)
+    x, weight, dy = wide(c["x"], 3), wide(c["weight"], 5), wide(c["dy"], 1)
+    y, low = adapter_linear(x, weight, d["bias"], d["a"], d["b"], g, scale=d["scale"], keep_low=True)
+    _check(y, ref.forward(c)[0], ref.forward(c, True)[0], 72, kind)
+    got = adapter_linear_backward(dy, x, weight, d["a"], d["b"], g, low, scale=d["scale"])
+    for t, want, size, terms in zip(got, ref.backward(c, low.cpu()), ref.backward(c, low.cpu(), True), (56, 48 + n, n)):
+        _check(t, want, size, terms, kind)
+    c["x"] = c["x"][:1].expand(n, 64)
+    y = adapter_linear(d["x"][:1].expand(n, 64), weight, d["bias"], d["a"], d["b"], g, scale=d["scale"])
+    _check(y, ref.forward(c)[0], ref.forward(c, True)[0], 72, kind)
+
+
+def test_number_as_scale_and_no_bias():
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    c = ref.case(41, 90, 64, 64, 16, 3, torch.float32)
+    c["scale"].fill_(0.5)
+    c["bias"].zero_()
+    d = ref.to_gpu(c)
+    g = group_rows(d["ids"], 3)
+    args = (d["a"], d["b"], g)
+    y, low = adapter_linear(d["x"], d["weight"], d["bias"], *args, scale=d["scale"], keep_low=True)
+    assert torch.equal(y, adapter_linear(d["x"], d["weight"], None, *args, scale=0.5))
+    one = adapter_linear_backward(d["dy"], d["x"], d["weight"], *args, low, scale=d["scale"])
+    two = adapter_linear_backward(d["dy"], d["x"], d["weight"], *args, low, scale=0.5)
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+
+
+def test_no_rows():
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    c = ref.to_gpu(ref.case(1, 3, 16, 8, 4, 2, torch.bfloat16))
+    g = group_rows(c["ids"][:0], 2)
+    y, low = adapter_linear(c["x"][:0], c["weight"], c["bias"], c["a"], c["b"], g, keep_low=True)
+    assert y.shape == (0, 8) and low.shape == (0, 4)
+    dx, da, db = adapter_linear_backward(c["dy"][:0], c["x"][:0], c["weight"], c["a"], c["b"], g, low)
+    assert dx.shape == (0, 16) and (da == 0).all() and (db == 0).all()
+
+
+def _train_pass(d, out):
+    """Sort, forward, backward, clip: what a training step does."""
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    from flatland_marl_amd.gradients import clip_grad_norm_
+    g = group_rows(d["ids"], d["a"].shape[0])
+    y, low = adapter_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], g, scale=d["scale"], keep_low=True)
+    dx, da, db = adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low, scale=d["scale"])
+    norm = clip_grad_norm_([da, db], 0.5)
+    out[:] = [y, dx, da, db, norm]
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("n", [33, 140])
+def test_together_in_a_graph_on_another_stream(n, kind):
+    """Two captured graphs, replayed in turn with new inputs and eager work between, give the eager results."""
+    sizes = [(n, 128, 96, 16, 5), (n + 9, 72, 200, 7, 3)]
+    held, graphs, outs = [], [], []
+    side = torch.cuda.Stream()
+    for i, (rows, k, n_out, r, e) in enumerate(sizes):
+        d = ref.to_gpu(ref.case(70 + i, rows, k, n_out, r, e, kind))
+        out = []
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _train_pass(d, out)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            _train_pass(d, out)
+        held.append(d)
+        graphs.append(graph)
+        outs.append(out)
+    for turn in range(4):
+        for i, (rows, k, n_out, r, e) in enumerate(sizes):
+            new = ref.to_gpu(ref.case(100 + 10 * turn + i, rows, k, n_out, r, e, kind))
+            for name in new:
+                held[i][name].copy_(new[name])
+        for i in (1, 0):
+            graphs[i].replay()
+        for i in range(2):
+            eager = []
+            _train_pass(held[i], eager)
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(outs[i], eager)), (turn, i)
+
+
+def test_repeated_calls_give_the_same_bits():
+    d = ref.to_gpu(ref.case(5, 700, 300, 200, 24, 11, torch.bfloat16, skew=True))
+    first = []
+    _train_pass(d, first)
+    for _ in range(3):
+        again = []
+        _train_pass(d, again)
+        assert all(torch.equal(p, q) for p, q in zip(first, again))
