@@ -90,7 +90,7 @@ _SIGNATURES = {
     "flm_group_rows_ints": [_i, _i],
     "flm_group_rows_workspace": [_i, _i],
     "flm_group_rows": [_p, _i, _i, _i, _p, _p, _p],
-    "flm_adapter_workspace": [_i] * 5,
+    "flm_adapter_workspace": [_i] * 6,
     "flm_adapter_linear": [_p, C.c_long, _p, C.c_long, _p, _p, _p, _p, _p, C.c_float, _i, _i, _i, _i, _i, _i, _p, _p, C.c_long,
                            _p, _p],
     "flm_adapter_backward_workspace": [_i] * 7,

@@ -112,7 +112,7 @@ def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False):
     y = torch.empty((n, n_out), dtype=x.dtype, device=dev)
     low = torch.empty((n, r), dtype=torch.float32, device=dev) if keep_low else None
     if n:
-        work = torch.empty(query("flm_adapter_workspace", n, k, n_out, r, e), dtype=torch.uint8, device=dev)
+        work = torch.empty(query("flm_adapter_workspace", n, k, n_out, r, e, DTYPES[x.dtype]), dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             call("flm_adapter_linear", x.data_ptr(), ldx, weight.data_ptr(), ldw, bias.data_ptr() if bias is not None else None,
                  a.data_ptr(), b.data_ptr(), groups.buf.data_ptr(), *scales, n, k, n_out, r, e, DTYPES[x.dtype], work.data_ptr(),

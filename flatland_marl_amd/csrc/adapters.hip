@@ -28,17 +28,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // ---- eight consecutive elements, at any alignment the type allows ------------------------------------------------
 template <typename T> struct Vec8 { T v[8]; };
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Packed8 { T v[8]; };
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Packed4 { T v[4]; };
+// (as words: an array of 16-bit elements at 2-byte alignment may be loaded one by one, words at that alignment are not)
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Packed8 { unsigned w[2 * sizeof(T)]; };
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Packed4 { unsigned w[sizeof(T)]; };
+template <typename T> struct Vec4 { T v[4]; };
 
 // avail: elements that exist from p on (may be <= 0: zeros, nothing is read)
 template <typename T>
 __device__ __forceinline__ Vec8<T> load8(const T* p, long avail) {
   Vec8<T> o;
   if (avail >= 8) {
-    const Packed8<T> t = *reinterpret_cast<const Packed8<T>*>(p);
-#pragma unroll
-    for (int j = 0; j < 8; j++) o.v[j] = t.v[j];
+    o = __builtin_bit_cast(Vec8<T>, *reinterpret_cast<const Packed8<T>*>(p));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; j++) o.v[j] = j < avail ? p[j] : (T)0.f;
@@ -57,10 +57,10 @@ __device__ __forceinline__ Vec8<T> load8_strided(const T* p, long stride, long a
 template <typename T>
 __device__ __forceinline__ void store4(T* p, const float (&v)[4], long avail) {
   if (avail >= 4) {
-    Packed4<T> t;
+    Vec4<T> t;
 #pragma unroll
     for (int j = 0; j < 4; j++) t.v[j] = (T)v[j];
-    *reinterpret_cast<Packed4<T>*>(p) = t;
+    *reinterpret_cast<Packed4<T>*>(p) = __builtin_bit_cast(Packed4<T>, t);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; j++)
@@ -169,8 +169,9 @@ __device__ __forceinline__ f32x16 mul32(f16x8 a, f16x8 b, f32x16 c) { return __b
 // which k a lane holds is the same for both operands, so their order does not matter), and meet in LDS.  Nothing is reused
 // between workgroups but through the L2, so this form is for operands that are read once: few rows, or few columns.
 // result: lane (c = lane & 15, q = lane >> 4) holds D[v = 16*ni + 4q .. +3][x = 16*mi + c]
-#define MINI_K 64
-template <typename T, int MR, int NR, bool V_STRIDED>
+// The loads of a wave's next step are in flight while the matrix cores work on the one before.
+// S: steps of 32 k taken together (a lane then holds 8*S consecutive elements of a row).
+template <typename T, int MR, int NR, int S, bool V_STRIDED>
 __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* const (&vr)[NR], long v_stride, int k_begin,
                                              int k_end, f32x4 (&acc)[MR][NR]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 4;
@@ -178,22 +179,39 @@ __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* 
   for (int mi = 0; mi < MR; mi++)
 #pragma unroll
     for (int ni = 0; ni < NR; ni++) acc[mi][ni] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k0 = k_begin + w * MINI_K; k0 < k_end; k0 += 4 * MINI_K) {
+  Vec8<T> rx[S][MR], rv[S][NR];
+  auto fetch = [&](int k0) {
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      const int k = k0 + q * 16 + s * 8;
+    for (int s = 0; s < S; s++) {
+      const int k = k0 + q * (8 * S) + s * 8;
       const int avail = k_end - k;
-      Wide<T> x[MR];
-#pragma unroll
-      for (int mi = 0; mi < MR; mi++) x[mi] = wide(load8(xr[mi] + k, xr[mi] ? avail : 0));
 #pragma unroll
       for (int ni = 0; ni < NR; ni++) {
         const int have = vr[ni] ? avail : 0;
-        const Wide<T> v = wide(V_STRIDED ? load8_strided(vr[ni] + (long)k * v_stride, v_stride, have) : load8(vr[ni] + k, have));
-#pragma unroll
-        for (int mi = 0; mi < MR; mi++) acc[mi][ni] = mul16(v, x[mi], acc[mi][ni]);
+        rv[s][ni] = V_STRIDED ? load8_strided(vr[ni] + (long)k * v_stride, v_stride, have) : load8(vr[ni] + k, have);
       }
+#pragma unroll
+      for (int mi = 0; mi < MR; mi++) rx[s][mi] = load8(xr[mi] + k, xr[mi] ? avail : 0);
     }
+  };
+  int k0 = k_begin + w * (32 * S);
+  if (k0 < k_end) fetch(k0);
+  for (; k0 < k_end; k0 += 4 * 32 * S) {
+    Wide<T> x[S][MR], v[S][NR];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+#pragma unroll
+      for (int mi = 0; mi < MR; mi++) x[s][mi] = wide(rx[s][mi]);
+#pragma unroll
+      for (int ni = 0; ni < NR; ni++) v[s][ni] = wide(rv[s][ni]);
+    }
+    if (k0 + 4 * 32 * S < k_end) fetch(k0 + 4 * 32 * S);
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+      for (int ni = 0; ni < NR; ni++)
+#pragma unroll
+        for (int mi = 0; mi < MR; mi++) acc[mi][ni] = mul16(v[s][ni], x[s][mi], acc[mi][ni]);
   }
 }
 
@@ -243,7 +261,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(ShrinkArgs a, RowGroups g) 
     vr[ni] = j < a.r ? (const T*)a.v + (long)e * a.v_group + (long)j * a.v_row : nullptr;
   }
   f32x4 acc[MR][NR];
-  mini_product<T, MR, NR, V_STRIDED>(xr, vr, a.v_k, k_begin, k_end, acc);
+  mini_product<T, MR, NR, (MR + NR <= 4 ? 2 : 1), V_STRIDED>(xr, vr, a.v_k, k_begin, k_end, acc);
   mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
     const int m = mi * 16 + c, j = ni * 16 + 4 * q;
     if (m < rows && j < a.rp)
@@ -258,93 +276,27 @@ struct BaseArgs {
   float* part;                           // [slice][n][N]
 };
 
-// the projection of up to 16*MR rows: 16 outputs a workgroup, grid (outputs / 16, K slices)
-template <typename T, int MR>
+// the projection of up to 16*MR rows: 16*NR outputs a workgroup, grid (outputs / (16*NR), K slices)
+template <typename T, int MR, int NR>
 __global__ __launch_bounds__(256) void base_rows_kernel(BaseArgs a) {
-  __shared__ f32x4 red[4 * MR * 64];
+  __shared__ f32x4 red[4 * MR * NR * 64];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * (16 * NR);
   const int k_begin = blockIdx.y * a.kslice, k_end = min(a.K, k_begin + a.kslice);
-  const T *xr[MR], *vr[1];
+  const T *xr[MR], *vr[NR];
 #pragma unroll
   for (int mi = 0; mi < MR; mi++) xr[mi] = mi * 16 + c < a.n ? (const T*)a.x + (long)(mi * 16 + c) * a.ldx : nullptr;
-  vr[0] = n0 + c < a.N ? (const T*)a.w + (long)(n0 + c) * a.ldw : nullptr;
-  f32x4 acc[MR][1];
-  mini_product<T, MR, 1, false>(xr, vr, 1, k_begin, k_end, acc);
-  mini_meet<MR, 1>(acc, red, [&](int mi, int, const f32x4& v) {
-    const int m = mi * 16 + c, n = n0 + 4 * q;
+#pragma unroll
+  for (int ni = 0; ni < NR; ni++) vr[ni] = n0 + ni * 16 + c < a.N ? (const T*)a.w + (long)(n0 + ni * 16 + c) * a.ldw : nullptr;
+  f32x4 acc[MR][NR];
+  mini_product<T, MR, NR, 2, false>(xr, vr, 1, k_begin, k_end, acc);
+  mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
+    const int m = mi * 16 + c, n = n0 + ni * 16 + 4 * q;
     if (m < a.n) {
       const float f[4] = {v[0], v[1], v[2], v[3]};
       store4(a.part + ((long)blockIdx.y * a.n + m) * a.N + n, f, a.N - n);
     }
   });
-}
-
-// ---- the projection of many rows, 16-bit types -------------------------------------------------------------------------
-// part[slice][n][N] = X[n,K] * W[N,K]^T: tiles of 128 x 128, four waves of 64 x 64, 32 k a stage, the next stage fetched
-// into registers while the matrix cores work on the one in LDS.  Any sizes and strides.
-#define BT_ROW 40                        // elements per LDS row of 32 k
-template <typename T>
-__global__ __launch_bounds__(256) void base_tile_kernel(BaseArgs a) {
-  __shared__ __attribute__((aligned(16))) T lx[128 * BT_ROW], lw[128 * BT_ROW];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, h = lane >> 5;
-  const int m0 = blockIdx.y * 128, n0 = blockIdx.x * 128, wm = (w >> 1) * 64, wn = (w & 1) * 64;
-  const int k_begin = blockIdx.z * a.kslice, k_end = min(a.K, k_begin + a.kslice);
-  f32x16 acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
-  Vec8<T> fx[2], fw[2];
-  auto fetch = [&](int k0) {
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-      const int row = (tid >> 2) + 64 * s, k = k0 + (tid & 3) * 8;
-      fx[s] = load8((const T*)a.x + (long)(m0 + row) * a.ldx + k, m0 + row < a.n ? k_end - k : 0);
-      fw[s] = load8((const T*)a.w + (long)(n0 + row) * a.ldw + k, n0 + row < a.N ? k_end - k : 0);
-    }
-  };
-  fetch(k_begin);
-  for (int k0 = k_begin; k0 < k_end; k0 += 32) {
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-      const int at = ((tid >> 2) + 64 * s) * BT_ROW + (tid & 3) * 8;
-      *reinterpret_cast<uint4*>(lx + at) = __builtin_bit_cast(uint4, fx[s]);
-      *reinterpret_cast<uint4*>(lw + at) = __builtin_bit_cast(uint4, fw[s]);
-    }
-    __syncthreads();
-    if (k0 + 32 < k_end) fetch(k0 + 32);
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-      typedef typename Operand<T>::V V;
-      V x[2], v[2];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        x[i] = __builtin_bit_cast(V, *reinterpret_cast<const uint4*>(lx + (wm + i * 32 + c) * BT_ROW + s * 16 + h * 8));
-        v[i] = __builtin_bit_cast(V, *reinterpret_cast<const uint4*>(lw + (wn + i * 32 + c) * BT_ROW + s * 16 + h * 8));
-      }
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) acc[i][j] = mul32(v[j], x[i], acc[i][j]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int m = m0 + wm + i * 32 + c;
-    if (m >= a.n) continue;
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int r4 = 0; r4 < 4; r4++) {
-        const int n = n0 + wn + j * 32 + 8 * r4 + 4 * h;
-        const float f[4] = {acc[i][j][4 * r4], acc[i][j][4 * r4 + 1], acc[i][j][4 * r4 + 2], acc[i][j][4 * r4 + 3]};
-        store4(a.part + ((long)blockIdx.z * a.n + m) * a.N + n, f, a.N - n);
-      }
-  }
 }
 
 // out[C][R] = in[R][C] (the weight with its contraction axis last, for the gradient of the inputs)
@@ -381,100 +333,314 @@ struct FinishArgs {
 
 __device__ __forceinline__ float adapter_scale(const float* scale, float all, int e) { return scale ? scale[e] : all; }
 
-// Adds s_e * low_i . V_e(n, .) to acc: lane (c, h) of the wave holds row (sorted position) pos + c of a tile of 32, outputs
-// n0 + 8*(r >> 2) + 4*h + (r & 3).  The rows of a tile may use several adapters: each adapter's product is formed apart and
-// added to its own rows only, so that no value of one adapter (an infinity, a NaN) can reach the rows of another.
-// key: the lane's adapter (E or more: none).  All lanes of the wave take part.
-template <typename T, bool V_STRIDED>
-__device__ __forceinline__ void add_adapters(const FinishArgs& a, long pos, int key, int n0, f32x16& acc) {
-  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-  unsigned todo = (unsigned)__ballot(key < a.E);                  // (both halves of the wave hold the same 32 rows)
-  while (todo) {
-    const int first = __builtin_ctz(todo);
-    const int e = __builtin_amdgcn_readlane(key, first);
-    todo &= ~(unsigned)__ballot(key == e);
-    const float s = adapter_scale(a.scale, a.scale_all, e);
-    f32x16 t;
+// The scaled narrow products of `rows` sorted positions from pos on, as bf16 terms in LDS: lt[(term*rows + row)*stride + j],
+// stride = low_stride(rp).  threads of the workgroup share the work; a barrier follows at the caller.
+__device__ __forceinline__ int low_stride(int rp) { return rp + 8; }          // (16 bytes more: rows fall into different banks)
+template <int LOW>
+__device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& g, long pos, int rows, __bf16* lt) {
+  const int per = a.rp >> 3, stride = low_stride(a.rp);
+  for (int i = threadIdx.x; i < rows * per; i += blockDim.x) {
+    const int row = i / per, j = (i - row * per) * 8;
+    float f[8];
 #pragma unroll
-    for (int r = 0; r < 16; r++) t[r] = 0.f;
-    const bool mine = key == e;
-    for (int j0 = 0; j0 < a.r; j0 += 16) {
-      const int j = j0 + 8 * h;
-      float f[8];
+    for (int u = 0; u < 8; u++) f[u] = 0.f;
+    const int e = pos + row < a.n ? g.key[pos + row] : a.E;
+    if (e < a.E) {
+      const float* p = a.low + (pos + row) * a.rp + j;
+      const long step = (long)a.n * a.rp;
+      int z = 0;
+      for (; z + 4 <= a.low_slices; z += 4) {
+        f32x4 v[4][2];
 #pragma unroll
-      for (int i = 0; i < 8; i++) f[i] = 0.f;
-      if (mine)
-        for (int z = 0; z < a.low_slices; z++) {
-          const float* p = a.low + ((long)z * a.n + pos + c) * a.rp + j;
-          const f32x4 p0 = reinterpret_cast<const f32x4*>(p)[0], p1 = reinterpret_cast<const f32x4*>(p)[1];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            f[i] += p0[i];
-            f[4 + i] += p1[i];
-          }
+        for (int k = 0; k < 4; k++) {
+          v[k][0] = reinterpret_cast<const f32x4*>(p + (z + k) * step)[0];
+          v[k][1] = reinterpret_cast<const f32x4*>(p + (z + k) * step)[1];
         }
 #pragma unroll
-      for (int i = 0; i < 8; i++) f[i] = j + i < a.r ? f[i] * s : 0.f;
-      bf16x8 lt[Terms<T>::low], vt[Terms<T>::own];
-      split_terms<Terms<T>::low>(f, lt);
-      const int n = n0 + c;
-      const T* vp = (const T*)a.v + (long)e * a.v_group + (long)n * a.v_row + (long)j * a.v_j;
-      const int have = n < a.N ? a.r - j : 0;
-      own_terms<T>(V_STRIDED ? load8_strided(vp, a.v_j, have) : load8(vp, have), vt);
-      t = mul_terms32<Terms<T>::own, Terms<T>::low>(vt, lt, t);
-    }
+        for (int k = 0; k < 4; k++)
 #pragma unroll
-    for (int r = 0; r < 16; r++) acc[r] = mine ? acc[r] + t[r] : acc[r];
+          for (int u = 0; u < 8; u++) f[u] += v[k][u >> 2][u & 3];
+      }
+      for (; z < a.low_slices; z++) {
+        const f32x4 v0 = reinterpret_cast<const f32x4*>(p + z * step)[0], v1 = reinterpret_cast<const f32x4*>(p + z * step)[1];
+#pragma unroll
+        for (int u = 0; u < 8; u++) f[u] += u < 4 ? v0[u] : v1[u - 4];
+      }
+      const float s = adapter_scale(a.scale, a.scale_all, e);
+#pragma unroll
+      for (int u = 0; u < 8; u++) f[u] = j + u < a.r ? f[u] * s : 0.f;
+    }
+    bf16x8 t[LOW];
+    split_terms<LOW>(f, t);
+#pragma unroll
+    for (int k = 0; k < LOW; k++) *reinterpret_cast<bf16x8*>(lt + (k * rows + row) * stride + j) = t[k];
   }
 }
 
-// y = sum of the K slices + bias + adapters, for 32 sorted rows and 128 outputs a workgroup
-template <typename T, bool V_STRIDED>
-__global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
-  const int n0 = blockIdx.x * 128 + w * 32;
-  const long pos = (long)blockIdx.y * 32;
-  const bool in = pos + c < a.n;
-  const int row = in ? g.order[pos + c] : 0;
-  const int key = in ? g.key[pos + c] : a.E;
-  if (n0 >= a.N) return;
-  f32x16 acc;
+// Adds s_e * low_i . V_e(n, .) to acc[mi]: lane (c, h) holds row lds_row0 + 32*mi + c of the staged tile of lds_rows rows,
+// outputs n0 + 8*(r >> 2) + 4*h + (r & 3).  The rows may use several adapters: each adapter's product is formed apart and
+// added to its own rows only, so that no value of one adapter (an infinity, a NaN) can reach the rows of another.
+// key[mi]: the lane's adapter (E: none), ascending over the rows.  V comes straight from memory (the L2): NB adapters and
+// 16*JB ranks at a time, so that NB*JB loads are in flight.  All lanes of the wave take part.
+template <typename T, bool V_STRIDED, int MI, int JB, int NB>
+__device__ __forceinline__ void add_adapters(const FinishArgs& a, const __bf16* lt, int lds_rows, int lds_row0,
+                                             const int (&key)[MI], int n0, f32x16 (&acc)[MI]) {
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, stride = low_stride(a.rp);
+  for (int j0 = 0; j0 < a.r; j0 += 16 * JB) {
+    unsigned todo[MI];
 #pragma unroll
-  for (int r = 0; r < 16; r++) acc[r] = 0.f;
-  if (in) {
-    for (int z = 0; z < a.slices; z++) {
-      const float* p = a.part + ((long)z * a.n + row) * a.N;
+    for (int mi = 0; mi < MI; mi++) todo[mi] = (unsigned)__ballot(key[mi] < a.E);   // (both halves of the wave: the same rows)
+    while (true) {
+      int es[NB];
 #pragma unroll
-      for (int r4 = 0; r4 < 4; r4++) {
-        const int n = n0 + 8 * r4 + 4 * h;
-        if (n + 4 <= a.N) {
-          const Packed4<float> f = *reinterpret_cast<const Packed4<float>*>(p + n);
+      for (int b = 0; b < NB; b++) {
+        es[b] = -1;
 #pragma unroll
-          for (int i = 0; i < 4; i++) acc[4 * r4 + i] += f.v[i];
-        } else {
+        for (int mi = 0; mi < MI; mi++)
+          if (es[b] < 0 && todo[mi]) es[b] = __builtin_amdgcn_readlane(key[mi], __builtin_ctz(todo[mi]));
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (n + i < a.N) acc[4 * r4 + i] += p[n + i];
+        for (int mi = 0; mi < MI; mi++) todo[mi] &= ~(unsigned)__ballot(key[mi] == es[b]);
+      }
+      if (es[0] < 0) break;
+      Vec8<T> v[NB][JB];
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int jj = 0; jj < JB; jj++) {
+          const int n = n0 + c, j = j0 + 16 * jj + 8 * h;
+          const T* p = (const T*)a.v + (long)es[b] * a.v_group + (long)n * a.v_row + (long)j * a.v_j;
+          const int have = es[b] >= 0 && n < a.N ? a.r - j : 0;
+          v[b][jj] = V_STRIDED ? load8_strided(p, a.v_j, have) : load8(p, have);
+        }
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        if (es[b] >= 0) {
+          bf16x8 vt[JB][Terms<T>::own];
+#pragma unroll
+          for (int jj = 0; jj < JB; jj++) own_terms<T>(v[b][jj], vt[jj]);
+#pragma unroll
+          for (int mi = 0; mi < MI; mi++) {
+            const bool mine = key[mi] == es[b];
+            if (__ballot(mine) != 0) {
+              f32x16 t;
+#pragma unroll
+              for (int r = 0; r < 16; r++) t[r] = 0.f;
+#pragma unroll
+              for (int jj = 0; jj < JB; jj++)
+                if (j0 + 16 * jj < a.r) {
+                  bf16x8 l[Terms<T>::low];
+#pragma unroll
+                  for (int k = 0; k < Terms<T>::low; k++)
+                    l[k] = *reinterpret_cast<const bf16x8*>(lt + (k * lds_rows + lds_row0 + 32 * mi + c) * stride + j0 + 16 * jj + 8 * h);
+                  t = mul_terms32<Terms<T>::own, Terms<T>::low>(vt[jj], l, t);
+                }
+#pragma unroll
+              for (int r = 0; r < 16; r++) acc[mi][r] = mine ? acc[mi][r] + t[r] : acc[mi][r];
+            }
+          }
         }
       }
     }
+  }
+}
+
+// y = sum of the K slices + bias + adapters: 32 sorted rows and 32 outputs a wave
+template <typename T, bool V_STRIDED>
+__global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) {
+  extern __shared__ __attribute__((aligned(16))) __bf16 lt[];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+  const int n0 = (blockIdx.x * (blockDim.x >> 6) + w) * 32;
+  const long pos = (long)blockIdx.y * 32;
+  const bool in = pos + c < a.n;
+  const int row = in ? g.order[pos + c] : 0;
+  const int key[1] = {in ? g.key[pos + c] : a.E};
+  f32x16 acc[1];
+#pragma unroll
+  for (int r = 0; r < 16; r++) acc[0][r] = 0.f;
+  if (in && n0 < a.N) {
     if (a.bias) {
 #pragma unroll
       for (int r = 0; r < 16; r++) {
         const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
-        if (n < a.N) acc[r] += (float)((const T*)a.bias)[n];
+        if (n < a.N) acc[0][r] = (float)((const T*)a.bias)[n];
       }
     }
+    const float* p = a.part + (long)row * a.N;
+    const long step = (long)a.n * a.N;
+    if (n0 + 32 <= a.N) {
+      int z = 0;
+      for (; z + 4 <= a.slices; z += 4) {
+        Vec4<float> f[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; r4++)
+            f[k][r4] = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + (z + k) * step + n0 + 8 * r4 + 4 * h));
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[0][r] += f[k][r >> 2].v[r & 3];
+      }
+      for (; z < a.slices; z++)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+          const Vec4<float> f = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + z * step + n0 + 8 * r4 + 4 * h));
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[0][4 * r4 + i] += f.v[i];
+        }
+    } else {
+      for (int z = 0; z < a.slices; z++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
+          if (n < a.N) acc[0][r] += p[z * step + n];
+        }
+    }
   }
-  add_adapters<T, V_STRIDED>(a, pos, key, n0, acc);
+  stage_low<Terms<T>::low>(a, g, pos, 32, lt);
+  __syncthreads();
+  if (n0 >= a.N) return;
+  add_adapters<T, V_STRIDED, 1, 2, 4>(a, lt, 32, 0, key, n0, acc);
   if (in) {
     T* y = (T*)a.y + (long)row * a.ldy;
 #pragma unroll
     for (int r4 = 0; r4 < 4; r4++) {
       const int n = n0 + 8 * r4 + 4 * h;
-      const float f[4] = {acc[4 * r4], acc[4 * r4 + 1], acc[4 * r4 + 2], acc[4 * r4 + 3]};
+      const float f[4] = {acc[0][4 * r4], acc[0][4 * r4 + 1], acc[0][4 * r4 + 2], acc[0][4 * r4 + 3]};
       store4(y + n, f, a.N - n);
     }
+  }
+}
+
+// ---- the projection of many rows, 16-bit types -------------------------------------------------------------------------
+// Tiles of BM sorted rows x BN outputs, waves as WM x WN of them, 64 k a stage, two stages in LDS.  A thread fetches its
+// share of the stage after next into registers while the matrix cores work on one stage; it goes to LDS one stage later.
+// A stage's row is 128 bytes; the 16-byte piece p of row r lies at slot p ^ (r & 7), so that the eight rows a group of lanes
+// reads at once fall into different banks.  The weight is the instruction's first operand: a lane then holds one row's
+// outputs, four consecutive ones at a time.
+// part == nullptr: with bias and adapters, straight to y.  Otherwise one K slice per blockIdx.z to part[slice][row][N].
+#define WIDE_K 64
+template <typename T, int BM, int BN, int WM, int WN, bool V_STRIDED>
+__global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, FinishArgs a, RowGroups g) {
+  constexpr int NT = 64 * WM * WN, MI = BM / (32 * WM), NI = BN / (32 * WN), RX = BM * 8 / NT, RW = BN * 8 / NT;
+  constexpr int STAGE = (BM + BN) * 128;                  // bytes
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  typedef typename Operand<T>::V V;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, h = lane >> 5;
+  const int wm = w / WN, wn = w % WN;
+  // workgroups go round-robin to the 8 XCDs: consecutive tiles of one XCD share eight row tiles' and a few column tiles' data
+  unsigned li = blockIdx.x;
+  const unsigned tm = (b.n + BM - 1) / BM, tn = (b.N + BN - 1) / BN, nwg = tm * tn;
+  if ((nwg & 7) == 0) li = (li & 7) * (nwg >> 3) + (li >> 3);
+  const unsigned band = li / (8 * tn), rows_in_band = min(8u, tm - band * 8), in_band = li - band * 8 * tn;
+  const int m0 = (band * 8 + in_band % rows_in_band) * BM, n0 = (in_band / rows_in_band) * BN;
+  const int k_begin = blockIdx.y * b.kslice, k_end = min(b.K, k_begin + b.kslice);
+  // (rows behind the last are fetched from the last: their results are not stored)
+  const T *xp[RX], *wp[RW];
+  const int piece = tid & 7;
+#pragma unroll
+  for (int i = 0; i < RX; i++) xp[i] = (const T*)b.x + (long)g.order[min(m0 + (tid >> 3) + i * (NT / 8), b.n - 1)] * b.ldx + piece * 8;
+#pragma unroll
+  for (int i = 0; i < RW; i++) wp[i] = (const T*)b.w + (long)min(n0 + (tid >> 3) + i * (NT / 8), b.N - 1) * b.ldw + piece * 8;
+  f32x16 acc[NI][MI];
+#pragma unroll
+  for (int ni = 0; ni < NI; ni++)
+#pragma unroll
+    for (int mi = 0; mi < MI; mi++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[ni][mi][r] = 0.f;
+  Vec8<T> fx[RX], fw[RW];
+  auto fetch = [&](int k0) {
+    if (k0 + WIDE_K <= k_end) {
+#pragma unroll
+      for (int i = 0; i < RX; i++) fx[i] = load8(xp[i] + k0, 8);
+#pragma unroll
+      for (int i = 0; i < RW; i++) fw[i] = load8(wp[i] + k0, 8);
+    } else {
+      const int avail = k_end - k0 - piece * 8;
+#pragma unroll
+      for (int i = 0; i < RX; i++) fx[i] = load8(xp[i] + k0, avail);
+#pragma unroll
+      for (int i = 0; i < RW; i++) fw[i] = load8(wp[i] + k0, avail);
+    }
+  };
+  const int slot = ((piece ^ ((tid >> 3) & 7)) << 4) + (tid >> 3) * 128;
+  auto place = [&](char* st) {
+#pragma unroll
+    for (int i = 0; i < RX; i++) *reinterpret_cast<uint4*>(st + slot + i * (NT / 8) * 128) = __builtin_bit_cast(uint4, fx[i]);
+#pragma unroll
+    for (int i = 0; i < RW; i++)
+      *reinterpret_cast<uint4*>(st + BM * 128 + slot + i * (NT / 8) * 128) = __builtin_bit_cast(uint4, fw[i]);
+  };
+  auto products = [&](const char* st) {
+    const char* sx = st + (wm * (BM / WM) + c) * 128;
+    const char* sw = st + BM * 128 + (wn * (BN / WN) + c) * 128;
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      const int at = ((2 * s + h) ^ (c & 7)) << 4;
+      V x[MI], v[NI];
+#pragma unroll
+      for (int ni = 0; ni < NI; ni++) v[ni] = __builtin_bit_cast(V, *reinterpret_cast<const uint4*>(sw + ni * 32 * 128 + at));
+#pragma unroll
+      for (int mi = 0; mi < MI; mi++) x[mi] = __builtin_bit_cast(V, *reinterpret_cast<const uint4*>(sx + mi * 32 * 128 + at));
+#pragma unroll
+      for (int mi = 0; mi < MI; mi++)
+#pragma unroll
+        for (int ni = 0; ni < NI; ni++) acc[ni][mi] = mul32(v[ni], x[mi], acc[ni][mi]);
+    }
+  };
+  if (k_begin < k_end) {
+    fetch(k_begin);
+    place(lds);
+    if (k_begin + WIDE_K < k_end) fetch(k_begin + WIDE_K);
+    __syncthreads();
+    int st = 0;
+    for (int k0 = k_begin; k0 < k_end; k0 += WIDE_K) {
+      if (k0 + WIDE_K < k_end) place(lds + (st ^ 1) * STAGE);
+      if (k0 + 2 * WIDE_K < k_end) fetch(k0 + 2 * WIDE_K);
+      products(lds + st * STAGE);
+      __syncthreads();
+      st ^= 1;
+    }
+  }
+  int row[MI], key[MI];
+#pragma unroll
+  for (int mi = 0; mi < MI; mi++) {
+    const long pos = m0 + wm * (BM / WM) + 32 * mi + c;
+    row[mi] = pos < b.n ? g.order[pos] : -1;
+    key[mi] = pos < b.n ? g.key[pos] : a.E;
+  }
+  const int nw = n0 + wn * (BN / WN);
+  if (!b.part) {
+    __bf16* lt = reinterpret_cast<__bf16*>(lds);
+    stage_low<Terms<T>::low>(a, g, m0, BM, lt);
+    __syncthreads();
+#pragma unroll
+    for (int ni = 0; ni < NI; ni++)
+      if (nw + 32 * ni < b.N) add_adapters<T, V_STRIDED, MI, 4, 1>(a, lt, BM, wm * (BM / WM), key, nw + 32 * ni, acc[ni]);
+  }
+#pragma unroll
+  for (int mi = 0; mi < MI; mi++) {
+    if (row[mi] < 0) continue;
+#pragma unroll
+    for (int ni = 0; ni < NI; ni++)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; r4++) {
+        const int n = nw + 32 * ni + 8 * r4 + 4 * h;
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = acc[ni][mi][4 * r4 + i];
+        if (b.part) {
+          store4(b.part + ((long)blockIdx.y * b.n + row[mi]) * b.N + n, f, b.N - n);
+        } else {
+          if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if (n + i < b.N) f[i] += (float)((const T*)a.bias)[n + i];
+          }
+          store4((T*)a.y + (long)row[mi] * a.ldy + n, f, b.N - n);
+        }
+      }
   }
 }
 
@@ -627,16 +793,37 @@ static int k_slices(long tiles, long want, int K, int min_k, int max_slices, int
 // Up to this many rows the projection's weight is streamed past all rows at once (base_rows_kernel).
 #define BASE_ROWS_MAX 64
 
-struct BaseSlices { int slices, kslice; };
-static BaseSlices base_slices(int n, int K, int N) {
-  BaseSlices b;
-  if (n <= BASE_ROWS_MAX) b.slices = k_slices((N + 15) / 16, 768, K, 512, 32, &b.kslice);
-  else b.slices = k_slices((long)((n + 127) / 128) * ((N + 127) / 128), 512, K, 512, 16, &b.kslice);
+// How the projection [n,K] x [N,K]^T is formed.
+enum { BASE_ROWS, BASE_X3, BASE_128, BASE_256 };
+struct BasePlan { int form, slices, kslice; };
+static BasePlan base_plan(int n, int K, int N, bool f32) {
+  BasePlan b;
+  b.slices = 1;
+  b.kslice = K;
+  const long t128 = (long)((n + 127) / 128) * ((N + 127) / 128), t256 = (long)((n + 255) / 256) * ((N + 255) / 256);
+  if (n <= BASE_ROWS_MAX) {
+    b.form = BASE_ROWS;
+    const int cols = n <= 16 ? 16 : 32;
+    b.slices = k_slices((N + cols - 1) / cols, 768, K, 512, 32, &b.kslice);
+  } else if (f32) {
+    b.form = BASE_X3;
+    b.slices = k_slices(t128, 512, K, 512, 16, &b.kslice);
+  } else if (t256 >= 200) {
+    b.form = BASE_256;
+  } else {
+    b.form = BASE_128;
+    if (t128 < 256) b.slices = k_slices(t128, 512, K, 256, 16, &b.kslice);
+  }
   return b;
 }
-static BaseSlices shrink_slices(int n, int K, int E) {
-  BaseSlices b;
-  b.slices = k_slices(row_tiles_cap(n, E), 512, K, 256, 32, &b.kslice);
+// bytes of the projection's partial sums (0: it goes straight to the result)
+static long base_part_bytes(const BasePlan& b, int n, int N) {
+  return b.slices == 1 && b.form >= BASE_128 ? 0 : 4L * b.slices * n * N;
+}
+struct ShrinkPlan { int slices, kslice; };
+static ShrinkPlan shrink_plan(int n, int K, int E) {
+  ShrinkPlan b;
+  b.slices = k_slices(row_tiles_cap(n, E), 512, K, 512, 16, &b.kslice);
   return b;
 }
 
@@ -658,28 +845,52 @@ static int launch_shrink(const ShrinkArgs& a, const RowGroups& g, int slices, hi
   return FLM_OK;
 }
 
-// part = X * W^T (W [N,K]), any type
-template <typename T>
-static int launch_base(const BaseArgs& a, int slices, hipStream_t st) {
-  if (a.n <= BASE_ROWS_MAX) {
-    const dim3 grid((a.N + 15) / 16, slices);
-    if (a.n <= 16) hipLaunchKernelGGL((base_rows_kernel<T, 1>), grid, dim3(256), 0, st, a);
-    else if (a.n <= 32) hipLaunchKernelGGL((base_rows_kernel<T, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((base_rows_kernel<T, 4>), grid, dim3(256), 0, st, a);
-  } else if constexpr (sizeof(T) == 4) {
-    return gemm_x3_slices((const float*)a.x, a.ldx, (const float*)a.w, a.ldw, true, a.part, a.n, a.N, a.K, slices, a.kslice, st);
-  } else {
-    hipLaunchKernelGGL(base_tile_kernel<T>, dim3((a.N + 127) / 128, (a.n + 127) / 128, slices), dim3(256), 0, st, a);
-  }
+template <typename T, int BM, int BN, int WM, int WN, bool V_STRIDED>
+static int launch_wide(const BaseArgs& b, int slices, const FinishArgs& f, const RowGroups& g, hipStream_t st) {
+  FLM_RAISE_LDS_ONCE((base_wide_kernel<T, BM, BN, WM, WN, V_STRIDED>));
+  size_t lds = 2 * (BM + BN) * 128;
+  const size_t tail = (size_t)Terms<T>::low * BM * (f.rp + 8) * 2;
+  if (!b.part && tail > lds) lds = tail;
+  hipLaunchKernelGGL((base_wide_kernel<T, BM, BN, WM, WN, V_STRIDED>),
+                     dim3(((b.n + BM - 1) / BM) * ((b.N + BN - 1) / BN), slices), dim3(64 * WM * WN), lds, st, b, f, g);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
 
 template <typename T, bool V_STRIDED>
 static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st) {
-  hipLaunchKernelGGL((finish_kernel<T, V_STRIDED>), dim3((a.N + 127) / 128, (a.n + 31) / 32), dim3(256), 0, st, a, g);
+  const long waves = (long)((a.N + 31) / 32) * ((a.n + 31) / 32);
+  const int per = waves <= 1024 ? 1 : 4;                              // (few waves: one a workgroup, spread over the CUs)
+  const size_t lds = (size_t)Terms<T>::low * 32 * (a.rp + 8) * 2;
+  hipLaunchKernelGGL((finish_kernel<T, V_STRIDED>), dim3((a.N + 32 * per - 1) / (32 * per), (a.n + 31) / 32), dim3(64 * per), lds, st,
+                     a, g);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
+}
+
+// y = X * W^T + bias + adapters, any type and size.  w_nk: W is [N,K]; otherwise [K,N] (fp32 through BASE_X3 only).
+// f.part / b.part: base_part_bytes() of workspace
+template <typename T, bool V_STRIDED>
+static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, FinishArgs f, const RowGroups& g, hipStream_t st) {
+  if (plan.form == BASE_ROWS) {
+    const int cols = b.n <= 16 ? 16 : 32;
+    const dim3 grid((b.N + cols - 1) / cols, plan.slices);
+    if (b.n <= 16) hipLaunchKernelGGL((base_rows_kernel<T, 1, 1>), grid, dim3(256), 0, st, b);
+    else if (b.n <= 32) hipLaunchKernelGGL((base_rows_kernel<T, 2, 2>), grid, dim3(256), 0, st, b);
+    else if (b.n <= 48) hipLaunchKernelGGL((base_rows_kernel<T, 3, 2>), grid, dim3(256), 0, st, b);
+    else hipLaunchKernelGGL((base_rows_kernel<T, 4, 2>), grid, dim3(256), 0, st, b);
+    FLM_CHECK_LAUNCH();
+  } else if constexpr (sizeof(T) == 4) {
+    const int rc = gemm_x3_slices((const float*)b.x, b.ldx, (const float*)b.w, b.ldw, w_nk, b.part, b.n, b.N, b.K, plan.slices,
+                                  b.kslice, st);
+    if (rc) return rc;
+  } else {
+    if (plan.slices == 1) b.part = nullptr;
+    const int rc = plan.form == BASE_256 ? launch_wide<T, 256, 256, 2, 4, V_STRIDED>(b, plan.slices, f, g, st)
+                                         : launch_wide<T, 128, 128, 2, 2, V_STRIDED>(b, plan.slices, f, g, st);
+    if (rc || !b.part) return rc;
+  }
+  return launch_finish<T, V_STRIDED>(f, g, st);
 }
 
 template <typename T>
@@ -710,16 +921,14 @@ static int forward(const void* x, long ldx, const void* w, long ldw, const void*
                    const RowGroups& g, const float* scale, float scale_all, int n, int K, int N, int r, int E, char* ws, void* y,
                    long ldy, float* low, hipStream_t st) {
   const int rp = ranks_padded(r);
-  const BaseSlices ss = shrink_slices(n, K, E), bs = base_slices(n, K, N);
+  const ShrinkPlan ss = shrink_plan(n, K, E);
+  const BasePlan bs = base_plan(n, K, N, sizeof(T) == 4);
   float* low_part = (float*)ws;
   float* part = (float*)(ws + round16(4L * ss.slices * n * rp));
   int rc = launch_shrink<T, false>(ShrinkArgs{x, a, ldx, (long)r * K, K, 1, K, r, rp, n, ss.kslice, low_part}, g, ss.slices, st);
   if (rc) return rc;
-  if ((rc = launch_base<T>(BaseArgs{x, w, ldx, ldw, n, K, N, bs.kslice, part}, bs.slices, st))) return rc;
-  if ((rc = launch_finish<T, false>(FinishArgs{part, bs.slices, bias, low_part, ss.slices, r, rp, b, (long)N * r, r, 1, scale,
-                                               scale_all, n, N, E, y, ldy},
-                                    g, st)))
-    return rc;
+  const FinishArgs f{part, bs.slices, bias, low_part, ss.slices, r, rp, b, (long)N * r, r, 1, scale, scale_all, n, N, E, y, ldy};
+  if ((rc = launch_projection<T, false>(BaseArgs{x, w, ldx, ldw, n, K, N, bs.kslice, part}, bs, true, f, g, st))) return rc;
   if (low) {
     hipLaunchKernelGGL(low_rows_kernel, dim3((unsigned)(((long)n * rp + 255) / 256)), dim3(256), 0, st, low_part, ss.slices, n, r,
                        rp, E, g, low);
@@ -733,7 +942,7 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
                     const RowGroups& g, const float* scale, float scale_all, const float* low, int n, int K, int N, int r, int E,
                     char* ws, void* dx, long lddx, void* da, void* db, hipStream_t st) {
   const int rp = ranks_padded(r);
-  const BaseSlices ss = shrink_slices(n, N, E);
+  const ShrinkPlan ss = shrink_plan(n, N, E);
   float* u = (float*)ws;                                             // s_e is applied where u is used
   ws += round16(4L * ss.slices * n * rp);
   int rc = launch_shrink<T, true>(ShrinkArgs{dy, b, lddy, (long)N * r, 1, r, N, r, rp, n, ss.kslice, u}, g, ss.slices, st);
@@ -746,23 +955,18 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
   if ((rc = launch_outer<T>(OuterArgs{low, 1, r, 1, 0, dy, lddy, N, r, E, n, cb, scale, scale_all, part, db, 1, r}, g, st)))
     return rc;
   if (!dx) return FLM_OK;
-  const BaseSlices bs = base_slices(n, N, K);
+  const BasePlan bs = base_plan(n, N, K, sizeof(T) == 4);
   float* dx_part = (float*)ws;
-  if constexpr (sizeof(T) == 4) {
-    if (n > BASE_ROWS_MAX) {
-      rc = gemm_x3_slices((const float*)dy, lddy, (const float*)w, ldw, false, dx_part, n, K, N, bs.slices, bs.kslice, st);
-      if (rc) return rc;
-    }
-  }
-  if (sizeof(T) != 4 || n <= BASE_ROWS_MAX) {
-    T* wt = (T*)(ws + round16(4L * bs.slices * n * K));
+  const bool turn = bs.form != BASE_X3;                              // the contraction runs down W: turned once
+  if (turn) {
+    T* wt = (T*)(ws + round16(base_part_bytes(bs, n, K)));
     hipLaunchKernelGGL(transpose_kernel<T>, dim3((K + 63) / 64, (N + 63) / 64), dim3(256), 0, st, (const T*)w, ldw, N, K, wt);
     FLM_CHECK_LAUNCH();
-    if ((rc = launch_base<T>(BaseArgs{dy, wt, lddy, N, n, N, K, bs.kslice, dx_part}, bs.slices, st))) return rc;
+    w = wt;
+    ldw = N;
   }
-  return launch_finish<T, true>(FinishArgs{dx_part, bs.slices, nullptr, u, ss.slices, r, rp, a, (long)r * K, 1, K, scale, scale_all,
-                                           n, K, E, dx, lddx},
-                                g, st);
+  const FinishArgs f{dx_part, bs.slices, nullptr, u, ss.slices, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
+  return launch_projection<T, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, turn, f, g, st);
 }
 
 }  // namespace flm
@@ -774,9 +978,10 @@ static bool adapter_sizes(int n, int K, int N, int r, int E, int dtype) {
          E <= FLM_GROUPS_MAX && dtype >= FLM_F32 && dtype <= FLM_F16;
 }
 
-extern "C" long flm_adapter_workspace(int n, int K, int N, int r, int E) {
-  if (!adapter_sizes(n, K, N, r, E, FLM_F32)) return 0;
-  return round16(4L * shrink_slices(n, K, E).slices * n * ranks_padded(r)) + round16(4L * base_slices(n, K, N).slices * n * N);
+extern "C" long flm_adapter_workspace(int n, int K, int N, int r, int E, int dtype) {
+  if (!adapter_sizes(n, K, N, r, E, dtype)) return 0;
+  return round16(4L * shrink_plan(n, K, E).slices * n * ranks_padded(r)) + base_part_bytes(base_plan(n, K, N, dtype == FLM_F32), n, N) +
+         256;
 }
 
 extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E, int dtype, int need_dx) {
@@ -785,11 +990,11 @@ extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E
   const long pa = 8L * ((n + ca - 1) / ca) * r * K, pb = 8L * ((n + cb - 1) / cb) * r * N;
   long rest = pa > pb ? pa : pb;
   if (need_dx) {
-    const long base = round16(4L * base_slices(n, N, K).slices * n * K) +
-                      (dtype == FLM_F32 && n > BASE_ROWS_MAX ? 0 : (dtype == FLM_F32 ? 4L : 2L) * K * N);
+    const BasePlan bs = base_plan(n, N, K, dtype == FLM_F32);
+    const long base = round16(base_part_bytes(bs, n, K)) + (bs.form == BASE_X3 ? 0 : (dtype == FLM_F32 ? 4L : 2L) * K * N);
     if (base > rest) rest = base;
   }
-  return round16(4L * shrink_slices(n, N, E).slices * n * ranks_padded(r)) + rest;
+  return round16(4L * shrink_plan(n, N, E).slices * n * ranks_padded(r)) + rest + 256;
 }
 
 extern "C" int flm_adapter_linear(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* a, const void* b,

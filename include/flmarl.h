@@ -645,11 +645,11 @@ int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* gro
  *   a [E,r,K], b [E,N,r] contiguous; all of type dtype (FLM_F32 / FLM_BF16 / FLM_F16)
  *   groups: flm_group_rows(ids, ., n, E, ...); scale [E] float or NULL (then scale_all for every adapter)
  *   low [n,r] float out (or NULL): A_e x_i, not scaled, zeros for rows without an adapter: what the backward pass takes
- *   workspace: flm_adapter_workspace(n, K, N, r, E) bytes, 16-byte aligned; one per call in flight
+ *   workspace: flm_adapter_workspace(n, K, N, r, E, dtype) bytes, 16-byte aligned; one per call in flight
  * Sums are fp32, rounded once.  fp32 operands are multiplied as three bf16 terms each (fp32 accuracy; a row that meets an
  * infinity or NaN becomes NaN, other rows do not).  An adapter's values reach the rows of that adapter only.
  * n, K, N <= 2^20, r <= FLM_ADAPTER_MAX_RANK, E <= FLM_GROUPS_MAX.  y must not overlap an input. */
-long flm_adapter_workspace(int n, int K, int N, int r, int E);
+long flm_adapter_workspace(int n, int K, int N, int r, int E, int dtype);
 int flm_adapter_linear(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* a, const void* b,
                        const int32_t* groups, const float* scale, float scale_all, int n, int K, int N, int r, int E,
                        int dtype, void* workspace, void* y, long ldy, float* low, void* stream);

@@ -22,6 +22,8 @@ SIZES = [
     (300, 512, 256, 64, 9, True),
     (517, 264, 384, 128, 6, False),
     (1031, 200, 72, 8, 1, False),
+    (2100, 136, 2050, 9, 3, False),
+    (3700, 328, 3655, 70, 6, True),
 ]
 
 

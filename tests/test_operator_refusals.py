@@ -20,9 +20,9 @@ def test_size_queries():
     assert lib.flm_group_rows_workspace(8192, 100) == 0 and lib.flm_group_rows_workspace(8193, 100) == (9 + 1) * 101
     for n, k, n_out, r, e in ((0, 8, 8, 4, 1), (8, 0, 8, 4, 1), (8, 8, 8, 0, 1), (8, 8, 8, 129, 1), (8, 8, 8, 4, 2048),
                               (1 << 21, 8, 8, 4, 1)):
-        assert lib.flm_adapter_workspace(n, k, n_out, r, e) == 0
+        assert lib.flm_adapter_workspace(n, k, n_out, r, e, 0) == 0
         assert lib.flm_adapter_backward_workspace(n, k, n_out, r, e, 0, 1) == 0
-    assert lib.flm_adapter_workspace(8, 64, 32, 4, 1) > 0
+    assert lib.flm_adapter_workspace(8, 64, 32, 4, 1, 2) > 0
     assert lib.flm_adapter_backward_workspace(8, 64, 32, 4, 1, 3, 1) == 0
 
 
