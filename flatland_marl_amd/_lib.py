@@ -4,6 +4,7 @@ There is no CPU fallback: if the shared library is missing or a call fails,
 the caller gets an exception.
 """
 import ctypes as C
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -11,11 +12,12 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FLMARL_LIB") or os.path.join(_HERE, "libflmarl_hip.so")
 
 FLM_OK = 0
+E_OVERLAP = -4                                            # FLM_E_OVERLAP of include/flmarl.h
 AGENT_ERRORS = {2: IndexError, 3: KeyError, 4: AssertionError, 5: OverflowError}
 GRAPH_ERR_NODES, GRAPH_ERR_RAILS, GRAPH_ERR_CELLS, GRAPH_ERR_STATES = 1, 2, 4, 8
 MAX_NODES = 2048
 ABI_VERSION = 4
-GROUPS_MAX, ADAPTER_MAX_RANK, GRAD_MAX_TENSORS, GRAD_WORKSPACE = 2047, 128, 65536, 2048
+GROUPS_MAX, ADAPTER_MAX_RANK, GRAD_MAX_TENSORS, GRAD_WORKSPACE = 2047, 128, 65536, 4096
 DQN_MAX_ACTIONS = 16                                       # FLM_DQN_MAX_ACTIONS of include/flmarl.h
 
 _p = C.c_void_p
@@ -148,4 +150,22 @@ def query(name, *args):
 def call(name, *args):
     rc = getattr(load(), name)(*args)
     if rc != FLM_OK:
+        if rc == E_OVERLAP:
+            raise ValueError("%s: tensors that are written share memory" % name)
         raise FlmError("%s failed with code %d" % (name, rc))
+
+
+def launch(dev, name, *args):
+    """call(name, *args, stream) on the current stream of dev, a GPU that need not be the current one."""
+    import torch
+    if torch.cuda.current_device() == dev.index:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
+@functools.lru_cache(maxsize=4096)
+def size_of(name, *args):
+    """query() of a size that depends on its arguments alone, remembered by them."""
+    return query(name, *args)

@@ -3,7 +3,7 @@ flm_adapter_linear_backward).  The reference trains one network for all maps (sr
 stays shared and every map (or whatever the caller tells apart) adds a correction of low rank to a dense layer."""
 import torch
 
-from ._lib import ADAPTER_MAX_RANK, GROUPS_MAX, FlmError, call, query
+from ._lib import ADAPTER_MAX_RANK, GROUPS_MAX, FlmError, launch, size_of
 from .gradients import DTYPES
 
 
@@ -48,12 +48,11 @@ def group_rows(ids, n_groups):
         raise ValueError("more than 2^30 rows")
     if not ids.is_contiguous():
         ids = ids.contiguous()
-    buf = torch.empty(query("flm_group_rows_ints", n, n_groups), dtype=torch.int32, device=dev)
-    need = query("flm_group_rows_workspace", n, n_groups)
+    buf = torch.empty(size_of("flm_group_rows_ints", n, n_groups), dtype=torch.int32, device=dev)
+    need = size_of("flm_group_rows_workspace", n, n_groups)
     work = torch.empty(need, dtype=torch.int32, device=dev) if need else None
-    with torch.cuda.device(dev):
-        call("flm_group_rows", ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, n, n_groups, buf.data_ptr(),
-             work.data_ptr() if need else None, torch.cuda.current_stream(dev).cuda_stream)
+    launch(dev, "flm_group_rows", ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, n, n_groups, buf.data_ptr(),
+           work.data_ptr() if need else None)
     return RowGroups(buf, n, n_groups)
 
 
@@ -112,11 +111,10 @@ def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False):
     y = torch.empty((n, n_out), dtype=x.dtype, device=dev)
     low = torch.empty((n, r), dtype=torch.float32, device=dev) if keep_low else None
     if n:
-        work = torch.empty(query("flm_adapter_workspace", n, k, n_out, r, e, DTYPES[x.dtype]), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            call("flm_adapter_linear", x.data_ptr(), ldx, weight.data_ptr(), ldw, bias.data_ptr() if bias is not None else None,
-                 a.data_ptr(), b.data_ptr(), groups.buf.data_ptr(), *scales, n, k, n_out, r, e, DTYPES[x.dtype], work.data_ptr(),
-                 y.data_ptr(), n_out, low.data_ptr() if keep_low else None, torch.cuda.current_stream(dev).cuda_stream)
+        work = torch.empty(size_of("flm_adapter_workspace", n, k, n_out, r, e, DTYPES[x.dtype]), dtype=torch.uint8, device=dev)
+        launch(dev, "flm_adapter_linear", x.data_ptr(), ldx, weight.data_ptr(), ldw, bias.data_ptr() if bias is not None else None,
+               a.data_ptr(), b.data_ptr(), groups.buf.data_ptr(), *scales, n, k, n_out, r, e, DTYPES[x.dtype], work.data_ptr(),
+               y.data_ptr(), n_out, low.data_ptr() if keep_low else None)
     return (y, low) if keep_low else y
 
 
@@ -144,10 +142,9 @@ def adapter_linear_backward(dy, x, weight, a, b, groups, low, scale=1.0, need_dx
         db.zero_()
         return dx, da, db
     kind = DTYPES[x.dtype]
-    work = torch.empty(query("flm_adapter_backward_workspace", n, k, n_out, r, e, kind, 1 if need_dx else 0), dtype=torch.uint8,
+    work = torch.empty(size_of("flm_adapter_backward_workspace", n, k, n_out, r, e, kind, 1 if need_dx else 0), dtype=torch.uint8,
                        device=dev)
-    with torch.cuda.device(dev):
-        call("flm_adapter_linear_backward", dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr() if need_dx else None, ldw,
-             a.data_ptr(), b.data_ptr(), groups.buf.data_ptr(), *scales, low.data_ptr(), n, k, n_out, r, e, kind, work.data_ptr(),
-             dx.data_ptr() if need_dx else None, k, da.data_ptr(), db.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+    launch(dev, "flm_adapter_linear_backward", dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr() if need_dx else None, ldw,
+           a.data_ptr(), b.data_ptr(), groups.buf.data_ptr(), *scales, low.data_ptr(), n, k, n_out, r, e, kind, work.data_ptr(),
+           dx.data_ptr() if need_dx else None, k, da.data_ptr(), db.data_ptr())
     return dx, da, db

@@ -248,7 +248,6 @@ __global__ __launch_bounds__(256) void shrink_kernel(ShrinkArgs a, RowGroups g) 
   if (rows == 0) return;
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int k_begin = blockIdx.y * a.kslice, k_end = min(a.K, k_begin + a.kslice);
-  // (a tile holds up to 32 rows; MR = 1 is only launched for calls of up to 16 rows)
   const T *xr[MR], *vr[NR];
 #pragma unroll
   for (int mi = 0; mi < MR; mi++) {
@@ -276,27 +275,51 @@ struct BaseArgs {
   float* part;                           // [slice][n][N]
 };
 
-// the projection of up to 16*MR rows: 16*NR outputs a workgroup, grid (outputs / (16*NR), K slices)
-template <typename T, int MR, int NR>
-__global__ __launch_bounds__(256) void base_rows_kernel(BaseArgs a) {
-  __shared__ f32x4 red[4 * MR * NR * 64];
+// Up to 64 rows: the projection (16*MR rows x 16*NR outputs a workgroup) and the narrow products (32 rows x 16 ranks) in one
+// launch.  The first base_groups workgroups are (output block, K slice) pairs of the projection, the others (tile, K slice,
+// rank block) of the narrow product: at these sizes both are streams of weights with little else to do.
+template <typename T, int MRS, int MR, int NR, bool V_STRIDED>
+__global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s, RowGroups g, int base_groups, int low_slices) {
+  __shared__ f32x4 red[4 * (MR * NR > MRS ? MR * NR : MRS) * 64];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * (16 * NR);
-  const int k_begin = blockIdx.y * a.kslice, k_end = min(a.K, k_begin + a.kslice);
-  const T *xr[MR], *vr[NR];
+  if ((int)blockIdx.x < base_groups) {
+    const int cols = (a.N + 16 * NR - 1) / (16 * NR), slice = blockIdx.x / cols;
+    const int n0 = (blockIdx.x - slice * cols) * (16 * NR);
+    const int k_begin = slice * a.kslice, k_end = min(a.K, k_begin + a.kslice);
+    const T *xr[MR], *vr[NR];
 #pragma unroll
-  for (int mi = 0; mi < MR; mi++) xr[mi] = mi * 16 + c < a.n ? (const T*)a.x + (long)(mi * 16 + c) * a.ldx : nullptr;
+    for (int mi = 0; mi < MR; mi++) xr[mi] = mi * 16 + c < a.n ? (const T*)a.x + (long)(mi * 16 + c) * a.ldx : nullptr;
 #pragma unroll
-  for (int ni = 0; ni < NR; ni++) vr[ni] = n0 + ni * 16 + c < a.N ? (const T*)a.w + (long)(n0 + ni * 16 + c) * a.ldw : nullptr;
-  f32x4 acc[MR][NR];
-  mini_product<T, MR, NR, 2, false>(xr, vr, 1, k_begin, k_end, acc);
-  mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
-    const int m = mi * 16 + c, n = n0 + ni * 16 + 4 * q;
-    if (m < a.n) {
-      const float f[4] = {v[0], v[1], v[2], v[3]};
-      store4(a.part + ((long)blockIdx.y * a.n + m) * a.N + n, f, a.N - n);
+    for (int ni = 0; ni < NR; ni++) vr[ni] = n0 + ni * 16 + c < a.N ? (const T*)a.w + (long)(n0 + ni * 16 + c) * a.ldw : nullptr;
+    f32x4 acc[MR][NR];
+    mini_product<T, MR, NR, 2, false>(xr, vr, 1, k_begin, k_end, acc);
+    mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
+      const int m = mi * 16 + c, n = n0 + ni * 16 + 4 * q;
+      if (m < a.n) {
+        const float f[4] = {v[0], v[1], v[2], v[3]};
+        store4(a.part + ((long)slice * a.n + m) * a.N + n, f, a.N - n);
+      }
+    });
+  } else {
+    const int i = blockIdx.x - base_groups, rest = i / g.cap, rank = rest / low_slices * 16, slice = rest % low_slices;
+    const int2 tile = g.tiles[i - rest * g.cap];
+    const int rows = tile.y >> 16, e = tile.y & 0xffff;
+    if (rows == 0) return;
+    const int k_begin = slice * s.kslice, k_end = min(s.K, k_begin + s.kslice);
+    const T *xr[MRS], *vr[1];
+#pragma unroll
+    for (int mi = 0; mi < MRS; mi++) {
+      const int m = mi * 16 + c;
+      xr[mi] = m < rows ? (const T*)s.x + (long)g.order[tile.x + m] * s.ldx : nullptr;
     }
-  });
+    vr[0] = rank + c < s.r ? (const T*)s.v + (long)e * s.v_group + (long)(rank + c) * s.v_row : nullptr;
+    f32x4 acc[MRS][1];
+    mini_product<T, MRS, 1, 2, V_STRIDED>(xr, vr, s.v_k, k_begin, k_end, acc);
+    mini_meet<MRS, 1>(acc, red, [&](int mi, int, const f32x4& v) {
+      const int m = mi * 16 + c;
+      if (m < rows) *reinterpret_cast<f32x4*>(s.out + ((long)slice * s.n + tile.x + m) * s.rp + rank + 4 * q) = v;
+    });
+  }
 }
 
 // out[C][R] = in[R][C] (the weight with its contraction axis last, for the gradient of the inputs)
@@ -349,15 +372,15 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
       const float* p = a.low + (pos + row) * a.rp + j;
       const long step = (long)a.n * a.rp;
       int z = 0;
-      for (; z + 4 <= a.low_slices; z += 4) {
-        f32x4 v[4][2];
+      for (; z + 8 <= a.low_slices; z += 8) {
+        f32x4 v[8][2];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 8; k++) {
           v[k][0] = reinterpret_cast<const f32x4*>(p + (z + k) * step)[0];
           v[k][1] = reinterpret_cast<const f32x4*>(p + (z + k) * step)[1];
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < 8; k++)
 #pragma unroll
           for (int u = 0; u < 8; u++) f[u] += v[k][u >> 2][u & 3];
       }
@@ -452,36 +475,35 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
   const int n0 = (blockIdx.x * (blockDim.x >> 6) + w) * 32;
   const long pos = (long)blockIdx.y * 32;
   const bool in = pos + c < a.n;
-  const int row = in ? g.order[pos + c] : 0;
   const int key[1] = {in ? g.key[pos + c] : a.E};
+  // Where fewer than 17 rows are left, the lanes of the missing rows take K slices of the others: lane c sums every
+  // (32 / span)-th slice of row c mod span.
+  int span = 32;
+  while (span > 1 && pos + span / 2 >= a.n) span >>= 1;
+  const int mine = c & (span - 1);
+  const int row = pos + mine < a.n ? g.order[pos + mine] : -1;
   f32x16 acc[1];
 #pragma unroll
   for (int r = 0; r < 16; r++) acc[0][r] = 0.f;
-  if (in && n0 < a.N) {
-    if (a.bias) {
-#pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
-        if (n < a.N) acc[0][r] = (float)((const T*)a.bias)[n];
-      }
-    }
+  if (row >= 0 && n0 < a.N) {
     const float* p = a.part + (long)row * a.N;
     const long step = (long)a.n * a.N;
+    const int stride = 32 / span;
     if (n0 + 32 <= a.N) {
-      int z = 0;
-      for (; z + 4 <= a.slices; z += 4) {
+      int z = c / span;
+      for (; z + 3 * stride < a.slices; z += 4 * stride) {
         Vec4<float> f[4][4];
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
           for (int r4 = 0; r4 < 4; r4++)
-            f[k][r4] = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + (z + k) * step + n0 + 8 * r4 + 4 * h));
+            f[k][r4] = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + (z + k * stride) * step + n0 + 8 * r4 + 4 * h));
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
           for (int r = 0; r < 16; r++) acc[0][r] += f[k][r >> 2].v[r & 3];
       }
-      for (; z < a.slices; z++)
+      for (; z < a.slices; z += stride)
 #pragma unroll
         for (int r4 = 0; r4 < 4; r4++) {
           const Vec4<float> f = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + z * step + n0 + 8 * r4 + 4 * h));
@@ -489,12 +511,22 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
           for (int i = 0; i < 4; i++) acc[0][4 * r4 + i] += f.v[i];
         }
     } else {
-      for (int z = 0; z < a.slices; z++)
+      for (int z = c / span; z < a.slices; z += stride)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
           if (n < a.N) acc[0][r] += p[z * step + n];
         }
+    }
+  }
+  for (int o = span; o < 32; o <<= 1)
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[0][r] += __shfl_xor(acc[0][r], o);
+  if (a.bias) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
+      if (n < a.N) acc[0][r] += (float)((const T*)a.bias)[n];
     }
   }
   stage_low<Terms<T>::low>(a, g, pos, 32, lt);
@@ -790,7 +822,7 @@ static int k_slices(long tiles, long want, int K, int min_k, int max_slices, int
   return (K + *kslice - 1) / *kslice;
 }
 
-// Up to this many rows the projection's weight is streamed past all rows at once (base_rows_kernel).
+// Up to this many rows the projection's weight is streamed past all rows at once (few_rows_kernel).
 #define BASE_ROWS_MAX 64
 
 // How the projection [n,K] x [N,K]^T is formed.
@@ -830,17 +862,23 @@ static ShrinkPlan shrink_plan(int n, int K, int E) {
 template <typename T, bool V_STRIDED>
 static int launch_shrink(const ShrinkArgs& a, const RowGroups& g, int slices, hipStream_t st) {
   const dim3 grid(g.cap, slices);
-  if (a.n <= 16) {
-    if (a.rp <= 16) hipLaunchKernelGGL((shrink_kernel<T, 1, 1, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-    else if (a.rp <= 32) hipLaunchKernelGGL((shrink_kernel<T, 1, 2, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-    else if (a.rp <= 64) hipLaunchKernelGGL((shrink_kernel<T, 1, 4, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-    else hipLaunchKernelGGL((shrink_kernel<T, 1, 8, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-  } else {
-    if (a.rp <= 16) hipLaunchKernelGGL((shrink_kernel<T, 2, 1, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-    else if (a.rp <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, 2, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-    else if (a.rp <= 64) hipLaunchKernelGGL((shrink_kernel<T, 2, 4, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-    else hipLaunchKernelGGL((shrink_kernel<T, 2, 8, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-  }
+  if (a.rp <= 16) hipLaunchKernelGGL((shrink_kernel<T, 2, 1, V_STRIDED>), grid, dim3(256), 0, st, a, g);
+  else if (a.rp <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, 2, V_STRIDED>), grid, dim3(256), 0, st, a, g);
+  else if (a.rp <= 64) hipLaunchKernelGGL((shrink_kernel<T, 2, 4, V_STRIDED>), grid, dim3(256), 0, st, a, g);
+  else hipLaunchKernelGGL((shrink_kernel<T, 2, 8, V_STRIDED>), grid, dim3(256), 0, st, a, g);
+  FLM_CHECK_LAUNCH();
+  return FLM_OK;
+}
+
+// the projection's K slices and the narrow product's of up to 64 rows
+template <typename T, bool V_STRIDED>
+static int launch_few_rows(const BaseArgs& a, int base_slices, const ShrinkArgs& s, int low_slices, const RowGroups& g, hipStream_t st) {
+  const int cols = a.n <= 16 ? 16 : 32, base_groups = (a.N + cols - 1) / cols * base_slices;
+  const dim3 grid(base_groups + g.cap * low_slices * (s.rp / 16));
+  if (a.n <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, 1, 1, V_STRIDED>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
+  else if (a.n <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, 2, 2, V_STRIDED>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
+  else if (a.n <= 48) hipLaunchKernelGGL((few_rows_kernel<T, 2, 3, 2, V_STRIDED>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
+  else hipLaunchKernelGGL((few_rows_kernel<T, 2, 4, 2, V_STRIDED>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
@@ -868,27 +906,30 @@ static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st
   return FLM_OK;
 }
 
-// y = X * W^T + bias + adapters, any type and size.  w_nk: W is [N,K]; otherwise [K,N] (fp32 through BASE_X3 only).
-// f.part / b.part: base_part_bytes() of workspace
-template <typename T, bool V_STRIDED>
-static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, FinishArgs f, const RowGroups& g, hipStream_t st) {
+// The narrow product and y = X * W^T + bias + adapters, any type and size.  w_nk: W is [N,K]; otherwise [K,N] (fp32 through
+// BASE_X3 only).  low_done: s has been formed already.  f.part / b.part: base_part_bytes() of workspace
+template <typename T, bool V_STRIDED, bool S_STRIDED>
+static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const ShrinkArgs& s, int low_slices, bool low_done,
+                             const FinishArgs& f, const RowGroups& g, hipStream_t st) {
   if (plan.form == BASE_ROWS) {
-    const int cols = b.n <= 16 ? 16 : 32;
-    const dim3 grid((b.N + cols - 1) / cols, plan.slices);
-    if (b.n <= 16) hipLaunchKernelGGL((base_rows_kernel<T, 1, 1>), grid, dim3(256), 0, st, b);
-    else if (b.n <= 32) hipLaunchKernelGGL((base_rows_kernel<T, 2, 2>), grid, dim3(256), 0, st, b);
-    else if (b.n <= 48) hipLaunchKernelGGL((base_rows_kernel<T, 3, 2>), grid, dim3(256), 0, st, b);
-    else hipLaunchKernelGGL((base_rows_kernel<T, 4, 2>), grid, dim3(256), 0, st, b);
-    FLM_CHECK_LAUNCH();
-  } else if constexpr (sizeof(T) == 4) {
-    const int rc = gemm_x3_slices((const float*)b.x, b.ldx, (const float*)b.w, b.ldw, w_nk, b.part, b.n, b.N, b.K, plan.slices,
-                                  b.kslice, st);
+    // (a narrow product that is there already is not formed again: no workgroups for it)
+    RowGroups tiles = g;
+    if (low_done) tiles.cap = 0;
+    const int rc = launch_few_rows<T, S_STRIDED>(b, plan.slices, s, low_slices, tiles, st);
     if (rc) return rc;
   } else {
-    if (plan.slices == 1) b.part = nullptr;
-    const int rc = plan.form == BASE_256 ? launch_wide<T, 256, 256, 2, 4, V_STRIDED>(b, plan.slices, f, g, st)
-                                         : launch_wide<T, 128, 128, 2, 2, V_STRIDED>(b, plan.slices, f, g, st);
-    if (rc || !b.part) return rc;
+    int rc = low_done ? FLM_OK : launch_shrink<T, S_STRIDED>(s, g, low_slices, st);
+    if (rc) return rc;
+    if constexpr (sizeof(T) == 4) {
+      if ((rc = gemm_x3_slices((const float*)b.x, b.ldx, (const float*)b.w, b.ldw, w_nk, b.part, b.n, b.N, b.K, plan.slices,
+                               b.kslice, st)))
+        return rc;
+    } else {
+      if (plan.slices == 1) b.part = nullptr;
+      rc = plan.form == BASE_256 ? launch_wide<T, 256, 256, 2, 4, V_STRIDED>(b, plan.slices, f, g, st)
+                                 : launch_wide<T, 128, 128, 2, 2, V_STRIDED>(b, plan.slices, f, g, st);
+      if (rc || !b.part) return rc;
+    }
   }
   return launch_finish<T, V_STRIDED>(f, g, st);
 }
@@ -925,10 +966,11 @@ static int forward(const void* x, long ldx, const void* w, long ldw, const void*
   const BasePlan bs = base_plan(n, K, N, sizeof(T) == 4);
   float* low_part = (float*)ws;
   float* part = (float*)(ws + round16(4L * ss.slices * n * rp));
-  int rc = launch_shrink<T, false>(ShrinkArgs{x, a, ldx, (long)r * K, K, 1, K, r, rp, n, ss.kslice, low_part}, g, ss.slices, st);
-  if (rc) return rc;
+  const ShrinkArgs s{x, a, ldx, (long)r * K, K, 1, K, r, rp, n, ss.kslice, low_part};
   const FinishArgs f{part, bs.slices, bias, low_part, ss.slices, r, rp, b, (long)N * r, r, 1, scale, scale_all, n, N, E, y, ldy};
-  if ((rc = launch_projection<T, false>(BaseArgs{x, w, ldx, ldw, n, K, N, bs.kslice, part}, bs, true, f, g, st))) return rc;
+  const int rc = launch_projection<T, false, false>(BaseArgs{x, w, ldx, ldw, n, K, N, bs.kslice, part}, bs, true, s, ss.slices, false, f,
+                                                    g, st);
+  if (rc) return rc;
   if (low) {
     hipLaunchKernelGGL(low_rows_kernel, dim3((unsigned)(((long)n * rp + 255) / 256)), dim3(256), 0, st, low_part, ss.slices, n, r,
                        rp, E, g, low);
@@ -945,7 +987,8 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
   const ShrinkPlan ss = shrink_plan(n, N, E);
   float* u = (float*)ws;                                             // s_e is applied where u is used
   ws += round16(4L * ss.slices * n * rp);
-  int rc = launch_shrink<T, true>(ShrinkArgs{dy, b, lddy, (long)N * r, 1, r, N, r, rp, n, ss.kslice, u}, g, ss.slices, st);
+  const ShrinkArgs s{dy, b, lddy, (long)N * r, 1, r, N, r, rp, n, ss.kslice, u};
+  int rc = launch_shrink<T, true>(s, g, ss.slices, st);
   if (rc) return rc;
   const int ca = outer_chunk(n, K), cb = outer_chunk(n, N);
   float* part = (float*)ws;                                          // both gradients in turn
@@ -966,7 +1009,8 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
     ldw = N;
   }
   const FinishArgs f{dx_part, bs.slices, nullptr, u, ss.slices, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
-  return launch_projection<T, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, turn, f, g, st);
+  return launch_projection<T, true, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, turn, s, ss.slices, true, f, g,
+                                          st);
 }
 
 }  // namespace flm

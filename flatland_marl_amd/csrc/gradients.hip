@@ -10,6 +10,11 @@
 // workgroups finish.
 // The tensors' addresses travel in the launch's arguments, FLM_GRAD_LIST tensors a launch: no table in device memory has to be
 // kept or refreshed by the caller.
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
+
 #include "flm_common.h"
 
 namespace flm {
@@ -18,7 +23,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 #define FLM_GRAD_LIST 112                // tensors per launch: 32 bytes each of the 4 KiB a launch's arguments may take
-#define GRAD_CHUNK 8192                  // elements a workgroup takes at a time
 #define GRAD_PARTS FLM_GRAD_WORKSPACE    // partial results at most
 
 struct GradItem {
@@ -31,6 +35,7 @@ struct GradItem {
 struct GradList {
   GradItem item[FLM_GRAD_LIST];
   int count, chunks;
+  int chunk;                             // elements a workgroup takes at a time, a multiple of 2048
 };
 // What the gradient holds beside the listed tensors: `times` copies of the outer products g_i (x) r, r [64], over the
 // 512 + 512 values of two vectors (the first dense layer's gradient under empty rows, formed by the optimizer pass).
@@ -40,15 +45,23 @@ struct GradOuter {
 };
 
 template <typename T> struct Pack8;
-template <> struct Pack8<float> { struct __attribute__((packed, aligned(4))) V { float v[8]; }; };
-template <> struct Pack8<__bf16> { struct __attribute__((packed, aligned(2))) V { __bf16 v[8]; }; };
-template <> struct Pack8<_Float16> { struct __attribute__((packed, aligned(2))) V { _Float16 v[8]; }; };
+template <> struct Pack8<float> { struct V { float v[8]; }; struct __attribute__((packed, aligned(4))) W { unsigned w[8]; }; };
+template <> struct Pack8<__bf16> { struct V { __bf16 v[8]; }; struct __attribute__((packed, aligned(2))) W { unsigned w[4]; }; };
+template <> struct Pack8<_Float16> { struct V { _Float16 v[8]; }; struct __attribute__((packed, aligned(2))) W { unsigned w[4]; }; };
+// (memory is accessed as words at the element's alignment: the first elements of a tensor up to a 16-byte boundary are
+// taken apart, but source and destination need not be aligned alike)
+template <typename T> __device__ __forceinline__ typename Pack8<T>::V get8(const T* p, int i) {
+  return __builtin_bit_cast(typename Pack8<T>::V, reinterpret_cast<const typename Pack8<T>::W*>(p)[i]);
+}
+template <typename T> __device__ __forceinline__ void put8(T* p, int i, const typename Pack8<T>::V& v) {
+  reinterpret_cast<typename Pack8<T>::W*>(p)[i] = __builtin_bit_cast(typename Pack8<T>::W, v);
+}
 
 __device__ __forceinline__ double larger(double m, double v) { return (m == m && !(v <= m)) ? v : m; }   // NaN stays
 
 // f(value array, count) over one chunk of a tensor, eight elements a thread and step
 template <typename T>
-__device__ __forceinline__ void grad_norm_chunk(const T* p, int n, int tid, int threads, bool inf_norm, double (&acc)[4]) {
+__device__ __forceinline__ void grad_norm_chunk(const T* p, int n, int lead, int tid, int threads, bool inf_norm, double (&acc)[4]) {
   typedef typename Pack8<T>::V V;
   const int whole = n >> 3;
   auto take = [&](const V& v) {
@@ -63,19 +76,19 @@ __device__ __forceinline__ void grad_norm_chunk(const T* p, int n, int tid, int 
   for (; i + 3 * threads < whole; i += 4 * threads) {
     V v[4];
 #pragma unroll
-    for (int u = 0; u < 4; u++) v[u] = reinterpret_cast<const V*>(p)[i + u * threads];
+    for (int u = 0; u < 4; u++) v[u] = get8(p, i + u * threads);
 #pragma unroll
     for (int u = 0; u < 4; u++) take(v[u]);
   }
-  for (; i < whole; i += threads) take(reinterpret_cast<const V*>(p)[i]);
-  if (tid < (n & 7)) {
-    const double g = (double)(float)p[(whole << 3) + tid];
+  for (; i < whole; i += threads) take(get8(p, i));
+  if (tid < (n & 7) + lead) {
+    const double g = (double)(float)p[tid < lead ? tid - lead : (whole << 3) + tid - lead];
     acc[0] = inf_norm ? larger(acc[0], __builtin_fabs(g)) : __builtin_fma(g, g, acc[0]);
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void grad_scale_chunk(const T* p, T* q, int n, int tid, int threads, double coef) {
+__device__ __forceinline__ void grad_scale_chunk(const T* p, T* q, int n, int lead, int tid, int threads, double coef) {
   typedef typename Pack8<T>::V V;
   const int whole = n >> 3;
   auto scaled = [&](const V& v) {
@@ -88,13 +101,13 @@ __device__ __forceinline__ void grad_scale_chunk(const T* p, T* q, int n, int ti
   for (; i + 3 * threads < whole; i += 4 * threads) {
     V v[4];
 #pragma unroll
-    for (int u = 0; u < 4; u++) v[u] = reinterpret_cast<const V*>(p)[i + u * threads];
+    for (int u = 0; u < 4; u++) v[u] = get8(p, i + u * threads);
 #pragma unroll
-    for (int u = 0; u < 4; u++) reinterpret_cast<V*>(q)[i + u * threads] = scaled(v[u]);
+    for (int u = 0; u < 4; u++) put8(q, i + u * threads, scaled(v[u]));
   }
-  for (; i < whole; i += threads) reinterpret_cast<V*>(q)[i] = scaled(reinterpret_cast<const V*>(p)[i]);
-  if (tid < (n & 7)) {
-    const int j = (whole << 3) + tid;
+  for (; i < whole; i += threads) put8(q, i, scaled(get8(p, i)));
+  if (tid < (n & 7) + lead) {
+    const int j = tid < lead ? tid - lead : (whole << 3) + tid - lead;
     q[j] = (T)(float)((double)(float)p[j] * coef);
   }
 }
@@ -114,26 +127,35 @@ __device__ __forceinline__ double grad_fold(double v, bool inf_norm, double* red
   return t;
 }
 
-// walks the chunks first, first + stride, ... of the list
-template <typename F>
+// Walks the chunks first, first + stride, ... of the list, or (BACK) the same chunks from the other end: the scaling pass
+// starts with what the norm pass has read last.  A tensor's first chunk also holds the elements in front of its first
+// 16-byte boundary; f(item, offset, count, leading) gets them as `leading` (0..7) elements before `offset`.
+template <bool BACK, typename F>
 __device__ __forceinline__ void grad_chunks(const GradList& list, int first, int stride, F&& f) {
-  int t = 0;
-  for (int c = first; c < list.chunks; c += stride) {
-    while (t + 1 < list.count && list.item[t + 1].first <= c) t++;
+  int t = BACK ? list.count - 1 : 0;
+  for (int i = first; i < list.chunks; i += stride) {
+    const int c = BACK ? list.chunks - 1 - i : i;
+    if (BACK) {
+      while (list.item[t].first > c) t--;
+    } else {
+      while (t + 1 < list.count && list.item[t + 1].first <= c) t++;
+    }
     const GradItem& it = list.item[t];
-    const long off = (long)(c - it.first) * GRAD_CHUNK;
-    const long left = it.numel - off;
-    f(it, off, (int)(left < GRAD_CHUNK ? left : GRAD_CHUNK));
+    const int size = it.dtype == FLM_F32 ? 4 : 2;
+    const long odd = min(it.numel, (long)((-(uintptr_t)it.src & 15) / size));
+    const long off = odd + (long)(c - it.first) * list.chunk;
+    const long left = max(it.numel - off, 0L);               // (0: the leading elements made one chunk fewer)
+    f(it, off, (int)(left < list.chunk ? left : list.chunk), c == it.first ? (int)odd : 0);
   }
 }
 
 __device__ __forceinline__ double grad_norm_share(const GradList& list, int first, int stride, bool inf_norm, double* red) {
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
   const int tid = threadIdx.x, threads = blockDim.x;
-  grad_chunks(list, first, stride, [&](const GradItem& it, long off, int n) {
-    if (it.dtype == FLM_F32) grad_norm_chunk((const float*)it.src + off, n, tid, threads, inf_norm, acc);
-    else if (it.dtype == FLM_BF16) grad_norm_chunk((const __bf16*)it.src + off, n, tid, threads, inf_norm, acc);
-    else grad_norm_chunk((const _Float16*)it.src + off, n, tid, threads, inf_norm, acc);
+  grad_chunks<false>(list, first, stride, [&](const GradItem& it, long off, int n, int lead) {
+    if (it.dtype == FLM_F32) grad_norm_chunk((const float*)it.src + off, n, lead, tid, threads, inf_norm, acc);
+    else if (it.dtype == FLM_BF16) grad_norm_chunk((const __bf16*)it.src + off, n, lead, tid, threads, inf_norm, acc);
+    else grad_norm_chunk((const _Float16*)it.src + off, n, lead, tid, threads, inf_norm, acc);
   });
   const double v = inf_norm ? larger(larger(acc[0], acc[1]), larger(acc[2], acc[3])) : (acc[0] + acc[1]) + (acc[2] + acc[3]);
   return grad_fold(v, inf_norm, red);
@@ -141,11 +163,11 @@ __device__ __forceinline__ double grad_norm_share(const GradList& list, int firs
 
 __device__ __forceinline__ void grad_scale_share(const GradList& list, int first, int stride, double coef) {
   const int tid = threadIdx.x, threads = blockDim.x;
-  grad_chunks(list, first, stride, [&](const GradItem& it, long off, int n) {
+  grad_chunks<true>(list, first, stride, [&](const GradItem& it, long off, int n, int lead) {
     if (!it.dst || (it.dst == it.src && coef == 1.0)) return;
-    if (it.dtype == FLM_F32) grad_scale_chunk((const float*)it.src + off, (float*)it.dst + off, n, tid, threads, coef);
-    else if (it.dtype == FLM_BF16) grad_scale_chunk((const __bf16*)it.src + off, (__bf16*)it.dst + off, n, tid, threads, coef);
-    else grad_scale_chunk((const _Float16*)it.src + off, (_Float16*)it.dst + off, n, tid, threads, coef);
+    if (it.dtype == FLM_F32) grad_scale_chunk((const float*)it.src + off, (float*)it.dst + off, n, lead, tid, threads, coef);
+    else if (it.dtype == FLM_BF16) grad_scale_chunk((const __bf16*)it.src + off, (__bf16*)it.dst + off, n, lead, tid, threads, coef);
+    else grad_scale_chunk((const _Float16*)it.src + off, (_Float16*)it.dst + off, n, lead, tid, threads, coef);
   });
 }
 
@@ -195,9 +217,10 @@ __global__ __launch_bounds__(1024) void grad_clip_small_kernel(GradList list, in
 
 // tensors [lo, lo + count) of the caller's arrays as one launch's list
 static bool grad_list(GradList& list, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype,
-                      int lo, int count) {
+                      int lo, int count, int chunk) {
   long chunks = 0;
   list.count = 0;
+  list.chunk = chunk;
   for (int i = lo; i < lo + count; i++) {
     if (numel[i] < 0 || (numel[i] > 0 && !src[i]) || dtype[i] < FLM_F32 || dtype[i] > FLM_F16) return false;
     if (numel[i] == 0) continue;
@@ -207,15 +230,36 @@ static bool grad_list(GradList& list, const void* const* src, void* const* dst, 
     it.numel = numel[i];
     it.dtype = dtype[i];
     it.first = (int)chunks;
-    chunks += (numel[i] + GRAD_CHUNK - 1) / GRAD_CHUNK;
+    chunks += (numel[i] + chunk - 1) / chunk;
     if (chunks >= (1L << 30)) return false;
   }
   list.chunks = (int)chunks;
   return true;
 }
 
-// A list that one workgroup handles alone: up to this many elements in all.
-#define GRAD_SMALL 65536
+// Whether a place would be written twice, or written as one tensor's and read as another's: sorted by address, two
+// neighbouring spans must not overlap (a destination that is its own source counts once).
+static int grad_overlap(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count) {
+  try {
+    std::vector<std::pair<uintptr_t, uintptr_t>> span;
+    span.reserve(2 * (size_t)count);
+    for (int i = 0; i < count; i++) {
+      if (numel[i] == 0 || !dst[i]) continue;
+      const uintptr_t bytes = (uintptr_t)numel[i] * (dtype[i] == FLM_F32 ? 4 : 2);
+      span.emplace_back((uintptr_t)src[i], (uintptr_t)src[i] + bytes);
+      if (dst[i] != src[i]) span.emplace_back((uintptr_t)dst[i], (uintptr_t)dst[i] + bytes);
+    }
+    if (!std::is_sorted(span.begin(), span.end())) std::sort(span.begin(), span.end());
+    for (size_t i = 1; i < span.size(); i++)
+      if (span[i].first < span[i - 1].second) return FLM_E_OVERLAP;
+  } catch (const std::bad_alloc&) {
+    return FLM_E_CAPACITY;
+  }
+  return FLM_OK;
+}
+
+// A list that one workgroup handles alone: up to this many elements in all, in up to 4 tensors.
+#define GRAD_SMALL 8192
 
 static int grad_clip_run(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count,
                          const GradOuter& outer, double max_norm, int inf_norm, double* workspace, float* norm_out,
@@ -223,21 +267,28 @@ static int grad_clip_run(const void* const* src, void* const* dst, const int64_t
   GradList list;
   long total = 0;
   for (int lo = 0; lo < count; lo += FLM_GRAD_LIST) {       // every tensor is checked before anything is launched
-    if (!grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST)) return FLM_E_ARG;
+    if (!grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST, 8192)) return FLM_E_ARG;
     for (int i = 0; i < list.count; i++) total += list.item[i].numel;
   }
-  if (count <= FLM_GRAD_LIST && total <= GRAD_SMALL && !outer.r) {
+  if (dst) {
+    const int rc = grad_overlap(src, dst, numel, dtype, count);
+    if (rc) return rc;
+  }
+  if (list.count == count && count <= 4 && total <= GRAD_SMALL && !outer.r) {
     hipLaunchKernelGGL(grad_clip_small_kernel, dim3(1), dim3(1024), 0, stream, list, inf_norm, max_norm, norm_out);
     FLM_CHECK_LAUNCH();
     return FLM_OK;
   }
+  // chunks: short enough to occupy the card, long enough that a workgroup's four 16-byte loads per thread are many
+  long chunk = (total / 2048 + 2047) / 2048 * 2048;
+  chunk = chunk < 2048 ? 2048 : (chunk > 32768 ? 32768 : chunk);
   // partial results are dealt to the launches in proportion to their chunks, at least one each
   const int launches = (count + FLM_GRAD_LIST - 1) / FLM_GRAD_LIST;
-  const long all_chunks = total / GRAD_CHUNK + count;
+  const long all_chunks = total / chunk + count;
   const int parts_max = GRAD_PARTS - launches;             // (at most 586 launches)
   int n_part = 0;
   for (int lo = 0; lo < count; lo += FLM_GRAD_LIST) {
-    grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST);
+    grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST, (int)chunk);
     long blocks = all_chunks <= parts_max ? list.chunks : (long)((double)list.chunks / all_chunks * parts_max);
     if (blocks < 1) blocks = 1;
     GradOuter o = outer;
@@ -246,12 +297,13 @@ static int grad_clip_run(const void* const* src, void* const* dst, const int64_t
     FLM_CHECK_LAUNCH();
     n_part += (int)blocks;
   }
-  for (int lo = 0; lo < count; lo += FLM_GRAD_LIST) {
-    grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST);
+  for (int i = launches - 1; i >= 0; i--) {
+    const int lo = i * FLM_GRAD_LIST;
+    grad_list(list, src, dst, numel, dtype, lo, count - lo < FLM_GRAD_LIST ? count - lo : FLM_GRAD_LIST, (int)chunk);
     if (!dst) list.chunks = 0;                              // the norm alone
-    const int blocks = list.chunks < 1 ? 1 : (list.chunks < GRAD_PARTS ? list.chunks : GRAD_PARTS);
+    const int blocks = list.chunks < 1 ? 1 : (list.chunks < 2048 ? list.chunks : 2048);
     hipLaunchKernelGGL(grad_clip_kernel, dim3(blocks), dim3(256), 0, stream, list, inf_norm, workspace, n_part, max_norm,
-                       lo == 0 ? norm_out : (float*)nullptr);
+                       i == launches - 1 ? norm_out : (float*)nullptr);
     FLM_CHECK_LAUNCH();
     if (!dst) break;
   }

@@ -11,7 +11,8 @@
 namespace flm {
 
 #define GROUP_SMALL 8192
-#define GROUP_RUN 1024                   // rows of a wave (at least) in the large form
+#define GROUP_RUN 512                    // rows of a wave (at least) in the large form
+#define GROUP_KEYS 8                     // rows a lane holds at a time: their ids are fetched together
 #define GROUP_RUNS_MAX 4096
 
 __device__ __forceinline__ int row_key(const void* ids, int ids64, long i, int E) {
@@ -56,27 +57,45 @@ __device__ __forceinline__ int block_scan(int v, int* scratch, int* total) {
   return base + inc - v;
 }
 
-// places rows [lo, hi) of a wave; next [E+1]: the wave's next position per group
-__device__ __forceinline__ void place_rows(const void* ids, int ids64, int lo, int hi, int E, int bits, int* next, int* order,
+// the keys of rows lo + 64*u + lane (E for rows from hi on)
+__device__ __forceinline__ void load_keys(const void* ids, int ids64, long lo, long hi, int E, int (&key)[GROUP_KEYS]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int u = 0; u < GROUP_KEYS; u++) {
+    const long i = lo + 64 * u + lane;
+    key[u] = i < hi ? row_key(ids, ids64, i, E) : E;
+  }
+}
+
+__device__ __forceinline__ void count_keys(const int (&key)[GROUP_KEYS], long lo, long hi, int* cnt) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int u = 0; u < GROUP_KEYS; u++)
+    if (lo + 64 * u + lane < hi) atomicAdd(&cnt[key[u]], 1);
+}
+
+// places the rows of these keys; next [E+1]: the wave's next position per group
+__device__ __forceinline__ void place_keys(const int (&key)[GROUP_KEYS], long lo, long hi, int bits, int* next, int* order,
                                            int* keys) {
   const int lane = threadIdx.x & 63;
-  for (int i0 = lo; i0 < hi; i0 += 64) {
-    const int i = i0 + lane;
+#pragma unroll
+  for (int u = 0; u < GROUP_KEYS; u++) {
+    if (lo + 64 * u >= hi) break;
+    const long i = lo + 64 * u + lane;
     const bool in = i < hi;
-    const int key = in ? row_key(ids, ids64, i, E) : E;
-    const unsigned long long same = same_key(key, bits) & __ballot(in);
+    const unsigned long long same = same_key(key[u], bits) & __ballot(in);
     const int rank = __popcll(same & lanemask_lt());
     int pos = 0;
-    if (in) pos = next[key] + rank;
+    if (in) pos = next[key[u]] + rank;
     // (all lanes have read before one lane a group writes, and that write is there before the next 64 rows read)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (in && rank == 0) next[key] += __popcll(same);
+    if (in && rank == 0) next[key[u]] = pos + __popcll(same);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (in) {
-      order[pos] = i;
-      keys[pos] = key;
+      order[pos] = (int)i;
+      keys[pos] = key[u];
     }
   }
 }
@@ -132,16 +151,19 @@ __device__ __forceinline__ void scan_groups(int* off, int* tstart, int E, int* s
 __global__ __launch_bounds__(1024) void group_small_kernel(const void* ids, int ids64, int n, int E, int bits, int* order, int* keys,
                                                            int* offsets, int2* tiles, int cap) {
   extern __shared__ int lds[];
-  const int nw = blockDim.x >> 6, w = threadIdx.x >> 6, lane = threadIdx.x & 63, E1 = E + 1;
+  const int nw = blockDim.x >> 6, w = threadIdx.x >> 6, E1 = E + 1;
   int* cnt = lds;
   int* off = cnt + nw * E1;
   int* tstart = off + E1;
   int* scratch = tstart + E1;
-  for (int i = threadIdx.x; i < nw * E1; i += blockDim.x) cnt[i] = 0;
-  __syncthreads();
+  // (a wave's run is at most 64 * GROUP_KEYS rows: GROUP_SMALL rows over 16 waves)
   const int run = ((n + nw - 1) / nw + 63) & ~63;
   const int lo = min(n, w * run), hi = min(n, lo + run);
-  for (int i = lo + lane; i < hi; i += 64) atomicAdd(&cnt[w * E1 + row_key(ids, ids64, i, E)], 1);
+  int key[GROUP_KEYS];
+  load_keys(ids, ids64, lo, hi, E, key);
+  for (int i = threadIdx.x; i < nw * E1; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  count_keys(key, lo, hi, cnt + w * E1);
   __syncthreads();
   // per group: counts of the waves -> rows before each wave; the group's total to off
   for (int g = threadIdx.x; g < E1; g += blockDim.x) {
@@ -155,10 +177,13 @@ __global__ __launch_bounds__(1024) void group_small_kernel(const void* ids, int 
   }
   __syncthreads();
   scan_groups(off, tstart, E, scratch);
-  for (int i = threadIdx.x; i < nw * E1; i += blockDim.x) cnt[i] += off[i % E1];
-  for (int g = threadIdx.x; g < E1; g += blockDim.x) offsets[g] = off[g];
+  for (int g = threadIdx.x; g < E1; g += blockDim.x) {
+    const int o = off[g];
+    for (int k = 0; k < nw; k++) cnt[k * E1 + g] += o;
+    offsets[g] = o;
+  }
   __syncthreads();
-  place_rows(ids, ids64, lo, hi, E, bits, cnt + w * E1, order, keys);
+  place_keys(key, lo, hi, bits, cnt + w * E1, order, keys);
   write_tiles(off, tstart, E, cap, threadIdx.x, blockDim.x, tiles);
 }
 
@@ -169,7 +194,11 @@ __global__ __launch_bounds__(64) void group_count_kernel(const void* ids, int id
   for (int i = threadIdx.x; i < E1; i += 64) lds[i] = 0;
   __syncthreads();
   const long lo = (long)blockIdx.x * run, hi = min((long)n, lo + run);
-  for (long i = lo + threadIdx.x; i < hi; i += 64) atomicAdd(&lds[row_key(ids, ids64, i, E)], 1);
+  for (long at = lo; at < hi; at += 64 * GROUP_KEYS) {
+    int key[GROUP_KEYS];
+    load_keys(ids, ids64, at, hi, E, key);
+    count_keys(key, at, hi, lds);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < E1; i += 64) counts[(long)blockIdx.x * E1 + i] = lds[i];
 }
@@ -230,18 +259,23 @@ __global__ __launch_bounds__(256) void group_place_kernel(const void* ids, int i
   int* off = next + 4 * E1;
   int* tstart = off + E1;
   int* scratch = tstart + E1;
+  const int r = blockIdx.x * 4 + w;
+  int key[GROUP_KEYS];                     // (fetched ahead of the scan)
+  if (r < runs) load_keys(ids, ids64, (long)r * run, min((long)n, (long)(r + 1) * run), E, key);
   for (int g = threadIdx.x; g < E1; g += 256) off[g] = totals[g];
   __syncthreads();
   scan_groups(off, tstart, E, scratch);
-  const int r = blockIdx.x * 4 + w;
   if (r < runs)
     for (int g = lane; g < E1; g += 64) next[w * E1 + g] = off[g] + counts[(long)r * E1 + g];
   if (blockIdx.x == 0)
     for (int g = threadIdx.x; g < E1; g += 256) offsets[g] = off[g];
   __syncthreads();
   if (r < runs) {
-    const long lo = (long)r * run;
-    place_rows(ids, ids64, (int)lo, (int)min((long)n, lo + run), E, bits, next + w * E1, order, keys);
+    const long lo = (long)r * run, hi = min((long)n, lo + run);
+    for (long at = lo; at < hi; at += 64 * GROUP_KEYS) {
+      if (at > lo) load_keys(ids, ids64, at, hi, E, key);
+      place_keys(key, at, hi, bits, next + w * E1, order, keys);
+    }
   }
   write_tiles(off, tstart, E, cap, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, tiles);
 }

@@ -1,15 +1,14 @@
 """Global norm of many gradient tensors, and clipping (flm_grad_clip): the norm of all elements together in one launch per
 112 tensors, the scaling in as many.  The reference's optimizer never clips (src/agent.py:111-116); DQNAgent does when its
 args hold max_grad_norm."""
-import ctypes as C
+from array import array
 from operator import attrgetter
 
 import torch
 
-from ._lib import GRAD_MAX_TENSORS, GRAD_WORKSPACE, FlmError, call, ptr
+from ._lib import GRAD_MAX_TENSORS, GRAD_WORKSPACE, FlmError, launch
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_dtype = attrgetter("dtype")
 
 
 def _dense(t):
@@ -24,8 +23,12 @@ def _dense(t):
     return True
 
 
-def _spans(tensors, sizes):
-    return [(p, p + n * t.element_size()) for p, n, t in zip(map(torch.Tensor.data_ptr, tensors), sizes, tensors) if n]
+_place, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_device, _dtype, _layout, _shape = map(attrgetter, ("device", "dtype", "layout", "shape"))
+
+
+def _address(values):
+    return values.buffer_info()[0]
 
 
 def _inf_norm(norm_type):
@@ -46,39 +49,33 @@ def _run(grads, max_norm, norm_type, outs):
     dev = grads[0].device
     if dev.type != "cuda":
         raise FlmError("gradients must live on a GPU: there is no CPU norm")
-    if set(map(attrgetter("device"), grads)) != {dev}:
+    if set(map(_device, grads)) != {dev}:
         raise ValueError("gradients of several devices")
-    kinds = list(map(_dtype, grads))
-    if not set(kinds) <= set(DTYPES):
-        raise ValueError("gradients must be float32, bfloat16 or float16")
-    if set(map(attrgetter("layout"), grads)) != {torch.strided}:
+    if set(map(_layout, grads)) != {torch.strided}:
         raise ValueError("sparse gradients are not taken")
-    if not all(map(_dense, grads)):
+    types = list(map(_dtype, grads))
+    if not set(types) <= DTYPES.keys():
+        raise ValueError("gradients must be float32, bfloat16 or float16")
+    straight = all(map(_contiguous, grads))
+    if not straight and not all(map(_dense, grads)):
         raise ValueError("a gradient with gaps or repeated places between its elements")
-    sizes = list(map(torch.Tensor.numel, grads))
-    src = (C.c_void_p * count)(*map(torch.Tensor.data_ptr, grads))
+    src, sizes = array("Q", map(_place, grads)), array("q", map(_numel, grads))
+    kinds = array("i", map(DTYPES.__getitem__, types))
     dst = None
-    if outs is not None:
-        spans = _spans(grads, sizes)
+    if outs is not None:                                    # (whether any of them share memory is checked by the call)
         dst = src
         if outs is not grads:
-            if len(outs) != count:
-                raise ValueError("as many outputs as gradients expected")
-            for g, o in zip(grads, outs):
-                if o.shape != g.shape or o.dtype != g.dtype or o.device != dev or \
-                        (not (o.is_contiguous() and g.is_contiguous()) and o.stride() != g.stride()):
-                    raise ValueError("an output differs from its gradient in shape, type, device or strides")
-            dst = (C.c_void_p * count)(*map(torch.Tensor.data_ptr, outs))
-            # (an output that is its own gradient's memory counts once)
-            spans = spans + [s for s, g in zip(_spans(outs, sizes), spans) if s != g]
-        spans.sort()
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise ValueError("gradients (or their outputs) share memory: an element would be scaled twice")
+            if list(map(_shape, outs)) != list(map(_shape, grads)) or list(map(_dtype, outs)) != types or \
+                    set(map(_device, outs)) != {dev}:
+                raise ValueError("an output differs from its gradient in shape, type or device")
+            if not (straight and all(map(_contiguous, outs))) and \
+                    any(o.stride() != g.stride() for o, g in zip(outs, grads)):
+                raise ValueError("an output differs from its gradient in strides")
+            dst = array("Q", map(_place, outs))
     work = torch.empty(GRAD_WORKSPACE, dtype=torch.float64, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        call("flm_grad_clip", src, dst, (C.c_int64 * count)(*sizes), (C.c_int32 * count)(*[DTYPES[k] for k in kinds]), count,
-             float(max_norm), inf, ptr(work), norm.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+    launch(dev, "flm_grad_clip", _address(src), None if dst is None else _address(dst), _address(sizes), _address(kinds), count,
+           float(max_norm), inf, work.data_ptr(), norm.data_ptr())
     return norm
 
 

@@ -40,6 +40,7 @@ extern "C" {
 #define FLM_E_ARG (-1)      /* bad size, null pointer, unsupported capacity */
 #define FLM_E_LAUNCH (-2)   /* the HIP runtime refused a launch or a memset */
 #define FLM_E_CAPACITY (-3) /* the call needs more than a fixed-size internal buffer holds */
+#define FLM_E_OVERLAP (-4)  /* buffers that must not share memory do */
 
 #define FLM_AGENT_OK 0
 #define FLM_AGENT_INDEX_ERROR 2   /* src/rail_observations.py:350, :367 */
@@ -669,11 +670,11 @@ int flm_adapter_linear_backward(const void* dy, long lddy, const void* x, long l
  * absolute value), dst = src * min(1, max_norm / (norm + 1e-6)).
  *   src, dst, numel, dtype: HOST arrays of count device pointers, element counts and FLM_F32 / FLM_BF16 / FLM_F16;
  *   dst[i] == src[i] clips in place, dst[i] == NULL only counts in the norm, dst == NULL: the norm alone.  A dst overlaps no
- *   src but its own, and no other dst
+ *   src but its own, and no other dst, and two src that are clipped do not overlap (FLM_E_OVERLAP)
  *   workspace [FLM_GRAD_WORKSPACE] double; norm_out [1] float
  * Sums are kept in 64 bits and have a fixed order.  A NaN norm makes every gradient NaN, an infinite one makes the finite
  * ones zero, as the formula does.  count <= FLM_GRAD_MAX_TENSORS, max_norm >= 0. */
-#define FLM_GRAD_WORKSPACE 2048
+#define FLM_GRAD_WORKSPACE 4096
 int flm_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count,
                   double max_norm, int inf_norm, double* workspace, float* norm_out, void* stream);
 

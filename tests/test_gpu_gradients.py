@@ -130,3 +130,15 @@ def test_captured_and_replayed():
             n2 = clip_grad_norm_(grads, 1.0, out=eager)
             torch.cuda.synchronize()
             assert torch.equal(norm, n2) and all(torch.equal(a, b) for a, b in zip(outs, eager)), turn
+
+
+def test_shared_memory_is_refused():
+    from flatland_marl_amd.gradients import clip_grad_norm_, grad_norm
+    g, h = torch.ones(100).cuda(), torch.ones(100).cuda()
+    for grads, out in (([g, g], None), ([g[:60], g[50:]], None), ([g, h], [h, g]), ([g, h], [torch.empty_like(g)] * 2)):
+        with pytest.raises(ValueError):
+            clip_grad_norm_(grads, 1.0, out=out)
+    assert (g == 1).all() and abs(grad_norm([g, g]).item() - math.sqrt(200)) < 1e-5      # the norm alone may count twice
+    for out in ([g], [g, h[:50]], [g, h.double()]):
+        with pytest.raises(ValueError):
+            clip_grad_norm_([g.clone(), h], 1.0, out=out)
