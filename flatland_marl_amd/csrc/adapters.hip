@@ -102,8 +102,7 @@ template <> struct Terms<_Float16> { static constexpr int own = 2, low = 2; };
 template <typename T>
 __device__ __forceinline__ void own_terms(const Vec8<T>& v, bf16x8 (&t)[Terms<T>::own]) {
   if constexpr (Terms<T>::own == 1) {
-#pragma unroll
-    for (int j = 0; j < 8; j++) t[0][j] = v.v[j];
+    t[0] = __builtin_bit_cast(bf16x8, v);
   } else {
     float f[8];
 #pragma unroll
@@ -131,14 +130,12 @@ template <> struct Wide<float> { bf16x8 t[3]; };
 
 __device__ __forceinline__ Wide<__bf16> wide(const Vec8<__bf16>& v) {
   Wide<__bf16> w;
-#pragma unroll
-  for (int j = 0; j < 8; j++) w.t[0][j] = v.v[j];
+  w.t[0] = __builtin_bit_cast(bf16x8, v);
   return w;
 }
 __device__ __forceinline__ Wide<_Float16> wide(const Vec8<_Float16>& v) {
   Wide<_Float16> w;
-#pragma unroll
-  for (int j = 0; j < 8; j++) w.t[0][j] = v.v[j];
+  w.t[0] = __builtin_bit_cast(f16x8, v);
   return w;
 }
 __device__ __forceinline__ Wide<float> wide(const Vec8<float>& v) {
@@ -691,10 +688,13 @@ __global__ __launch_bounds__(256) void low_rows_kernel(const float* __restrict__
 
 // ---- gradients of the adapters -----------------------------------------------------------------------------------------
 // G_e(j, q) = sum over the rows i of e of s_e * P(i, j) * Q(i, q), with P fp32 and narrow (u or low), Q wide (x or dy).
-// The sorted rows are cut into chunks of equal length whatever the groups' sizes; a workgroup walks the groups inside its
-// chunk for 256 columns of Q.  A group that lies inside one chunk is written at once; a longer one leaves a partial sum
-// per chunk (at most two a chunk: the group it begins in and the one it ends in), added up in order by a second launch,
-// which also clears the groups without rows.
+// The row tiles of the grouping are cut into chunks of `chunk` tiles whatever the groups' sizes; a workgroup walks a chunk
+// for 4 waves of 32*CPL columns of Q.  A tile's 32 rows are two matrix instructions deep: a lane fetches CPL neighbouring
+// columns of eight rows each, which are the operands of CPL instructions whose outputs interleave; P goes through LDS as
+// bf16 terms, rows contiguous.  Row numbers run two tiles ahead, Q and P one.
+// A group that lies inside one chunk is written at once; a longer one leaves a partial sum per chunk (at most two a chunk: the
+// group it begins in and the one it ends in), added up in order by a second launch, which also clears the groups without
+// rows.
 struct OuterArgs {
   const float* p;                        // [p_slices][.][pld]: by sorted position, or (p_gather) by row
   int p_slices, pld, p_gather;
@@ -704,108 +704,224 @@ struct OuterArgs {
   int KQ, r, E, n, chunk;
   const float* scale;
   float scale_all;
-  float* part;                           // [chunks][2][r][KQ]
+  float* part;                           // [chunks][2][r*KQ], laid out as out
   void* out;                             // out[e*r*KQ + j*o_j + q*o_q]
   long o_j, o_q;
 };
 
-template <typename T, int NRJ>
+// CPL neighbouring elements as words
+template <typename T, int CPL> struct __attribute__((packed, aligned(sizeof(T)))) ColWords { unsigned w[CPL * sizeof(T) / 4]; };
+
+// Column u of eight rows' words, as eight elements.
+template <typename T, int CPL>
+__device__ __forceinline__ Vec8<T> column(const ColWords<T, CPL> (&q)[8], int u) {
+  if constexpr (sizeof(T) == 4) {
+    Vec8<T> v;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v.v[i] = __uint_as_float(q[i].w[u]);
+    return v;
+  } else {
+    uint4 o;
+    const unsigned sel = u & 1 ? 0x07060302u : 0x05040100u;
+    o.x = __builtin_amdgcn_perm(q[1].w[u >> 1], q[0].w[u >> 1], sel);
+    o.y = __builtin_amdgcn_perm(q[3].w[u >> 1], q[2].w[u >> 1], sel);
+    o.z = __builtin_amdgcn_perm(q[5].w[u >> 1], q[4].w[u >> 1], sel);
+    o.w = __builtin_amdgcn_perm(q[7].w[u >> 1], q[6].w[u >> 1], sel);
+    return __builtin_bit_cast(Vec8<T>, o);
+  }
+}
+
+#define OUTER_ROW 40                     // bf16 per LDS row of 32 rows of P
+template <typename T, int NRJ, int CPL>
 __global__ __launch_bounds__(256) void outer_kernel(OuterArgs a, RowGroups g) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
-  const int q0 = blockIdx.x * 256 + w * 64;
-  if (q0 >= a.KQ) return;
-  const int c0 = blockIdx.y * a.chunk;
-  const int c1 = min(c0 + a.chunk, g.offsets[a.E]);
-  int pos = c0;
-  while (pos < c1) {
-    const int e = g.key[pos];
-    const int begin = g.offsets[e], finish = g.offsets[e + 1];
-    const int end = min(finish, c1);
-    const float s = adapter_scale(a.scale, a.scale_all, e);
-    f32x16 acc[2][NRJ];
+  constexpr int LOW = Terms<T>::low, PI = (32 * NRJ * 4 + 255) / 256;     // pieces of eight P values per thread
+  __shared__ __attribute__((aligned(16))) __bf16 pt[LOW * NRJ * 32 * OUTER_ROW];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, h = lane >> 5;
+  const int t0 = blockIdx.y * a.chunk, t1 = min(t0 + a.chunk, g.first_tile[a.E]);
+  const int q0 = (blockIdx.x * 4 + w) * (32 * CPL), q = q0 + c * CPL;
+  if (t0 >= t1) return;
+  f32x16 acc[NRJ][CPL];
+  int rows_of[2][8];                       // row numbers of the lane's rows of a tile, -1 behind its last
+  ColWords<T, CPL> qv[2][8];
+  float pv[PI][8];
+  auto fetch_rows = [&](int2 tile) {
+    const int rows = tile.y >> 16;
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < NRJ; j++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
-    for (int p = pos; p < end; p += 16) {
-      int row[8];
+    for (int s = 0; s < 2; s++)
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const int at = p + 8 * h + i;
-        row[i] = at < end ? g.order[at] : -1;
+        const int m = 16 * s + 8 * h + i;
+        rows_of[s][i] = m < rows ? g.order[tile.x + m] : -1;
       }
-      bf16x8 qt[2][Terms<T>::own];
+  };
+  auto fetch_q = [&]() {
 #pragma unroll
-      for (int sub = 0; sub < 2; sub++) {
-        const int q = q0 + sub * 32 + c;
-        Vec8<T> v;
+    for (int s = 0; s < 2; s++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v.v[i] = row[i] >= 0 && q < a.KQ ? ((const T*)a.q)[(long)row[i] * a.ldq + q] : (T)0.f;
-        own_terms<T>(v, qt[sub]);
-      }
+      for (int i = 0; i < 8; i++) {
+        const T* p = (const T*)a.q + (long)rows_of[s][i] * a.ldq + q;
 #pragma unroll
-      for (int jj = 0; jj < NRJ; jj++) {
-        const int j = jj * 32 + c;
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          f[i] = 0.f;
-          if (row[i] >= 0 && j < a.r) {
-            const long at = (long)(a.p_gather ? row[i] : p + 8 * h + i) * a.pld + j;
-            for (int z = 0; z < a.p_slices; z++) f[i] += a.p[z * a.p_slice + at];
-            f[i] *= s;
-          }
-        }
-        bf16x8 pt[Terms<T>::low];
-        split_terms<Terms<T>::low>(f, pt);
-#pragma unroll
-        for (int sub = 0; sub < 2; sub++) acc[sub][jj] = mul_terms32<Terms<T>::own, Terms<T>::low>(qt[sub], pt, acc[sub][jj]);
-      }
-    }
-    const bool whole = begin >= c0 && finish <= c0 + a.chunk;
-    float* part = a.part + ((long)blockIdx.y * 2 + (begin < c0 ? 0 : 1)) * a.r * a.KQ;
-    T* out = (T*)a.out + (long)e * a.r * a.KQ;
-#pragma unroll
-    for (int sub = 0; sub < 2; sub++)
-#pragma unroll
-      for (int jj = 0; jj < NRJ; jj++) {
-        const int j = jj * 32 + c;
-        if (j >= a.r) continue;
-#pragma unroll
-        for (int r4 = 0; r4 < 4; r4++) {
-          const int q = q0 + sub * 32 + 8 * r4 + 4 * h;
-          const float f[4] = {acc[sub][jj][4 * r4], acc[sub][jj][4 * r4 + 1], acc[sub][jj][4 * r4 + 2], acc[sub][jj][4 * r4 + 3]};
-          if (!whole) {
-            store4(part + (long)j * a.KQ + q, f, a.KQ - q);
-          } else if (a.o_q == 1) {
-            store4(out + (long)j * a.o_j + q, f, a.KQ - q);
+        for (int u = 0; u < CPL * (int)sizeof(T) / 4; u++) qv[s][i].w[u] = 0;
+        if (rows_of[s][i] >= 0) {
+          if (q + CPL <= a.KQ) {
+            qv[s][i] = *reinterpret_cast<const ColWords<T, CPL>*>(p);
           } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              if (q + i < a.KQ) out[(long)j * a.o_j + (long)(q + i) * a.o_q] = (T)f[i];
+            for (int u = 0; u < CPL; u++)
+              if (q + u < a.KQ) {
+                if constexpr (sizeof(T) == 4) qv[s][i].w[u] = __float_as_uint((float)p[u]);
+                else qv[s][i].w[u >> 1] |= (unsigned)__builtin_bit_cast(unsigned short, p[u]) << (16 * (u & 1));
+              }
           }
         }
       }
-    pos = end;
+  };
+  // piece i of the tile's P: row i / (4*NRJ), values 8*(i % (4*NRJ)) ..
+  auto fetch_p = [&](int2 tile) {
+    const int rows = tile.y >> 16;
+#pragma unroll
+    for (int k = 0; k < PI; k++) {
+      const int i = tid + 256 * k, m = i / (4 * NRJ), j = (i - m * (4 * NRJ)) * 8;
+#pragma unroll
+      for (int u = 0; u < 8; u++) pv[k][u] = 0.f;
+      if (m < rows && j < a.r) {
+        const float* p = a.p + (long)(a.p_gather ? g.order[tile.x + m] : tile.x + m) * a.pld + j;
+        for (int z = 0; z < a.p_slices; z++) {
+          const Vec8<float> f = load8(p + z * a.p_slice, a.r - j);
+#pragma unroll
+          for (int u = 0; u < 8; u++) pv[k][u] += f.v[u];
+        }
+      }
+    }
+  };
+  auto place_p = [&](float s) {
+#pragma unroll
+    for (int k = 0; k < PI; k++) {
+      const int i = tid + 256 * k, m = i / (4 * NRJ), j = (i - m * (4 * NRJ)) * 8;
+      if (PI * 256 > 32 * NRJ * 4 && i >= 32 * NRJ * 4) continue;
+#pragma unroll
+      for (int u = 0; u < 8; u++) pv[k][u] *= s;
+      bf16x8 t[LOW];
+      split_terms<LOW>(pv[k], t);
+#pragma unroll
+      for (int o = 0; o < LOW; o++)
+#pragma unroll
+        for (int u = 0; u < 8; u++) pt[(o * NRJ * 32 + j + u) * OUTER_ROW + m] = t[o][u];
+    }
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (int jj = 0; jj < NRJ; jj++)
+#pragma unroll
+      for (int u = 0; u < CPL; u++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[jj][u][r] = 0.f;
+  };
+  auto flush = [&](int e) {
+    const int first = g.first_tile[e], last = g.first_tile[e + 1] - 1;
+    const bool whole = first >= t0 && last < t0 + a.chunk;
+    float* part = a.part + ((long)blockIdx.y * 2 + (first < t0 ? 0 : 1)) * a.r * a.KQ;
+    T* out = (T*)a.out + (long)e * a.r * a.KQ;
+    // (the places are worked out here, not kept in registers over the whole walk: hundreds of them)
+    int col = q0, rank = c;
+    asm volatile("" : "+v"(col), "+v"(rank));
+#pragma unroll
+    for (int jj = 0; jj < NRJ; jj++) {
+      const int j = jj * 32 + rank;
+      if (j >= a.r) continue;
+#pragma unroll
+      for (int r4 = 0; r4 < 4; r4++) {
+        const int qq = col + (8 * r4 + 4 * h) * CPL;                // 4*CPL neighbouring columns
+        if (a.o_q == 1) {
+#pragma unroll
+          for (int i4 = 0; i4 < CPL; i4++) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) f[i] = acc[jj][(4 * i4 + i) % CPL][4 * r4 + (4 * i4 + i) / CPL];
+            if (whole) store4(out + (long)j * a.o_j + qq + 4 * i4, f, a.KQ - qq - 4 * i4);
+            else store4(part + (long)j * a.o_j + qq + 4 * i4, f, a.KQ - qq - 4 * i4);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4 * CPL; i++) {
+            const float f = acc[jj][i % CPL][4 * r4 + i / CPL];
+            const long at = (long)j * a.o_j + (long)(qq + i) * a.o_q;
+            if (qq + i < a.KQ) {
+              if (whole) out[at] = (T)f;
+              else part[at] = f;
+            }
+          }
+        }
+      }
+    }
+  };
+  clear();
+  int2 tile = g.tiles[t0];
+  int2 next = t0 + 1 < t1 ? g.tiles[t0 + 1] : make_int2(0, 0);
+  fetch_rows(tile);
+  fetch_p(tile);
+  fetch_q();
+  fetch_rows(next);
+  for (int t = t0; t < t1; t++) {
+    const int e = tile.y & 0xffff;
+    __syncthreads();                       // (the products of the tile before have read pt)
+    place_p(adapter_scale(a.scale, a.scale_all, e));
+    __syncthreads();
+    bf16x8 qt[2][CPL][Terms<T>::own];
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int u = 0; u < CPL; u++) own_terms<T>(column<T, CPL>(qv[s], u), qt[s][u]);
+    const int2 after = t + 2 < t1 ? g.tiles[t + 2] : make_int2(0, 0);
+    if (t + 1 < t1) {
+      fetch_p(next);
+      fetch_q();
+      fetch_rows(after);
+    }
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int jj = 0; jj < NRJ; jj++) {
+        bf16x8 l[LOW];
+#pragma unroll
+        for (int o = 0; o < LOW; o++)
+          l[o] = *reinterpret_cast<const bf16x8*>(pt + (o * NRJ * 32 + jj * 32 + c) * OUTER_ROW + 16 * s + 8 * h);
+#pragma unroll
+        for (int u = 0; u < CPL; u++) acc[jj][u] = mul_terms32<Terms<T>::own, LOW>(qt[s][u], l, acc[jj][u]);
+      }
+    if (t + 1 == t1 || (next.y & 0xffff) != e) {
+      flush(e);
+      clear();
+    }
+    tile = next;
+    next = after;
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void outer_join_kernel(OuterArgs a, RowGroups g) {
   const int e = blockIdx.y;
-  const int begin = g.offsets[e], end = g.offsets[e + 1];
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   const long total = (long)a.r * a.KQ;
   if (i >= total) return;
+  const int begin = g.first_tile[e], end = g.first_tile[e + 1];
   const int first = begin / a.chunk, last = (end - 1) / a.chunk;
   if (begin < end && first == last) return;
-  const int j = (int)(i / a.KQ), q = (int)(i - (long)j * a.KQ);
-  float s = 0.f;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (begin < end)
-    for (int k = first; k <= last; k++) s += a.part[((long)k * 2 + (begin < k * a.chunk ? 0 : 1)) * total + i];
-  ((T*)a.out)[(long)e * total + (long)j * a.o_j + (long)q * a.o_q] = (T)s;
+    for (int k = first; k <= last; k++) {
+      const float* p = a.part + ((long)k * 2 + (begin < k * a.chunk ? 0 : 1)) * total + i;
+      if (i + 4 <= total) {
+        const Vec4<float> f = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p));
+#pragma unroll
+        for (int u = 0; u < 4; u++) s[u] += f.v[u];
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+          if (i + u < total) s[u] += p[u];
+      }
+    }
+  store4((T*)a.out + (long)e * total + i, s, total - i);
 }
 
 // ---- sizes and launches ------------------------------------------------------------------------------------------------
@@ -934,27 +1050,32 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const 
   return launch_finish<T, V_STRIDED>(f, g, st);
 }
 
-template <typename T>
-static int launch_outer(const OuterArgs& a, const RowGroups& g, hipStream_t st) {
-  const dim3 grid((a.KQ + 255) / 256, (a.n + a.chunk - 1) / a.chunk);
-  if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, dim3(256), 0, st, a, g);
-  else if (a.r <= 64) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, dim3(256), 0, st, a, g);
-  else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, dim3(256), 0, st, a, g);
+template <typename T, int CPL>
+static int launch_outer_cols(const OuterArgs& a, const RowGroups& g, hipStream_t st) {
+  const dim3 grid((a.KQ + 128 * CPL - 1) / (128 * CPL), (g.cap + a.chunk - 1) / a.chunk);
+  if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 1, CPL>), grid, dim3(256), 0, st, a, g);
+  else if (a.r <= 64) hipLaunchKernelGGL((outer_kernel<T, 2, CPL>), grid, dim3(256), 0, st, a, g);
+  else hipLaunchKernelGGL((outer_kernel<T, 4, 2>), dim3((a.KQ + 255) / 256, grid.y), dim3(256), 0, st, a, g);
   FLM_CHECK_LAUNCH();
-  hipLaunchKernelGGL(outer_join_kernel<T>, dim3((unsigned)(((long)a.r * a.KQ + 255) / 256), a.E), dim3(256), 0, st, a, g);
+  hipLaunchKernelGGL(outer_join_kernel<T>, dim3((unsigned)(((long)a.r * a.KQ + 1023) / 1024), a.E), dim3(256), 0, st, a, g);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
 
+// columns a lane holds: 8 bytes' worth, 4 where the ranks leave no registers
+template <typename T>
+static int launch_outer(const OuterArgs& a, const RowGroups& g, hipStream_t st) {
+  return launch_outer_cols<T, sizeof(T) == 4 ? 2 : 4>(a, g, st);
+}
+
 static long round16(long bytes) { return (bytes + 255) & ~255L; }
 
-// rows of sorted positions a workgroup of outer_kernel takes
-static int outer_chunk(int n, int KQ) {
-  const long cols = (KQ + 255) / 256;
-  long chunks = (768 + cols - 1) / cols;
-  long c = ((n + chunks - 1) / chunks + 15) & ~15L;
-  if (c < 64) c = 64;
-  return (int)c;
+// Tiles a workgroup of outer_kernel takes: as many as leave about 512 workgroups (128 ranks: 256 columns each, otherwise 512
+// of 16-bit types): a group that spans several chunks costs a partial sum in each.
+static int outer_chunk(long tiles, int KQ, int r, bool f32) {
+  const int cols = f32 || r > 64 ? 256 : 512;
+  const long c = tiles * ((KQ + cols - 1) / cols) / 512;
+  return (int)(c < 1 ? 1 : c);
 }
 
 template <typename T>
@@ -990,7 +1111,7 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
   const ShrinkArgs s{dy, b, lddy, (long)N * r, 1, r, N, r, rp, n, ss.kslice, u};
   int rc = launch_shrink<T, true>(s, g, ss.slices, st);
   if (rc) return rc;
-  const int ca = outer_chunk(n, K), cb = outer_chunk(n, N);
+  const int ca = outer_chunk(g.cap, K, r, sizeof(T) == 4), cb = outer_chunk(g.cap, N, r, sizeof(T) == 4);
   float* part = (float*)ws;                                          // both gradients in turn
   if ((rc = launch_outer<T>(OuterArgs{u, ss.slices, rp, 0, (long)n * rp, x, ldx, K, r, E, n, ca, scale, scale_all, part, da, K, 1},
                             g, st)))
@@ -1030,8 +1151,9 @@ extern "C" long flm_adapter_workspace(int n, int K, int N, int r, int E, int dty
 
 extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E, int dtype, int need_dx) {
   if (!adapter_sizes(n, K, N, r, E, dtype)) return 0;
-  const int ca = outer_chunk(n, K), cb = outer_chunk(n, N);
-  const long pa = 8L * ((n + ca - 1) / ca) * r * K, pb = 8L * ((n + cb - 1) / cb) * r * N;
+  const long tiles = row_tiles_cap(n, E);
+  const int ca = outer_chunk(tiles, K, r, dtype == FLM_F32), cb = outer_chunk(tiles, N, r, dtype == FLM_F32);
+  const long pa = 8L * ((tiles + ca - 1) / ca) * r * K, pb = 8L * ((tiles + cb - 1) / cb) * r * N;
   long rest = pa > pb ? pa : pb;
   if (need_dx) {
     const BasePlan bs = base_plan(n, N, K, dtype == FLM_F32);

@@ -149,7 +149,7 @@ __device__ __forceinline__ void scan_groups(int* off, int* tstart, int E, int* s
 
 // LDS: cnt [waves][E+1], off [E+1], tstart [E+1], scratch [17]
 __global__ __launch_bounds__(1024) void group_small_kernel(const void* ids, int ids64, int n, int E, int bits, int* order, int* keys,
-                                                           int* offsets, int2* tiles, int cap) {
+                                                           int* offsets, int* first_tile, int2* tiles, int cap) {
   extern __shared__ int lds[];
   const int nw = blockDim.x >> 6, w = threadIdx.x >> 6, E1 = E + 1;
   int* cnt = lds;
@@ -181,6 +181,7 @@ __global__ __launch_bounds__(1024) void group_small_kernel(const void* ids, int 
     const int o = off[g];
     for (int k = 0; k < nw; k++) cnt[k * E1 + g] += o;
     offsets[g] = o;
+    first_tile[g] = tstart[g];
   }
   __syncthreads();
   place_keys(key, lo, hi, bits, cnt + w * E1, order, keys);
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(1024) void group_scan_kernel(int* counts, int runs,
 // four runs a workgroup.  LDS: next [4][E+1], off [E+1], tstart [E+1], scratch [17]
 __global__ __launch_bounds__(256) void group_place_kernel(const void* ids, int ids64, int n, int run, int runs, int E, int bits,
                                                           const int* counts, const int* totals, int* order, int* keys,
-                                                          int* offsets, int2* tiles, int cap) {
+                                                          int* offsets, int* first_tile, int2* tiles, int cap) {
   extern __shared__ int lds[];
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, E1 = E + 1;
   int* next = lds;
@@ -268,7 +269,10 @@ __global__ __launch_bounds__(256) void group_place_kernel(const void* ids, int i
   if (r < runs)
     for (int g = lane; g < E1; g += 64) next[w * E1 + g] = off[g] + counts[(long)r * E1 + g];
   if (blockIdx.x == 0)
-    for (int g = threadIdx.x; g < E1; g += 256) offsets[g] = off[g];
+    for (int g = threadIdx.x; g < E1; g += 256) {
+      offsets[g] = off[g];
+      first_tile[g] = tstart[g];
+    }
   __syncthreads();
   if (r < runs) {
     const long lo = (long)r * run, hi = min((long)n, lo + run);
@@ -307,6 +311,7 @@ extern "C" int flm_group_rows(const void* ids, int ids64, int n, int n_groups, i
   int* order = const_cast<int*>(g.order);
   int* keys = const_cast<int*>(g.key);
   int* offsets = const_cast<int*>(g.offsets);
+  int* first_tile = const_cast<int*>(g.first_tile);
   int2* tiles = const_cast<int2*>(g.tiles);
   int bits = 0;
   while ((1 << bits) <= E) bits++;
@@ -317,7 +322,7 @@ extern "C" int flm_group_rows(const void* ids, int ids64, int n, int n_groups, i
     const size_t lds = sizeof(int) * ((size_t)(waves + 2) * E1 + 17);
     if (lds > 64 * 1024) FLM_RAISE_LDS_ONCE(group_small_kernel);
     hipLaunchKernelGGL(group_small_kernel, dim3(1), dim3(64 * waves), lds, st, ids, ids64, n, E, bits, order, keys, offsets,
-                       tiles, g.cap);
+                       first_tile, tiles, g.cap);
     FLM_CHECK_LAUNCH();
     return FLM_OK;
   }
@@ -329,7 +334,8 @@ extern "C" int flm_group_rows(const void* ids, int ids64, int n, int n_groups, i
   hipLaunchKernelGGL(group_scan_kernel, dim3((E1 + 63) / 64), dim3(1024), 0, st, workspace, runs, E, totals);
   FLM_CHECK_LAUNCH();
   hipLaunchKernelGGL(group_place_kernel, dim3((runs + 3) / 4), dim3(256), sizeof(int) * (6 * E1 + 17), st, ids, ids64, n, run,
-                     runs, E, bits, workspace, totals, order, keys, offsets, tiles, g.cap);
+                     runs, E, bits, workspace, totals, order, keys, offsets, first_tile, tiles,
+                     g.cap);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }

@@ -632,7 +632,7 @@ int flm_dqn_soft_update(float* target, const float* local, long n, double tau, v
  *   ids [n] int32 (ids64 = 0) or int64 (ids64 = 1): 0..n_groups-1; any other value = the row has no group
  *   groups [flm_group_rows_ints(n, n_groups)] int32 out, 16-byte aligned: order [n] (row numbers by group, rows without a
  *     group last), key [n] (the group of order[i], n_groups for none), offsets [n_groups+1] (first position of each group;
- *     offsets[n_groups] = rows that have one) and a table of row tiles.  key starts at the next multiple of four ints
+ *     offsets[n_groups] = rows that have one) and tables of row tiles.  key starts at the next multiple of four ints
  *     behind order, offsets at the next one behind key
  *   workspace [flm_group_rows_workspace(n, n_groups)] int32 (0: may be NULL)
  * n <= 2^30, n_groups <= FLM_GROUPS_MAX. */

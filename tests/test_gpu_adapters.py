@@ -50,6 +50,9 @@ def test_rows_sorted(n, e):
     assert np.array_equal(g.offsets.cpu().numpy(), offsets)
     # the tile table covers every row that has a group once, tiles inside one group
     at = (n + 3) // 4 * 8 + (e + 4) // 4 * 4
+    first = np.concatenate([[0], np.cumsum(-(-np.diff(offsets) // 32))])
+    assert np.array_equal(g.buf[at:at + e + 1].cpu().numpy(), first)
+    at += (e + 4) // 4 * 4
     tiles = g.buf[at:].cpu().numpy().reshape(-1, 2)
     want = [(lo + i, grp, min(32, hi - lo - i)) for grp, (lo, hi) in enumerate(zip(offsets[:-1], offsets[1:]))
             for i in range(0, hi - lo, 32)]

@@ -15,8 +15,8 @@ P = ctypes.c_void_p(4096)                     # a pointer that is never followed
 def test_size_queries():
     lib = _lib.load()
     assert lib.flm_group_rows_ints(0, 4) == 0 and lib.flm_group_rows_ints(10, 0) == 0
-    # order and key padded to 12, four offsets, tiles of 32 rows: one full tile's worth and one per group
-    assert lib.flm_group_rows_ints(10, 3) == 12 + 12 + 4 + 2 * (1 + 3)
+    # order and key padded to 12, twice four offsets, tiles of 32 rows: one full tile's worth and one per group
+    assert lib.flm_group_rows_ints(10, 3) == 12 + 12 + 4 + 4 + 2 * (1 + 3)
     assert lib.flm_group_rows_workspace(8192, 100) == 0 and lib.flm_group_rows_workspace(8193, 100) >= 101
     for n, k, n_out, r, e in ((0, 8, 8, 4, 1), (8, 0, 8, 4, 1), (8, 8, 8, 0, 1), (8, 8, 8, 129, 1), (8, 8, 8, 4, 2048),
                               (1 << 21, 8, 8, 4, 1)):
