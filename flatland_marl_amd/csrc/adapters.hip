@@ -579,19 +579,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[ni][mi][r] = 0.f;
   Vec8<T> fx[RX], fw[RW];
+  auto fetch_whole = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < RX; i++) fx[i] = load8(xp[i] + k0, 8);
+#pragma unroll
+    for (int i = 0; i < RW; i++) fw[i] = load8(wp[i] + k0, 8);
+  };
   auto fetch = [&](int k0) {
-    if (k0 + WIDE_K <= k_end) {
+    const int avail = k_end - k0 - piece * 8;
 #pragma unroll
-      for (int i = 0; i < RX; i++) fx[i] = load8(xp[i] + k0, 8);
+    for (int i = 0; i < RX; i++) fx[i] = load8(xp[i] + k0, avail);
 #pragma unroll
-      for (int i = 0; i < RW; i++) fw[i] = load8(wp[i] + k0, 8);
-    } else {
-      const int avail = k_end - k0 - piece * 8;
-#pragma unroll
-      for (int i = 0; i < RX; i++) fx[i] = load8(xp[i] + k0, avail);
-#pragma unroll
-      for (int i = 0; i < RW; i++) fw[i] = load8(wp[i] + k0, avail);
-    }
+    for (int i = 0; i < RW; i++) fw[i] = load8(wp[i] + k0, avail);
   };
   const int slot = ((piece ^ ((tid >> 3) & 7)) << 4) + (tid >> 3) * 128;
   auto place = [&](char* st) {
@@ -604,32 +603,55 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
   auto products = [&](const char* st) {
     const char* sx = st + (wm * (BM / WM) + c) * 128;
     const char* sw = st + BM * 128 + (wn * (BN / WN) + c) * 128;
+    V x[2][MI], v[2][NI];
+    auto operands = [&](int s) {
+      const int at = ((2 * s + h) ^ (c & 7)) << 4;
+#pragma unroll
+      for (int ni = 0; ni < NI; ni++) v[s & 1][ni] = __builtin_bit_cast(V, *reinterpret_cast<const uint4*>(sw + ni * 32 * 128 + at));
+#pragma unroll
+      for (int mi = 0; mi < MI; mi++) x[s & 1][mi] = __builtin_bit_cast(V, *reinterpret_cast<const uint4*>(sx + mi * 32 * 128 + at));
+    };
+    operands(0);
 #pragma unroll
     for (int s = 0; s < 4; s++) {
-      const int at = ((2 * s + h) ^ (c & 7)) << 4;
-      V x[MI], v[NI];
-#pragma unroll
-      for (int ni = 0; ni < NI; ni++) v[ni] = __builtin_bit_cast(V, *reinterpret_cast<const uint4*>(sw + ni * 32 * 128 + at));
-#pragma unroll
-      for (int mi = 0; mi < MI; mi++) x[mi] = __builtin_bit_cast(V, *reinterpret_cast<const uint4*>(sx + mi * 32 * 128 + at));
+      if (s < 3) operands(s + 1);
 #pragma unroll
       for (int mi = 0; mi < MI; mi++)
 #pragma unroll
-        for (int ni = 0; ni < NI; ni++) acc[ni][mi] = mul32(v[ni], x[mi], acc[ni][mi]);
+        for (int ni = 0; ni < NI; ni++) acc[ni][mi] = mul32(v[s & 1][ni], x[s & 1][mi], acc[ni][mi]);
     }
+    // order: the first operands, then a matrix instruction at a time with a read of the next operands in its shadow
+    constexpr int READS = MI + NI, MULS = MI * NI;
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+      for (int j = 0; j < MULS; j++) {
+        if (s < 3 && j < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
   };
-  if (k_begin < k_end) {
+  const int whole = (k_end - k_begin) / WIDE_K, stages = (k_end - k_begin + WIDE_K - 1) / WIDE_K;
+  if (stages > 0) {
     fetch(k_begin);
     place(lds);
-    if (k_begin + WIDE_K < k_end) fetch(k_begin + WIDE_K);
+    fetch(k_begin + WIDE_K);                                // (behind the end: zeros)
     __syncthreads();
-    int st = 0;
-    for (int k0 = k_begin; k0 < k_end; k0 += WIDE_K) {
-      if (k0 + WIDE_K < k_end) place(lds + (st ^ 1) * STAGE);
-      if (k0 + 2 * WIDE_K < k_end) fetch(k0 + 2 * WIDE_K);
-      products(lds + st * STAGE);
+    int i = 0;
+    for (; i + 2 < whole; i++) {
+      char* st = lds + (i & 1) * STAGE;
+      place(lds + ((i & 1) ^ 1) * STAGE);
+      fetch_whole(k_begin + (i + 2) * WIDE_K);
+      __builtin_amdgcn_sched_barrier(0);                    // (the loads are not moved behind the products: a stage's time ahead)
+      products(st);
       __syncthreads();
-      st ^= 1;
+    }
+    for (; i < stages; i++) {
+      char* st = lds + (i & 1) * STAGE;
+      if (i + 1 < stages) place(lds + ((i & 1) ^ 1) * STAGE);
+      if (i + 2 < stages) fetch(k_begin + (i + 2) * WIDE_K);
+      products(st);
+      __syncthreads();
     }
   }
   int row[MI], key[MI];
@@ -733,7 +755,7 @@ __device__ __forceinline__ Vec8<T> column(const ColWords<T, CPL> (&q)[8], int u)
 
 #define OUTER_ROW 40                     // bf16 per LDS row of 32 rows of P
 template <typename T, int NRJ, int CPL>
-__global__ __launch_bounds__(256) void outer_kernel(OuterArgs a, RowGroups g) {
+__global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs a, RowGroups g) {
   constexpr int LOW = Terms<T>::low, PI = (32 * NRJ * 4 + 255) / 256;     // pieces of eight P values per thread
   __shared__ __attribute__((aligned(16))) __bf16 pt[LOW * NRJ * 32 * OUTER_ROW];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, h = lane >> 5;
