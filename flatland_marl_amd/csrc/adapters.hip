@@ -654,15 +654,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
       __syncthreads();
     }
   }
-  int row[MI], key[MI];
-#pragma unroll
-  for (int mi = 0; mi < MI; mi++) {
-    const long pos = m0 + wm * (BM / WM) + 32 * mi + c;
-    row[mi] = pos < b.n ? g.order[pos] : -1;
-    key[mi] = pos < b.n ? g.key[pos] : a.E;
-  }
   const int nw = n0 + wn * (BN / WN);
   if (!b.part) {
+    int key[MI];
+#pragma unroll
+    for (int mi = 0; mi < MI; mi++) {
+      const long pos = m0 + wm * (BM / WM) + 32 * mi + c;
+      key[mi] = pos < b.n ? g.key[pos] : a.E;
+    }
     __bf16* lt = reinterpret_cast<__bf16*>(lds);
     stage_low<Terms<T>::low>(a, g, m0, BM, lt);
     __syncthreads();
@@ -670,29 +669,51 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
     for (int ni = 0; ni < NI; ni++)
       if (nw + 32 * ni < b.N) add_adapters<T, V_STRIDED, MI, 4, 1>(a, lt, BM, wm * (BM / WM), key, nw + 32 * ni, acc[ni]);
   }
-#pragma unroll
-  for (int mi = 0; mi < MI; mi++) {
-    if (row[mi] < 0) continue;
+  // The tile goes through LDS and out in whole rows, 16 bytes a lane: as the matrix cores leave it, a row's line would be
+  // written sixteen bytes at a time by eight instructions, and the L2 takes one such piece a cycle and channel (measured:
+  // 28 us per 33 MB of a round of tiles, 8 in whole rows).
+  auto store_tile = [&](auto* out, long ld, auto zero) {
+    typedef decltype(zero) O;
+    constexpr int ROW = BN * sizeof(O) + 16, PER = BN * sizeof(O) / 16;        // bytes and 16-byte pieces of a row
+    __syncthreads();
 #pragma unroll
     for (int ni = 0; ni < NI; ni++)
 #pragma unroll
       for (int r4 = 0; r4 < 4; r4++) {
-        const int n = nw + 32 * ni + 8 * r4 + 4 * h;
-        float f[4];
+        const int n = wn * (BN / WN) + 32 * ni + 8 * r4 + 4 * h;
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!b.part && a.bias) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = acc[ni][mi][4 * r4 + i];
-        if (b.part) {
-          store4(b.part + ((long)blockIdx.y * b.n + row[mi]) * b.N + n, f, b.N - n);
-        } else {
-          if (a.bias) {
+          for (int i = 0; i < 4; i++)
+            if (n0 + n + i < b.N) bias[i] = (float)((const T*)a.bias)[n0 + n + i];
+        }
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              if (n + i < b.N) f[i] += (float)((const T*)a.bias)[n + i];
-          }
-          store4((T*)a.y + (long)row[mi] * a.ldy + n, f, b.N - n);
+        for (int mi = 0; mi < MI; mi++) {
+          Vec4<O> v;
+#pragma unroll
+          for (int i = 0; i < 4; i++) v.v[i] = (O)(acc[ni][mi][4 * r4 + i] + bias[i]);
+          *reinterpret_cast<Vec4<O>*>(lds + (wm * (BM / WM) + 32 * mi + c) * ROW + n * sizeof(O)) = v;
         }
       }
-  }
+    __syncthreads();
+    for (int i = tid; i < BM * PER; i += NT) {
+      const int m = i / PER, n = n0 + (i - m * PER) * (16 / (int)sizeof(O));
+      if (m0 + m >= b.n || n >= b.N) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(lds + m * ROW + (i - m * PER) * 16);
+      O* p = out + (long)g.order[m0 + m] * ld + n;
+      struct __attribute__((packed, aligned(sizeof(O)))) Piece { unsigned w[4]; };
+      if (n + 16 / (int)sizeof(O) <= b.N) {
+        *reinterpret_cast<Piece*>(p) = Piece{{v.x, v.y, v.z, v.w}};
+      } else {
+        struct { O v[16 / sizeof(O)]; } e = __builtin_bit_cast(decltype(e), v);
+#pragma unroll
+        for (int u = 0; u < 16 / (int)sizeof(O); u++)
+          if (n + u < b.N) p[u] = e.v[u];
+      }
+    }
+  };
+  if (b.part) store_tile(b.part + (long)blockIdx.y * b.n * b.N, (long)b.N, 0.f);
+  else store_tile((T*)a.y, a.ldy, (T)0.f);
 }
 
 // low[row][r] of every row, in the rows' own order, from the K slices; rows without an adapter get zeros
@@ -1027,6 +1048,8 @@ static int launch_wide(const BaseArgs& b, int slices, const FinishArgs& f, const
   size_t lds = 2 * (BM + BN) * 128;
   const size_t tail = (size_t)Terms<T>::low * BM * (f.rp + 8) * 2;
   if (!b.part && tail > lds) lds = tail;
+  const size_t out = (size_t)BM * (BN * (b.part ? 4 : sizeof(T)) + 16);
+  if (out > lds) lds = out;
   hipLaunchKernelGGL((base_wide_kernel<T, BM, BN, WM, WN, V_STRIDED>),
                      dim3(((b.n + BM - 1) / BM) * ((b.N + BN - 1) / BN), slices), dim3(64 * WM * WN), lds, st, b, f, g);
   FLM_CHECK_LAUNCH();
