@@ -161,7 +161,7 @@ __device__ __forceinline__ f32x16 mul32(bf16x8 a, bf16x8 b, f32x16 c) { return _
 __device__ __forceinline__ f32x16 mul32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 // ---- few rows times few columns over a long K ------------------------------------------------------------------------
-// A workgroup of four waves forms 16*MR rows of X times 16*NR rows of V over k_begin..k_end: the waves take 64 k in turn,
+// Waves form 16*MR rows of X times 16*NR rows of V over k_begin..k_end, `parts` of them taking 32*S k in turn (part: which),
 // both operands straight from memory in the matrix instruction's layout (a lane reads 16 consecutive elements of one row;
 // which k a lane holds is the same for both operands, so their order does not matter), and meet in LDS.  Nothing is reused
 // between workgroups but through the L2, so this form is for operands that are read once: few rows, or few columns.
@@ -170,8 +170,8 @@ __device__ __forceinline__ f32x16 mul32(f16x8 a, f16x8 b, f32x16 c) { return __b
 // S: steps of 32 k taken together (a lane then holds 8*S consecutive elements of a row).
 template <typename T, int MR, int NR, int S, bool V_STRIDED>
 __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* const (&vr)[NR], long v_stride, int k_begin,
-                                             int k_end, f32x4 (&acc)[MR][NR]) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 4;
+                                             int k_end, f32x4 (&acc)[MR][NR], int part, int parts) {
+  const int lane = threadIdx.x & 63, q = lane >> 4;
 #pragma unroll
   for (int mi = 0; mi < MR; mi++)
 #pragma unroll
@@ -191,9 +191,9 @@ __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* 
       for (int mi = 0; mi < MR; mi++) rx[s][mi] = load8(xr[mi] + k, xr[mi] ? avail : 0);
     }
   };
-  int k0 = k_begin + w * (32 * S);
+  int k0 = k_begin + part * (32 * S);
   if (k0 < k_end) fetch(k0);
-  for (; k0 < k_end; k0 += 4 * 32 * S) {
+  for (; k0 < k_end; k0 += parts * 32 * S) {
     Wide<T> x[S][MR], v[S][NR];
 #pragma unroll
     for (int s = 0; s < S; s++) {
@@ -202,7 +202,7 @@ __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* 
 #pragma unroll
       for (int ni = 0; ni < NR; ni++) v[s][ni] = wide(rv[s][ni]);
     }
-    if (k0 + 4 * 32 * S < k_end) fetch(k0 + 4 * 32 * S);
+    if (k0 + parts * 32 * S < k_end) fetch(k0 + parts * 32 * S);
 #pragma unroll
     for (int s = 0; s < S; s++)
 #pragma unroll
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(ShrinkArgs a, RowGroups g) 
     vr[ni] = j < a.r ? (const T*)a.v + (long)e * a.v_group + (long)j * a.v_row : nullptr;
   }
   f32x4 acc[MR][NR];
-  mini_product<T, MR, NR, (MR + NR <= 4 ? 2 : 1), V_STRIDED>(xr, vr, a.v_k, k_begin, k_end, acc);
+  mini_product<T, MR, NR, (MR + NR <= 4 ? 2 : 1), V_STRIDED>(xr, vr, a.v_k, k_begin, k_end, acc, threadIdx.x >> 6, 4);
   mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
     const int m = mi * 16 + c, j = ni * 16 + 4 * q;
     if (m < rows && j < a.rp)
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s,
 #pragma unroll
     for (int ni = 0; ni < NR; ni++) vr[ni] = n0 + ni * 16 + c < a.N ? (const T*)a.w + (long)(n0 + ni * 16 + c) * a.ldw : nullptr;
     f32x4 acc[MR][NR];
-    mini_product<T, MR, NR, 2, false>(xr, vr, 1, k_begin, k_end, acc);
+    mini_product<T, MR, NR, 2, false>(xr, vr, 1, k_begin, k_end, acc, threadIdx.x >> 6, 4);
     mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
       const int m = mi * 16 + c, n = n0 + ni * 16 + 4 * q;
       if (m < a.n) {
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s,
     }
     vr[0] = rank + c < s.r ? (const T*)s.v + (long)e * s.v_group + (long)(rank + c) * s.v_row : nullptr;
     f32x4 acc[MRS][1];
-    mini_product<T, MRS, 1, 2, V_STRIDED>(xr, vr, s.v_k, k_begin, k_end, acc);
+    mini_product<T, MRS, 1, 2, V_STRIDED>(xr, vr, s.v_k, k_begin, k_end, acc, threadIdx.x >> 6, 4);
     mini_meet<MRS, 1>(acc, red, [&](int mi, int, const f32x4& v) {
       const int m = mi * 16 + c;
       if (m < rows) *reinterpret_cast<f32x4*>(s.out + ((long)slice * s.n + tile.x + m) * s.rp + rank + 4 * q) = v;
@@ -337,10 +337,11 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ in
 
 // ---- the adapters' part and the result ---------------------------------------------------------------------------------
 struct FinishArgs {
-  const float* part;                     // [slices][n][N], rows in their own order
-  int slices;
+  const float* part;                     // [slices][n][N]
+  int slices, part_sorted;               // rows of part: in their own order, or (part_sorted) by position
   const void* bias;
-  const float* low;                      // [low_slices][sorted position][rp]
+  const float* low;                      // [low_slices][sorted position][rp], low_step floats a slice
+  long low_step;
   int low_slices, r, rp;
   const void* v;                         // V_e(n, j) = v[e*v_group + n*v_row + j*v_j]
   long v_group, v_row, v_j;
@@ -367,7 +368,7 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
     const int e = pos + row < a.n ? g.key[pos + row] : a.E;
     if (e < a.E) {
       const float* p = a.low + (pos + row) * a.rp + j;
-      const long step = (long)a.n * a.rp;
+      const long step = a.low_step;
       int z = 0;
       for (; z + 8 <= a.low_slices; z += 8) {
         f32x4 v[8][2];
@@ -482,39 +483,39 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
   f32x16 acc[1];
 #pragma unroll
   for (int r = 0; r < 16; r++) acc[0][r] = 0.f;
-  if (row >= 0 && n0 < a.N) {
-    const float* p = a.part + (long)row * a.N;
-    const long step = (long)a.n * a.N;
-    const int stride = 32 / span;
-    if (n0 + 32 <= a.N) {
-      int z = c / span;
-      for (; z + 3 * stride < a.slices; z += 4 * stride) {
-        Vec4<float> f[4][4];
+  const float* p = a.part + (a.part_sorted ? pos + mine : (long)row) * a.N;
+  const long step = (long)a.n * a.N;
+  const int stride = 32 / span;
+  const bool some = row >= 0 && n0 < a.N, whole = some && n0 + 32 <= a.N;
+  // four slices at a time; the first four are on their way while the narrow products are staged
+  Vec4<float> f[4][4];
+  auto fetch = [&](int z) {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+    for (int k = 0; k < 4; k++)
 #pragma unroll
-          for (int r4 = 0; r4 < 4; r4++)
-            f[k][r4] = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + (z + k * stride) * step + n0 + 8 * r4 + 4 * h));
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) acc[0][r] += f[k][r >> 2].v[r & 3];
+      for (int r4 = 0; r4 < 4; r4++) {
+        f[k][r4] = Vec4<float>{{0.f, 0.f, 0.f, 0.f}};
+        if (whole && z + k * stride < a.slices)
+          f[k][r4] = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + (z + k * stride) * step + n0 + 8 * r4 + 4 * h));
       }
-      for (; z < a.slices; z += stride)
+  };
+  fetch(c / span);
+  stage_low<Terms<T>::low>(a, g, pos, 32, lt);
+  if (whole) {
+    for (int z = c / span; z < a.slices; z += 4 * stride) {
 #pragma unroll
-        for (int r4 = 0; r4 < 4; r4++) {
-          const Vec4<float> f = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + z * step + n0 + 8 * r4 + 4 * h));
+      for (int k = 0; k < 4; k++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) acc[0][4 * r4 + i] += f.v[i];
-        }
-    } else {
-      for (int z = c / span; z < a.slices; z += stride)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (n < a.N) acc[0][r] += p[z * step + n];
-        }
+        for (int r = 0; r < 16; r++) acc[0][r] += f[k][r >> 2].v[r & 3];
+      if (z + 4 * stride < a.slices) fetch(z + 4 * stride);
     }
+  } else if (some) {
+    for (int z = c / span; z < a.slices; z += stride)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
+        if (n < a.N) acc[0][r] += p[z * step + n];
+      }
   }
   for (int o = span; o < 32; o <<= 1)
 #pragma unroll
@@ -526,7 +527,6 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
       if (n < a.N) acc[0][r] += (float)((const T*)a.bias)[n];
     }
   }
-  stage_low<Terms<T>::low>(a, g, pos, 32, lt);
   __syncthreads();
   if (n0 >= a.N) return;
   add_adapters<T, V_STRIDED, 1, 2, 4>(a, lt, 32, 0, key, n0, acc);
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
 // A stage's row is 128 bytes; the 16-byte piece p of row r lies at slot p ^ (r & 7), so that the eight rows a group of lanes
 // reads at once fall into different banks.  The weight is the instruction's first operand: a lane then holds one row's
 // outputs, four consecutive ones at a time.
-// part == nullptr: with bias and adapters, straight to y.  Otherwise one K slice per blockIdx.z to part[slice][row][N].
+// part == nullptr: with bias and adapters, straight to y.  Otherwise one K slice per blockIdx.z to part[slice][position][N].
 #define WIDE_K 64
 template <typename T, int BM, int BN, int WM, int WN, bool V_STRIDED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, FinishArgs a, RowGroups g) {
@@ -700,7 +700,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
       const int m = i / PER, n = n0 + (i - m * PER) * (16 / (int)sizeof(O));
       if (m0 + m >= b.n || n >= b.N) continue;
       const uint4 v = *reinterpret_cast<const uint4*>(lds + m * ROW + (i - m * PER) * 16);
-      O* p = out + (long)g.order[m0 + m] * ld + n;
+      O* p = out + (long)(b.part ? m0 + m : g.order[m0 + m]) * ld + n;
       struct __attribute__((packed, aligned(sizeof(O)))) Piece { unsigned w[4]; };
       if (n + 16 / (int)sizeof(O) <= b.N) {
         *reinterpret_cast<Piece*>(p) = Piece{{v.x, v.y, v.z, v.w}};
@@ -750,6 +750,7 @@ struct OuterArgs {
   float* part;                           // [chunks][2][r*KQ], laid out as out
   void* out;                             // out[e*r*KQ + j*o_j + q*o_q]
   long o_j, o_q;
+  int across;                            // workgroups over the columns
 };
 
 // CPL neighbouring elements as words
@@ -776,12 +777,16 @@ __device__ __forceinline__ Vec8<T> column(const ColWords<T, CPL> (&q)[8], int u)
 
 #define OUTER_ROW 40                     // bf16 per LDS row of 32 rows of P
 template <typename T, int NRJ, int CPL>
-__global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs a, RowGroups g) {
+__global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArgs second, int groups, RowGroups g) {
   constexpr int LOW = Terms<T>::low, PI = (32 * NRJ * 4 + 255) / 256;     // pieces of eight P values per thread
   __shared__ __attribute__((aligned(16))) __bf16 pt[LOW * NRJ * 32 * OUTER_ROW];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, h = lane >> 5;
-  const int t0 = blockIdx.y * a.chunk, t1 = min(t0 + a.chunk, g.first_tile[a.E]);
-  const int q0 = (blockIdx.x * 4 + w) * (32 * CPL), q = q0 + c * CPL;
+  // the first `groups` workgroups form one gradient, the others the other
+  const bool one = (int)blockIdx.x < groups;
+  const OuterArgs a = one ? first : second;
+  const int block = one ? blockIdx.x : blockIdx.x - groups, chunk = block / a.across;
+  const int t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, g.first_tile[a.E]);
+  const int q0 = ((block - chunk * a.across) * 4 + w) * (32 * CPL), q = q0 + c * CPL;
   if (t0 >= t1) return;
   f32x16 acc[NRJ][CPL];
   int rows_of[2][8];                       // row numbers of the lane's rows of a tile, -1 behind its last
@@ -861,9 +866,9 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs a, RowGroups g)
         for (int r = 0; r < 16; r++) acc[jj][u][r] = 0.f;
   };
   auto flush = [&](int e) {
-    const int first = g.first_tile[e], last = g.first_tile[e + 1] - 1;
-    const bool whole = first >= t0 && last < t0 + a.chunk;
-    float* part = a.part + ((long)blockIdx.y * 2 + (first < t0 ? 0 : 1)) * a.r * a.KQ;
+    const int head = g.first_tile[e], last = g.first_tile[e + 1] - 1;
+    const bool whole = head >= t0 && last < t0 + a.chunk;
+    float* part = a.part + ((long)chunk * 2 + (head < t0 ? 0 : 1)) * a.r * a.KQ;
     T* out = (T*)a.out + (long)e * a.r * a.KQ;
     // (the places are worked out here, not kept in registers over the whole walk: hundreds of them)
     int col = q0, rank = c;
@@ -942,7 +947,8 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs a, RowGroups g)
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void outer_join_kernel(OuterArgs a, RowGroups g) {
+__global__ __launch_bounds__(256) void outer_join_kernel(OuterArgs one, OuterArgs other, RowGroups g) {
+  const OuterArgs a = blockIdx.z == 0 ? one : other;
   const int e = blockIdx.y;
   const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   const long total = (long)a.r * a.KQ;
@@ -984,37 +990,83 @@ static int k_slices(long tiles, long want, int K, int min_k, int max_slices, int
 // Up to this many rows the projection's weight is streamed past all rows at once (few_rows_kernel).
 #define BASE_ROWS_MAX 64
 
-// How the projection [n,K] x [N,K]^T is formed.
-enum { BASE_ROWS, BASE_X3, BASE_128, BASE_256 };
-struct BasePlan { int form, slices, kslice; };
+// How the projection [n,K] x [N,K]^T is formed.  16-bit types with more than 64 rows: whole tiles of 256 x 256 for the first
+// `rows` rows (sorted positions), tiles of 128 x 128, in K slices if need be, for the others.
+enum { BASE_ROWS, BASE_X3, BASE_TILES };
+struct BasePlan {
+  int form, slices, kslice;              // of the rows behind the first `rows`
+  int rows;
+};
+
+// The time of 128 x 128 tiles for n rows, in units of one round of 256 x 256 tiles (one a CU), and the K slices to take.
+// Measured: a round of 512 tiles of 128 x 128 (two a CU) takes 0.62 of one of 256 tiles of 256 x 256 that do twice its work,
+// half a round 0.4.  Slices are added up by a launch of its own: 5 us and 4 bytes per slice and output at 5 TB/s, against
+// 28.7 ns per k for a round.
+static double tiles_128_time(int n, int K, int N, int* slices, int* kslice) {
+  const double t = (double)((n + 127) / 128) * ((N + 127) / 128), rest = t - 512.0 * (long)(t / 512);
+  *slices = 1;
+  *kslice = K;
+  const double whole = 0.62 * (long)(t / 512) + (rest == 0 ? 0 : (rest <= 256 ? 0.4 : 0.62));
+  int ks;
+  const int s = k_slices((long)t, 512, K, 256, 16, &ks);
+  if (s <= 1) return whole;
+  const double cut = 0.62 * t / 512 + (5000.0 + (4.0 * (2 * s) + 2) * n * N / 5000) / (28.7 * K);
+  if (cut >= whole) return whole;
+  *slices = s;
+  *kslice = ks;
+  return cut;
+}
+
 static BasePlan base_plan(int n, int K, int N, bool f32) {
   BasePlan b;
+  b.rows = 0;
   b.slices = 1;
   b.kslice = K;
-  const long t128 = (long)((n + 127) / 128) * ((N + 127) / 128), t256 = (long)((n + 255) / 256) * ((N + 255) / 256);
+  const int tn = (N + 255) / 256, tm = (n + 255) / 256;
   if (n <= BASE_ROWS_MAX) {
     b.form = BASE_ROWS;
     const int cols = n <= 16 ? 16 : 32;
     b.slices = k_slices((N + cols - 1) / cols, 768, K, 512, 32, &b.kslice);
-  } else if (f32) {
+    return b;
+  }
+  if (f32) {
     b.form = BASE_X3;
-    b.slices = k_slices(t128, 512, K, 512, 16, &b.kslice);
-  } else if (t256 >= 200) {
-    b.form = BASE_256;
-  } else {
-    b.form = BASE_128;
-    if (t128 < 256) b.slices = k_slices(t128, 512, K, 256, 16, &b.kslice);
+    b.slices = k_slices((long)((n + 127) / 128) * ((N + 127) / 128), 512, K, 512, 16, &b.kslice);
+    return b;
+  }
+  b.form = BASE_TILES;
+  double best = tiles_128_time(n, K, N, &b.slices, &b.kslice);
+  // all rows in large tiles, or as many row tiles as fill whole rounds and the rest in small ones
+  const int rounds = (int)(((long)tm * tn + 255) / 256);
+  if (rounds < best) {
+    best = rounds;
+    b.rows = n;
+    b.slices = 1;
+    b.kslice = K;
+  }
+  const int full = (int)((rounds - 1) * 256L / tn);
+  if (full > 0 && full * 256 < n) {
+    int s, ks;
+    const double t = rounds - 1 + tiles_128_time(n - full * 256, K, N, &s, &ks) + 3000.0 / (28.7 * K);
+    if (t < best) {
+      b.rows = full * 256;
+      b.slices = s;
+      b.kslice = ks;
+    }
   }
   return b;
 }
 // bytes of the projection's partial sums (0: it goes straight to the result)
 static long base_part_bytes(const BasePlan& b, int n, int N) {
-  return b.slices == 1 && b.form >= BASE_128 ? 0 : 4L * b.slices * n * N;
+  return b.form == BASE_TILES && (b.slices == 1 || b.rows == n) ? 0 : 4L * b.slices * (n - b.rows) * N;
 }
+#ifndef SHRINK_WANT
+#define SHRINK_WANT 512
+#endif
 struct ShrinkPlan { int slices, kslice; };
 static ShrinkPlan shrink_plan(int n, int K, int E) {
   ShrinkPlan b;
-  b.slices = k_slices(row_tiles_cap(n, E), 512, K, 512, 16, &b.kslice);
+  b.slices = k_slices(row_tiles_cap(n, E), SHRINK_WANT, K, 512, 16, &b.kslice);
   return b;
 }
 
@@ -1071,7 +1123,7 @@ static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st
 // BASE_X3 only).  low_done: s has been formed already.  f.part / b.part: base_part_bytes() of workspace
 template <typename T, bool V_STRIDED, bool S_STRIDED>
 static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const ShrinkArgs& s, int low_slices, bool low_done,
-                             const FinishArgs& f, const RowGroups& g, hipStream_t st) {
+                             FinishArgs f, const RowGroups& g, hipStream_t st) {
   if (plan.form == BASE_ROWS) {
     // (a narrow product that is there already is not formed again: no workgroups for it)
     RowGroups tiles = g;
@@ -1086,31 +1138,48 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const 
                                b.kslice, st)))
         return rc;
     } else {
+      if (plan.rows) {
+        BaseArgs large = b;
+        FinishArgs fl = f;
+        large.n = fl.n = plan.rows;
+        large.part = nullptr;
+        large.kslice = b.K;
+        if ((rc = launch_wide<T, 256, 256, 2, 4, V_STRIDED>(large, 1, fl, g, st))) return rc;
+        if (plan.rows == b.n) return FLM_OK;
+      }
+      // the rows behind: the same with the sorted positions from plan.rows on
+      RowGroups rest = g;
+      rest.order += plan.rows;
+      rest.key += plan.rows;
+      b.n = f.n = b.n - plan.rows;
+      f.low += (long)plan.rows * f.rp;
+      f.part_sorted = 1;
       if (plan.slices == 1) b.part = nullptr;
-      rc = plan.form == BASE_256 ? launch_wide<T, 256, 256, 2, 4, V_STRIDED>(b, plan.slices, f, g, st)
-                                 : launch_wide<T, 128, 128, 2, 2, V_STRIDED>(b, plan.slices, f, g, st);
+      rc = launch_wide<T, 128, 128, 2, 2, V_STRIDED>(b, plan.slices, f, rest, st);
       if (rc || !b.part) return rc;
+      return launch_finish<T, V_STRIDED>(f, rest, st);
     }
   }
   return launch_finish<T, V_STRIDED>(f, g, st);
 }
 
-template <typename T, int CPL>
-static int launch_outer_cols(const OuterArgs& a, const RowGroups& g, hipStream_t st) {
-  const dim3 grid((a.KQ + 128 * CPL - 1) / (128 * CPL), (g.cap + a.chunk - 1) / a.chunk);
-  if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 1, CPL>), grid, dim3(256), 0, st, a, g);
-  else if (a.r <= 64) hipLaunchKernelGGL((outer_kernel<T, 2, CPL>), grid, dim3(256), 0, st, a, g);
-  else hipLaunchKernelGGL((outer_kernel<T, 4, 2>), dim3((a.KQ + 255) / 256, grid.y), dim3(256), 0, st, a, g);
+// both gradients; CPL: 8 bytes' worth of columns a lane, half where the ranks leave no registers
+template <typename T>
+static int launch_outer(OuterArgs a, OuterArgs b, const RowGroups& g, hipStream_t st) {
+  constexpr int CPL = sizeof(T) == 4 ? 2 : 4;
+  const int cols = 128 * (a.r > 64 ? 2 : CPL);
+  a.across = (a.KQ + cols - 1) / cols;
+  b.across = (b.KQ + cols - 1) / cols;
+  const int groups = a.across * ((g.cap + a.chunk - 1) / a.chunk);
+  const dim3 grid(groups + b.across * ((g.cap + b.chunk - 1) / b.chunk));
+  if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 1, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
+  else if (a.r <= 64) hipLaunchKernelGGL((outer_kernel<T, 2, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
+  else hipLaunchKernelGGL((outer_kernel<T, 4, 2>), grid, dim3(256), 0, st, a, b, groups, g);
   FLM_CHECK_LAUNCH();
-  hipLaunchKernelGGL(outer_join_kernel<T>, dim3((unsigned)(((long)a.r * a.KQ + 1023) / 1024), a.E), dim3(256), 0, st, a, g);
+  const long most = (long)a.r * (a.KQ > b.KQ ? a.KQ : b.KQ);
+  hipLaunchKernelGGL(outer_join_kernel<T>, dim3((unsigned)((most + 1023) / 1024), a.E, 2), dim3(256), 0, st, a, b, g);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
-}
-
-// columns a lane holds: 8 bytes' worth, 4 where the ranks leave no registers
-template <typename T>
-static int launch_outer(const OuterArgs& a, const RowGroups& g, hipStream_t st) {
-  return launch_outer_cols<T, sizeof(T) == 4 ? 2 : 4>(a, g, st);
 }
 
 static long round16(long bytes) { return (bytes + 255) & ~255L; }
@@ -1123,6 +1192,9 @@ static int outer_chunk(long tiles, int KQ, int r, bool f32) {
   return (int)(c < 1 ? 1 : c);
 }
 
+// partial sums of outer_kernel: two a chunk
+static long outer_part(long tiles, int chunk) { return 2 * ((tiles + chunk - 1) / chunk); }
+
 template <typename T>
 static int forward(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* a, const void* b,
                    const RowGroups& g, const float* scale, float scale_all, int n, int K, int N, int r, int E, char* ws, void* y,
@@ -1133,7 +1205,7 @@ static int forward(const void* x, long ldx, const void* w, long ldw, const void*
   float* low_part = (float*)ws;
   float* part = (float*)(ws + round16(4L * ss.slices * n * rp));
   const ShrinkArgs s{x, a, ldx, (long)r * K, K, 1, K, r, rp, n, ss.kslice, low_part};
-  const FinishArgs f{part, bs.slices, bias, low_part, ss.slices, r, rp, b, (long)N * r, r, 1, scale, scale_all, n, N, E, y, ldy};
+  const FinishArgs f{part, bs.slices, 0, bias, low_part, (long)n * rp, ss.slices, r, rp, b, (long)N * r, r, 1, scale, scale_all, n, N, E, y, ldy};
   const int rc = launch_projection<T, false, false>(BaseArgs{x, w, ldx, ldw, n, K, N, bs.kslice, part}, bs, true, s, ss.slices, false, f,
                                                     g, st);
   if (rc) return rc;
@@ -1157,11 +1229,9 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
   int rc = launch_shrink<T, true>(s, g, ss.slices, st);
   if (rc) return rc;
   const int ca = outer_chunk(g.cap, K, r, sizeof(T) == 4), cb = outer_chunk(g.cap, N, r, sizeof(T) == 4);
-  float* part = (float*)ws;                                          // both gradients in turn
-  if ((rc = launch_outer<T>(OuterArgs{u, ss.slices, rp, 0, (long)n * rp, x, ldx, K, r, E, n, ca, scale, scale_all, part, da, K, 1},
-                            g, st)))
-    return rc;
-  if ((rc = launch_outer<T>(OuterArgs{low, 1, r, 1, 0, dy, lddy, N, r, E, n, cb, scale, scale_all, part, db, 1, r}, g, st)))
+  float *part_a = (float*)ws, *part_b = part_a + outer_part(g.cap, ca) * r * K;
+  if ((rc = launch_outer<T>(OuterArgs{u, ss.slices, rp, 0, (long)n * rp, x, ldx, K, r, E, n, ca, scale, scale_all, part_a, da, K, 1, 0},
+                            OuterArgs{low, 1, r, 1, 0, dy, lddy, N, r, E, n, cb, scale, scale_all, part_b, db, 1, r, 0}, g, st)))
     return rc;
   if (!dx) return FLM_OK;
   const BasePlan bs = base_plan(n, N, K, sizeof(T) == 4);
@@ -1174,7 +1244,7 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
     w = wt;
     ldw = N;
   }
-  const FinishArgs f{dx_part, bs.slices, nullptr, u, ss.slices, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
+  const FinishArgs f{dx_part, bs.slices, 0, nullptr, u, (long)n * rp, ss.slices, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
   return launch_projection<T, true, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, turn, s, ss.slices, true, f, g,
                                           st);
 }
@@ -1198,8 +1268,7 @@ extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E
   if (!adapter_sizes(n, K, N, r, E, dtype)) return 0;
   const long tiles = row_tiles_cap(n, E);
   const int ca = outer_chunk(tiles, K, r, dtype == FLM_F32), cb = outer_chunk(tiles, N, r, dtype == FLM_F32);
-  const long pa = 8L * ((tiles + ca - 1) / ca) * r * K, pb = 8L * ((tiles + cb - 1) / cb) * r * N;
-  long rest = pa > pb ? pa : pb;
+  long rest = 4L * r * (outer_part(tiles, ca) * K + outer_part(tiles, cb) * N);
   if (need_dx) {
     const BasePlan bs = base_plan(n, N, K, dtype == FLM_F32);
     const long base = round16(base_part_bytes(bs, n, K)) + (bs.form == BASE_X3 ? 0 : (dtype == FLM_F32 ? 4L : 2L) * K * N);

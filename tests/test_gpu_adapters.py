@@ -24,6 +24,11 @@ SIZES = [
     (1031, 200, 72, 8, 1, False),
     (2100, 136, 2050, 9, 3, False),
     (3700, 328, 3655, 70, 6, True),
+    (4099, 600, 4096, 24, 9, True),
+    (4099, 4096, 600, 7, 4, False),
+    (500, 96, 64, 40, 400, False),
+    (6000, 72, 40, 100, 300, True),
+    (13000, 328, 136, 10, 3, True),
 ]
 
 
