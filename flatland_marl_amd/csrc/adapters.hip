@@ -69,9 +69,9 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], long avail) {
 }
 
 // ---- operands as bf16 terms ---------------------------------------------------------------------------------------
-// x = t[0] + t[1] + ... with every term rounded to nearest.  A value that is infinite in bf16 keeps zero in its further
-// terms (its difference from itself would be NaN).
-template <int N>
+// x = t[0] + t[1] + ... with every term rounded to nearest.  KEEP_INF: a value that is infinite in bf16 keeps zero in its
+// further terms (its difference from itself is NaN); without, an infinity becomes NaN, which saves a third of the work.
+template <int N, bool KEEP_INF>
 __device__ __forceinline__ void split_terms(const float (&x)[8], bf16x8 (&t)[N]) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -85,8 +85,8 @@ __device__ __forceinline__ void split_terms(const float (&x)[8], bf16x8 (&t)[N])
       t[s][2 * i + 1] = h[1];
       if (s + 1 < N) {
         const f32x2 f = __builtin_convertvector(h, f32x2);
-        r[0] = __builtin_fabsf(f[0]) < __builtin_inff() ? r[0] - f[0] : 0.f;
-        r[1] = __builtin_fabsf(f[1]) < __builtin_inff() ? r[1] - f[1] : 0.f;
+        r[0] = !KEEP_INF || __builtin_fabsf(f[0]) < __builtin_inff() ? r[0] - f[0] : 0.f;
+        r[1] = !KEEP_INF || __builtin_fabsf(f[1]) < __builtin_inff() ? r[1] - f[1] : 0.f;
       }
     }
   }
@@ -107,7 +107,7 @@ __device__ __forceinline__ void own_terms(const Vec8<T>& v, bf16x8 (&t)[Terms<T>
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) f[j] = (float)v.v[j];
-    split_terms<Terms<T>::own>(f, t);
+    split_terms<Terms<T>::own, sizeof(T) != 4>(f, t);
   }
 }
 
@@ -140,7 +140,7 @@ __device__ __forceinline__ Wide<_Float16> wide(const Vec8<_Float16>& v) {
 }
 __device__ __forceinline__ Wide<float> wide(const Vec8<float>& v) {
   Wide<float> w;
-  split_terms<3>(v.v, w.t);
+  split_terms<3, false>(v.v, w.t);
   return w;
 }
 __device__ __forceinline__ f32x4 mul16(const Wide<__bf16>& a, const Wide<__bf16>& b, f32x4 c) {
@@ -168,10 +168,12 @@ __device__ __forceinline__ f32x16 mul32(f16x8 a, f16x8 b, f32x16 c) { return __b
 // result: lane (c = lane & 15, q = lane >> 4) holds D[v = 16*ni + 4q .. +3][x = 16*mi + c]
 // The loads of a wave's next step are in flight while the matrix cores work on the one before.
 // S: steps of 32 k taken together (a lane then holds 8*S consecutive elements of a row).
+// Every row pointer must be readable: a lane without a row of its own is given another's, its results are not used.  The
+// loop then has no test around a load: launches of a few microseconds run cold, and straight code costs what it is long.
 template <typename T, int MR, int NR, int S, bool V_STRIDED>
 __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* const (&vr)[NR], long v_stride, int k_begin,
                                              int k_end, f32x4 (&acc)[MR][NR], int part, int parts) {
-  const int lane = threadIdx.x & 63, q = lane >> 4;
+  const int q = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int mi = 0; mi < MR; mi++)
 #pragma unroll
@@ -181,20 +183,22 @@ __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* 
 #pragma unroll
     for (int s = 0; s < S; s++) {
       const int k = k0 + q * (8 * S) + s * 8;
-      const int avail = k_end - k;
 #pragma unroll
-      for (int ni = 0; ni < NR; ni++) {
-        const int have = vr[ni] ? avail : 0;
-        rv[s][ni] = V_STRIDED ? load8_strided(vr[ni] + (long)k * v_stride, v_stride, have) : load8(vr[ni] + k, have);
-      }
+      for (int ni = 0; ni < NR; ni++)
+        rv[s][ni] = V_STRIDED ? load8_strided(vr[ni] + (long)k * v_stride, v_stride, 8) : load8(vr[ni] + k, 8);
 #pragma unroll
-      for (int mi = 0; mi < MR; mi++) rx[s][mi] = load8(xr[mi] + k, xr[mi] ? avail : 0);
+      for (int mi = 0; mi < MR; mi++) rx[s][mi] = load8(xr[mi] + k, 8);
     }
   };
-  int k0 = k_begin + part * (32 * S);
-  if (k0 < k_end) fetch(k0);
-  for (; k0 < k_end; k0 += parts * 32 * S) {
-    Wide<T> x[S][MR], v[S][NR];
+  auto products = [&](const Wide<T> (&x)[S][MR], const Wide<T> (&v)[S][NR]) {
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+      for (int ni = 0; ni < NR; ni++)
+#pragma unroll
+        for (int mi = 0; mi < MR; mi++) acc[mi][ni] = mul16(v[s][ni], x[s][mi], acc[mi][ni]);
+  };
+  auto convert = [&](Wide<T> (&x)[S][MR], Wide<T> (&v)[S][NR]) {
 #pragma unroll
     for (int s = 0; s < S; s++) {
 #pragma unroll
@@ -202,13 +206,30 @@ __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* 
 #pragma unroll
       for (int ni = 0; ni < NR; ni++) v[s][ni] = wide(rv[s][ni]);
     }
-    if (k0 + parts * 32 * S < k_end) fetch(k0 + parts * 32 * S);
+  };
+  constexpr int STEP = 32 * S;
+  const int whole = k_begin + (k_end - k_begin) / STEP * STEP;       // steps that lie inside; one more may not
+  int k0 = k_begin + part * STEP;
+  if (k0 < whole) fetch(k0);
+  for (; k0 < whole; k0 += parts * STEP) {
+    Wide<T> x[S][MR], v[S][NR];
+    convert(x, v);
+    if (k0 + parts * STEP < whole) fetch(k0 + parts * STEP);
+    products(x, v);
+  }
+  if (k0 == whole && k0 < k_end) {                                   // this wave's turn is the last, ragged step
 #pragma unroll
-    for (int s = 0; s < S; s++)
+    for (int s = 0; s < S; s++) {
+      const int k = k0 + q * (8 * S) + s * 8, avail = k_end - k;
 #pragma unroll
       for (int ni = 0; ni < NR; ni++)
+        rv[s][ni] = V_STRIDED ? load8_strided(vr[ni] + (long)k * v_stride, v_stride, avail) : load8(vr[ni] + k, avail);
 #pragma unroll
-        for (int mi = 0; mi < MR; mi++) acc[mi][ni] = mul16(v[s][ni], x[s][mi], acc[mi][ni]);
+      for (int mi = 0; mi < MR; mi++) rx[s][mi] = load8(xr[mi] + k, avail);
+    }
+    Wide<T> x[S][MR], v[S][NR];
+    convert(x, v);
+    products(x, v);
   }
 }
 
@@ -233,7 +254,7 @@ struct ShrinkArgs {
   const void *x, *v;
   long ldx, v_group, v_row, v_k;         // V_e(j, k) = v[e*v_group + j*v_row + k*v_k]
   int K, r, rp, n, kslice;
-  float* out;                            // [slice][sorted position][rp]
+  float* out;                            // [slice][sorted position][rp]; what lies behind r is not meant to be read
 };
 
 // low (or u): tiles of rows of one adapter times its r vectors; grid (tiles, K slices)
@@ -248,13 +269,13 @@ __global__ __launch_bounds__(256) void shrink_kernel(ShrinkArgs a, RowGroups g) 
   const T *xr[MR], *vr[NR];
 #pragma unroll
   for (int mi = 0; mi < MR; mi++) {
-    const int m = mi * 16 + c;
-    xr[mi] = m < rows ? (const T*)a.x + (long)g.order[tile.x + m] * a.ldx : nullptr;
+    const int m = min(mi * 16 + c, rows - 1);
+    xr[mi] = (const T*)a.x + (long)g.order[tile.x + m] * a.ldx;
   }
 #pragma unroll
   for (int ni = 0; ni < NR; ni++) {
-    const int j = ni * 16 + c;
-    vr[ni] = j < a.r ? (const T*)a.v + (long)e * a.v_group + (long)j * a.v_row : nullptr;
+    const int j = min(ni * 16 + c, a.r - 1);
+    vr[ni] = (const T*)a.v + (long)e * a.v_group + (long)j * a.v_row;
   }
   f32x4 acc[MR][NR];
   mini_product<T, MR, NR, (MR + NR <= 4 ? 2 : 1), V_STRIDED>(xr, vr, a.v_k, k_begin, k_end, acc, threadIdx.x >> 6, 4);
@@ -285,9 +306,9 @@ __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s,
     const int k_begin = slice * a.kslice, k_end = min(a.K, k_begin + a.kslice);
     const T *xr[MR], *vr[NR];
 #pragma unroll
-    for (int mi = 0; mi < MR; mi++) xr[mi] = mi * 16 + c < a.n ? (const T*)a.x + (long)(mi * 16 + c) * a.ldx : nullptr;
+    for (int mi = 0; mi < MR; mi++) xr[mi] = (const T*)a.x + (long)min(mi * 16 + c, a.n - 1) * a.ldx;
 #pragma unroll
-    for (int ni = 0; ni < NR; ni++) vr[ni] = n0 + ni * 16 + c < a.N ? (const T*)a.w + (long)(n0 + ni * 16 + c) * a.ldw : nullptr;
+    for (int ni = 0; ni < NR; ni++) vr[ni] = (const T*)a.w + (long)min(n0 + ni * 16 + c, a.N - 1) * a.ldw;
     f32x4 acc[MR][NR];
     mini_product<T, MR, NR, 2, false>(xr, vr, 1, k_begin, k_end, acc, threadIdx.x >> 6, 4);
     mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
@@ -306,10 +327,10 @@ __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s,
     const T *xr[MRS], *vr[1];
 #pragma unroll
     for (int mi = 0; mi < MRS; mi++) {
-      const int m = mi * 16 + c;
-      xr[mi] = m < rows ? (const T*)s.x + (long)g.order[tile.x + m] * s.ldx : nullptr;
+      const int m = min(mi * 16 + c, rows - 1);
+      xr[mi] = (const T*)s.x + (long)g.order[tile.x + m] * s.ldx;
     }
-    vr[0] = rank + c < s.r ? (const T*)s.v + (long)e * s.v_group + (long)(rank + c) * s.v_row : nullptr;
+    vr[0] = (const T*)s.v + (long)e * s.v_group + (long)min(rank + c, s.r - 1) * s.v_row;
     f32x4 acc[MRS][1];
     mini_product<T, MRS, 1, 2, V_STRIDED>(xr, vr, s.v_k, k_begin, k_end, acc, threadIdx.x >> 6, 4);
     mini_meet<MRS, 1>(acc, red, [&](int mi, int, const f32x4& v) {
@@ -343,7 +364,7 @@ struct FinishArgs {
   const float* low;                      // [low_slices][sorted position][rp], low_step floats a slice
   long low_step;
   int low_slices, r, rp;
-  const void* v;                         // V_e(n, j) = v[e*v_group + n*v_row + j*v_j]
+  const void* v;                         // V_e(n, j) = v[e*v_group + n*v_row + j*v_j]; without V_STRIDED v_j = 1, r % 8 = 0
   long v_group, v_row, v_j;
   const float* scale;                    // per adapter, or nullptr: scale_all
   float scale_all;
@@ -360,6 +381,7 @@ __device__ __forceinline__ int low_stride(int rp) { return rp + 8; }          //
 template <int LOW>
 __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& g, long pos, int rows, __bf16* lt) {
   const int per = a.rp >> 3, stride = low_stride(a.rp);
+#pragma unroll 1
   for (int i = threadIdx.x; i < rows * per; i += blockDim.x) {
     const int row = i / per, j = (i - row * per) * 8;
     float f[8];
@@ -370,6 +392,7 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
       const float* p = a.low + (pos + row) * a.rp + j;
       const long step = a.low_step;
       int z = 0;
+#pragma unroll 1
       for (; z + 8 <= a.low_slices; z += 8) {
         f32x4 v[8][2];
 #pragma unroll
@@ -382,6 +405,7 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
 #pragma unroll
           for (int u = 0; u < 8; u++) f[u] += v[k][u >> 2][u & 3];
       }
+#pragma unroll 1
       for (; z < a.low_slices; z++) {
         const f32x4 v0 = reinterpret_cast<const f32x4*>(p + z * step)[0], v1 = reinterpret_cast<const f32x4*>(p + z * step)[1];
 #pragma unroll
@@ -392,7 +416,7 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
       for (int u = 0; u < 8; u++) f[u] = j + u < a.r ? f[u] * s : 0.f;
     }
     bf16x8 t[LOW];
-    split_terms<LOW>(f, t);
+    split_terms<LOW, true>(f, t);
 #pragma unroll
     for (int k = 0; k < LOW; k++) *reinterpret_cast<bf16x8*>(lt + (k * rows + row) * stride + j) = t[k];
   }
@@ -402,37 +426,68 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
 // outputs n0 + 8*(r >> 2) + 4*h + (r & 3).  The rows may use several adapters: each adapter's product is formed apart and
 // added to its own rows only, so that no value of one adapter (an infinity, a NaN) can reach the rows of another.
 // key[mi]: the lane's adapter (E: none), ascending over the rows.  V comes straight from memory (the L2): NB adapters and
-// 16*JB ranks at a time, so that NB*JB loads are in flight.  All lanes of the wave take part.
+// 16*JB ranks at a time, so that NB*JB loads are in flight; start() fetches the first of them, before the narrow products are
+// staged if the caller likes.  All lanes of the wave take part.
 template <typename T, bool V_STRIDED, int MI, int JB, int NB>
-__device__ __forceinline__ void add_adapters(const FinishArgs& a, const __bf16* lt, int lds_rows, int lds_row0,
-                                             const int (&key)[MI], int n0, f32x16 (&acc)[MI]) {
-  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, stride = low_stride(a.rp);
-  for (int j0 = 0; j0 < a.r; j0 += 16 * JB) {
-    unsigned todo[MI];
+struct AddAdapters {
+  int es[NB], j0;
+  unsigned todo[MI];
+  Vec8<T> v[NB][JB];
+
+  __device__ __forceinline__ void restart(const FinishArgs& a, const int (&key)[MI]) {
 #pragma unroll
     for (int mi = 0; mi < MI; mi++) todo[mi] = (unsigned)__ballot(key[mi] < a.E);   // (both halves of the wave: the same rows)
-    while (true) {
-      int es[NB];
+  }
+  // the next adapters of the rows and their vectors; es[0] < 0: none left
+  __device__ __forceinline__ void fetch(const FinishArgs& a, const int (&key)[MI], int n0) {
+    const int lane = threadIdx.x & 63, n = min(n0 + (lane & 31), a.N - 1), h = lane >> 5;
 #pragma unroll
-      for (int b = 0; b < NB; b++) {
-        es[b] = -1;
+    for (int b = 0; b < NB; b++) {
+      es[b] = -1;
 #pragma unroll
-        for (int mi = 0; mi < MI; mi++)
-          if (es[b] < 0 && todo[mi]) es[b] = __builtin_amdgcn_readlane(key[mi], __builtin_ctz(todo[mi]));
+      for (int mi = 0; mi < MI; mi++)
+        if (es[b] < 0 && todo[mi]) es[b] = __builtin_amdgcn_readlane(key[mi], __builtin_ctz(todo[mi]));
 #pragma unroll
-        for (int mi = 0; mi < MI; mi++) todo[mi] &= ~(unsigned)__ballot(key[mi] == es[b]);
-      }
-      if (es[0] < 0) break;
-      Vec8<T> v[NB][JB];
+      for (int mi = 0; mi < MI; mi++) todo[mi] &= ~(unsigned)__ballot(key[mi] == es[b]);
+    }
 #pragma unroll
-      for (int b = 0; b < NB; b++)
+    for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int jj = 0; jj < JB; jj++) {
-          const int n = n0 + c, j = j0 + 16 * jj + 8 * h;
-          const T* p = (const T*)a.v + (long)es[b] * a.v_group + (long)n * a.v_row + (long)j * a.v_j;
-          const int have = es[b] >= 0 && n < a.N ? a.r - j : 0;
-          v[b][jj] = V_STRIDED ? load8_strided(p, a.v_j, have) : load8(p, have);
+      for (int jj = 0; jj < JB; jj++) {
+        const int j = j0 + 16 * jj + 8 * h;
+        const T* p = (const T*)a.v + (long)max(es[b], 0) * a.v_group + (long)n * a.v_row;
+        // (no test around a load: ranks behind the last are read from the last, or the first eight, and cleared)
+        if (V_STRIDED) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const T x = p[(long)min(j + i, a.r - 1) * a.v_j];
+            v[b][jj].v[i] = j + i < a.r ? x : (T)0.f;
+          }
+        } else {
+          uint4 x[sizeof(T) / 2];
+          __builtin_memcpy(x, p + (j < a.r ? j : 0), sizeof(x));
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(T) / 2; i++) x[i] = j < a.r ? x[i] : make_uint4(0, 0, 0, 0);
+          __builtin_memcpy(&v[b][jj], x, sizeof(x));
         }
+      }
+  }
+  __device__ __forceinline__ void start(const FinishArgs& a, const int (&key)[MI], int n0) {
+    j0 = 0;
+    restart(a, key);
+    fetch(a, key, n0);
+  }
+  __device__ __forceinline__ void run(const FinishArgs& a, const __bf16* lt, int lds_rows, int lds_row0, const int (&key)[MI],
+                                      int n0, f32x16 (&acc)[MI]) {
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, stride = low_stride(a.rp);
+    while (true) {
+      if (es[0] < 0) {                     // the rows are through: the next ranks
+        j0 += 16 * JB;
+        if (j0 >= a.r) break;
+        restart(a, key);
+        fetch(a, key, n0);
+        if (es[0] < 0) break;
+      }
 #pragma unroll
       for (int b = 0; b < NB; b++) {
         if (es[b] >= 0) {
@@ -461,16 +516,19 @@ __device__ __forceinline__ void add_adapters(const FinishArgs& a, const __bf16* 
           }
         }
       }
+      fetch(a, key, n0);
     }
   }
-}
+};
 
-// y = sum of the K slices + bias + adapters: 32 sorted rows and 32 outputs a wave
-template <typename T, bool V_STRIDED>
+// y = sum of the K slices + bias + adapters: 32 sorted rows and 32 outputs a wave, or (SHARED) a workgroup of four waves
+// that take the K slices in turn and meet in LDS.
+template <typename T, bool V_STRIDED, bool SHARED>
 __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) {
   extern __shared__ __attribute__((aligned(16))) __bf16 lt[];
+  __shared__ float meet[SHARED ? 3 : 1][16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
-  const int n0 = (blockIdx.x * (blockDim.x >> 6) + w) * 32;
+  const int n0 = (SHARED ? blockIdx.x : blockIdx.x * (blockDim.x >> 6) + w) * 32;
   const long pos = (long)blockIdx.y * 32;
   const bool in = pos + c < a.n;
   const int key[1] = {in ? g.key[pos + c] : a.E};
@@ -485,41 +543,49 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
   for (int r = 0; r < 16; r++) acc[0][r] = 0.f;
   const float* p = a.part + (a.part_sorted ? pos + mine : (long)row) * a.N;
   const long step = (long)a.n * a.N;
-  const int stride = 32 / span;
+  const int first = SHARED ? c / span * 4 + w : c / span, stride = SHARED ? 128 / span : 32 / span;
   const bool some = row >= 0 && n0 < a.N, whole = some && n0 + 32 <= a.N;
-  // four slices at a time; the first four are on their way while the narrow products are staged
-  Vec4<float> f[4][4];
-  auto fetch = [&](int z) {
+  auto slice = [&](int z) {
+    Vec4<float> f[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++)
+    for (int r4 = 0; r4 < 4; r4++)
+      f[r4] = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + z * step + n0 + 8 * r4 + 4 * h));
 #pragma unroll
-      for (int r4 = 0; r4 < 4; r4++) {
-        f[k][r4] = Vec4<float>{{0.f, 0.f, 0.f, 0.f}};
-        if (whole && z + k * stride < a.slices)
-          f[k][r4] = __builtin_bit_cast(Vec4<float>, *reinterpret_cast<const Packed4<float>*>(p + (z + k * stride) * step + n0 + 8 * r4 + 4 * h));
-      }
+    for (int r = 0; r < 16; r++) acc[0][r] += f[r >> 2].v[r & 3];
   };
-  fetch(c / span);
-  stage_low<Terms<T>::low>(a, g, pos, 32, lt);
+  AddAdapters<T, V_STRIDED, 1, 2, 2> add;
+  if (!SHARED || w == 0) add.start(a, key, n0);
   if (whole) {
-    for (int z = c / span; z < a.slices; z += 4 * stride) {
+    int z = first;
+    for (; z + 3 * stride < a.slices; z += 4 * stride) {
 #pragma unroll
-      for (int k = 0; k < 4; k++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) acc[0][r] += f[k][r >> 2].v[r & 3];
-      if (z + 4 * stride < a.slices) fetch(z + 4 * stride);
+      for (int k = 0; k < 4; k++) slice(z + k * stride);
     }
+#pragma unroll 1
+    for (; z < a.slices; z += stride) slice(z);
   } else if (some) {
-    for (int z = c / span; z < a.slices; z += stride)
+#pragma unroll 1
+    for (int z = first; z < a.slices; z += stride)
 #pragma unroll
       for (int r = 0; r < 16; r++) {
         const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
         if (n < a.N) acc[0][r] += p[z * step + n];
       }
   }
+  stage_low<Terms<T>::low>(a, g, pos, 32, lt);
   for (int o = span; o < 32; o <<= 1)
 #pragma unroll
     for (int r = 0; r < 16; r++) acc[0][r] += __shfl_xor(acc[0][r], o);
+  if (SHARED && w > 0)
+#pragma unroll
+    for (int r = 0; r < 16; r++) meet[w - 1][r][lane] = acc[0][r];
+  __syncthreads();
+  if (n0 >= a.N || (SHARED && w > 0)) return;
+  if (SHARED)
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[0][r] += meet[k][r][lane];
   if (a.bias) {
 #pragma unroll
     for (int r = 0; r < 16; r++) {
@@ -527,16 +593,14 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
       if (n < a.N) acc[0][r] += (float)((const T*)a.bias)[n];
     }
   }
-  __syncthreads();
-  if (n0 >= a.N) return;
-  add_adapters<T, V_STRIDED, 1, 2, 4>(a, lt, 32, 0, key, n0, acc);
+  add.run(a, lt, 32, 0, key, n0, acc);
   if (in) {
     T* y = (T*)a.y + (long)row * a.ldy;
 #pragma unroll
     for (int r4 = 0; r4 < 4; r4++) {
       const int n = n0 + 8 * r4 + 4 * h;
-      const float f[4] = {acc[0][4 * r4], acc[0][4 * r4 + 1], acc[0][4 * r4 + 2], acc[0][4 * r4 + 3]};
-      store4(y + n, f, a.N - n);
+      const float v[4] = {acc[0][4 * r4], acc[0][4 * r4 + 1], acc[0][4 * r4 + 2], acc[0][4 * r4 + 3]};
+      store4(y + n, v, a.N - n);
     }
   }
 }
@@ -667,7 +731,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
     __syncthreads();
 #pragma unroll
     for (int ni = 0; ni < NI; ni++)
-      if (nw + 32 * ni < b.N) add_adapters<T, V_STRIDED, MI, 4, 1>(a, lt, BM, wm * (BM / WM), key, nw + 32 * ni, acc[ni]);
+      if (nw + 32 * ni < b.N) {
+        AddAdapters<T, V_STRIDED, MI, 4, 1> add;
+        add.start(a, key, nw + 32 * ni);
+        add.run(a, lt, BM, wm * (BM / WM), key, nw + 32 * ni, acc[ni]);
+      }
   }
   // The tile goes through LDS and out in whole rows, 16 bytes a lane: as the matrix cores leave it, a row's line would be
   // written sixteen bytes at a time by eight instructions, and the L2 takes one such piece a cycle and channel (measured:
@@ -802,27 +870,38 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
         rows_of[s][i] = m < rows ? g.order[tile.x + m] : -1;
       }
   };
+  const bool inside = q0 + 32 * CPL <= a.KQ;
   auto fetch_q = [&]() {
+    if (inside) {
 #pragma unroll
-    for (int s = 0; s < 2; s++)
+      for (int s = 0; s < 2; s++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const T* p = (const T*)a.q + (long)rows_of[s][i] * a.ldq + q;
-#pragma unroll
-        for (int u = 0; u < CPL * (int)sizeof(T) / 4; u++) qv[s][i].w[u] = 0;
-        if (rows_of[s][i] >= 0) {
-          if (q + CPL <= a.KQ) {
-            qv[s][i] = *reinterpret_cast<const ColWords<T, CPL>*>(p);
-          } else {
-#pragma unroll
-            for (int u = 0; u < CPL; u++)
-              if (q + u < a.KQ) {
-                if constexpr (sizeof(T) == 4) qv[s][i].w[u] = __float_as_uint((float)p[u]);
-                else qv[s][i].w[u >> 1] |= (unsigned)__builtin_bit_cast(unsigned short, p[u]) << (16 * (u & 1));
-              }
-          }
+        for (int i = 0; i < 8; i++) {
+          const T* p = (const T*)a.q + (long)max(rows_of[s][i], 0) * a.ldq + q;
+          qv[s][i] = *reinterpret_cast<const ColWords<T, CPL>*>(p);
         }
-      }
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+          for (int u = 0; u < CPL * (int)sizeof(T) / 4; u++) qv[s][i].w[u] = rows_of[s][i] >= 0 ? qv[s][i].w[u] : 0u;
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const T* p = (const T*)a.q + (long)rows_of[s][i] * a.ldq + q;
+#pragma unroll
+          for (int u = 0; u < CPL * (int)sizeof(T) / 4; u++) qv[s][i].w[u] = 0;
+#pragma unroll
+          for (int u = 0; u < CPL; u++)
+            if (rows_of[s][i] >= 0 && q + u < a.KQ) {
+              if constexpr (sizeof(T) == 4) qv[s][i].w[u] = __float_as_uint((float)p[u]);
+              else qv[s][i].w[u >> 1] |= (unsigned)__builtin_bit_cast(unsigned short, p[u]) << (16 * (u & 1));
+            }
+        }
+    }
   };
   // piece i of the tile's P: row i / (4*NRJ), values 8*(i % (4*NRJ)) ..
   auto fetch_p = [&](int2 tile) {
@@ -850,7 +929,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
 #pragma unroll
       for (int u = 0; u < 8; u++) pv[k][u] *= s;
       bf16x8 t[LOW];
-      split_terms<LOW>(pv[k], t);
+      split_terms<LOW, true>(pv[k], t);
 #pragma unroll
       for (int o = 0; o < LOW; o++)
 #pragma unroll
@@ -1110,11 +1189,16 @@ static int launch_wide(const BaseArgs& b, int slices, const FinishArgs& f, const
 
 template <typename T, bool V_STRIDED>
 static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st) {
-  const long waves = (long)((a.N + 31) / 32) * ((a.n + 31) / 32);
-  const int per = waves <= 1024 ? 1 : 4;                              // (few waves: one a workgroup, spread over the CUs)
+  const long tiles = (long)((a.N + 31) / 32) * ((a.n + 31) / 32);
   const size_t lds = (size_t)Terms<T>::low * 32 * (a.rp + 8) * 2;
-  hipLaunchKernelGGL((finish_kernel<T, V_STRIDED>), dim3((a.N + 32 * per - 1) / (32 * per), (a.n + 31) / 32), dim3(64 * per), lds, st,
-                     a, g);
+  const unsigned down = (a.n + 31) / 32;
+  if (tiles <= 1024 && a.slices >= 4) {                               // few tiles and a sum worth sharing
+    hipLaunchKernelGGL((finish_kernel<T, V_STRIDED, true>), dim3((a.N + 31) / 32, down), dim3(256), lds, st, a, g);
+  } else {
+    const int per = tiles <= 1024 ? 1 : 4;                            // (few tiles: one a workgroup, spread over the CUs)
+    hipLaunchKernelGGL((finish_kernel<T, V_STRIDED, false>), dim3((a.N + 32 * per - 1) / (32 * per), down), dim3(64 * per), lds, st, a,
+                       g);
+  }
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
@@ -1206,8 +1290,9 @@ static int forward(const void* x, long ldx, const void* w, long ldw, const void*
   float* part = (float*)(ws + round16(4L * ss.slices * n * rp));
   const ShrinkArgs s{x, a, ldx, (long)r * K, K, 1, K, r, rp, n, ss.kslice, low_part};
   const FinishArgs f{part, bs.slices, 0, bias, low_part, (long)n * rp, ss.slices, r, rp, b, (long)N * r, r, 1, scale, scale_all, n, N, E, y, ldy};
-  const int rc = launch_projection<T, false, false>(BaseArgs{x, w, ldx, ldw, n, K, N, bs.kslice, part}, bs, true, s, ss.slices, false, f,
-                                                    g, st);
+  const BaseArgs base{x, w, ldx, ldw, n, K, N, bs.kslice, part};
+  const int rc = r % 8 == 0 ? launch_projection<T, false, false>(base, bs, true, s, ss.slices, false, f, g, st)
+                            : launch_projection<T, true, false>(base, bs, true, s, ss.slices, false, f, g, st);
   if (rc) return rc;
   if (low) {
     hipLaunchKernelGGL(low_rows_kernel, dim3((unsigned)(((long)n * rp + 255) / 256)), dim3(256), 0, st, low_part, ss.slices, n, r,
