@@ -122,6 +122,16 @@ __device__ __forceinline__ f32x16 mul_terms32(const bf16x8 (&a)[OWN], const bf16
   return c;
 }
 
+template <int OWN, int LOW>
+__device__ __forceinline__ f32x4 mul_terms16(const bf16x8 (&a)[OWN], const bf16x8 (&b)[LOW], f32x4 c) {
+#pragma unroll
+  for (int order = LOW - 1; order >= 0; order--)
+#pragma unroll
+    for (int i = 0; i < OWN; i++)
+      if (order - i >= 0 && order - i < LOW) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[order - i], c, 0, 0, 0);
+  return c;
+}
+
 // operands of the wide products: 16-bit types as they are, fp32 as three bf16 terms
 template <typename T> struct Operand { typedef bf16x8 V; };
 template <> struct Operand<_Float16> { typedef f16x8 V; };
@@ -732,7 +742,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
 #pragma unroll
     for (int ni = 0; ni < NI; ni++)
       if (nw + 32 * ni < b.N) {
-        AddAdapters<T, V_STRIDED, MI, 4, 1> add;
+        AddAdapters<T, V_STRIDED, MI, V_STRIDED ? 2 : 4, 1> add;
         add.start(a, key, nw + 32 * ni);
         add.run(a, lt, BM, wm * (BM / WM), key, nw + 32 * ni, acc[ni]);
       }
@@ -800,9 +810,10 @@ __global__ __launch_bounds__(256) void low_rows_kernel(const float* __restrict__
 // ---- gradients of the adapters -----------------------------------------------------------------------------------------
 // G_e(j, q) = sum over the rows i of e of s_e * P(i, j) * Q(i, q), with P fp32 and narrow (u or low), Q wide (x or dy).
 // The row tiles of the grouping are cut into chunks of `chunk` tiles whatever the groups' sizes; a workgroup walks a chunk
-// for 4 waves of 32*CPL columns of Q.  A tile's 32 rows are two matrix instructions deep: a lane fetches CPL neighbouring
-// columns of eight rows each, which are the operands of CPL instructions whose outputs interleave; P goes through LDS as
-// bf16 terms, rows contiguous.  Row numbers run two tiles ahead, Q and P one.
+// for 4 waves of 16*CPL columns of Q.  A tile's 32 rows are one matrix instruction deep: a lane fetches CPL neighbouring
+// columns of eight rows, which are the operands of CPL instructions whose outputs interleave (a lane ends up with 4*CPL
+// neighbouring columns of one rank); P goes through LDS as bf16 terms, rows contiguous.  Row numbers run two tiles ahead, Q
+// and P one.
 // A group that lies inside one chunk is written at once; a longer one leaves a partial sum per chunk (at most two a chunk: the
 // group it begins in and the one it ends in), added up in order by a second launch, which also clears the groups without
 // rows.
@@ -846,73 +857,61 @@ __device__ __forceinline__ Vec8<T> column(const ColWords<T, CPL> (&q)[8], int u)
 #define OUTER_ROW 40                     // bf16 per LDS row of 32 rows of P
 template <typename T, int NRJ, int CPL>
 __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArgs second, int groups, RowGroups g) {
-  constexpr int LOW = Terms<T>::low, PI = (32 * NRJ * 4 + 255) / 256;     // pieces of eight P values per thread
-  __shared__ __attribute__((aligned(16))) __bf16 pt[LOW * NRJ * 32 * OUTER_ROW];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, h = lane >> 5;
+  constexpr int LOW = Terms<T>::low, PER = 2 * NRJ, PI = (32 * PER + 255) / 256;     // pieces of eight P values: a row, a thread
+  __shared__ __attribute__((aligned(16))) __bf16 pt[LOW * NRJ * 16 * OUTER_ROW];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, h = lane >> 4;
   // the first `groups` workgroups form one gradient, the others the other
   const bool one = (int)blockIdx.x < groups;
   const OuterArgs a = one ? first : second;
   const int block = one ? blockIdx.x : blockIdx.x - groups, chunk = block / a.across;
   const int t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, g.first_tile[a.E]);
-  const int q0 = ((block - chunk * a.across) * 4 + w) * (32 * CPL), q = q0 + c * CPL;
+  const int q0 = ((block - chunk * a.across) * 4 + w) * (16 * CPL), q = q0 + c * CPL;
   if (t0 >= t1) return;
-  f32x16 acc[NRJ][CPL];
-  int rows_of[2][8];                       // row numbers of the lane's rows of a tile, -1 behind its last
-  ColWords<T, CPL> qv[2][8];
+  f32x4 acc[NRJ][CPL];
+  int rows_of[8];                          // row numbers of the lane's rows of a tile, -1 behind its last
+  ColWords<T, CPL> qv[8];
   float pv[PI][8];
   auto fetch_rows = [&](int2 tile) {
     const int rows = tile.y >> 16;
 #pragma unroll
-    for (int s = 0; s < 2; s++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int m = 16 * s + 8 * h + i;
-        rows_of[s][i] = m < rows ? g.order[tile.x + m] : -1;
-      }
+    for (int i = 0; i < 8; i++) rows_of[i] = 8 * h + i < rows ? g.order[tile.x + 8 * h + i] : -1;
   };
-  const bool inside = q0 + 32 * CPL <= a.KQ;
+  const bool inside = q0 + 16 * CPL <= a.KQ;
   auto fetch_q = [&]() {
     if (inside) {
 #pragma unroll
-      for (int s = 0; s < 2; s++)
+      for (int i = 0; i < 8; i++)
+        qv[i] = *reinterpret_cast<const ColWords<T, CPL>*>((const T*)a.q + (long)max(rows_of[i], 0) * a.ldq + q);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const T* p = (const T*)a.q + (long)max(rows_of[s][i], 0) * a.ldq + q;
-          qv[s][i] = *reinterpret_cast<const ColWords<T, CPL>*>(p);
-        }
+      for (int i = 0; i < 8; i++)
 #pragma unroll
-      for (int s = 0; s < 2; s++)
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-          for (int u = 0; u < CPL * (int)sizeof(T) / 4; u++) qv[s][i].w[u] = rows_of[s][i] >= 0 ? qv[s][i].w[u] : 0u;
+        for (int u = 0; u < CPL * (int)sizeof(T) / 4; u++) qv[i].w[u] = rows_of[i] >= 0 ? qv[i].w[u] : 0u;
     } else {
 #pragma unroll
-      for (int s = 0; s < 2; s++)
+      for (int i = 0; i < 8; i++) {
+        const T* p = (const T*)a.q + (long)rows_of[i] * a.ldq + q;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const T* p = (const T*)a.q + (long)rows_of[s][i] * a.ldq + q;
+        for (int u = 0; u < CPL * (int)sizeof(T) / 4; u++) qv[i].w[u] = 0;
 #pragma unroll
-          for (int u = 0; u < CPL * (int)sizeof(T) / 4; u++) qv[s][i].w[u] = 0;
-#pragma unroll
-          for (int u = 0; u < CPL; u++)
-            if (rows_of[s][i] >= 0 && q + u < a.KQ) {
-              if constexpr (sizeof(T) == 4) qv[s][i].w[u] = __float_as_uint((float)p[u]);
-              else qv[s][i].w[u >> 1] |= (unsigned)__builtin_bit_cast(unsigned short, p[u]) << (16 * (u & 1));
-            }
-        }
+        for (int u = 0; u < CPL; u++)
+          if (rows_of[i] >= 0 && q + u < a.KQ) {
+            if constexpr (sizeof(T) == 4) qv[i].w[u] = __float_as_uint((float)p[u]);
+            else qv[i].w[u >> 1] |= (unsigned)__builtin_bit_cast(unsigned short, p[u]) << (16 * (u & 1));
+          }
+      }
     }
   };
-  // piece i of the tile's P: row i / (4*NRJ), values 8*(i % (4*NRJ)) ..
+  // piece i of the tile's P: row i / PER, values 8*(i % PER) ..
   auto fetch_p = [&](int2 tile) {
     const int rows = tile.y >> 16;
 #pragma unroll
     for (int k = 0; k < PI; k++) {
-      const int i = tid + 256 * k, m = i / (4 * NRJ), j = (i - m * (4 * NRJ)) * 8;
+      const int i = tid + 256 * k, m = i / PER, j = (i - m * PER) * 8;
 #pragma unroll
       for (int u = 0; u < 8; u++) pv[k][u] = 0.f;
       if (m < rows && j < a.r) {
         const float* p = a.p + (long)(a.p_gather ? g.order[tile.x + m] : tile.x + m) * a.pld + j;
+#pragma unroll 1
         for (int z = 0; z < a.p_slices; z++) {
           const Vec8<float> f = load8(p + z * a.p_slice, a.r - j);
 #pragma unroll
@@ -924,8 +923,8 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
   auto place_p = [&](float s) {
 #pragma unroll
     for (int k = 0; k < PI; k++) {
-      const int i = tid + 256 * k, m = i / (4 * NRJ), j = (i - m * (4 * NRJ)) * 8;
-      if (PI * 256 > 32 * NRJ * 4 && i >= 32 * NRJ * 4) continue;
+      const int i = tid + 256 * k, m = i / PER, j = (i - m * PER) * 8;
+      if (PI * 256 > 32 * PER && i >= 32 * PER) continue;
 #pragma unroll
       for (int u = 0; u < 8; u++) pv[k][u] *= s;
       bf16x8 t[LOW];
@@ -933,16 +932,14 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
 #pragma unroll
       for (int o = 0; o < LOW; o++)
 #pragma unroll
-        for (int u = 0; u < 8; u++) pt[(o * NRJ * 32 + j + u) * OUTER_ROW + m] = t[o][u];
+        for (int u = 0; u < 8; u++) pt[(o * NRJ * 16 + j + u) * OUTER_ROW + m] = t[o][u];
     }
   };
   auto clear = [&]() {
 #pragma unroll
     for (int jj = 0; jj < NRJ; jj++)
 #pragma unroll
-      for (int u = 0; u < CPL; u++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) acc[jj][u][r] = 0.f;
+      for (int u = 0; u < CPL; u++) acc[jj][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
   auto flush = [&](int e) {
     const int head = g.first_tile[e], last = g.first_tile[e + 1] - 1;
@@ -950,33 +947,29 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
     float* part = a.part + ((long)chunk * 2 + (head < t0 ? 0 : 1)) * a.r * a.KQ;
     T* out = (T*)a.out + (long)e * a.r * a.KQ;
     // (the places are worked out here, not kept in registers over the whole walk: hundreds of them)
-    int col = q0, rank = c;
+    int col = q0 + 4 * h * CPL, rank = c;
     asm volatile("" : "+v"(col), "+v"(rank));
 #pragma unroll
     for (int jj = 0; jj < NRJ; jj++) {
-      const int j = jj * 32 + rank;
+      const int j = jj * 16 + rank;
       if (j >= a.r) continue;
+      float f[4 * CPL];                                             // 4*CPL neighbouring columns
 #pragma unroll
-      for (int r4 = 0; r4 < 4; r4++) {
-        const int qq = col + (8 * r4 + 4 * h) * CPL;                // 4*CPL neighbouring columns
-        if (a.o_q == 1) {
+      for (int i = 0; i < 4 * CPL; i++) f[i] = acc[jj][i % CPL][i / CPL];
+      if (a.o_q == 1) {
 #pragma unroll
-          for (int i4 = 0; i4 < CPL; i4++) {
-            float f[4];
+        for (int i = 0; i < CPL; i++) {
+          const float v[4] = {f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
+          if (whole) store4(out + (long)j * a.o_j + col + 4 * i, v, a.KQ - col - 4 * i);
+          else store4(part + (long)j * a.o_j + col + 4 * i, v, a.KQ - col - 4 * i);
+        }
+      } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) f[i] = acc[jj][(4 * i4 + i) % CPL][4 * r4 + (4 * i4 + i) / CPL];
-            if (whole) store4(out + (long)j * a.o_j + qq + 4 * i4, f, a.KQ - qq - 4 * i4);
-            else store4(part + (long)j * a.o_j + qq + 4 * i4, f, a.KQ - qq - 4 * i4);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4 * CPL; i++) {
-            const float f = acc[jj][i % CPL][4 * r4 + i / CPL];
-            const long at = (long)j * a.o_j + (long)(qq + i) * a.o_q;
-            if (qq + i < a.KQ) {
-              if (whole) out[at] = (T)f;
-              else part[at] = f;
-            }
+        for (int i = 0; i < 4 * CPL; i++) {
+          const long at = (long)j * a.o_j + (long)(col + i) * a.o_q;
+          if (col + i < a.KQ) {
+            if (whole) out[at] = (T)f[i];
+            else part[at] = f[i];
           }
         }
       }
@@ -986,36 +979,32 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
   int2 tile = g.tiles[t0];
   int2 next = t0 + 1 < t1 ? g.tiles[t0 + 1] : make_int2(0, 0);
   fetch_rows(tile);
-  fetch_p(tile);
-  fetch_q();
-  fetch_rows(next);
-  for (int t = t0; t < t1; t++) {
+  for (int t = t0 - 1; t < t1; t++) {
+    // (the step before the first only fetches)
     const int e = tile.y & 0xffff;
-    __syncthreads();                       // (the products of the tile before have read pt)
-    place_p(adapter_scale(a.scale, a.scale_all, e));
-    __syncthreads();
-    bf16x8 qt[2][CPL][Terms<T>::own];
+    bf16x8 qt[CPL][Terms<T>::own];
+    if (t >= t0) {
+      __syncthreads();                     // (the products of the tile before have read pt)
+      place_p(adapter_scale(a.scale, a.scale_all, e));
+      __syncthreads();
 #pragma unroll
-    for (int s = 0; s < 2; s++)
-#pragma unroll
-      for (int u = 0; u < CPL; u++) own_terms<T>(column<T, CPL>(qv[s], u), qt[s][u]);
-    const int2 after = t + 2 < t1 ? g.tiles[t + 2] : make_int2(0, 0);
+      for (int u = 0; u < CPL; u++) own_terms<T>(column<T, CPL>(qv, u), qt[u]);
+    }
+    const int2 ahead = t < t0 ? tile : next, after = t < t0 ? next : (t + 2 < t1 ? g.tiles[t + 2] : make_int2(0, 0));
     if (t + 1 < t1) {
-      fetch_p(next);
+      fetch_p(ahead);
       fetch_q();
       fetch_rows(after);
     }
+    if (t < t0) continue;
 #pragma unroll
-    for (int s = 0; s < 2; s++)
+    for (int jj = 0; jj < NRJ; jj++) {
+      bf16x8 l[LOW];
 #pragma unroll
-      for (int jj = 0; jj < NRJ; jj++) {
-        bf16x8 l[LOW];
+      for (int o = 0; o < LOW; o++) l[o] = *reinterpret_cast<const bf16x8*>(pt + (o * NRJ * 16 + jj * 16 + c) * OUTER_ROW + 8 * h);
 #pragma unroll
-        for (int o = 0; o < LOW; o++)
-          l[o] = *reinterpret_cast<const bf16x8*>(pt + (o * NRJ * 32 + jj * 32 + c) * OUTER_ROW + 16 * s + 8 * h);
-#pragma unroll
-        for (int u = 0; u < CPL; u++) acc[jj][u] = mul_terms32<Terms<T>::own, LOW>(qt[s][u], l, acc[jj][u]);
-      }
+      for (int u = 0; u < CPL; u++) acc[jj][u] = mul_terms16<Terms<T>::own, LOW>(qt[u], l, acc[jj][u]);
+    }
     if (t + 1 == t1 || (next.y & 0xffff) != e) {
       flush(e);
       clear();
@@ -1247,18 +1236,22 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const 
   return launch_finish<T, V_STRIDED>(f, g, st);
 }
 
-// both gradients; CPL: 8 bytes' worth of columns a lane, half where the ranks leave no registers
+// Columns a lane of outer_kernel holds: 16 bytes' worth, half where 128 ranks leave no registers.
+static int outer_cols(int r, bool f32) { return f32 || r > 64 ? 4 : 8; }
+
+// both gradients
 template <typename T>
 static int launch_outer(OuterArgs a, OuterArgs b, const RowGroups& g, hipStream_t st) {
-  constexpr int CPL = sizeof(T) == 4 ? 2 : 4;
-  const int cols = 128 * (a.r > 64 ? 2 : CPL);
+  constexpr int CPL = sizeof(T) == 4 ? 4 : 8;
+  const int cols = 64 * outer_cols(a.r, sizeof(T) == 4);
   a.across = (a.KQ + cols - 1) / cols;
   b.across = (b.KQ + cols - 1) / cols;
   const int groups = a.across * ((g.cap + a.chunk - 1) / a.chunk);
   const dim3 grid(groups + b.across * ((g.cap + b.chunk - 1) / b.chunk));
-  if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 1, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
-  else if (a.r <= 64) hipLaunchKernelGGL((outer_kernel<T, 2, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
-  else hipLaunchKernelGGL((outer_kernel<T, 4, 2>), grid, dim3(256), 0, st, a, b, groups, g);
+  if (a.r <= 16) hipLaunchKernelGGL((outer_kernel<T, 1, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
+  else if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 2, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
+  else if (a.r <= 64) hipLaunchKernelGGL((outer_kernel<T, 4, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
+  else hipLaunchKernelGGL((outer_kernel<T, 8, 4>), grid, dim3(256), 0, st, a, b, groups, g);
   FLM_CHECK_LAUNCH();
   const long most = (long)a.r * (a.KQ > b.KQ ? a.KQ : b.KQ);
   hipLaunchKernelGGL(outer_join_kernel<T>, dim3((unsigned)((most + 1023) / 1024), a.E, 2), dim3(256), 0, st, a, b, g);
@@ -1268,11 +1261,14 @@ static int launch_outer(OuterArgs a, OuterArgs b, const RowGroups& g, hipStream_
 
 static long round16(long bytes) { return (bytes + 255) & ~255L; }
 
-// Tiles a workgroup of outer_kernel takes: as many as leave about 512 workgroups (128 ranks: 256 columns each, otherwise 512
-// of 16-bit types): a group that spans several chunks costs a partial sum in each.
+// Tiles a workgroup of outer_kernel takes: as many as leave about 512 workgroups; a group that spans several chunks costs a
+// partial sum in each.
+#ifndef OUTER_WANT
+#define OUTER_WANT 512
+#endif
 static int outer_chunk(long tiles, int KQ, int r, bool f32) {
-  const int cols = f32 || r > 64 ? 256 : 512;
-  const long c = tiles * ((KQ + cols - 1) / cols) / 512;
+  const int cols = 64 * outer_cols(r, f32);
+  const long c = tiles * ((KQ + cols - 1) / cols) / OUTER_WANT;
   return (int)(c < 1 ? 1 : c);
 }
 
