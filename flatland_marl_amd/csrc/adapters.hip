@@ -122,13 +122,13 @@ __device__ __forceinline__ f32x16 mul_terms32(const bf16x8 (&a)[OWN], const bf16
   return c;
 }
 
-template <int OWN, int LOW>
-__device__ __forceinline__ f32x4 mul_terms16(const bf16x8 (&a)[OWN], const bf16x8 (&b)[LOW], f32x4 c) {
+template <int OWN, int LOW, int A, int B>
+__device__ __forceinline__ f32x4 mul_terms16(const bf16x8 (&a)[A], const bf16x8 (&b)[B], f32x4 c) {
 #pragma unroll
   for (int order = LOW - 1; order >= 0; order--)
 #pragma unroll
-    for (int i = 0; i < OWN; i++)
-      if (order - i >= 0 && order - i < LOW) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[order - i], c, 0, 0, 0);
+    for (int i = 0; i < A; i++)
+      if (order - i >= 0 && order - i < B) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[order - i], c, 0, 0, 0);
   return c;
 }
 
@@ -794,6 +794,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
   else store_tile((T*)a.y, a.ldy, (T)0.f);
 }
 
+// part[0] = sum of the K slices part[z], n4 float4 each
+__global__ __launch_bounds__(256) void sum_slices_kernel(float* part, int slices, long n4) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n4) return;
+  f32x4* p = reinterpret_cast<f32x4*>(part) + i;
+  f32x4 s = p[0];
+#pragma unroll 4
+  for (int z = 1; z < slices; z++) s += p[z * n4];
+  p[0] = s;
+}
+
 // low[row][r] of every row, in the rows' own order, from the K slices; rows without an adapter get zeros
 __global__ __launch_bounds__(256) void low_rows_kernel(const float* __restrict__ part, int slices, int n, int r, int rp, int E,
                                                        RowGroups g, float* __restrict__ low) {
@@ -818,9 +829,8 @@ __global__ __launch_bounds__(256) void low_rows_kernel(const float* __restrict__
 // group it begins in and the one it ends in), added up in order by a second launch, which also clears the groups without
 // rows.
 struct OuterArgs {
-  const float* p;                        // [p_slices][.][pld]: by sorted position, or (p_gather) by row
-  int p_slices, pld, p_gather;
-  long p_slice;                          // floats per slice
+  const float* p;                        // [.][pld]: by sorted position, or (p_gather) by row
+  int pld, p_gather;
   const void* q;
   long ldq;
   int KQ, r, E, n, chunk;
@@ -867,6 +877,9 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
   const int t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, g.first_tile[a.E]);
   const int q0 = ((block - chunk * a.across) * 4 + w) * (16 * CPL), q = q0 + c * CPL;
   if (t0 >= t1) return;
+  // whichever axis is contiguous in the result ends up four neighbouring elements a lane: the ranks' (by_rank: a lane holds
+  // one rank and 4*CPL neighbouring columns) or the columns' (one column and four neighbouring ranks)
+  const bool by_rank = a.o_q == 1;
   f32x4 acc[NRJ][CPL];
   int rows_of[8];                          // row numbers of the lane's rows of a tile, -1 behind its last
   ColWords<T, CPL> qv[8];
@@ -901,32 +914,35 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
       }
     }
   };
-  // piece i of the tile's P: row i / PER, values 8*(i % PER) ..
+  // Piece i of the tile's P: row i / PER, values 8*(i % PER) ..  Values behind the last rank belong to outputs that are not
+  // stored; rows behind the last are cleared.
+  int p_row[PI];
+  auto fetch_p_rows = [&](int2 tile) {
+#pragma unroll
+    for (int k = 0; k < PI; k++) {
+      const int at = tile.x + max(min((tid + 256 * k) / PER, (tile.y >> 16) - 1), 0);
+      p_row[k] = a.p_gather ? g.order[at] : at;
+    }
+  };
   auto fetch_p = [&](int2 tile) {
-    const int rows = tile.y >> 16;
 #pragma unroll
     for (int k = 0; k < PI; k++) {
       const int i = tid + 256 * k, m = i / PER, j = (i - m * PER) * 8;
+      const float* p = a.p + (long)p_row[k] * a.pld + (j < a.r ? j : 0);
+      Vec8<float> f;
+      if (j + 8 <= a.pld || j >= a.r) f = load8(p, min(8, a.pld));
+      else f = load8(p, a.r - j);
 #pragma unroll
-      for (int u = 0; u < 8; u++) pv[k][u] = 0.f;
-      if (m < rows && j < a.r) {
-        const float* p = a.p + (long)(a.p_gather ? g.order[tile.x + m] : tile.x + m) * a.pld + j;
-#pragma unroll 1
-        for (int z = 0; z < a.p_slices; z++) {
-          const Vec8<float> f = load8(p + z * a.p_slice, a.r - j);
-#pragma unroll
-          for (int u = 0; u < 8; u++) pv[k][u] += f.v[u];
-        }
-      }
+      for (int u = 0; u < 8; u++) pv[k][u] = f.v[u];
     }
   };
-  auto place_p = [&](float s) {
+  auto place_p = [&](float s, int rows) {
 #pragma unroll
     for (int k = 0; k < PI; k++) {
       const int i = tid + 256 * k, m = i / PER, j = (i - m * PER) * 8;
       if (PI * 256 > 32 * PER && i >= 32 * PER) continue;
 #pragma unroll
-      for (int u = 0; u < 8; u++) pv[k][u] *= s;
+      for (int u = 0; u < 8; u++) pv[k][u] = m < rows ? pv[k][u] * s : 0.f;
       bf16x8 t[LOW];
       split_terms<LOW, true>(pv[k], t);
 #pragma unroll
@@ -947,30 +963,34 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
     float* part = a.part + ((long)chunk * 2 + (head < t0 ? 0 : 1)) * a.r * a.KQ;
     T* out = (T*)a.out + (long)e * a.r * a.KQ;
     // (the places are worked out here, not kept in registers over the whole walk: hundreds of them)
-    int col = q0 + 4 * h * CPL, rank = c;
-    asm volatile("" : "+v"(col), "+v"(rank));
+    int at = c;
+    asm volatile("" : "+v"(at));
+    if (by_rank) {
+      const int col = q0 + 4 * h * CPL;
 #pragma unroll
-    for (int jj = 0; jj < NRJ; jj++) {
-      const int j = jj * 16 + rank;
-      if (j >= a.r) continue;
-      float f[4 * CPL];                                             // 4*CPL neighbouring columns
-#pragma unroll
-      for (int i = 0; i < 4 * CPL; i++) f[i] = acc[jj][i % CPL][i / CPL];
-      if (a.o_q == 1) {
+      for (int jj = 0; jj < NRJ; jj++) {
+        const int j = jj * 16 + at;
+        if (j >= a.r) continue;
 #pragma unroll
         for (int i = 0; i < CPL; i++) {
-          const float v[4] = {f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
+          float v[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) v[u] = acc[jj][(4 * i + u) % CPL][(4 * i + u) / CPL];
           if (whole) store4(out + (long)j * a.o_j + col + 4 * i, v, a.KQ - col - 4 * i);
           else store4(part + (long)j * a.o_j + col + 4 * i, v, a.KQ - col - 4 * i);
         }
-      } else {
+      }
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4 * CPL; i++) {
-          const long at = (long)j * a.o_j + (long)(col + i) * a.o_q;
-          if (col + i < a.KQ) {
-            if (whole) out[at] = (T)f[i];
-            else part[at] = f[i];
-          }
+      for (int u = 0; u < CPL; u++) {
+        const int col = q0 + at * CPL + u;
+        if (col >= a.KQ) continue;
+#pragma unroll
+        for (int jj = 0; jj < NRJ; jj++) {
+          const int j = jj * 16 + 4 * h;
+          const float v[4] = {acc[jj][u][0], acc[jj][u][1], acc[jj][u][2], acc[jj][u][3]};
+          if (whole) store4(out + (long)col * a.o_q + j, v, a.r - j);
+          else store4(part + (long)col * a.o_q + j, v, a.r - j);
         }
       }
     }
@@ -979,13 +999,14 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
   int2 tile = g.tiles[t0];
   int2 next = t0 + 1 < t1 ? g.tiles[t0 + 1] : make_int2(0, 0);
   fetch_rows(tile);
+  fetch_p_rows(tile);
   for (int t = t0 - 1; t < t1; t++) {
     // (the step before the first only fetches)
     const int e = tile.y & 0xffff;
     bf16x8 qt[CPL][Terms<T>::own];
     if (t >= t0) {
       __syncthreads();                     // (the products of the tile before have read pt)
-      place_p(adapter_scale(a.scale, a.scale_all, e));
+      place_p(adapter_scale(a.scale, a.scale_all, e), tile.y >> 16);
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < CPL; u++) own_terms<T>(column<T, CPL>(qv, u), qt[u]);
@@ -995,6 +1016,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
       fetch_p(ahead);
       fetch_q();
       fetch_rows(after);
+      fetch_p_rows(after);
     }
     if (t < t0) continue;
 #pragma unroll
@@ -1003,7 +1025,8 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
 #pragma unroll
       for (int o = 0; o < LOW; o++) l[o] = *reinterpret_cast<const bf16x8*>(pt + (o * NRJ * 16 + jj * 16 + c) * OUTER_ROW + 8 * h);
 #pragma unroll
-      for (int u = 0; u < CPL; u++) acc[jj][u] = mul_terms16<Terms<T>::own, LOW>(qt[u], l, acc[jj][u]);
+      for (int u = 0; u < CPL; u++)
+        acc[jj][u] = by_rank ? mul_terms16<Terms<T>::own, LOW>(qt[u], l, acc[jj][u]) : mul_terms16<Terms<T>::own, LOW>(l, qt[u], acc[jj][u]);
     }
     if (t + 1 == t1 || (next.y & 0xffff) != e) {
       flush(e);
@@ -1261,15 +1284,15 @@ static int launch_outer(OuterArgs a, OuterArgs b, const RowGroups& g, hipStream_
 
 static long round16(long bytes) { return (bytes + 255) & ~255L; }
 
-// Tiles a workgroup of outer_kernel takes: as many as leave about 512 workgroups; a group that spans several chunks costs a
-// partial sum in each.
-#ifndef OUTER_WANT
-#define OUTER_WANT 512
-#endif
-static int outer_chunk(long tiles, int KQ, int r, bool f32) {
+// Tiles a workgroup of outer_kernel takes.  Enough workgroups (512) come first; where groups are long, each chunk that one
+// spans costs a partial sum, and half as many workgroups are better (4099 rows of 24 adapters, chunks of 2 / 4 tiles: product
+// and join 65 / 54 us; 512 rows of 20, 3 / 7 tiles: 23 / 34 us).
+static int outer_chunk(long tiles, int n, int E, int KQ, int r, bool f32) {
   const int cols = 64 * outer_cols(r, f32);
-  const long c = tiles * ((KQ + cols - 1) / cols) / OUTER_WANT;
-  return (int)(c < 1 ? 1 : c);
+  const long work = tiles * ((KQ + cols - 1) / cols), group = n / (32L * E);
+  const long c = work / 512, most = work / 256;
+  const long wish = group < most ? group : most;
+  return (int)(c > wish ? (c < 1 ? 1 : c) : (wish < 1 ? 1 : wish));
 }
 
 // partial sums of outer_kernel: two a chunk
@@ -1309,10 +1332,14 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
   const ShrinkArgs s{dy, b, lddy, (long)N * r, 1, r, N, r, rp, n, ss.kslice, u};
   int rc = launch_shrink<T, true>(s, g, ss.slices, st);
   if (rc) return rc;
-  const int ca = outer_chunk(g.cap, K, r, sizeof(T) == 4), cb = outer_chunk(g.cap, N, r, sizeof(T) == 4);
+  if (ss.slices > 1) {                                               // read many times below: added up once
+    hipLaunchKernelGGL(sum_slices_kernel, dim3((unsigned)(((long)n * rp / 4 + 255) / 256)), dim3(256), 0, st, u, ss.slices, (long)n * rp / 4);
+    FLM_CHECK_LAUNCH();
+  }
+  const int ca = outer_chunk(g.cap, n, E, K, r, sizeof(T) == 4), cb = outer_chunk(g.cap, n, E, N, r, sizeof(T) == 4);
   float *part_a = (float*)ws, *part_b = part_a + outer_part(g.cap, ca) * r * K;
-  if ((rc = launch_outer<T>(OuterArgs{u, ss.slices, rp, 0, (long)n * rp, x, ldx, K, r, E, n, ca, scale, scale_all, part_a, da, K, 1, 0},
-                            OuterArgs{low, 1, r, 1, 0, dy, lddy, N, r, E, n, cb, scale, scale_all, part_b, db, 1, r, 0}, g, st)))
+  if ((rc = launch_outer<T>(OuterArgs{u, rp, 0, x, ldx, K, r, E, n, ca, scale, scale_all, part_a, da, K, 1, 0},
+                            OuterArgs{low, r, 1, dy, lddy, N, r, E, n, cb, scale, scale_all, part_b, db, 1, r, 0}, g, st)))
     return rc;
   if (!dx) return FLM_OK;
   const BasePlan bs = base_plan(n, N, K, sizeof(T) == 4);
@@ -1325,7 +1352,7 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
     w = wt;
     ldw = N;
   }
-  const FinishArgs f{dx_part, bs.slices, 0, nullptr, u, (long)n * rp, ss.slices, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
+  const FinishArgs f{dx_part, bs.slices, 0, nullptr, u, (long)n * rp, 1, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
   return launch_projection<T, true, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, turn, s, ss.slices, true, f, g,
                                           st);
 }
@@ -1348,7 +1375,7 @@ extern "C" long flm_adapter_workspace(int n, int K, int N, int r, int E, int dty
 extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E, int dtype, int need_dx) {
   if (!adapter_sizes(n, K, N, r, E, dtype)) return 0;
   const long tiles = row_tiles_cap(n, E);
-  const int ca = outer_chunk(tiles, K, r, dtype == FLM_F32), cb = outer_chunk(tiles, N, r, dtype == FLM_F32);
+  const int ca = outer_chunk(tiles, n, E, K, r, dtype == FLM_F32), cb = outer_chunk(tiles, n, E, N, r, dtype == FLM_F32);
   long rest = 4L * r * (outer_part(tiles, ca) * K + outer_part(tiles, cb) * N);
   if (need_dx) {
     const BasePlan bs = base_plan(n, N, K, dtype == FLM_F32);
