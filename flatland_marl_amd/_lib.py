@@ -98,6 +98,9 @@ _SIGNATURES = {
     "flm_adapter_backward_workspace": [_i] * 7,
     "flm_adapter_linear_backward": [_p, C.c_long, _p, C.c_long, _p, C.c_long, _p, _p, _p, _p, C.c_float, _p, _i, _i, _i, _i, _i,
                                     _i, _p, _p, C.c_long, _p, _p, _p],
+    "flm_dqn_features_u8": [_p, _p, _i, _i, _i, _i, _i, _p, _p],
+    "flm_dqn_heads": [_p, _p, _i, _i, _i, _i, _p, _p],
+    "flm_dqn_hidden_grads": [_p] * 8 + [C.c_float, _i, _i, _i, _i, _i, _p, _p, _p, _p],
     "flm_grad_clip": [_p, _p, _p, _p, _i, C.c_double, _i, _p, _p, _p],
     "flm_dqn_grad_clip": [_p, _i, _i, _i, _i, _i, _p, C.c_double, _i, _p, _p, _p],
 }

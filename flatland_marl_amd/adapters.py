@@ -96,11 +96,12 @@ def _weights(x, weight, a, b, groups, scale):
         _rows(weight, "weight", k, dev, kind) if weight is not None else 0
 
 
-def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False):
+def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False, out=None):
     """y[i] = weight x[i] + bias + scale[e] * b[e] (a[e] x[i]) for the adapter e of row i (groups = group_rows(ids, E)); rows
     without an adapter get the projection alone.  x [n, K], weight [N, K], bias [N] or None, a [E, r, K], b [E, N, r], all
     of one type (float32, bfloat16, float16); scale: a number or float32 [E].  keep_low: returns (y, low) with low [n, r]
-    float32 = a[e] x[i], which the backward pass takes.  Runs on the current stream; no autograd."""
+    float32 = a[e] x[i], which the backward pass takes.  out: a tensor [n, N] with contiguous rows that receives y (it must
+    not overlap an input).  Runs on the current stream; no autograd."""
     n, k, n_out, r, e, scales, ldx, ldw = _weights(x, weight, a, b, groups, scale)
     if weight.shape[0] != n_out:
         raise ValueError("weight [%d, %d] expected" % (n_out, k))
@@ -108,13 +109,19 @@ def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False):
                              not bias.is_contiguous()):
         raise ValueError("contiguous bias [%d] in the type and on the device of x expected" % n_out)
     dev = x.device
-    y = torch.empty((n, n_out), dtype=x.dtype, device=dev)
+    ldy = n_out
+    if out is None:
+        y = torch.empty((n, n_out), dtype=x.dtype, device=dev)
+    else:
+        y, ldy = out, _rows(out, "out", n_out, dev, x.dtype)
+        if y.shape[0] != n or ldy < n_out:
+            raise ValueError("out [%d, %d] with rows of its own expected" % (n, n_out))
     low = torch.empty((n, r), dtype=torch.float32, device=dev) if keep_low else None
     if n:
         work = torch.empty(size_of("flm_adapter_workspace", n, k, n_out, r, e, DTYPES[x.dtype]), dtype=torch.uint8, device=dev)
         launch(dev, "flm_adapter_linear", x.data_ptr(), ldx, weight.data_ptr(), ldw, bias.data_ptr() if bias is not None else None,
                a.data_ptr(), b.data_ptr(), groups.buf.data_ptr(), *scales, n, k, n_out, r, e, DTYPES[x.dtype], work.data_ptr(),
-               y.data_ptr(), n_out, low.data_ptr() if keep_low else None)
+               y.data_ptr(), ldy, low.data_ptr() if keep_low else None)
     return (y, low) if keep_low else y
 
 
@@ -148,3 +155,111 @@ def adapter_linear_backward(dy, x, weight, a, b, groups, low, scale=1.0, need_dx
            a.data_ptr(), b.data_ptr(), groups.buf.data_ptr(), *scales, low.data_ptr(), n, k, n_out, r, e, kind, work.data_ptr(),
            dx.data_ptr() if need_dx else None, k, da.data_ptr(), db.data_ptr())
     return dx, da, db
+
+
+class NetworkAdapters:
+    """Low-rank adapters of a Dueling_DQN's two first dense layers (98 % of its weights), n_adapters of them: the network is
+    shared, a map (or whatever an id stands for) owns (a, b) of either layer.  All parameters are one flat float32 buffer;
+    a starts uniform within 1/sqrt(inputs), b as zeros, so that a new adapter changes nothing.  scale = alpha / rank
+    (alpha None: 1)."""
+
+    PARTS = ("a_adv", "a_val", "b_adv", "b_val")
+
+    def __init__(self, network, n_adapters, rank, alpha=None):
+        n_adapters, rank = int(n_adapters), int(rank)
+        if not 1 <= n_adapters <= GROUPS_MAX or not 1 <= rank <= ADAPTER_MAX_RANK:
+            raise ValueError("1..%d adapters of rank 1..%d" % (GROUPS_MAX, ADAPTER_MAX_RANK))
+        self.n_adapters, self.rank = n_adapters, rank
+        self.inputs, self.outputs = network.fc1_adv.in_features, network.fc1_adv.out_features
+        self.scale = 1.0 if alpha is None else float(alpha) / rank
+        self.device = network.flat_params().device
+        self.flat = torch.zeros(sum(n for _, n in self._layout()), dtype=torch.float32, device=self.device)
+        views = self.views(self.flat)
+        for name in ("a_adv", "a_val"):
+            views[name].uniform_(-self.inputs ** -0.5, self.inputs ** -0.5)
+        self.__dict__.update(views)
+
+    def _layout(self):
+        e, r, k, n = self.n_adapters, self.rank, self.inputs, self.outputs
+        return [((e, r, k), e * r * k), ((e, r, k), e * r * k), ((e, n, r), e * n * r), ((e, n, r), e * n * r)]
+
+    def views(self, flat):
+        """The four parameters (or their gradients, in a buffer of the same layout) by name."""
+        out, at = {}, 0
+        for name, (shape, n) in zip(self.PARTS, self._layout()):
+            out[name] = flat[at:at + n].view(shape)
+            at += n
+        return out
+
+    def state_dict(self):
+        return {name: getattr(self, name).clone() for name in self.PARTS}
+
+    def load_state_dict(self, state):
+        for name in self.PARTS:
+            if tuple(state[name].shape) != tuple(getattr(self, name).shape):
+                raise ValueError("%s %s expected" % (name, tuple(getattr(self, name).shape)))
+            getattr(self, name).copy_(state[name])
+
+    def copy_for(self, network):
+        """The same adapters, values and scale, beside another network of the same shape (the target network)."""
+        other = NetworkAdapters(network, self.n_adapters, self.rank, self.scale * self.rank)
+        other.flat.copy_(self.flat)
+        return other
+
+    def q_values(self, network, obs_u8, plane_stride, groups, out=None, features=None, keep=False):
+        """Q-values [n, actions] of uint8 observations [n, 3, plane_stride] with the adapters of groups = group_rows(ids,
+        n_adapters), ids the adapter of each observation; observations without one get the network's own values.  All rails
+        are computed.  out: a float32 buffer of at least n rows; features: one of n * inputs floats (both optional).
+        keep: returns (q, what gradients() takes)."""
+        if network.height % 3:
+            raise ValueError("observations have three planes: the network height must be 3*max_rails")
+        n = obs_u8.shape[0]
+        if obs_u8.dtype != torch.uint8 or tuple(obs_u8.shape[1:]) != (3, plane_stride) or not obs_u8.is_contiguous():
+            raise ValueError("contiguous uint8 observations [n, 3, plane_stride] expected")
+        flat = network.flat_params()
+        q = torch.empty((n, network.action_space), dtype=torch.float32, device=flat.device) if out is None else out[:n]
+        x = torch.empty(n * self.inputs, dtype=torch.float32, device=flat.device) if features is None else features
+        x = x[:n * self.inputs].view(n, self.inputs)
+        hidden = torch.empty((n, 2 * self.outputs), dtype=torch.float32, device=flat.device)
+        if n:
+            launch(flat.device, "flm_dqn_features_u8", flat.data_ptr(), obs_u8.data_ptr(), n, network.height // 3, network.width,
+                   int(plane_stride), network.action_space, x.data_ptr())
+            half = self.outputs
+            res = [adapter_linear(x, layer.weight.data, layer.bias.data, a, b, groups, scale=self.scale, keep_low=keep, out=y)
+                   for layer, a, b, y in ((network.fc1_adv, self.a_adv, self.b_adv, hidden[:, :half]),
+                                          (network.fc1_val, self.a_val, self.b_val, hidden[:, half:]))]
+            launch(flat.device, "flm_dqn_heads", flat.data_ptr(), hidden.data_ptr(), n, network.height, network.width,
+                   network.action_space, q.data_ptr())
+        if not keep:
+            return q
+        return q, (x, hidden, groups, res[0][1], res[1][1])
+
+    def gradients(self, kept, dhidden, grads):
+        """The adapters' gradients from the gradient dhidden [n, 1024] of the layers' pre-activations, into the flat buffer
+        grads; kept: from q_values."""
+        x, _, groups, low_adv, low_val = kept
+        into, half = self.views(grads), self.outputs
+        for dy, low, part in ((dhidden[:, :half], low_adv, "adv"), (dhidden[:, half:], low_val, "val")):
+            adapter_linear_backward(dy, x, None, getattr(self, "a_" + part), getattr(self, "b_" + part), groups, low, scale=self.scale,
+                                    need_dx=False, da=into["a_" + part], db=into["b_" + part])
+
+
+class AdapterAdam:
+    """torch.optim.Adam (default options) over the flat parameters of a NetworkAdapters (flm_dqn_adam).  An adapter without
+    rows in a step has a zero gradient; its moments decay and move it as Adam's do."""
+
+    def __init__(self, adapters, lr, betas=(0.9, 0.999), eps=1e-8):
+        self.adapters, self.lr, self.betas, self.eps = adapters, lr, betas, eps
+        self.m, self.v, self.grads = (torch.zeros_like(adapters.flat) for _ in range(3))
+        self.step_count = 0
+
+    def step(self, target=None, tau=None):
+        """One step with self.grads; with target (the target's NetworkAdapters) and tau its soft update in the same pass."""
+        self.step_count += 1
+        p = self.adapters.flat
+        args = [t.data_ptr() for t in (p, self.grads, self.m, self.v)]
+        hyper = (float(self.lr), float(self.betas[0]), float(self.betas[1]), float(self.eps), self.step_count)
+        if target is None:
+            launch(p.device, "flm_dqn_adam", *args, p.numel(), *hyper)
+        else:
+            launch(p.device, "flm_dqn_adam_soft_update", *args, target.flat.data_ptr(), p.numel(), *hyper, float(tau))

@@ -1,7 +1,7 @@
 """Drop-in for the reference's DQNAgent and ReplayBuffer (src/agent.py:17-198).
 
 Same constructor arguments (args.prediction_depth, lr, buffer_size, batch_size, update_every, gamma,
-tau), methods and attributes.  Forward, loss, backward, Adam and the soft update are HIP kernels over flat
+tau), methods and attributes; args.max_grad_norm, if there, bounds the gradient's global norm.  Forward, loss, backward, Adam and the soft update are HIP kernels over flat
 fp32 parameter buffers; with more than one process the gradient is averaged over ranks (one all-reduce
 of the flat buffer) before the optimizer step.
 """
@@ -13,7 +13,9 @@ import numpy as np
 import torch
 
 from . import parallel
-from ._lib import call, ptr, query
+from ._lib import GRAD_WORKSPACE, call, launch, ptr, query
+from .adapters import AdapterAdam, NetworkAdapters, group_rows
+from .gradients import clip_grad_norm_
 from .model import Dueling_DQN
 from .replay import DeviceReplay
 
@@ -81,6 +83,23 @@ class FlatAdam:
         self._ensure()
         return self._uniform_from is not None and self._uniform_from <= int(rails4)
 
+    def clip_grad_norm_(self, max_norm, rails=None):
+        """Scales the gradient so that its global norm is at most max_norm; returns the norm it had (a float32 tensor [],
+        nothing waited for).  rails: as for step(), when the learn step left the packed form; the gradient under the empty
+        rows, which step() forms itself, counts in the norm and is scaled with the bias gradient it is formed from."""
+        self._ensure()
+        net, dev = self.network, self.grads.device
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        work = torch.empty(GRAD_WORKSPACE, dtype=torch.float64, device=dev)
+        if rails is not None:
+            Rp, T1, NA, rails4, rcb, packed = rails
+            if not packed:
+                raise ValueError("the used rails' gradient lies among rows that were not written: only the packed form can be clipped")
+            launch(dev, "flm_dqn_grad_clip", ptr(self.grads), int(Rp), int(T1), int(NA), int(rails4), 1, ptr(rcb), float(max_norm), 0,
+                   ptr(work), norm.data_ptr())
+            return norm
+        return clip_grad_norm_(self.grads, max_norm)
+
     def step(self, target=None, tau=None, rails=None):
         """One Adam step; with target (the target network's flat parameters) and tau also its soft update with
         the new parameters, in the same pass.  rails = (Rp, T1, NA, rails4, rcb, packed): the learn step ran over the
@@ -141,18 +160,68 @@ class DQNAgent:
         self.optimizer = FlatAdam(self.qnetwork_local, lr=self.args.lr)
         self.memory = ReplayBuffer(action_space, self.args.buffer_size, self.args.batch_size, self.width, self.height)
         self.t_step = 0
-        self.last_loss = None
+        self.last_loss = self.last_grad_norm = None
         self._ws = None
+        # bound of the gradient's global norm (args.max_grad_norm; None, as in the reference: not clipped)
+        self.max_grad_norm = getattr(args, "max_grad_norm", None)
+        self.adapters = self.adapters_target = self.adapter_optimizer = None
 
     def save(self, filename):
         torch.save(self.qnetwork_local.state_dict(), filename + ".local")
         torch.save(self.qnetwork_target.state_dict(), filename + ".target")
+        if self.adapters is not None:
+            torch.save({"local": self.adapters.state_dict(), "target": self.adapters_target.state_dict()}, filename + ".adapters")
 
     def load(self, filename):
         if os.path.exists(filename + ".local"):
             self.qnetwork_local.load_state_dict(torch.load(filename + ".local", weights_only=True))
         if os.path.exists(filename + ".target"):
             self.qnetwork_target.load_state_dict(torch.load(filename + ".target", weights_only=True))
+        if self.adapters is not None and os.path.exists(filename + ".adapters"):
+            state = torch.load(filename + ".adapters", weights_only=True)
+            self.adapters.load_state_dict(state["local"])
+            self.adapters_target.load_state_dict(state["target"])
+
+    def attach_adapters(self, n_adapters, rank, alpha=None, lr=None):
+        """Low-rank adapters beside the networks' first dense layers: from now on learn_adapters() trains them (Adam, lr or
+        the agent's) and the networks stay as they are.  Returns the local network's NetworkAdapters."""
+        self.adapters = NetworkAdapters(self.qnetwork_local, n_adapters, rank, alpha)
+        self.adapters_target = self.adapters.copy_for(self.qnetwork_target)
+        self.adapter_optimizer = AdapterAdam(self.adapters, self.args.lr if lr is None else lr)
+        return self.adapters
+
+    def learn_adapters(self, experiences, ids, gamma, plane_stride):
+        """One learn step (src/agent.py:94-118) of the adapters alone, on uint8 observations [B, 3, plane_stride]: ids [B] is
+        the adapter each transition belongs to (any value outside 0..n_adapters-1: none, the transition teaches nothing).
+        The networks are not changed; the adapters' gradient is averaged over the ranks, clipped (max_grad_norm) and
+        applied, and the target's adapters follow softly."""
+        states, actions, rewards, next_states, dones = experiences
+        ad, opt = self.adapters, self.adapter_optimizer
+        if ad is None:
+            raise ValueError("attach_adapters() first")
+        B, net = states.size(0), self.qnetwork_local
+        dev = net.flat_params().device
+        groups = group_rows(ids, ad.n_adapters)
+        s, sn = states.contiguous(), next_states.contiguous()
+        q, kept = ad.q_values(net, s, plane_stride, groups, keep=True)
+        q_next = ad.q_values(net, sn, plane_stride, groups) if self.double_dqn else None
+        q_target = self.adapters_target.q_values(self.qnetwork_target, sn, plane_stride, groups)
+        a = actions.to(dev, torch.int64).contiguous()
+        r = rewards.to(dev, torch.float32).contiguous()
+        d = dones.to(dev, torch.float32).contiguous()
+        hidden = kept[1]
+        dhidden = torch.empty_like(hidden)
+        loss = torch.empty(1, dtype=torch.float32, device=dev)
+        work = torch.empty((2 * self.action_space + 2) * B, dtype=torch.float32, device=dev)
+        launch(dev, "flm_dqn_hidden_grads", ptr(net.flat_params()), ptr(hidden), ptr(q), ptr(q_next), ptr(q_target), ptr(a), ptr(r),
+               ptr(d), float(gamma), 1 if self.double_dqn else 0, B, self.height, self.width, self.action_space, ptr(work),
+               ptr(dhidden), ptr(loss))
+        ad.gradients(kept, dhidden, opt.grads)
+        parallel.allreduce_mean_(opt.grads)
+        if self.max_grad_norm is not None:
+            self.last_grad_norm = clip_grad_norm_(opt.grads, self.max_grad_norm)
+        self.last_loss = loss
+        opt.step(self.adapters_target, self.args.tau)
 
     def step(self, state, action, reward, next_state, done, train=True):
         self.memory.add(state, action, reward, next_state, done)
@@ -194,6 +263,8 @@ class DQNAgent:
                 ptr(self.optimizer.grads), ptr(loss))
         self._grads_and_exchange("flm_dqn_learn_grads", args, st)
         self.last_loss = loss
+        if self.max_grad_norm is not None:
+            self.last_grad_norm = self.optimizer.clip_grad_norm_(self.max_grad_norm)
         self._update(target)
 
     def learn_obs(self, experiences, gamma, plane_stride, rails_used=0):
@@ -229,6 +300,7 @@ class DQNAgent:
         rails4 = query("flm_dqn_learn_rails", B, Rp, self.width, int(rails_used))
         fused = rails4 > 0 and type(self).soft_update is DQNAgent.soft_update and 512 * 64 * self.height < (1 << 24)
         packed = fused and self.optimizer.compact_for(Rp, self.width, self.action_space, rails4)
+        fused = fused and (packed or self.max_grad_norm is None)     # (a gradient with rows left out cannot be clipped)
         args = (ptr(local), ptr(target), ptr(s), ptr(sn), int(plane_stride), ptr(a), ptr(r), ptr(d),
                 float(gamma), 1 if self.double_dqn else 0, B, Rp, self.width, self.action_space, int(rails_used),
                 ptr(self._ws), ptr(self.optimizer.grads), ptr(loss), (2 if packed else 0) if fused else 1)
@@ -237,9 +309,13 @@ class DQNAgent:
         self.last_loss = loss
         if fused:
             off = query("flm_dqn_learn_rails_rcb_offset", B, Rp, self.width, self.action_space)
-            self.optimizer.step(target=target, tau=self.args.tau,
-                                rails=(Rp, self.width, self.action_space, rails4, self._ws[off:off + 64], packed))
+            rails = (Rp, self.width, self.action_space, rails4, self._ws[off:off + 64], packed)
+            if self.max_grad_norm is not None:
+                self.last_grad_norm = self.optimizer.clip_grad_norm_(self.max_grad_norm, rails=rails)
+            self.optimizer.step(target=target, tau=self.args.tau, rails=rails)
         else:
+            if self.max_grad_norm is not None:
+                self.last_grad_norm = self.optimizer.clip_grad_norm_(self.max_grad_norm)
             self._update(target)
 
     def _grads_and_exchange(self, entry, args, stream, phased_entry=False, packed_cols=0):

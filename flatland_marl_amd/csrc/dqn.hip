@@ -892,6 +892,14 @@ __global__ __launch_bounds__(1024) void td_loss_plain_kernel(const float* __rest
   }
 }
 
+__global__ __launch_bounds__(256) void relu_kernel(float4* x, long n4) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n4) return;
+  float4 v = x[i];                                   // (as the fused forms clamp: a NaN becomes 0)
+  v.x = v.x > 0.f ? v.x : 0.f; v.y = v.y > 0.f ? v.y : 0.f; v.z = v.z > 0.f ? v.z : 0.f; v.w = v.w > 0.f ? v.w : 0.f;
+  x[i] = v;
+}
+
 __global__ __launch_bounds__(64) void mean_kernel(const float* __restrict__ x, int n, float* __restrict__ out) {
   float s = 0.f;
   for (int i = threadIdx.x; i < n; i += 64) s += x[i];
@@ -2262,6 +2270,49 @@ extern "C" int flm_dqn_forward_u8(const float* params, const uint8_t* obs, int n
   float* hid = workspace + (long)n * 64 * H3;
   float* part = hid + (long)n * 1024;
   return dqn_forward_impl(params, nullptr, obs, plane_stride, n, H3, T1, NA, x1, hid, part, q, (hipStream_t)stream);
+}
+
+extern "C" int flm_dqn_features_u8(const float* params, const uint8_t* obs, int n, int Rp, int T1, int plane_stride, int NA,
+                                   float* features, void* stream) {
+  if (!params || !obs || !features || n <= 0 || Rp <= 0 || T1 <= 0 || (long)plane_stride < (long)Rp * T1 || !actions_ok(NA))
+    return FLM_E_ARG;
+  return dqn_conv_stage(params, nullptr, obs, plane_stride, n, 3 * Rp, T1, NA, features, (hipStream_t)stream);
+}
+
+extern "C" int flm_dqn_heads(const float* params, float* hidden, int B, int H3, int T1, int NA, float* q, void* stream) {
+  if (!params || !hidden || !q || B <= 0 || H3 <= 0 || T1 <= 0 || !actions_ok(NA) || ((uintptr_t)hidden & 15)) return FLM_E_ARG;
+  const DqnLayout L(H3, T1, NA);
+  hipLaunchKernelGGL(flm::relu_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream, reinterpret_cast<float4*>(hidden),
+                     (long)B * 256);
+  FLM_CHECK_LAUNCH();
+  hipLaunchKernelGGL(flm::head_forward_kernel, dim3(B), dim3(64), 0, (hipStream_t)stream, hidden, params + L.a2_w, params + L.a2_b,
+                     params + L.v2_w, params + L.v2_b, B, NA, q);
+  FLM_CHECK_LAUNCH();
+  return FLM_OK;
+}
+
+extern "C" int flm_dqn_hidden_grads(const float* params, const float* hidden, const float* q, const float* q_next,
+                                    const float* q_target, const int64_t* action, const float* reward, const float* done,
+                                    float gamma, int double_dqn, int B, int H3, int T1, int NA, float* workspace, float* dhidden,
+                                    float* loss_out, void* stream) {
+  if (!params || !hidden || !q || !q_target || (double_dqn && !q_next) || !action || !reward || !done || !workspace || !dhidden ||
+      !loss_out || B <= 0 || H3 <= 0 || T1 <= 0 || !actions_ok(NA))
+    return FLM_E_ARG;
+  const DqnLayout L(H3, T1, NA);
+  hipStream_t st = (hipStream_t)stream;
+  float *dq = workspace, *dadv = dq + (long)NA * B, *dval = dadv + (long)NA * B, *sq = dval + B;
+  if (double_dqn)
+    hipLaunchKernelGGL(flm::td_loss_kernel, dim3((B + 255) / 256), dim3(256), 0, st, q, q_next, q_target, action, reward, done, gamma,
+                       B, NA, dq, sq, (float*)nullptr);
+  else
+    hipLaunchKernelGGL(flm::td_loss_plain_kernel, dim3(1), dim3(1024), 0, st, q, q_target, action, reward, done, gamma, B, NA, dq, sq);
+  FLM_CHECK_LAUNCH();
+  hipLaunchKernelGGL(flm::mean_kernel, dim3(1), dim3(64), 0, st, sq, B, loss_out);
+  FLM_CHECK_LAUNCH();
+  hipLaunchKernelGGL(flm::head_backward_hidden_kernel, dim3(B), dim3(64), 0, st, hidden, dq, params + L.a2_w, params + L.v2_w, B, NA,
+                     dhidden, dadv, dval);
+  FLM_CHECK_LAUNCH();
+  return FLM_OK;
 }
 
 extern "C" int flm_dqn_forward_u8_rails(const float* params, const uint8_t* obs, int n, int Rp, int T1, int plane_stride,

@@ -31,14 +31,31 @@ class DeviceReplay:
         self.head = 0
         self.seed = int(seed) & 0xFFFFFFFF
         self.draws = 0
+        self.group = None                                  # per transition, if the caller tells some apart (keep_groups)
         self._out = None
 
     def __len__(self):
         return self.size
 
-    def add(self, state, action, reward, next_state, done):
+    def keep_groups(self):
+        """From now on every transition has a group (an int32, -1 = none): add(groups=), store_step(groups_of_env=) set it,
+        sampled_groups() returns it.  Those already stored have none."""
+        if self.group is None:
+            # (one place more than the ring: where kernels leave a transition out, its group goes there)
+            self.group = torch.full((self.capacity + 1,), -1, dtype=torch.int32, device=self.device)
+
+    def sampled_groups(self):
+        """The groups [batch] of the last sample()'s transitions."""
+        return self.group.index_select(0, self._out[5].long())
+
+    def add(self, state, action, reward, next_state, done, groups=None):
         """Append n transitions (oldest entries are overwritten, as with deque(maxlen))."""
         n = state.shape[0]
+        if self.group is not None:
+            if groups is None:
+                groups = torch.full((n,), -1, dtype=torch.int32, device=self.device)
+            at = (torch.arange(max(0, n - self.capacity), n, device=self.device) - max(0, n - self.capacity) + self.head) % self.capacity
+            self.group[at] = groups.to(self.device, torch.int32)[max(0, n - self.capacity):]
         if n > self.capacity:
             state, action, reward, next_state, done = (x[-self.capacity:] for x in (state, action, reward, next_state, done))
             n = self.capacity
@@ -52,12 +69,13 @@ class DeviceReplay:
         self.head = (self.head + n) % self.capacity
         self.size = min(self.capacity, self.size + n)
 
-    def store_step(self, ro, req_ready, req_switch, sel_row, obs):
+    def store_step(self, ro, req_ready, req_switch, sel_row, obs, groups_of_env=None):
         """The default feeding mode of the training script (src/main.py:275-278) for one rollout step of every
         environment: the agents req_ready + req_switch that acted on row sel_row[i] >= 0 of obs [rows,3,plane_stride]
         are stored with the decision left by the crash checks, the step's reward and done flag, and their
         observation on the planes after the step, which flm_observations_req_columns_rows writes straight into
-        the ring.  Returns the number of transitions (one host read-back)."""
+        the ring.  groups_of_env [E] int32 (with keep_groups): the group of every environment's transitions.  Returns the
+        number of transitions (one host read-back)."""
         n1, n2 = req_ready.numel(), req_switch.numel()
         n = n1 + n2
         dev = self.device
@@ -75,6 +93,12 @@ class DeviceReplay:
              ptr(self._count), ro.stream)
         call("flm_observations_req_columns_rows", ptr(ro.cols), ptr(self._req), ptr(self._slot), n, ro.E, ro.A, b.Rp, b.T1,
              b.plane_stride, ptr(self.next_state), ro.stream)
+        if self.group is not None:
+            with torch.cuda.stream(ro.b.stream):
+                slot = self._slot[:n].long()
+                env = torch.div(self._req[:n], ro.A, rounding_mode="floor").long()
+                groups = groups_of_env[env] if groups_of_env is not None else torch.full_like(self._req[:n], -1)
+                self.group.index_copy_(0, torch.where(slot < 0, self.capacity, slot), groups)
         self._count_event.record(ro.b.stream)
         self._count_event.synchronize()
         k = int(self._count[0])
@@ -88,6 +112,8 @@ class DeviceReplay:
         every environment: flm_replay_store_slots.  req_ready / req_switch / sel_row / obs are None when nobody
         consulted the network.  `slots` holds the per-agent state (curr_obs, has_curr, buf_obs, has_buf, buf_rew)
         and the two flags.  Returns the number of transitions (one host read-back)."""
+        if self.group is not None:
+            raise ValueError("transitions have groups in the default feeding mode only")
         n1 = req_ready.numel() if req_ready is not None else 0
         n2 = req_switch.numel() if req_switch is not None else 0
         n = n1 + n2

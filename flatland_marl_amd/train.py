@@ -25,6 +25,7 @@ import torch
 
 from . import parallel
 from ._lib import call, ptr, query
+from .adapters import group_rows
 from .replay import DeviceReplay
 from .rollout import MAX_REQ, RolloutBatch
 
@@ -44,9 +45,10 @@ class DQNPolicy:
     agent and of every alternative of every agent in front of a switch, then the epsilon-greedy choice on the
     device (flm_policy_select).  `last` holds what the replay memory needs: a list with one group
     (agents e*A+a, their observations as shown to the network, the actions chosen).  `raw` are views of buffers
-    that the next call overwrites."""
+    that the next call overwrites.  adapter_of_env [E] int32: the agent's adapter (DQNAgent.attach_adapters) each
+    environment's decisions are taken with, -1 = the network alone; None: no adapters."""
 
-    def __init__(self, agent, eps=0.0, seed=0, chunk_bytes=2 << 30):
+    def __init__(self, agent, eps=0.0, seed=0, chunk_bytes=2 << 30, adapter_of_env=None):
         if agent.action_space != 2:                        # the rollout's decision is stop (0) or go (1), src/main.py:163-213
             raise ValueError("the rollout's policy chooses between two actions; the agent has %d" % agent.action_space)
         self.agent = agent
@@ -57,6 +59,28 @@ class DQNPolicy:
         self._last = None
         self._flat = self._sel = self._pool = None
         self._pool_limit = 0
+        if adapter_of_env is not None and agent.adapters is None:
+            raise ValueError("the agent has no adapters: attach_adapters() first")
+        self.adapter_of_env = adapter_of_env
+        self._features = None
+
+    def _adapted_q_values(self, ro, obs_u8, agents, out):
+        """q_values() with every row's environment's adapter; agents [n]: e*A + a of each row."""
+        b, n, ad = ro.b, obs_u8.shape[0], self.agent.adapters
+        net = self.agent.qnetwork_local
+        q = torch.empty((n, net.action_space), dtype=torch.float32, device=obs_u8.device) if out is None else out[:n]
+        chunk = max(1, min(1 << 20, self.chunk_bytes // (4 * ad.inputs)))
+        with torch.cuda.stream(b.stream):                  # (the observations were written on the rollout's stream)
+            ids = self.adapter_of_env[torch.div(agents, ro.A, rounding_mode="floor").long()]
+            rows = min(n, chunk)
+            if self._features is None or self._features.numel() < rows * ad.inputs:
+                self._features = None
+                self._features = torch.empty((rows + rows // 4) * ad.inputs, dtype=torch.float32, device=obs_u8.device)
+            for lo in range(0, n, chunk):
+                hi = min(n, lo + chunk)
+                ad.q_values(net, obs_u8[lo:hi], b.plane_stride, group_rows(ids[lo:hi], ad.n_adapters), out=q[lo:hi],
+                            features=self._features)
+        return q
 
     def q_values(self, ro, obs_u8, out=None, flat=None):
         b = ro.b
@@ -122,7 +146,7 @@ class DQNPolicy:
                 # what the forward pass needs apart from the number of rows is put together before the wait, so that
                 # the launch follows it at once (the same call as Dueling_DQN.forward_obs makes)
                 net_l, b = self.agent.qnetwork_local, ro.b
-                fast = rows_max <= max(1, self.chunk_bytes // (64 * 3 * b.Rp * 4))
+                fast = self.adapter_of_env is None and rows_max <= max(1, self.chunk_bytes // (64 * 3 * b.Rp * 4))
                 if fast:
                     head = (ptr(flat), ptr(obs_pool))
                     tail = (b.Rp, net_l.width, b.plane_stride, net_l.action_space, ro.rails_used(),
@@ -146,7 +170,10 @@ class DQNPolicy:
             self._pool_limit = ro.b.plane_stride            # (whole planes written)
         if rows == 0:                                       # agents before a switch, none with an alternative
             return net, best
-        q = q_pool[:rows] if q_done else self.q_values(ro, obs, out=q_pool, flat=flat)
+        if self.adapter_of_env is not None:
+            q = self._adapted_q_values(ro, obs, req1 if alt is None else alt["row_req"][:rows], q_pool)
+        else:
+            q = q_pool[:rows] if q_done else self.q_values(ro, obs, out=q_pool, flat=flat)
         sel_row, sel_act = self._sel[0][:n1 + n2], self._sel[1][:n1 + n2]
         call("flm_policy_select", ptr(q), ptr(req1) if n1 else None, n1, ptr(req2) if n2 else None, n2,
              ptr(alt["row_offset"]) if alt is not None else None, ptr(alt["count"]) if alt is not None else None,
@@ -175,7 +202,9 @@ class DQNPolicy:
 class BatchedTrainer:
     def __init__(self, rollout: RolloutBatch, agent, replay_capacity=None, max_steps=200, start_eps=1.0, end_eps=0.005,
                  eps_decay=0.998, crash_penalty=False, switch2switch=False, max_learns_per_step=None, seed=0,
-                 strict=False):
+                 strict=False, adapter_of_env=None):
+        """adapter_of_env [E] (integers): decisions are taken with the agent's adapter of each environment (-1: none) and the
+        learn steps train the adapters alone (DQNAgent.attach_adapters, learn_adapters), in the default feeding mode."""
         self.ro = rollout
         self.agent = agent
         b = rollout.b
@@ -184,7 +213,15 @@ class BatchedTrainer:
                              % (agent.height, agent.width, 3 * b.Rp, b.T1))
         cap = replay_capacity or agent.args.buffer_size
         self.replay = DeviceReplay(cap, (3, b.plane_stride), rollout.device, seed=seed + 1)
-        self.policy = DQNPolicy(agent, eps=start_eps, seed=seed)
+        if adapter_of_env is not None:
+            adapter_of_env = torch.as_tensor(adapter_of_env).to(rollout.device, torch.int32)
+            if adapter_of_env.shape != (rollout.E,):
+                raise ValueError("adapter_of_env [%d] expected" % rollout.E)
+            if crash_penalty or switch2switch:
+                raise ValueError("adapters are trained in the default feeding mode only")
+            self.replay.keep_groups()
+        self.adapter_of_env = adapter_of_env
+        self.policy = DQNPolicy(agent, eps=start_eps, seed=seed, adapter_of_env=adapter_of_env)
         self.max_steps = max_steps
         self.eps, self.end_eps, self.eps_decay = start_eps, end_eps, eps_decay
         self.crash_penalty = crash_penalty
@@ -210,6 +247,11 @@ class BatchedTrainer:
 
     def _learn(self):
         b = self.ro.b
+        if self.adapter_of_env is not None:
+            batch = self.replay.sample(self.agent.args.batch_size)
+            self.agent.learn_adapters(batch, self.replay.sampled_groups(), self.agent.args.gamma, b.plane_stride)
+            self.n_learn += 1
+            return
         # every observation in the memory comes from this batch of environments: rails beyond its largest count are
         # empty, neither gathered nor computed
         # (of anything ever stored; with several ranks the largest over the ranks, agreed on in step(): the ranks' learn
@@ -231,7 +273,7 @@ class BatchedTrainer:
             raw = self.policy.raw
             if raw is not None:
                 req1, req2, obs, sel_row, _ = raw
-                n_new = self.replay.store_step(ro, req1, req2, sel_row, obs)
+                n_new = self.replay.store_step(ro, req1, req2, sel_row, obs, groups_of_env=self.adapter_of_env)
         elif train:
             # crash penalty (src/main.py:271-273) and switch-to-switch (src/main.py:280-296): the observation each
             # agent last acted on, and the one kept since its last "go", live in per-agent slots on the device

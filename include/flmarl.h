@@ -666,6 +666,22 @@ int flm_adapter_linear_backward(const void* dy, long lddy, const void* x, long l
                                 int n, int K, int N, int r, int E, int dtype, void* workspace, void* dx, long lddx, void* da,
                                 void* db, void* stream);
 
+/* The pieces of the network around its first dense layers, for a caller that forms these itself (flm_adapter_linear with
+ * the network's own weights and an adapter per map; src/model.py:31-43, src/agent.py:94-114):
+ *   flm_dqn_features_u8   features [n, 64*3*Rp] = relu(convolution) of uint8 observations [n,3,plane_stride], all rails
+ *   flm_dqn_heads         hidden [B,1024] in: the two layers' pre-activations (advantage stream first), out: their ReLU
+ *                         (16-byte aligned); q [B,NA] out
+ *   flm_dqn_hidden_grads  loss_out [1] and dhidden [B,1024] = its gradient w.r.t. the pre-activations, from hidden (after
+ *                         flm_dqn_heads) and the Q-values of the states (q), of the next states by the local network
+ *                         (q_next, only with double_dqn) and by the target network (q_target); the loss as in
+ *                         flm_dqn_learn_grads.  workspace: (2*NA + 2) * B floats */
+int flm_dqn_features_u8(const float* params, const uint8_t* obs, int n, int Rp, int T1, int plane_stride, int NA,
+                        float* features, void* stream);
+int flm_dqn_heads(const float* params, float* hidden, int B, int H3, int T1, int NA, float* q, void* stream);
+int flm_dqn_hidden_grads(const float* params, const float* hidden, const float* q, const float* q_next, const float* q_target,
+                         const int64_t* action, const float* reward, const float* done, float gamma, int double_dqn, int B,
+                         int H3, int T1, int NA, float* workspace, float* dhidden, float* loss_out, void* stream);
+
 /* Global norm of many gradient tensors and clipping: norm = sqrt(sum of all squares) (inf_norm != 0: the largest
  * absolute value), dst = src * min(1, max_norm / (norm + 1e-6)).
  *   src, dst, numel, dtype: HOST arrays of count device pointers, element counts and FLM_F32 / FLM_BF16 / FLM_F16;
