@@ -11,19 +11,17 @@
 // largest); the narrow products low and u stay fp32 in memory and enter the next product as two bf16 terms beside bf16 or
 // fp16 operands (2^-17 of the value, far below the rounding of the result).
 #include "flm_adapters.h"
+#include "flm_gemm_x3.h"
 
 namespace flm {
 
-// the split-operand fp32 product of the dense layers (dqn.hip): C[slice][M,N] = A[M,K] * B over the K slices;
-// B is [N,K] (b_kc) or [K,N]
+// C[slice][M,N] = A[M,K] * B over K slices with the fp32 product of the dense layers (dqn.hip); B is [N,K] (b_kc) or [K,N]
 int gemm_x3_slices(const float* A, long lda, const float* B, long ldb, bool b_kc, float* C, int M, int N, int K, int slices,
                    int kslice, hipStream_t stream);
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // ---- eight consecutive elements, at any alignment the type allows ------------------------------------------------
@@ -243,8 +241,8 @@ __device__ __forceinline__ void mini_product(const T* const (&xr)[MR], const T* 
   }
 }
 
-// sums the four waves' results; f(mi, ni, values) is called by one wave per pair
-template <int MR, int NR, typename F>
+// sums the PARTS waves' results; f(mi, ni, values) is called by one wave per pair.  red: PARTS * MR * NR * 64 of LDS
+template <int MR, int NR, int PARTS, typename F>
 __device__ __forceinline__ void mini_meet(const f32x4 (&acc)[MR][NR], f32x4* red, F&& f) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
@@ -252,10 +250,10 @@ __device__ __forceinline__ void mini_meet(const f32x4 (&acc)[MR][NR], f32x4* red
 #pragma unroll
     for (int ni = 0; ni < NR; ni++) red[(w * MR * NR + mi * NR + ni) * 64 + lane] = acc[mi][ni];
   __syncthreads();
-  for (int s = w; s < MR * NR; s += 4) {
+  for (int s = w; s < MR * NR; s += PARTS) {
     f32x4 v = red[s * 64 + lane];
 #pragma unroll
-    for (int k = 1; k < 4; k++) v += red[(k * MR * NR + s) * 64 + lane];
+    for (int k = 1; k < PARTS; k++) v += red[(k * MR * NR + s) * 64 + lane];
     f(s / NR, s - s / NR * NR, v);
   }
 }
@@ -267,15 +265,15 @@ struct ShrinkArgs {
   float* out;                            // [slice][sorted position][rp]; what lies behind r is not meant to be read
 };
 
-// low (or u): tiles of rows of one adapter times its r vectors; grid (tiles, K slices)
-template <typename T, int MR, int NR, bool V_STRIDED>
-__global__ __launch_bounds__(256) void shrink_kernel(ShrinkArgs a, RowGroups g) {
-  __shared__ f32x4 red[4 * MR * NR * 64];
-  const int2 tile = g.tiles[blockIdx.x];
+// low (or u) of row tile t: its 16*MR rows times ranks rank .. rank + 16*NR - 1 of their adapter, over one K slice.
+// A workgroup of PARTS waves; red: PARTS * MR * NR * 64 of LDS
+template <typename T, int MR, int NR, int S, int PARTS, bool V_STRIDED>
+__device__ __forceinline__ void shrink_tile(const ShrinkArgs& a, const RowGroups& g, int t, int slice, int rank, f32x4* red) {
+  const int2 tile = g.tiles[t];
   const int rows = tile.y >> 16, e = tile.y & 0xffff;
   if (rows == 0) return;
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int k_begin = blockIdx.y * a.kslice, k_end = min(a.K, k_begin + a.kslice);
+  const int k_begin = slice * a.kslice, k_end = min(a.K, k_begin + a.kslice);
   const T *xr[MR], *vr[NR];
 #pragma unroll
   for (int mi = 0; mi < MR; mi++) {
@@ -284,16 +282,22 @@ __global__ __launch_bounds__(256) void shrink_kernel(ShrinkArgs a, RowGroups g) 
   }
 #pragma unroll
   for (int ni = 0; ni < NR; ni++) {
-    const int j = min(ni * 16 + c, a.r - 1);
+    const int j = min(rank + ni * 16 + c, a.r - 1);
     vr[ni] = (const T*)a.v + (long)e * a.v_group + (long)j * a.v_row;
   }
   f32x4 acc[MR][NR];
-  mini_product<T, MR, NR, (MR + NR <= 4 ? 2 : 1), V_STRIDED>(xr, vr, a.v_k, k_begin, k_end, acc, threadIdx.x >> 6, 4);
-  mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
-    const int m = mi * 16 + c, j = ni * 16 + 4 * q;
-    if (m < rows && j < a.rp)
-      *reinterpret_cast<f32x4*>(a.out + ((long)blockIdx.y * a.n + tile.x + m) * a.rp + j) = v;
+  mini_product<T, MR, NR, S, V_STRIDED>(xr, vr, a.v_k, k_begin, k_end, acc, threadIdx.x >> 6, PARTS);
+  mini_meet<MR, NR, PARTS>(acc, red, [&](int mi, int ni, const f32x4& v) {
+    const int m = mi * 16 + c, j = rank + ni * 16 + 4 * q;
+    if (m < rows && j < a.rp) *reinterpret_cast<f32x4*>(a.out + ((long)slice * a.n + tile.x + m) * a.rp + j) = v;
   });
+}
+
+// grid (tiles, K slices)
+template <typename T, int NR, bool V_STRIDED>
+__global__ __launch_bounds__(256) void shrink_kernel(ShrinkArgs a, RowGroups g) {
+  __shared__ f32x4 red[4 * 2 * NR * 64];
+  shrink_tile<T, 2, NR, (NR <= 2 ? 2 : 1), 4, V_STRIDED>(a, g, blockIdx.x, blockIdx.y, 0, red);
 }
 
 struct BaseArgs {
@@ -306,7 +310,7 @@ struct BaseArgs {
 // Up to 64 rows: the projection (16*MR rows x 16*NR outputs a workgroup) and the narrow products (32 rows x 16 ranks) in one
 // launch.  The first base_groups workgroups are (output block, K slice) pairs of the projection, the others (tile, K slice,
 // rank block) of the narrow product: at these sizes both are streams of weights with little else to do.
-template <typename T, int MRS, int MR, int NR, bool V_STRIDED>
+template <typename T, int MRS, int MR, int NR>
 __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s, RowGroups g, int base_groups, int low_slices) {
   __shared__ f32x4 red[4 * (MR * NR > MRS ? MR * NR : MRS) * 64];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
@@ -321,7 +325,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s,
     for (int ni = 0; ni < NR; ni++) vr[ni] = (const T*)a.w + (long)min(n0 + ni * 16 + c, a.N - 1) * a.ldw;
     f32x4 acc[MR][NR];
     mini_product<T, MR, NR, 2, false>(xr, vr, 1, k_begin, k_end, acc, threadIdx.x >> 6, 4);
-    mini_meet<MR, NR>(acc, red, [&](int mi, int ni, const f32x4& v) {
+    mini_meet<MR, NR, 4>(acc, red, [&](int mi, int ni, const f32x4& v) {
       const int m = mi * 16 + c, n = n0 + ni * 16 + 4 * q;
       if (m < a.n) {
         const float f[4] = {v[0], v[1], v[2], v[3]};
@@ -329,24 +333,8 @@ __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s,
       }
     });
   } else {
-    const int i = blockIdx.x - base_groups, rest = i / g.cap, rank = rest / low_slices * 16, slice = rest % low_slices;
-    const int2 tile = g.tiles[i - rest * g.cap];
-    const int rows = tile.y >> 16, e = tile.y & 0xffff;
-    if (rows == 0) return;
-    const int k_begin = slice * s.kslice, k_end = min(s.K, k_begin + s.kslice);
-    const T *xr[MRS], *vr[1];
-#pragma unroll
-    for (int mi = 0; mi < MRS; mi++) {
-      const int m = min(mi * 16 + c, rows - 1);
-      xr[mi] = (const T*)s.x + (long)g.order[tile.x + m] * s.ldx;
-    }
-    vr[0] = (const T*)s.v + (long)e * s.v_group + (long)min(rank + c, s.r - 1) * s.v_row;
-    f32x4 acc[MRS][1];
-    mini_product<T, MRS, 1, 2, V_STRIDED>(xr, vr, s.v_k, k_begin, k_end, acc, threadIdx.x >> 6, 4);
-    mini_meet<MRS, 1>(acc, red, [&](int mi, int, const f32x4& v) {
-      const int m = mi * 16 + c;
-      if (m < rows) *reinterpret_cast<f32x4*>(s.out + ((long)slice * s.n + tile.x + m) * s.rp + rank + 4 * q) = v;
-    });
+    const int i = blockIdx.x - base_groups, rest = i / g.cap;
+    shrink_tile<T, MRS, 1, 2, 4, false>(s, g, i - rest * g.cap, rest % low_slices, rest / low_slices * 16, red);
   }
 }
 
@@ -621,23 +609,22 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
 // A stage's row is 128 bytes; the 16-byte piece p of row r lies at slot p ^ (r & 7), so that the eight rows a group of lanes
 // reads at once fall into different banks.  The weight is the instruction's first operand: a lane then holds one row's
 // outputs, four consecutive ones at a time.
-// part == nullptr: with bias and adapters, straight to y.  Otherwise one K slice per blockIdx.z to part[slice][position][N].
+// FUSED: with bias and adapters, straight to y.  Otherwise one K slice to part[slice][position][N].
+// li: the workgroup's index among the tiles; lds: wide_lds_bytes()
 #define WIDE_K 64
-template <typename T, int BM, int BN, int WM, int WN, bool V_STRIDED>
-__global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, FinishArgs a, RowGroups g) {
+template <typename T, int BM, int BN, int WM, int WN, bool FUSED, bool V_STRIDED>
+__device__ __forceinline__ void wide_tile(const BaseArgs& b, const FinishArgs& a, const RowGroups& g, unsigned li, int slice, char* lds) {
   constexpr int NT = 64 * WM * WN, MI = BM / (32 * WM), NI = BN / (32 * WN), RX = BM * 8 / NT, RW = BN * 8 / NT;
   constexpr int STAGE = (BM + BN) * 128;                  // bytes
-  extern __shared__ __attribute__((aligned(16))) char lds[];
   typedef typename Operand<T>::V V;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, h = lane >> 5;
   const int wm = w / WN, wn = w % WN;
   // workgroups go round-robin to the 8 XCDs: consecutive tiles of one XCD share eight row tiles' and a few column tiles' data
-  unsigned li = blockIdx.x;
   const unsigned tm = (b.n + BM - 1) / BM, tn = (b.N + BN - 1) / BN, nwg = tm * tn;
   if ((nwg & 7) == 0) li = (li & 7) * (nwg >> 3) + (li >> 3);
   const unsigned band = li / (8 * tn), rows_in_band = min(8u, tm - band * 8), in_band = li - band * 8 * tn;
   const int m0 = (band * 8 + in_band % rows_in_band) * BM, n0 = (in_band / rows_in_band) * BN;
-  const int k_begin = blockIdx.y * b.kslice, k_end = min(b.K, k_begin + b.kslice);
+  const int k_begin = slice * b.kslice, k_end = min(b.K, k_begin + b.kslice);
   // (rows behind the last are fetched from the last: their results are not stored)
   const T *xp[RX], *wp[RW];
   const int piece = tid & 7;
@@ -729,7 +716,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
     }
   }
   const int nw = n0 + wn * (BN / WN);
-  if (!b.part) {
+  if constexpr (FUSED) {
     int key[MI];
 #pragma unroll
     for (int mi = 0; mi < MI; mi++) {
@@ -760,7 +747,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
       for (int r4 = 0; r4 < 4; r4++) {
         const int n = wn * (BN / WN) + 32 * ni + 8 * r4 + 4 * h;
         float bias[4] = {0.f, 0.f, 0.f, 0.f};
-        if (!b.part && a.bias) {
+        if (FUSED && a.bias) {
 #pragma unroll
           for (int i = 0; i < 4; i++)
             if (n0 + n + i < b.N) bias[i] = (float)((const T*)a.bias)[n0 + n + i];
@@ -778,7 +765,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
       const int m = i / PER, n = n0 + (i - m * PER) * (16 / (int)sizeof(O));
       if (m0 + m >= b.n || n >= b.N) continue;
       const uint4 v = *reinterpret_cast<const uint4*>(lds + m * ROW + (i - m * PER) * 16);
-      O* p = out + (long)(b.part ? m0 + m : g.order[m0 + m]) * ld + n;
+      O* p = out + (long)(FUSED ? g.order[m0 + m] : m0 + m) * ld + n;
       struct __attribute__((packed, aligned(sizeof(O)))) Piece { unsigned w[4]; };
       if (n + 16 / (int)sizeof(O) <= b.N) {
         *reinterpret_cast<Piece*>(p) = Piece{{v.x, v.y, v.z, v.w}};
@@ -790,8 +777,45 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
       }
     }
   };
-  if (b.part) store_tile(b.part + (long)blockIdx.y * b.n * b.N, (long)b.N, 0.f);
-  else store_tile((T*)a.y, a.ldy, (T)0.f);
+  if constexpr (FUSED) store_tile((T*)a.y, a.ldy, (T)0.f);
+  else store_tile(b.part + (long)slice * b.n * b.N, (long)b.N, 0.f);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool V_STRIDED>
+__global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, FinishArgs a, RowGroups g) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  wide_tile<T, BM, BN, WM, WN, true, V_STRIDED>(b, a, g, blockIdx.x, 0, lds);
+}
+
+// K slices of the projection, and beside them the narrow products (ranks in blocks of 16*NR), in one launch: the products of
+// the first `tiles` * slices workgroups keep the matrix cores busy, the others mostly wait for memory.
+template <typename T, int NR>
+__global__ __launch_bounds__(256, 2) void parts_kernel(BaseArgs b, ShrinkArgs s, RowGroups g, int tiles, int slices, int low_slices) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int i = (int)blockIdx.x - tiles * slices;
+  if (i < 0) {
+    const int slice = blockIdx.x / tiles;
+    wide_tile<T, 128, 128, 2, 2, false, false>(b, FinishArgs{}, g, blockIdx.x - slice * tiles, slice, lds);
+  } else {
+    const int rest = i / g.cap;
+    shrink_tile<T, 2, NR, (NR <= 2 ? 2 : 1), 4, false>(s, g, i - rest * g.cap, rest % low_slices, rest / low_slices * 16 * NR,
+                                                       reinterpret_cast<f32x4*>(lds));
+  }
+}
+
+// the same for fp32: the first gx * gy * gz workgroups are the dense layers' product over K slices
+template <int NR>
+__global__ __launch_bounds__(512, 4) void x3_parts_kernel(GemmArgs p, unsigned gx, unsigned gy, unsigned gz, ShrinkArgs s, RowGroups g,
+                                                          int low_slices) {
+  extern __shared__ __attribute__((aligned(16))) unsigned x3_lds[];
+  const int i = (int)blockIdx.x - (int)(gx * gy * gz);
+  if (i < 0) {
+    gemm_x3_body<true, true, EPI_PLAIN>(p, blockIdx.x, gx, gy, gz, x3_lds);
+  } else {
+    const int rest = i / g.cap;
+    shrink_tile<float, 2, NR, 1, 8, false>(s, g, i - rest * g.cap, rest % low_slices, rest / low_slices * 16 * NR,
+                                           reinterpret_cast<f32x4*>(x3_lds));
+  }
 }
 
 // part[0] = sum of the K slices part[z], n4 float4 each
@@ -1164,37 +1188,72 @@ static ShrinkPlan shrink_plan(int n, int K, int E) {
 template <typename T, bool V_STRIDED>
 static int launch_shrink(const ShrinkArgs& a, const RowGroups& g, int slices, hipStream_t st) {
   const dim3 grid(g.cap, slices);
-  if (a.rp <= 16) hipLaunchKernelGGL((shrink_kernel<T, 2, 1, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-  else if (a.rp <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, 2, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-  else if (a.rp <= 64) hipLaunchKernelGGL((shrink_kernel<T, 2, 4, V_STRIDED>), grid, dim3(256), 0, st, a, g);
-  else hipLaunchKernelGGL((shrink_kernel<T, 2, 8, V_STRIDED>), grid, dim3(256), 0, st, a, g);
+  if (a.rp <= 16) hipLaunchKernelGGL((shrink_kernel<T, 1, V_STRIDED>), grid, dim3(256), 0, st, a, g);
+  else if (a.rp <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, V_STRIDED>), grid, dim3(256), 0, st, a, g);
+  else if (a.rp <= 64) hipLaunchKernelGGL((shrink_kernel<T, 4, V_STRIDED>), grid, dim3(256), 0, st, a, g);
+  else hipLaunchKernelGGL((shrink_kernel<T, 8, V_STRIDED>), grid, dim3(256), 0, st, a, g);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
 
-// the projection's K slices and the narrow product's of up to 64 rows
-template <typename T, bool V_STRIDED>
+// the projection's K slices and (low_slices > 0) the narrow product's of up to 64 rows
+template <typename T>
 static int launch_few_rows(const BaseArgs& a, int base_slices, const ShrinkArgs& s, int low_slices, const RowGroups& g, hipStream_t st) {
   const int cols = a.n <= 16 ? 16 : 32, base_groups = (a.N + cols - 1) / cols * base_slices;
   const dim3 grid(base_groups + g.cap * low_slices * (s.rp / 16));
-  if (a.n <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, 1, 1, V_STRIDED>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
-  else if (a.n <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, 2, 2, V_STRIDED>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
-  else if (a.n <= 48) hipLaunchKernelGGL((few_rows_kernel<T, 2, 3, 2, V_STRIDED>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
-  else hipLaunchKernelGGL((few_rows_kernel<T, 2, 4, 2, V_STRIDED>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
+  if (a.n <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, 1, 1>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
+  else if (a.n <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, 2, 2>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
+  else if (a.n <= 48) hipLaunchKernelGGL((few_rows_kernel<T, 2, 3, 2>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
+  else hipLaunchKernelGGL((few_rows_kernel<T, 2, 4, 2>), grid, dim3(256), 0, st, a, s, g, base_groups, low_slices);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool V_STRIDED>
-static int launch_wide(const BaseArgs& b, int slices, const FinishArgs& f, const RowGroups& g, hipStream_t st) {
+static int launch_wide(const BaseArgs& b, const FinishArgs& f, const RowGroups& g, hipStream_t st) {
   FLM_RAISE_LDS_ONCE((base_wide_kernel<T, BM, BN, WM, WN, V_STRIDED>));
-  size_t lds = 2 * (BM + BN) * 128;
-  const size_t tail = (size_t)Terms<T>::low * BM * (f.rp + 8) * 2;
-  if (!b.part && tail > lds) lds = tail;
-  const size_t out = (size_t)BM * (BN * (b.part ? 4 : sizeof(T)) + 16);
+  size_t lds = 2 * (BM + BN) * 128;                                  // two stages; the narrow products' terms; the result
+  const size_t tail = (size_t)Terms<T>::low * BM * (f.rp + 8) * 2, out = (size_t)BM * (BN * sizeof(T) + 16);
+  if (tail > lds) lds = tail;
   if (out > lds) lds = out;
-  hipLaunchKernelGGL((base_wide_kernel<T, BM, BN, WM, WN, V_STRIDED>),
-                     dim3(((b.n + BM - 1) / BM) * ((b.N + BN - 1) / BN), slices), dim3(64 * WM * WN), lds, st, b, f, g);
+  hipLaunchKernelGGL((base_wide_kernel<T, BM, BN, WM, WN, V_STRIDED>), dim3(((b.n + BM - 1) / BM) * ((b.N + BN - 1) / BN)),
+                     dim3(64 * WM * WN), lds, st, b, f, g);
+  FLM_CHECK_LAUNCH();
+  return FLM_OK;
+}
+
+// K slices of the projection with W [N,K] into b.part and, with low_slices > 0, the narrow products beside them.  low: the
+// grouping of all rows (g may be a window of it)
+template <typename T>
+static int launch_parts(const BaseArgs& b, int slices, const RowGroups& g, const ShrinkArgs& s, int low_slices, hipStream_t st) {
+  const int nr = s.rp <= 16 ? 1 : 2, ranks = (s.rp + 16 * nr - 1) / (16 * nr);
+  const int low = g.cap * low_slices * ranks;
+  if constexpr (sizeof(T) == 4) {
+    GemmArgs p{};
+    p.A = (const float*)b.x; p.B = (const float*)b.w; p.C = b.part;
+    p.M = b.n; p.N = b.N; p.K = b.K; p.lda = b.ldx; p.ldb = b.ldw; p.ldc = b.N;
+    p.ksplit = slices > 1 ? b.kslice : 0; p.c_zs = (long)b.n * b.N;
+    const unsigned gx = (b.N + GBN - 1) / GBN, gy = (b.n + GBM - 1) / GBM;
+    const dim3 grid(gx * gy * slices + low);
+    if (nr == 1) {
+      FLM_RAISE_LDS_ONCE(x3_parts_kernel<1>);
+      hipLaunchKernelGGL(x3_parts_kernel<1>, grid, dim3(512), X3_LDS_BYTES, st, p, gx, gy, (unsigned)slices, s, g, low_slices);
+    } else {
+      FLM_RAISE_LDS_ONCE(x3_parts_kernel<2>);
+      hipLaunchKernelGGL(x3_parts_kernel<2>, grid, dim3(512), X3_LDS_BYTES, st, p, gx, gy, (unsigned)slices, s, g, low_slices);
+    }
+  } else {
+    const int tiles = ((b.n + 127) / 128) * ((b.N + 127) / 128);
+    const size_t lds = 128 * (128 * 4 + 16);                         // (the stages take 64 KiB, the result a little more)
+    const dim3 grid(tiles * slices + low);
+    if (nr == 1) {
+      FLM_RAISE_LDS_ONCE((parts_kernel<T, 1>));
+      hipLaunchKernelGGL((parts_kernel<T, 1>), grid, dim3(256), lds, st, b, s, g, tiles, slices, low_slices);
+    } else {
+      FLM_RAISE_LDS_ONCE((parts_kernel<T, 2>));
+      hipLaunchKernelGGL((parts_kernel<T, 2>), grid, dim3(256), lds, st, b, s, g, tiles, slices, low_slices);
+    }
+  }
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
@@ -1215,32 +1274,33 @@ static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st
   return FLM_OK;
 }
 
-// The narrow product and y = X * W^T + bias + adapters, any type and size.  w_nk: W is [N,K]; otherwise [K,N] (fp32 through
-// BASE_X3 only).  low_done: s has been formed already.  f.part / b.part: base_part_bytes() of workspace
-template <typename T, bool V_STRIDED, bool S_STRIDED>
-static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const ShrinkArgs& s, int low_slices, bool low_done,
-                             FinishArgs f, const RowGroups& g, hipStream_t st) {
+// The narrow product (low_slices = 0: it is there already) and y = X * W^T + bias + adapters, any type and size.  w_nk: W is
+// [N,K]; otherwise [K,N] (fp32 through BASE_X3 only).  f.part / b.part: base_part_bytes() of workspace
+template <typename T, bool V_STRIDED>
+static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const ShrinkArgs& s, int low_slices, FinishArgs f,
+                             const RowGroups& g, hipStream_t st) {
   if (plan.form == BASE_ROWS) {
-    // (a narrow product that is there already is not formed again: no workgroups for it)
-    RowGroups tiles = g;
-    if (low_done) tiles.cap = 0;
-    const int rc = launch_few_rows<T, S_STRIDED>(b, plan.slices, s, low_slices, tiles, st);
+    const int rc = launch_few_rows<T>(b, plan.slices, s, low_slices, g, st);
     if (rc) return rc;
-  } else {
-    int rc = low_done ? FLM_OK : launch_shrink<T, S_STRIDED>(s, g, low_slices, st);
-    if (rc) return rc;
+  } else if (plan.form == BASE_X3) {
     if constexpr (sizeof(T) == 4) {
-      if ((rc = gemm_x3_slices((const float*)b.x, b.ldx, (const float*)b.w, b.ldw, w_nk, b.part, b.n, b.N, b.K, plan.slices,
-                               b.kslice, st)))
-        return rc;
-    } else {
+      // (W [K,N] comes from the backward pass only, whose narrow product is there already)
+      const int rc = w_nk ? launch_parts<float>(b, plan.slices, g, s, low_slices, st)
+                          : gemm_x3_slices((const float*)b.x, b.ldx, (const float*)b.w, b.ldw, false, b.part, b.n, b.N, b.K, plan.slices,
+                                           b.kslice, st);
+      if (rc) return rc;
+    }
+  } else {
+    if constexpr (sizeof(T) != 4) {
+      const bool beside = plan.rows == 0 && plan.slices > 1;         // nothing needs low before it is through
+      int rc = low_slices == 0 || beside ? FLM_OK : launch_shrink<T, false>(s, g, low_slices, st);
+      if (rc) return rc;
       if (plan.rows) {
         BaseArgs large = b;
         FinishArgs fl = f;
         large.n = fl.n = plan.rows;
-        large.part = nullptr;
         large.kslice = b.K;
-        if ((rc = launch_wide<T, 256, 256, 2, 4, V_STRIDED>(large, 1, fl, g, st))) return rc;
+        if ((rc = launch_wide<T, 256, 256, 2, 4, V_STRIDED>(large, fl, g, st))) return rc;
         if (plan.rows == b.n) return FLM_OK;
       }
       // the rows behind: the same with the sorted positions from plan.rows on
@@ -1250,9 +1310,8 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const 
       b.n = f.n = b.n - plan.rows;
       f.low += (long)plan.rows * f.rp;
       f.part_sorted = 1;
-      if (plan.slices == 1) b.part = nullptr;
-      rc = launch_wide<T, 128, 128, 2, 2, V_STRIDED>(b, plan.slices, f, rest, st);
-      if (rc || !b.part) return rc;
+      if (plan.slices == 1) return launch_wide<T, 128, 128, 2, 2, V_STRIDED>(b, f, rest, st);
+      if ((rc = launch_parts<T>(b, plan.slices, rest, s, beside ? low_slices : 0, st))) return rc;
       return launch_finish<T, V_STRIDED>(f, rest, st);
     }
   }
@@ -1310,8 +1369,8 @@ static int forward(const void* x, long ldx, const void* w, long ldw, const void*
   const ShrinkArgs s{x, a, ldx, (long)r * K, K, 1, K, r, rp, n, ss.kslice, low_part};
   const FinishArgs f{part, bs.slices, 0, bias, low_part, (long)n * rp, ss.slices, r, rp, b, (long)N * r, r, 1, scale, scale_all, n, N, E, y, ldy};
   const BaseArgs base{x, w, ldx, ldw, n, K, N, bs.kslice, part};
-  const int rc = r % 8 == 0 ? launch_projection<T, false, false>(base, bs, true, s, ss.slices, false, f, g, st)
-                            : launch_projection<T, true, false>(base, bs, true, s, ss.slices, false, f, g, st);
+  const int rc = r % 8 == 0 ? launch_projection<T, false>(base, bs, true, s, ss.slices, f, g, st)
+                            : launch_projection<T, true>(base, bs, true, s, ss.slices, f, g, st);
   if (rc) return rc;
   if (low) {
     hipLaunchKernelGGL(low_rows_kernel, dim3((unsigned)(((long)n * rp + 255) / 256)), dim3(256), 0, st, low_part, ss.slices, n, r,
@@ -1353,8 +1412,7 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
     ldw = N;
   }
   const FinishArgs f{dx_part, bs.slices, 0, nullptr, u, (long)n * rp, 1, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
-  return launch_projection<T, true, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, turn, s, ss.slices, true, f, g,
-                                          st);
+  return launch_projection<T, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, turn, s, 0, f, g, st);
 }
 
 }  // namespace flm
