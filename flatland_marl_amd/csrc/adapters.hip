@@ -425,14 +425,16 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
 // added to its own rows only, so that no value of one adapter (an infinity, a NaN) can reach the rows of another.
 // key[mi]: the lane's adapter (E: none), ascending over the rows.  V comes straight from memory (the L2): NB adapters and
 // 16*JB ranks at a time, so that NB*JB loads are in flight; start() fetches the first of them, before the narrow products are
-// staged if the caller likes.  All lanes of the wave take part.
+// staged if the caller likes.  Waves that hold the same tile may share its adapters.  All lanes of the wave take part.
 template <typename T, bool V_STRIDED, int MI, int JB, int NB>
 struct AddAdapters {
-  int es[NB], j0;
+  int es[NB], j0, seen;
   unsigned todo[MI];
   Vec8<T> v[NB][JB];
+  int turn = 0, share = 1;                 // this wave takes the adapters whose number in the tile is turn modulo share
 
   __device__ __forceinline__ void restart(const FinishArgs& a, const int (&key)[MI]) {
+    seen = 0;
 #pragma unroll
     for (int mi = 0; mi < MI; mi++) todo[mi] = (unsigned)__ballot(key[mi] < a.E);   // (both halves of the wave: the same rows)
   }
@@ -441,12 +443,15 @@ struct AddAdapters {
     const int lane = threadIdx.x & 63, n = min(n0 + (lane & 31), a.N - 1), h = lane >> 5;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      es[b] = -1;
+      do {
+        es[b] = -1;
 #pragma unroll
-      for (int mi = 0; mi < MI; mi++)
-        if (es[b] < 0 && todo[mi]) es[b] = __builtin_amdgcn_readlane(key[mi], __builtin_ctz(todo[mi]));
+        for (int mi = 0; mi < MI; mi++)
+          if (es[b] < 0 && todo[mi]) es[b] = __builtin_amdgcn_readlane(key[mi], __builtin_ctz(todo[mi]));
 #pragma unroll
-      for (int mi = 0; mi < MI; mi++) todo[mi] &= ~(unsigned)__ballot(key[mi] == es[b]);
+        for (int mi = 0; mi < MI; mi++) todo[mi] &= ~(unsigned)__ballot(key[mi] == es[b]);
+        seen++;
+      } while (es[b] >= 0 && share > 1 && (seen & (share - 1)) != turn);
     }
 #pragma unroll
     for (int b = 0; b < NB; b++)
@@ -520,7 +525,7 @@ struct AddAdapters {
 };
 
 // y = sum of the K slices + bias + adapters: 32 sorted rows and 32 outputs a wave, or (SHARED) a workgroup of four waves
-// that take the K slices in turn and meet in LDS.
+// that take the K slices and the adapters in turn and meet in LDS.
 template <typename T, bool V_STRIDED, bool SHARED>
 __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) {
   extern __shared__ __attribute__((aligned(16))) __bf16 lt[];
@@ -552,7 +557,11 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
     for (int r = 0; r < 16; r++) acc[0][r] += f[r >> 2].v[r & 3];
   };
   AddAdapters<T, V_STRIDED, 1, 2, 2> add;
-  if (!SHARED || w == 0) add.start(a, key, n0);
+  if (SHARED) {
+    add.turn = w;
+    add.share = 4;
+  }
+  add.start(a, key, n0);
   if (whole) {
     int z = first;
     for (; z + 3 * stride < a.slices; z += 4 * stride) {
@@ -574,16 +583,20 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
   for (int o = span; o < 32; o <<= 1)
 #pragma unroll
     for (int r = 0; r < 16; r++) acc[0][r] += __shfl_xor(acc[0][r], o);
-  if (SHARED && w > 0)
-#pragma unroll
-    for (int r = 0; r < 16; r++) meet[w - 1][r][lane] = acc[0][r];
   __syncthreads();
-  if (n0 >= a.N || (SHARED && w > 0)) return;
-  if (SHARED)
+  if (n0 < a.N) add.run(a, lt, 32, 0, key, n0, acc);
+  if (SHARED) {
+    if (w > 0)
+#pragma unroll
+      for (int r = 0; r < 16; r++) meet[w - 1][r][lane] = acc[0][r];
+    __syncthreads();
+    if (w > 0) return;
 #pragma unroll
     for (int k = 0; k < 3; k++)
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[0][r] += meet[k][r][lane];
+  }
+  if (n0 >= a.N) return;
   if (a.bias) {
 #pragma unroll
     for (int r = 0; r < 16; r++) {
@@ -591,7 +604,6 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
       if (n < a.N) acc[0][r] += (float)((const T*)a.bias)[n];
     }
   }
-  add.run(a, lt, 32, 0, key, n0, acc);
   if (in) {
     T* y = (T*)a.y + (long)row * a.ldy;
 #pragma unroll
@@ -1141,7 +1153,9 @@ static BasePlan base_plan(int n, int K, int N, bool f32) {
   if (n <= BASE_ROWS_MAX) {
     b.form = BASE_ROWS;
     const int cols = n <= 16 ? 16 : 32;
-    b.slices = k_slices((N + cols - 1) / cols, 768, K, 512, 32, &b.kslice);
+    // (workgroups measured: one row of 13440 x 512 fp32, 256 / 512 / 768: 10.3 / 9.2 / 10.5 us; 37 rows of 4096 x 4096 bf16:
+    // 13.8 / 15.0 / 14.9)
+    b.slices = k_slices((N + cols - 1) / cols, n <= 16 ? 512 : 256, K, 512, 32, &b.kslice);
     return b;
   }
   if (f32) {
@@ -1175,13 +1189,10 @@ static BasePlan base_plan(int n, int K, int N, bool f32) {
 static long base_part_bytes(const BasePlan& b, int n, int N) {
   return b.form == BASE_TILES && (b.slices == 1 || b.rows == n) ? 0 : 4L * b.slices * (n - b.rows) * N;
 }
-#ifndef SHRINK_WANT
-#define SHRINK_WANT 512
-#endif
 struct ShrinkPlan { int slices, kslice; };
 static ShrinkPlan shrink_plan(int n, int K, int E) {
   ShrinkPlan b;
-  b.slices = k_slices(row_tiles_cap(n, E), SHRINK_WANT, K, 512, 16, &b.kslice);
+  b.slices = k_slices(row_tiles_cap(n, E), 512, K, 512, 16, &b.kslice);
   return b;
 }
 
@@ -1263,10 +1274,12 @@ static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st
   const long tiles = (long)((a.N + 31) / 32) * ((a.n + 31) / 32);
   const size_t lds = (size_t)Terms<T>::low * 32 * (a.rp + 8) * 2;
   const unsigned down = (a.n + 31) / 32;
-  if (tiles <= 1024 && a.slices >= 4) {                               // few tiles and a sum worth sharing
+  // Up to a tile a CU, four waves share each (37 rows of 24 adapters, 4096 outputs: 11.4 -> 8.0 us); up to 1024 a wave each,
+  // spread over the CUs (1001 rows, 515 outputs: 8.7 us, shared 11.9); beyond that four a workgroup
+  if (tiles <= 256) {
     hipLaunchKernelGGL((finish_kernel<T, V_STRIDED, true>), dim3((a.N + 31) / 32, down), dim3(256), lds, st, a, g);
   } else {
-    const int per = tiles <= 1024 ? 1 : 4;                            // (few tiles: one a workgroup, spread over the CUs)
+    const int per = tiles <= 1024 ? 1 : 4;
     hipLaunchKernelGGL((finish_kernel<T, V_STRIDED, false>), dim3((a.N + 32 * per - 1) / (32 * per), down), dim3(64 * per), lds, st, a,
                        g);
   }

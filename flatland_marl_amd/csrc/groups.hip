@@ -14,15 +14,7 @@ namespace flm {
 #define GROUP_RUN 512                    // rows of a wave (at least) in the large form
 #define GROUP_KEYS 8                     // rows a lane holds at a time: their ids are fetched together
 #define GROUP_RUNS_MAX 4096
-
-__device__ __forceinline__ int row_key(const void* ids, int ids64, long i, int E) {
-  if (ids64) {
-    const int64_t v = reinterpret_cast<const int64_t*>(ids)[i];
-    return v >= 0 && v < E ? (int)v : E;
-  }
-  const int v = reinterpret_cast<const int32_t*>(ids)[i];
-  return (unsigned)v < (unsigned)E ? v : E;
-}
+#define GROUP_WAVES 4                    // runs of a workgroup when rows are placed
 
 // lanes of the wave that hold the same key (all 64 lanes take part; bits: bits of a key)
 __device__ __forceinline__ unsigned long long same_key(int key, int bits) {
@@ -57,13 +49,34 @@ __device__ __forceinline__ int block_scan(int v, int* scratch, int* total) {
   return base + inc - v;
 }
 
-// the keys of rows lo + 64*u + lane (E for rows from hi on)
+// The keys of rows lo + 64*u + lane (E for rows from hi on), lo < hi.  All ids are on their way before the first is looked at.
 __device__ __forceinline__ void load_keys(const void* ids, int ids64, long lo, long hi, int E, int (&key)[GROUP_KEYS]) {
   const int lane = threadIdx.x & 63;
+  if (ids64) {
+    int64_t v[GROUP_KEYS];
 #pragma unroll
-  for (int u = 0; u < GROUP_KEYS; u++) {
-    const long i = lo + 64 * u + lane;
-    key[u] = i < hi ? row_key(ids, ids64, i, E) : E;
+    for (int u = 0; u < GROUP_KEYS; u++) v[u] = reinterpret_cast<const int64_t*>(ids)[min(lo + 64 * u + lane, hi - 1)];
+#pragma unroll
+    for (int u = 0; u < GROUP_KEYS; u++) key[u] = lo + 64 * u + lane < hi && v[u] >= 0 && v[u] < E ? (int)v[u] : E;
+  } else {
+    int v[GROUP_KEYS];
+#pragma unroll
+    for (int u = 0; u < GROUP_KEYS; u++) v[u] = reinterpret_cast<const int32_t*>(ids)[min(lo + 64 * u + lane, hi - 1)];
+#pragma unroll
+    for (int u = 0; u < GROUP_KEYS; u++) key[u] = lo + 64 * u + lane < hi && (unsigned)v[u] < (unsigned)E ? v[u] : E;
+  }
+}
+
+// f(i, src[i]) for i = first, first + stride, .. < n, eight loads in flight
+template <typename F>
+__device__ __forceinline__ void each_of(const int* src, int n, int first, int stride, F&& f) {
+  for (int i0 = first; i0 < n; i0 += 8 * stride) {
+    int v[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) v[u] = src[min(i0 + u * stride, n - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (i0 + u * stride < n) f(i0 + u * stride, v[u]);
   }
 }
 
@@ -160,7 +173,7 @@ __global__ __launch_bounds__(1024) void group_small_kernel(const void* ids, int 
   const int run = ((n + nw - 1) / nw + 63) & ~63;
   const int lo = min(n, w * run), hi = min(n, lo + run);
   int key[GROUP_KEYS];
-  load_keys(ids, ids64, lo, hi, E, key);
+  if (lo < hi) load_keys(ids, ids64, lo, hi, E, key);
   for (int i = threadIdx.x; i < nw * E1; i += blockDim.x) cnt[i] = 0;
   __syncthreads();
   count_keys(key, lo, hi, cnt + w * E1);
@@ -250,26 +263,28 @@ __global__ __launch_bounds__(1024) void group_scan_kernel(int* counts, int runs,
   if (w == 0) totals[g] = total;
 }
 
-// four runs a workgroup.  LDS: next [4][E+1], off [E+1], tstart [E+1], scratch [17]
-__global__ __launch_bounds__(256) void group_place_kernel(const void* ids, int ids64, int n, int run, int runs, int E, int bits,
+// GROUP_WAVES runs a workgroup.  LDS: next [GROUP_WAVES][E+1], off [E+1], tstart [E+1], scratch [17]
+__global__ __launch_bounds__(64 * GROUP_WAVES) void group_place_kernel(const void* ids, int ids64, int n, int run, int runs, int E, int bits,
                                                           const int* counts, const int* totals, int* order, int* keys,
                                                           int* offsets, int* first_tile, int2* tiles, int cap) {
   extern __shared__ int lds[];
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, E1 = E + 1;
   int* next = lds;
-  int* off = next + 4 * E1;
+  int* off = next + GROUP_WAVES * E1;
   int* tstart = off + E1;
   int* scratch = tstart + E1;
-  const int r = blockIdx.x * 4 + w;
+  const int r = blockIdx.x * GROUP_WAVES + w;
   int key[GROUP_KEYS];                     // (fetched ahead of the scan)
   if (r < runs) load_keys(ids, ids64, (long)r * run, min((long)n, (long)(r + 1) * run), E, key);
-  for (int g = threadIdx.x; g < E1; g += 256) off[g] = totals[g];
+  constexpr int NT = 64 * GROUP_WAVES;
+  each_of(totals, E1, threadIdx.x, NT, [&](int g, int v) { off[g] = v; });
+  if (r < runs) each_of(counts + (long)r * E1, E1, lane, 64, [&](int g, int v) { next[w * E1 + g] = v; });
   __syncthreads();
   scan_groups(off, tstart, E, scratch);
   if (r < runs)
-    for (int g = lane; g < E1; g += 64) next[w * E1 + g] = off[g] + counts[(long)r * E1 + g];
+    for (int g = lane; g < E1; g += 64) next[w * E1 + g] += off[g];
   if (blockIdx.x == 0)
-    for (int g = threadIdx.x; g < E1; g += 256) {
+    for (int g = threadIdx.x; g < E1; g += NT) {
       offsets[g] = off[g];
       first_tile[g] = tstart[g];
     }
@@ -281,7 +296,7 @@ __global__ __launch_bounds__(256) void group_place_kernel(const void* ids, int i
       place_keys(key, at, hi, bits, next + w * E1, order, keys);
     }
   }
-  write_tiles(off, tstart, E, cap, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, tiles);
+  write_tiles(off, tstart, E, cap, blockIdx.x * NT + threadIdx.x, gridDim.x * NT, tiles);
 }
 
 }  // namespace flm
@@ -333,9 +348,10 @@ extern "C" int flm_group_rows(const void* ids, int ids64, int n, int n_groups, i
   FLM_CHECK_LAUNCH();
   hipLaunchKernelGGL(group_scan_kernel, dim3((E1 + 63) / 64), dim3(1024), 0, st, workspace, runs, E, totals);
   FLM_CHECK_LAUNCH();
-  hipLaunchKernelGGL(group_place_kernel, dim3((runs + 3) / 4), dim3(256), sizeof(int) * (6 * E1 + 17), st, ids, ids64, n, run,
-                     runs, E, bits, workspace, totals, order, keys, offsets, first_tile, tiles,
-                     g.cap);
+  const size_t lds = sizeof(int) * ((size_t)(GROUP_WAVES + 2) * E1 + 17);
+  if (lds > 64 * 1024) FLM_RAISE_LDS_ONCE(group_place_kernel);
+  hipLaunchKernelGGL(group_place_kernel, dim3((runs + GROUP_WAVES - 1) / GROUP_WAVES), dim3(64 * GROUP_WAVES), lds, st, ids, ids64, n,
+                     run, runs, E, bits, workspace, totals, order, keys, offsets, first_tile, tiles, g.cap);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
