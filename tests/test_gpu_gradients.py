@@ -7,7 +7,7 @@ import torch
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 SETS = [[1], [7], [64], [0, 3, 0], [1, 2, 3, 4, 5, 6, 7, 8, 9], [65536], [65537], [5, 70000, 8191, 8192, 8193, 1],
-        [100] * 111, [100] * 112, [100] * 113, [37, 4099] * 200, [3000001, 12], [20000000]]
+        [100] * 111, [100] * 112, [100] * 113, [37, 4099] * 200, [3000001, 12], [20000000], [40000003, 5, 40000000]]
 
 
 def _grads(sizes, kind, seed=0, scale=0.1):
