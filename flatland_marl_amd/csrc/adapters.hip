@@ -293,6 +293,48 @@ __device__ __forceinline__ void shrink_tile(const ShrinkArgs& a, const RowGroups
   });
 }
 
+// Two neighbouring tiles of one adapter at a time (tiles of two adapters one after the other): half the way of the vectors
+// through the L2, which is longer than the rows' from 32 ranks on.  Eight waves; grid (tiles / 2, K slices)
+template <typename T, int NR>
+__global__ __launch_bounds__(512) void shrink_pair_kernel(ShrinkArgs a, RowGroups g) {
+  __shared__ f32x4 red[8 * 2 * NR * 64];
+  const int t = 2 * blockIdx.x;
+  const int2 one = g.tiles[t], two = t + 1 < g.cap ? g.tiles[t + 1] : make_int2(0, 0);
+  if ((one.y >> 16) == 0) return;
+  const int slice = blockIdx.y;
+  if ((two.y >> 16) == 0 || (one.y & 0xffff) != (two.y & 0xffff)) {
+#pragma unroll 1
+    for (int i = 0; i < 2; i++) {
+      if (t + i < g.cap) shrink_tile<T, 2, NR, 1, 8, false>(a, g, t + i, slice, 0, red);
+      __syncthreads();
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, e = one.y & 0xffff, rows = 32 + (two.y >> 16);
+  const int k_begin = slice * a.kslice, k_end = min(a.K, k_begin + a.kslice);
+  const T *xr[4], *vr[NR];
+#pragma unroll
+  for (int mi = 0; mi < 4; mi++) xr[mi] = (const T*)a.x + (long)g.order[one.x + min(mi * 16 + c, rows - 1)] * a.ldx;
+#pragma unroll
+  for (int ni = 0; ni < NR; ni++) vr[ni] = (const T*)a.v + (long)e * a.v_group + (long)min(ni * 16 + c, a.r - 1) * a.v_row;
+  f32x4 acc[4][NR];
+  mini_product<T, 4, NR, 1, false>(xr, vr, 1, k_begin, k_end, acc, threadIdx.x >> 6, 8);
+  // the waves meet in two halves of the rows
+#pragma unroll
+  for (int half = 0; half < 2; half++) {
+    f32x4 part[2][NR];
+#pragma unroll
+    for (int mi = 0; mi < 2; mi++)
+#pragma unroll
+      for (int ni = 0; ni < NR; ni++) part[mi][ni] = acc[2 * half + mi][ni];
+    if (half) __syncthreads();
+    mini_meet<2, NR, 8>(part, red, [&](int mi, int ni, const f32x4& v) {
+      const int m = 32 * half + mi * 16 + c, j = ni * 16 + 4 * q;
+      if (m < rows && j < a.rp) *reinterpret_cast<f32x4*>(a.out + ((long)slice * a.n + one.x + m) * a.rp + j) = v;
+    });
+  }
+}
+
 // grid (tiles, K slices)
 template <typename T, int NR, bool V_STRIDED>
 __global__ __launch_bounds__(256) void shrink_kernel(ShrinkArgs a, RowGroups g) {
@@ -338,22 +380,6 @@ __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s,
   }
 }
 
-// out[C][R] = in[R][C] (the weight with its contraction axis last, for the gradient of the inputs)
-template <typename T>
-__global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ in, long ld, int R, int C, T* __restrict__ out) {
-  __shared__ T t[64][66];
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int r = i >> 6, c = i & 63;
-    if (r0 + r < R && c0 + c < C) t[r][c] = in[(long)(r0 + r) * ld + c0 + c];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int c = i >> 6, r = i & 63;
-    if (r0 + r < R && c0 + c < C) out[(long)(c0 + c) * R + r0 + r] = t[r][c];
-  }
-}
-
 // ---- the adapters' part and the result ---------------------------------------------------------------------------------
 struct FinishArgs {
   const float* part;                     // [slices][n][N]
@@ -389,25 +415,19 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
     if (e < a.E) {
       const float* p = a.low + (pos + row) * a.rp + j;
       const long step = a.low_step;
-      int z = 0;
 #pragma unroll 1
-      for (; z + 8 <= a.low_slices; z += 8) {
+      for (int z = 0; z < a.low_slices; z += 8) {                    // eight slices in flight, the last one again behind the end
         f32x4 v[8][2];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-          v[k][0] = reinterpret_cast<const f32x4*>(p + (z + k) * step)[0];
-          v[k][1] = reinterpret_cast<const f32x4*>(p + (z + k) * step)[1];
+          const float* q = p + min(z + k, a.low_slices - 1) * step;
+          v[k][0] = reinterpret_cast<const f32x4*>(q)[0];
+          v[k][1] = reinterpret_cast<const f32x4*>(q)[1];
         }
 #pragma unroll
         for (int k = 0; k < 8; k++)
 #pragma unroll
-          for (int u = 0; u < 8; u++) f[u] += v[k][u >> 2][u & 3];
-      }
-#pragma unroll 1
-      for (; z < a.low_slices; z++) {
-        const f32x4 v0 = reinterpret_cast<const f32x4*>(p + z * step)[0], v1 = reinterpret_cast<const f32x4*>(p + z * step)[1];
-#pragma unroll
-        for (int u = 0; u < 8; u++) f[u] += u < 4 ? v0[u] : v1[u - 4];
+          for (int u = 0; u < 8; u++) f[u] += z + k < a.low_slices ? v[k][u >> 2][u & 3] : 0.f;
       }
       const float s = adapter_scale(a.scale, a.scale_all, e);
 #pragma unroll
@@ -624,7 +644,10 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
 // FUSED: with bias and adapters, straight to y.  Otherwise one K slice to part[slice][position][N].
 // li: the workgroup's index among the tiles; lds: wide_lds_bytes()
 #define WIDE_K 64
-template <typename T, int BM, int BN, int WM, int WN, bool FUSED, bool V_STRIDED>
+// W_KN: W is [K,N] with contiguous outputs (the gradient of the inputs).  A thread then fetches eight outputs of four
+// consecutive k and turns them in registers; lanes of a wave take the sixteen groups of k first, so that they write whole
+// LDS rows.
+template <typename T, int BM, int BN, int WM, int WN, bool FUSED, bool W_KN, bool V_STRIDED>
 __device__ __forceinline__ void wide_tile(const BaseArgs& b, const FinishArgs& a, const RowGroups& g, unsigned li, int slice, char* lds) {
   constexpr int NT = 64 * WM * WN, MI = BM / (32 * WM), NI = BN / (32 * WN), RX = BM * 8 / NT, RW = BN * 8 / NT;
   constexpr int STAGE = (BM + BN) * 128;                  // bytes
@@ -638,12 +661,16 @@ __device__ __forceinline__ void wide_tile(const BaseArgs& b, const FinishArgs& a
   const int m0 = (band * 8 + in_band % rows_in_band) * BM, n0 = (in_band / rows_in_band) * BN;
   const int k_begin = slice * b.kslice, k_end = min(b.K, k_begin + b.kslice);
   // (rows behind the last are fetched from the last: their results are not stored)
+  static_assert(!W_KN || RW % 4 == 0, "four rows of W a thread");
   const T *xp[RX], *wp[RW];
   const int piece = tid & 7;
 #pragma unroll
   for (int i = 0; i < RX; i++) xp[i] = (const T*)b.x + (long)g.order[min(m0 + (tid >> 3) + i * (NT / 8), b.n - 1)] * b.ldx + piece * 8;
 #pragma unroll
-  for (int i = 0; i < RW; i++) wp[i] = (const T*)b.w + (long)min(n0 + (tid >> 3) + i * (NT / 8), b.N - 1) * b.ldw + piece * 8;
+  for (int i = 0; i < RW; i++) {
+    if (W_KN) wp[i] = (const T*)b.w + (long)(4 * (tid & 15) + (i & 3)) * b.ldw + n0 + 8 * ((tid >> 4) + (NT / 16) * (i >> 2));
+    else wp[i] = (const T*)b.w + (long)min(n0 + (tid >> 3) + i * (NT / 8), b.N - 1) * b.ldw + piece * 8;
+  }
   f32x16 acc[NI][MI];
 #pragma unroll
   for (int ni = 0; ni < NI; ni++)
@@ -656,22 +683,54 @@ __device__ __forceinline__ void wide_tile(const BaseArgs& b, const FinishArgs& a
 #pragma unroll
     for (int i = 0; i < RX; i++) fx[i] = load8(xp[i] + k0, 8);
 #pragma unroll
-    for (int i = 0; i < RW; i++) fw[i] = load8(wp[i] + k0, 8);
+    for (int i = 0; i < RW; i++) fw[i] = load8(W_KN ? wp[i] + (long)k0 * b.ldw : wp[i] + k0, 8);
   };
   auto fetch = [&](int k0) {
     const int avail = k_end - k0 - piece * 8;
 #pragma unroll
     for (int i = 0; i < RX; i++) fx[i] = load8(xp[i] + k0, avail);
 #pragma unroll
-    for (int i = 0; i < RW; i++) fw[i] = load8(wp[i] + k0, avail);
+    for (int i = 0; i < RW; i++) {
+      if (W_KN) {
+        const bool in = k0 + 4 * (tid & 15) + (i & 3) < k_end;
+        fw[i] = load8(wp[i] + (long)k0 * b.ldw, in ? b.N - (n0 + 8 * ((tid >> 4) + (NT / 16) * (i >> 2))) : 0);
+      } else {
+        fw[i] = load8(wp[i] + k0, avail);
+      }
+    }
   };
   const int slot = ((piece ^ ((tid >> 3) & 7)) << 4) + (tid >> 3) * 128;
   auto place = [&](char* st) {
 #pragma unroll
     for (int i = 0; i < RX; i++) *reinterpret_cast<uint4*>(st + slot + i * (NT / 8) * 128) = __builtin_bit_cast(uint4, fx[i]);
+    if constexpr (W_KN) {
 #pragma unroll
-    for (int i = 0; i < RW; i++)
-      *reinterpret_cast<uint4*>(st + BM * 128 + slot + i * (NT / 8) * 128) = __builtin_bit_cast(uint4, fw[i]);
+      for (int i = 0; i < RW; i += 4) {
+        uint4 d[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) d[k] = __builtin_bit_cast(uint4, fw[i + k]);
+        const int row = 8 * ((tid >> 4) + (NT / 16) * (i >> 2)), kg = tid & 15;
+        auto put = [&](int j, unsigned w0, unsigned w1, unsigned w2, unsigned w3) {       // outputs 2j, 2j+1 of the four k
+#pragma unroll
+          for (int o = 0; o < 2; o++) {
+            // (lanes of one instruction write even and odd rows alike, so both halves of the banks)
+            const int odd = o ^ ((tid >> 4) & 1);
+            const unsigned sel = odd ? 0x07060302u : 0x05040100u;
+            const int r = row + 2 * j + odd;
+            *reinterpret_cast<uint2*>(st + BM * 128 + r * 128 + (((kg >> 1) ^ (r & 7)) << 4) + (kg & 1) * 8) =
+                make_uint2(__builtin_amdgcn_perm(w1, w0, sel), __builtin_amdgcn_perm(w3, w2, sel));
+          }
+        };
+        put(0, d[0].x, d[1].x, d[2].x, d[3].x);
+        put(1, d[0].y, d[1].y, d[2].y, d[3].y);
+        put(2, d[0].z, d[1].z, d[2].z, d[3].z);
+        put(3, d[0].w, d[1].w, d[2].w, d[3].w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < RW; i++)
+        *reinterpret_cast<uint4*>(st + BM * 128 + slot + i * (NT / 8) * 128) = __builtin_bit_cast(uint4, fw[i]);
+    }
   };
   auto products = [&](const char* st) {
     const char* sx = st + (wm * (BM / WM) + c) * 128;
@@ -704,7 +763,8 @@ __device__ __forceinline__ void wide_tile(const BaseArgs& b, const FinishArgs& a
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       }
   };
-  const int whole = (k_end - k_begin) / WIDE_K, stages = (k_end - k_begin + WIDE_K - 1) / WIDE_K;
+  // (W_KN: outputs behind the last must not be fetched either)
+  const int whole = W_KN && n0 + BN > b.N ? 0 : (k_end - k_begin) / WIDE_K, stages = (k_end - k_begin + WIDE_K - 1) / WIDE_K;
   if (stages > 0) {
     fetch(k_begin);
     place(lds);
@@ -793,21 +853,21 @@ __device__ __forceinline__ void wide_tile(const BaseArgs& b, const FinishArgs& a
   else store_tile(b.part + (long)slice * b.n * b.N, (long)b.N, 0.f);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool V_STRIDED>
+template <typename T, int BM, int BN, int WM, int WN, bool W_KN, bool V_STRIDED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, FinishArgs a, RowGroups g) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  wide_tile<T, BM, BN, WM, WN, true, V_STRIDED>(b, a, g, blockIdx.x, 0, lds);
+  wide_tile<T, BM, BN, WM, WN, true, W_KN, V_STRIDED>(b, a, g, blockIdx.x, 0, lds);
 }
 
 // K slices of the projection, and beside them the narrow products (ranks in blocks of 16*NR), in one launch: the products of
 // the first `tiles` * slices workgroups keep the matrix cores busy, the others mostly wait for memory.
-template <typename T, int NR>
+template <typename T, int NR, bool W_KN>
 __global__ __launch_bounds__(256, 2) void parts_kernel(BaseArgs b, ShrinkArgs s, RowGroups g, int tiles, int slices, int low_slices) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int i = (int)blockIdx.x - tiles * slices;
   if (i < 0) {
     const int slice = blockIdx.x / tiles;
-    wide_tile<T, 128, 128, 2, 2, false, false>(b, FinishArgs{}, g, blockIdx.x - slice * tiles, slice, lds);
+    wide_tile<T, 128, 128, 2, 2, false, W_KN, false>(b, FinishArgs{}, g, blockIdx.x - slice * tiles, slice, lds);
   } else {
     const int rest = i / g.cap;
     shrink_tile<T, 2, NR, (NR <= 2 ? 2 : 1), 4, false>(s, g, i - rest * g.cap, rest % low_slices, rest / low_slices * 16 * NR,
@@ -1144,13 +1204,14 @@ static double tiles_128_time(int n, int K, int N, int* slices, int* kslice) {
   return cut;
 }
 
-static BasePlan base_plan(int n, int K, int N, bool f32) {
+// w_kn: W is [K,N]: the few-row form is for [N,K] only.
+static BasePlan base_plan(int n, int K, int N, bool f32, bool w_kn = false) {
   BasePlan b;
   b.rows = 0;
   b.slices = 1;
   b.kslice = K;
   const int tn = (N + 255) / 256, tm = (n + 255) / 256;
-  if (n <= BASE_ROWS_MAX) {
+  if (n <= BASE_ROWS_MAX && !w_kn) {
     b.form = BASE_ROWS;
     const int cols = n <= 16 ? 16 : 32;
     // (workgroups measured: one row of 13440 x 512 fp32, 256 / 512 / 768: 10.3 / 9.2 / 10.5 us; 37 rows of 4096 x 4096 bf16:
@@ -1198,6 +1259,16 @@ static ShrinkPlan shrink_plan(int n, int K, int E) {
 
 template <typename T, bool V_STRIDED>
 static int launch_shrink(const ShrinkArgs& a, const RowGroups& g, int slices, hipStream_t st) {
+  if constexpr (!V_STRIDED) {
+    // pairs where they still leave a workgroup a CU, from 32 ranks (16384 rows of 4096, 64 ranks: 70 -> 60 us)
+    if (g.cap >= 512 && a.rp > 16 && a.rp <= 64) {
+      const dim3 pairs((g.cap + 1) / 2, slices);
+      if (a.rp <= 32) hipLaunchKernelGGL((shrink_pair_kernel<T, 2>), pairs, dim3(512), 0, st, a, g);
+      else hipLaunchKernelGGL((shrink_pair_kernel<T, 4>), pairs, dim3(512), 0, st, a, g);
+      FLM_CHECK_LAUNCH();
+      return FLM_OK;
+    }
+  }
   const dim3 grid(g.cap, slices);
   if (a.rp <= 16) hipLaunchKernelGGL((shrink_kernel<T, 1, V_STRIDED>), grid, dim3(256), 0, st, a, g);
   else if (a.rp <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, V_STRIDED>), grid, dim3(256), 0, st, a, g);
@@ -1220,53 +1291,46 @@ static int launch_few_rows(const BaseArgs& a, int base_slices, const ShrinkArgs&
   return FLM_OK;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool V_STRIDED>
+template <typename T, int BM, int BN, int WM, int WN, bool W_KN, bool V_STRIDED>
 static int launch_wide(const BaseArgs& b, const FinishArgs& f, const RowGroups& g, hipStream_t st) {
-  FLM_RAISE_LDS_ONCE((base_wide_kernel<T, BM, BN, WM, WN, V_STRIDED>));
+  FLM_RAISE_LDS_ONCE((base_wide_kernel<T, BM, BN, WM, WN, W_KN, V_STRIDED>));
   size_t lds = 2 * (BM + BN) * 128;                                  // two stages; the narrow products' terms; the result
   const size_t tail = (size_t)Terms<T>::low * BM * (f.rp + 8) * 2, out = (size_t)BM * (BN * sizeof(T) + 16);
   if (tail > lds) lds = tail;
   if (out > lds) lds = out;
-  hipLaunchKernelGGL((base_wide_kernel<T, BM, BN, WM, WN, V_STRIDED>), dim3(((b.n + BM - 1) / BM) * ((b.N + BN - 1) / BN)),
+  hipLaunchKernelGGL((base_wide_kernel<T, BM, BN, WM, WN, W_KN, V_STRIDED>), dim3(((b.n + BM - 1) / BM) * ((b.N + BN - 1) / BN)),
                      dim3(64 * WM * WN), lds, st, b, f, g);
   FLM_CHECK_LAUNCH();
   return FLM_OK;
 }
 
-// K slices of the projection with W [N,K] into b.part and, with low_slices > 0, the narrow products beside them.  low: the
-// grouping of all rows (g may be a window of it)
-template <typename T>
-static int launch_parts(const BaseArgs& b, int slices, const RowGroups& g, const ShrinkArgs& s, int low_slices, hipStream_t st) {
-  const int nr = s.rp <= 16 ? 1 : 2, ranks = (s.rp + 16 * nr - 1) / (16 * nr);
-  const int low = g.cap * low_slices * ranks;
+template <typename T, int NR, bool W_KN>
+static int launch_parts_ranks(const BaseArgs& b, int slices, const RowGroups& g, const ShrinkArgs& s, int low_slices, hipStream_t st) {
+  const int low = g.cap * low_slices * ((s.rp + 16 * NR - 1) / (16 * NR));
   if constexpr (sizeof(T) == 4) {
     GemmArgs p{};
     p.A = (const float*)b.x; p.B = (const float*)b.w; p.C = b.part;
     p.M = b.n; p.N = b.N; p.K = b.K; p.lda = b.ldx; p.ldb = b.ldw; p.ldc = b.N;
     p.ksplit = slices > 1 ? b.kslice : 0; p.c_zs = (long)b.n * b.N;
     const unsigned gx = (b.N + GBN - 1) / GBN, gy = (b.n + GBM - 1) / GBM;
-    const dim3 grid(gx * gy * slices + low);
-    if (nr == 1) {
-      FLM_RAISE_LDS_ONCE(x3_parts_kernel<1>);
-      hipLaunchKernelGGL(x3_parts_kernel<1>, grid, dim3(512), X3_LDS_BYTES, st, p, gx, gy, (unsigned)slices, s, g, low_slices);
-    } else {
-      FLM_RAISE_LDS_ONCE(x3_parts_kernel<2>);
-      hipLaunchKernelGGL(x3_parts_kernel<2>, grid, dim3(512), X3_LDS_BYTES, st, p, gx, gy, (unsigned)slices, s, g, low_slices);
-    }
+    FLM_RAISE_LDS_ONCE(x3_parts_kernel<NR>);
+    hipLaunchKernelGGL(x3_parts_kernel<NR>, dim3(gx * gy * slices + low), dim3(512), X3_LDS_BYTES, st, p, gx, gy, (unsigned)slices, s, g,
+                       low_slices);
   } else {
     const int tiles = ((b.n + 127) / 128) * ((b.N + 127) / 128);
     const size_t lds = 128 * (128 * 4 + 16);                         // (the stages take 64 KiB, the result a little more)
-    const dim3 grid(tiles * slices + low);
-    if (nr == 1) {
-      FLM_RAISE_LDS_ONCE((parts_kernel<T, 1>));
-      hipLaunchKernelGGL((parts_kernel<T, 1>), grid, dim3(256), lds, st, b, s, g, tiles, slices, low_slices);
-    } else {
-      FLM_RAISE_LDS_ONCE((parts_kernel<T, 2>));
-      hipLaunchKernelGGL((parts_kernel<T, 2>), grid, dim3(256), lds, st, b, s, g, tiles, slices, low_slices);
-    }
+    FLM_RAISE_LDS_ONCE((parts_kernel<T, NR, W_KN>));
+    hipLaunchKernelGGL((parts_kernel<T, NR, W_KN>), dim3(tiles * slices + low), dim3(256), lds, st, b, s, g, tiles, slices, low_slices);
   }
   FLM_CHECK_LAUNCH();
   return FLM_OK;
+}
+
+// K slices of the projection into b.part and, with low_slices > 0, the narrow products beside them
+template <typename T, bool W_KN>
+static int launch_parts(const BaseArgs& b, int slices, const RowGroups& g, const ShrinkArgs& s, int low_slices, hipStream_t st) {
+  return W_KN || s.rp <= 16 ? launch_parts_ranks<T, 1, W_KN>(b, slices, g, s, low_slices, st)
+                            : launch_parts_ranks<T, 2, false>(b, slices, g, s, low_slices, st);
 }
 
 template <typename T, bool V_STRIDED>
@@ -1287,46 +1351,44 @@ static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st
   return FLM_OK;
 }
 
-// The narrow product (low_slices = 0: it is there already) and y = X * W^T + bias + adapters, any type and size.  w_nk: W is
-// [N,K]; otherwise [K,N] (fp32 through BASE_X3 only).  f.part / b.part: base_part_bytes() of workspace
-template <typename T, bool V_STRIDED>
-static int launch_projection(BaseArgs b, const BasePlan& plan, bool w_nk, const ShrinkArgs& s, int low_slices, FinishArgs f,
-                             const RowGroups& g, hipStream_t st) {
-  if (plan.form == BASE_ROWS) {
-    const int rc = launch_few_rows<T>(b, plan.slices, s, low_slices, g, st);
+// The narrow product (low_slices = 0: it is there already, as always with W_KN) and y = X * W^T + bias + adapters, any type
+// and size.  W is [N,K], or (W_KN) [K,N].  f.part / b.part: base_part_bytes() of workspace
+template <typename T, bool W_KN, bool V_STRIDED>
+static int launch_projection(BaseArgs b, const BasePlan& plan, const ShrinkArgs& s, int low_slices, FinishArgs f, const RowGroups& g,
+                             hipStream_t st) {
+  int rc;
+  if constexpr (!W_KN) {
+    if (plan.form == BASE_ROWS) {
+      if ((rc = launch_few_rows<T>(b, plan.slices, s, low_slices, g, st))) return rc;
+      return launch_finish<T, V_STRIDED>(f, g, st);
+    }
+  }
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (W_KN) rc = gemm_x3_slices((const float*)b.x, b.ldx, (const float*)b.w, b.ldw, false, b.part, b.n, b.N, b.K, plan.slices,
+                                            b.kslice, st);
+    else rc = launch_parts<float, false>(b, plan.slices, g, s, low_slices, st);
     if (rc) return rc;
-  } else if (plan.form == BASE_X3) {
-    if constexpr (sizeof(T) == 4) {
-      // (W [K,N] comes from the backward pass only, whose narrow product is there already)
-      const int rc = w_nk ? launch_parts<float>(b, plan.slices, g, s, low_slices, st)
-                          : gemm_x3_slices((const float*)b.x, b.ldx, (const float*)b.w, b.ldw, false, b.part, b.n, b.N, b.K, plan.slices,
-                                           b.kslice, st);
-      if (rc) return rc;
-    }
   } else {
-    if constexpr (sizeof(T) != 4) {
-      const bool beside = plan.rows == 0 && plan.slices > 1;         // nothing needs low before it is through
-      int rc = low_slices == 0 || beside ? FLM_OK : launch_shrink<T, false>(s, g, low_slices, st);
-      if (rc) return rc;
-      if (plan.rows) {
-        BaseArgs large = b;
-        FinishArgs fl = f;
-        large.n = fl.n = plan.rows;
-        large.kslice = b.K;
-        if ((rc = launch_wide<T, 256, 256, 2, 4, V_STRIDED>(large, fl, g, st))) return rc;
-        if (plan.rows == b.n) return FLM_OK;
-      }
-      // the rows behind: the same with the sorted positions from plan.rows on
-      RowGroups rest = g;
-      rest.order += plan.rows;
-      rest.key += plan.rows;
-      b.n = f.n = b.n - plan.rows;
-      f.low += (long)plan.rows * f.rp;
-      f.part_sorted = 1;
-      if (plan.slices == 1) return launch_wide<T, 128, 128, 2, 2, V_STRIDED>(b, f, rest, st);
-      if ((rc = launch_parts<T>(b, plan.slices, rest, s, beside ? low_slices : 0, st))) return rc;
-      return launch_finish<T, V_STRIDED>(f, rest, st);
+    const bool beside = plan.rows == 0 && plan.slices > 1;           // nothing needs low before it is through
+    if (!W_KN && low_slices && !beside && (rc = launch_shrink<T, false>(s, g, low_slices, st))) return rc;
+    if (plan.rows) {
+      BaseArgs large = b;
+      FinishArgs fl = f;
+      large.n = fl.n = plan.rows;
+      large.kslice = b.K;
+      if ((rc = launch_wide<T, 256, 256, 2, 4, W_KN, V_STRIDED>(large, fl, g, st))) return rc;
+      if (plan.rows == b.n) return FLM_OK;
     }
+    // the rows behind: the same with the sorted positions from plan.rows on
+    RowGroups rest = g;
+    rest.order += plan.rows;
+    rest.key += plan.rows;
+    b.n = f.n = b.n - plan.rows;
+    f.low += (long)plan.rows * f.rp;
+    f.part_sorted = 1;
+    if (plan.slices == 1) return launch_wide<T, 128, 128, 2, 2, W_KN, V_STRIDED>(b, f, rest, st);
+    if ((rc = launch_parts<T, W_KN>(b, plan.slices, rest, s, beside ? low_slices : 0, st))) return rc;
+    return launch_finish<T, V_STRIDED>(f, rest, st);
   }
   return launch_finish<T, V_STRIDED>(f, g, st);
 }
@@ -1382,8 +1444,8 @@ static int forward(const void* x, long ldx, const void* w, long ldw, const void*
   const ShrinkArgs s{x, a, ldx, (long)r * K, K, 1, K, r, rp, n, ss.kslice, low_part};
   const FinishArgs f{part, bs.slices, 0, bias, low_part, (long)n * rp, ss.slices, r, rp, b, (long)N * r, r, 1, scale, scale_all, n, N, E, y, ldy};
   const BaseArgs base{x, w, ldx, ldw, n, K, N, bs.kslice, part};
-  const int rc = r % 8 == 0 ? launch_projection<T, false>(base, bs, true, s, ss.slices, f, g, st)
-                            : launch_projection<T, true>(base, bs, true, s, ss.slices, f, g, st);
+  const int rc = r % 8 == 0 ? launch_projection<T, false, false>(base, bs, s, ss.slices, f, g, st)
+                            : launch_projection<T, false, true>(base, bs, s, ss.slices, f, g, st);
   if (rc) return rc;
   if (low) {
     hipLaunchKernelGGL(low_rows_kernel, dim3((unsigned)(((long)n * rp + 255) / 256)), dim3(256), 0, st, low_part, ss.slices, n, r,
@@ -1414,18 +1476,10 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
                             OuterArgs{low, r, 1, dy, lddy, N, r, E, n, cb, scale, scale_all, part_b, db, 1, r, 0}, g, st)))
     return rc;
   if (!dx) return FLM_OK;
-  const BasePlan bs = base_plan(n, N, K, sizeof(T) == 4);
+  const BasePlan bs = base_plan(n, N, K, sizeof(T) == 4, true);
   float* dx_part = (float*)ws;
-  const bool turn = bs.form != BASE_X3;                              // the contraction runs down W: turned once
-  if (turn) {
-    T* wt = (T*)(ws + round16(base_part_bytes(bs, n, K)));
-    hipLaunchKernelGGL(transpose_kernel<T>, dim3((K + 63) / 64, (N + 63) / 64), dim3(256), 0, st, (const T*)w, ldw, N, K, wt);
-    FLM_CHECK_LAUNCH();
-    w = wt;
-    ldw = N;
-  }
   const FinishArgs f{dx_part, bs.slices, 0, nullptr, u, (long)n * rp, 1, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
-  return launch_projection<T, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, turn, s, 0, f, g, st);
+  return launch_projection<T, true, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, s, 0, f, g, st);
 }
 
 }  // namespace flm
@@ -1449,8 +1503,7 @@ extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E
   const int ca = outer_chunk(tiles, n, E, K, r, dtype == FLM_F32), cb = outer_chunk(tiles, n, E, N, r, dtype == FLM_F32);
   long rest = 4L * r * (outer_part(tiles, ca) * K + outer_part(tiles, cb) * N);
   if (need_dx) {
-    const BasePlan bs = base_plan(n, N, K, dtype == FLM_F32);
-    const long base = round16(base_part_bytes(bs, n, K)) + (bs.form == BASE_X3 ? 0 : (dtype == FLM_F32 ? 4L : 2L) * K * N);
+    const long base = base_part_bytes(base_plan(n, N, K, dtype == FLM_F32, true), n, K);
     if (base > rest) rest = base;
   }
   return round16(4L * shrink_plan(n, N, E).slices * n * ranks_padded(r)) + rest + 256;

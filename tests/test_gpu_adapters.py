@@ -29,6 +29,9 @@ SIZES = [
     (500, 96, 64, 40, 400, False),
     (6000, 72, 40, 100, 300, True),
     (13000, 328, 136, 10, 3, True),
+    # so many rows that the narrow product takes pairs of tiles, of one adapter and of two
+    (16500, 77, 40, 33, 9, False),
+    (16450, 264, 72, 20, 300, True),
 ]
 
 
