@@ -223,17 +223,16 @@ __global__ __launch_bounds__(1024) void group_scan_kernel(int* counts, int runs,
   __shared__ int part[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, E1 = E + 1, g = blockIdx.x * 64 + lane;
   const int per = (runs + 15) / 16, lo = min(runs, w * per), hi = min(runs, lo + per);
+  const int gg = min(g, E1 - 1);
+  // up to 32 runs a thread stay in registers between the two passes (512 runs: 262144 rows); longer shares are read twice
+  constexpr int KEEP = 32;
+  int c[KEEP];
   int s = 0;
-  if (g < E1) {
-    int k = lo;
-    for (; k + 8 <= hi; k += 8) {
-      int c[8];
+  for (int k0 = lo; k0 < hi; k0 += KEEP) {
 #pragma unroll
-      for (int u = 0; u < 8; u++) c[u] = counts[(long)(k + u) * E1 + g];
+    for (int u = 0; u < KEEP; u++) c[u] = counts[(long)min(k0 + u, hi - 1) * E1 + gg];
 #pragma unroll
-      for (int u = 0; u < 8; u++) s += c[u];
-    }
-    for (; k < hi; k++) s += counts[(long)k * E1 + g];
+    for (int u = 0; u < KEEP; u++) s += k0 + u < hi ? c[u] : 0;
   }
   part[w][lane] = s;
   __syncthreads();
@@ -244,21 +243,17 @@ __global__ __launch_bounds__(1024) void group_scan_kernel(int* counts, int runs,
     total += part[k][lane];
   }
   if (g >= E1) return;
-  int k = lo;
-  for (; k + 8 <= hi; k += 8) {
-    int c[8];
+  for (int k0 = lo; k0 < hi; k0 += KEEP) {
+    if (per > KEEP) {
 #pragma unroll
-    for (int u = 0; u < 8; u++) c[u] = counts[(long)(k + u) * E1 + g];
-#pragma unroll
-    for (int u = 0; u < 8; u++) {
-      counts[(long)(k + u) * E1 + g] = base;
-      base += c[u];
+      for (int u = 0; u < KEEP; u++) c[u] = counts[(long)min(k0 + u, hi - 1) * E1 + g];
     }
-  }
-  for (; k < hi; k++) {
-    const int c = counts[(long)k * E1 + g];
-    counts[(long)k * E1 + g] = base;
-    base += c;
+#pragma unroll
+    for (int u = 0; u < KEEP; u++)
+      if (k0 + u < hi) {
+        counts[(long)(k0 + u) * E1 + g] = base;
+        base += c[u];
+      }
   }
   if (w == 0) totals[g] = total;
 }
