@@ -1486,6 +1486,20 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
 
 using namespace flm;
 
+// Whether two operands may share an element: rows of `width` elements, ld apart (ld is no less than width, or 0 and more
+// where rows may coincide).  Columns of one matrix that do not meet do not overlap.
+struct Span { const void* p; long ld, rows, width; };
+static bool spans_meet(const Span& a, const Span& b, int size) {
+  if (!a.p || !b.p) return false;
+  const long pa = (long)(uintptr_t)a.p, pb = (long)(uintptr_t)b.p;
+  const long ea = pa + ((a.rows - 1) * a.ld + a.width) * size, eb = pb + ((b.rows - 1) * b.ld + b.width) * size;
+  if (pa >= eb || pb >= ea) return false;
+  const long ld = a.ld * size;
+  if (a.ld != b.ld || a.rows < 2 || b.rows < 2 || a.width + b.width > a.ld) return true;
+  const long d = ((pb - pa) % ld + ld) % ld;               // where b's rows begin within a's
+  return d < a.width * size || d + b.width * size > ld;
+}
+
 static bool adapter_sizes(int n, int K, int N, int r, int E, int dtype) {
   return n > 0 && n <= (1 << 20) && K > 0 && N > 0 && K <= (1 << 20) && N <= (1 << 20) && r > 0 && r <= FLM_ADAPTER_MAX_RANK && E > 0 &&
          E <= FLM_GROUPS_MAX && dtype >= FLM_F32 && dtype <= FLM_F16;
@@ -1515,6 +1529,10 @@ extern "C" int flm_adapter_linear(const void* x, long ldx, const void* w, long l
   if (!x || !w || !a || !b || !groups || !workspace || !y || !adapter_sizes(n, K, N, r, E, dtype) || ldx < 0 || ldw < 0 || ldy < N ||
       ((uintptr_t)workspace & 15))
     return FLM_E_ARG;
+  const int size = dtype == FLM_F32 ? 4 : 2;
+  const Span out{y, ldy, n, N};
+  for (const Span& in : {Span{x, ldx, n, K}, Span{w, ldw, N, K}, Span{bias, 0, 1, N}, Span{a, 0, 1, (long)E * r * K}, Span{b, 0, 1, (long)E * N * r}})
+    if (spans_meet(out, in, size)) return FLM_E_OVERLAP;
   const RowGroups g = row_groups(groups, n, E);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == FLM_F32) return forward<float>(x, ldx, w, ldw, bias, a, b, g, scale, scale_all, n, K, N, r, E, (char*)workspace, y, ldy, low, st);
@@ -1529,6 +1547,17 @@ extern "C" int flm_adapter_linear_backward(const void* dy, long lddy, const void
   if (!dy || !x || !b || !groups || !low || !workspace || !da || !db || !adapter_sizes(n, K, N, r, E, dtype) || lddy < 0 ||
       ldx < 0 || (dx && (!w || !a || ldw < 0 || lddx < K)) || ((uintptr_t)workspace & 15))
     return FLM_E_ARG;
+  const int size = dtype == FLM_F32 ? 4 : 2;
+  const long na = (long)E * r * K, nb = (long)E * N * r;
+  const Span in[] = {{dy, lddy, n, N}, {x, ldx, n, K}, {dx ? w : nullptr, ldw, N, K}, {dx ? a : nullptr, 0, 1, na}, {b, 0, 1, nb},
+                     {low, 0, 1, (long)n * r * (4 / size)}};
+  const Span out[] = {{da, 0, 1, na}, {db, 0, 1, nb}, {dx, lddx, n, K}};
+  for (int i = 0; i < 3; i++) {
+    for (const Span& s : in)
+      if (spans_meet(out[i], s, size)) return FLM_E_OVERLAP;
+    for (int j = 0; j < i; j++)
+      if (spans_meet(out[i], out[j], size)) return FLM_E_OVERLAP;
+  }
   const RowGroups g = row_groups(groups, n, E);
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;

@@ -649,7 +649,7 @@ int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* gro
  *   workspace: flm_adapter_workspace(n, K, N, r, E, dtype) bytes, 16-byte aligned; one per call in flight
  * Sums are fp32, rounded once.  fp32 operands are multiplied as three bf16 terms each (fp32 accuracy; a row that meets an
  * infinity or NaN becomes NaN, other rows do not).  An adapter's values reach the rows of that adapter only.
- * n, K, N <= 2^20, r <= FLM_ADAPTER_MAX_RANK, E <= FLM_GROUPS_MAX.  y must not overlap an input. */
+ * n, K, N <= 2^20, r <= FLM_ADAPTER_MAX_RANK, E <= FLM_GROUPS_MAX.  y shares no element with an input (FLM_E_OVERLAP). */
 long flm_adapter_workspace(int n, int K, int N, int r, int E, int dtype);
 int flm_adapter_linear(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* a, const void* b,
                        const int32_t* groups, const float* scale, float scale_all, int n, int K, int N, int r, int E,
@@ -658,7 +658,8 @@ int flm_adapter_linear(const void* x, long ldx, const void* w, long ldw, const v
 /* Its backward pass for the gradient dy [n,N] of y; the projection itself (w, bias) is held fixed.
  *   u_i = s_e B_e^T dy_i;  da_e = sum_{i of e} u_i x_i^T [E,r,K];  db_e = s_e sum_{i of e} dy_i low_i^T [E,N,r];
  *   dx_i = W^T dy_i + A_e^T u_i [n,K] (dx = NULL: not computed, w and a may then be NULL)
- * da and db are written whole: zeros for adapters without rows.  Sums have a fixed order.
+ * da and db are written whole: zeros for adapters without rows.  Sums have a fixed order.  No result shares an element
+ * with an input or another result (FLM_E_OVERLAP).
  * workspace: flm_adapter_backward_workspace(n, K, N, r, E, dtype, dx != NULL) bytes, 16-byte aligned. */
 long flm_adapter_backward_workspace(int n, int K, int N, int r, int E, int dtype, int need_dx);
 int flm_adapter_linear_backward(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* a,

@@ -11,6 +11,9 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # rows, inputs, outputs, rank, adapters, skewed
 SIZES = [
     (1, 64, 32, 16, 1, False),
+    (1, 1, 1, 1, 1, False),
+    (66, 1, 3, 2, 2, False),
+    (70, 3, 1, 1, 1, True),
     (1, 1000, 130, 4, 20, False),
     (2, 7, 5, 1, 3, False),
     (16, 515, 96, 5, 4, False),
@@ -237,6 +240,29 @@ def test_no_rows():
     assert y.shape == (0, 8) and low.shape == (0, 4)
     dx, da, db = adapter_linear_backward(c["dy"][:0], c["x"][:0], c["weight"], c["a"], c["b"], g, low)
     assert dx.shape == (0, 16) and (da == 0).all() and (db == 0).all()
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+def test_results_beside_their_inputs(kind):
+    """Columns of one matrix may be input and result of a call; results that meet an input are refused."""
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    c = ref.case(5, 100, 64, 32, 8, 3, kind)
+    d = ref.to_gpu(c)
+    g = group_rows(d["ids"], 3)
+    both = torch.zeros((100, 96), dtype=kind, device="cuda")
+    both[:, :64] = d["x"]
+    args = (d["weight"], d["bias"], d["a"], d["b"], g, d["scale"])
+    want = adapter_linear(d["x"], *args)
+    got = adapter_linear(both[:, :64], *args, out=both[:, 64:])
+    assert torch.equal(got, want) and torch.equal(both[:, 64:], want) and torch.equal(both[:, :64], d["x"])
+    with pytest.raises(ValueError):
+        adapter_linear(both[:, :64], *args, out=both[:, 40:72])
+    with pytest.raises(ValueError):
+        adapter_linear(d["x"], *args, out=d["x"][:, :32])
+    low = adapter_linear(d["x"], *args, keep_low=True)[1]
+    with pytest.raises(ValueError):
+        adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low, db=d["b"])
+    assert torch.equal(d["x"].cpu(), c["x"]) and torch.equal(d["b"].cpu(), c["b"])
 
 
 def _train_pass(d, out):

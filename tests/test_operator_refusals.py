@@ -53,6 +53,34 @@ def test_adapter_entries():
         assert lib.flm_adapter_linear_backward(*args) == -1, i
 
 
+def test_adapter_results_that_share_memory():
+    """Host addresses only: every call is refused before a launch.  n 8, K 64, N 32, r 4, E 2, bf16."""
+    lib = _lib.load()
+    at = ctypes.c_void_p
+    ok = [at(0x100000), 64, at(0x200000), 64, at(0x280000), at(0x300000), at(0x400000), P, None, 1.0, 8, 64, 32, 4, 2, 1, P, at(0x500000),
+          32, None, None]
+    sizes = {0: 8 * 64, 2: 32 * 64, 4: 32, 5: 2 * 4 * 64, 6: 2 * 32 * 4}          # elements of each input
+    for i, n in sizes.items():
+        for y in (ok[i].value, ok[i].value + 2 * n - 2, ok[i].value - 2 * 8 * 32 + 2):
+            args = list(ok)
+            args[17] = at(y)
+            assert lib.flm_adapter_linear(*args) == -4, (i, y)
+    # columns of one matrix: x and y share 16 of them
+    args = list(ok)
+    args[1], args[17], args[18] = 96, at(0x100000 + 2 * 48), 96
+    assert lib.flm_adapter_linear(*args) == -4
+    args[17] = at(0x100000 + 2 * 64 + 2 * 2)                                      # runs over into x's next row
+    assert lib.flm_adapter_linear(*args) == -4
+    ok = [at(0x100000), 32, at(0x200000), 64, at(0x300000), 64, at(0x400000), at(0x500000), P, None, 1.0, at(0x600000), 8, 64, 32, 4, 2, 1, P,
+          at(0x700000), 64, at(0x800000), at(0x900000), None]
+    for out in (19, 21, 22):
+        for other in (0, 2, 4, 6, 7, 11, 19, 21, 22):
+            if out != other:
+                args = list(ok)
+                args[out] = ok[other]
+                assert lib.flm_adapter_linear_backward(*args) == -4, (out, other)
+
+
 def test_gradient_entries():
     lib = _lib.load()
     src = (ctypes.c_void_p * 2)(4096, 8192)
