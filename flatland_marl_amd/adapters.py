@@ -100,8 +100,8 @@ def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False, out
     """y[i] = weight x[i] + bias + scale[e] * b[e] (a[e] x[i]) for the adapter e of row i (groups = group_rows(ids, E)); rows
     without an adapter get the projection alone.  x [n, K], weight [N, K], bias [N] or None, a [E, r, K], b [E, N, r], all
     of one type (float32, bfloat16, float16); scale: a number or float32 [E].  keep_low: returns (y, low) with low [n, r]
-    float32 = a[e] x[i], which the backward pass takes.  out: a tensor [n, N] with contiguous rows that receives y (it must
-    not overlap an input).  Runs on the current stream; no autograd."""
+    float32 = a[e] x[i], which the backward pass takes.  out: a tensor [n, N] with contiguous rows that receives y (it may
+    share no element with an input).  Runs on the current stream; no autograd."""
     n, k, n_out, r, e, scales, ldx, ldw = _weights(x, weight, a, b, groups, scale)
     if weight.shape[0] != n_out:
         raise ValueError("weight [%d, %d] expected" % (n_out, k))
@@ -128,7 +128,8 @@ def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False, out
 def adapter_linear_backward(dy, x, weight, a, b, groups, low, scale=1.0, need_dx=True, da=None, db=None):
     """Gradients (dx, da, db) of adapter_linear for the gradient dy [n, N] of y; the shared projection is held fixed.
     low: what adapter_linear kept.  need_dx = False: dx is None and weight is not read (None is taken).  da, db: contiguous
-    tensors like a and b that receive the gradients (fresh ones by default); adapters without rows get zeros."""
+    tensors like a and b that receive the gradients (fresh ones by default; they share no element with an input); adapters
+    without rows get zeros."""
     n, k, n_out, r, e, scales, ldx, ldw = _weights(x, weight if need_dx else None, a, b, groups, scale)
     if need_dx and weight.shape[0] != n_out:
         raise ValueError("weight [%d, %d] expected" % (n_out, k))
@@ -198,6 +199,7 @@ class NetworkAdapters:
         for name in self.PARTS:
             if tuple(state[name].shape) != tuple(getattr(self, name).shape):
                 raise ValueError("%s %s expected" % (name, tuple(getattr(self, name).shape)))
+        for name in self.PARTS:
             getattr(self, name).copy_(state[name])
 
     def copy_for(self, network):
@@ -217,6 +219,11 @@ class NetworkAdapters:
         if obs_u8.dtype != torch.uint8 or tuple(obs_u8.shape[1:]) != (3, plane_stride) or not obs_u8.is_contiguous():
             raise ValueError("contiguous uint8 observations [n, 3, plane_stride] expected")
         flat = network.flat_params()
+        if obs_u8.device != flat.device:
+            raise ValueError("observations on the network's device expected")
+        for name, t, want in (("out", out, n * network.action_space), ("features", features, n * self.inputs)):
+            if t is not None and (t.dtype != torch.float32 or t.device != flat.device or not t.is_contiguous() or t.numel() < want):
+                raise ValueError("%s: a contiguous float32 buffer of at least %d elements on the network's device expected" % (name, want))
         q = torch.empty((n, network.action_space), dtype=torch.float32, device=flat.device) if out is None else out[:n]
         x = torch.empty(n * self.inputs, dtype=torch.float32, device=flat.device) if features is None else features
         x = x[:n * self.inputs].view(n, self.inputs)

@@ -184,7 +184,8 @@ class DQNAgent:
 
     def attach_adapters(self, n_adapters, rank, alpha=None, lr=None):
         """Low-rank adapters beside the networks' first dense layers: from now on learn_adapters() trains them (Adam, lr or
-        the agent's) and the networks stay as they are.  Returns the local network's NetworkAdapters."""
+        the agent's) and the networks stay as they are.  Returns the local network's NetworkAdapters.  (Several ranks draw the
+        same start if they are seeded alike, as for the network itself.)"""
         self.adapters = NetworkAdapters(self.qnetwork_local, n_adapters, rank, alpha)
         self.adapters_target = self.adapters.copy_for(self.qnetwork_target)
         self.adapter_optimizer = AdapterAdam(self.adapters, self.args.lr if lr is None else lr)
@@ -201,6 +202,8 @@ class DQNAgent:
             raise ValueError("attach_adapters() first")
         B, net = states.size(0), self.qnetwork_local
         dev = net.flat_params().device
+        if not B == actions.numel() == rewards.numel() == dones.numel() == ids.numel() or B < 1:
+            raise ValueError("actions, rewards, dones and ids of %d transitions expected" % B)
         groups = group_rows(ids, ad.n_adapters)
         s, sn = states.contiguous(), next_states.contiguous()
         q, kept = ad.q_values(net, s, plane_stride, groups, keep=True)

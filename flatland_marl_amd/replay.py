@@ -43,14 +43,19 @@ class DeviceReplay:
         if self.group is None:
             # (one place more than the ring: where kernels leave a transition out, its group goes there)
             self.group = torch.full((self.capacity + 1,), -1, dtype=torch.int32, device=self.device)
+            torch.cuda.current_stream(self.device).synchronize()       # (steps may be stored on another stream)
 
     def sampled_groups(self):
         """The groups [batch] of the last sample()'s transitions."""
+        if self.group is None or self._out is None:
+            raise ValueError("keep_groups() and sample() first")
         return self.group.index_select(0, self._out[5].long())
 
     def add(self, state, action, reward, next_state, done, groups=None):
         """Append n transitions (oldest entries are overwritten, as with deque(maxlen))."""
         n = state.shape[0]
+        if groups is not None and (self.group is None or tuple(groups.shape) != (n,)):
+            raise ValueError("keep_groups() first, then a group for each of the %d transitions" % n)
         if self.group is not None:
             if groups is None:
                 groups = torch.full((n,), -1, dtype=torch.int32, device=self.device)
@@ -79,6 +84,9 @@ class DeviceReplay:
         n1, n2 = req_ready.numel(), req_switch.numel()
         n = n1 + n2
         dev = self.device
+        if groups_of_env is not None and (self.group is None or tuple(groups_of_env.shape) != (ro.E,) or
+                                          groups_of_env.dtype != torch.int32 or groups_of_env.device != self.group.device):
+            raise ValueError("keep_groups() first, then an int32 group for each of the %d environments, on the device" % ro.E)
         if getattr(self, "_slot", None) is None or self._slot.numel() < n:
             cap = max(n, 1024)
             self._slot = torch.empty((cap,), dtype=torch.int32, device=dev)

@@ -68,6 +68,8 @@ class DQNPolicy:
         """q_values() with every row's environment's adapter; agents [n]: e*A + a of each row."""
         b, n, ad = ro.b, obs_u8.shape[0], self.agent.adapters
         net = self.agent.qnetwork_local
+        if tuple(self.adapter_of_env.shape) != (ro.E,) or self.adapter_of_env.device != obs_u8.device:
+            raise ValueError("adapter_of_env [%d] on the device of the rollout expected" % ro.E)
         q = torch.empty((n, net.action_space), dtype=torch.float32, device=obs_u8.device) if out is None else out[:n]
         chunk = max(1, min(1 << 20, self.chunk_bytes // (4 * ad.inputs)))
         with torch.cuda.stream(b.stream):                  # (the observations were written on the rollout's stream)

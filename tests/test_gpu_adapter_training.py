@@ -289,5 +289,35 @@ def test_refusals():
         ad.q_values(agent.qnetwork_local, dev[0], ro.b.plane_stride, group_rows(torch.zeros(3, dtype=torch.int32).cuda(), 2))
     with pytest.raises(ValueError):
         ad.q_values(agent.qnetwork_local, dev[0].float(), ro.b.plane_stride, group_rows(torch.zeros(4, dtype=torch.int32).cuda(), 2))
+    ids = torch.zeros(4, dtype=torch.int32).cuda()
+    groups = group_rows(ids, 2)
+    net, stride = agent.qnetwork_local, ro.b.plane_stride
+    with pytest.raises(ValueError):                          # observations, results and features that are not where they should be
+        ad.q_values(net, dev[0].cpu(), stride, groups)
+    for kw in (dict(out=torch.zeros(3, 2).cuda()), dict(out=torch.zeros(4, 2)), dict(out=torch.zeros(4, 2).cuda().half()),
+               dict(features=torch.zeros(4 * ad.inputs - 1).cuda()), dict(features=torch.zeros(4 * ad.inputs))):
+        with pytest.raises(ValueError):
+            ad.q_values(net, dev[0], stride, groups, **kw)
+    for i in (1, 2, 4):                                      # an action, a reward, a flag too few
+        short = list(dev)
+        short[i] = short[i][:3]
+        with pytest.raises(ValueError):
+            agent.learn_adapters(short, ids, 0.9, stride)
+    policy = DQNPolicy(agent, adapter_of_env=torch.zeros(1, dtype=torch.int32).cuda())
+    with pytest.raises(ValueError):
+        policy._adapted_q_values(ro, dev[0], ids, None)
+    for groups_of in (None, ids[:3]):                        # groups without keep_groups(), too few of them
+        if groups_of is not None:
+            tr.replay.keep_groups()
+        with pytest.raises(ValueError):
+            tr.replay.add(dev[0], dev[1], dev[2], dev[3], dev[4], groups=ids if groups_of is None else groups_of)
+        with pytest.raises(ValueError):
+            tr.replay.sampled_groups()
+    before = ad.state_dict()
+    bad = dict(before, b_val=before["b_val"][:1])
+    bad["a_adv"] = before["a_adv"] + 1
+    with pytest.raises(ValueError):
+        ad.load_state_dict(bad)
+    assert all(torch.equal(before[k], v) for k, v in ad.state_dict().items())
     with pytest.raises(ValueError):
         agent.optimizer.clip_grad_norm_(1.0, rails=(100, 151, 2, 8, None, False))
