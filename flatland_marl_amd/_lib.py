@@ -151,21 +151,29 @@ def query(name, *args):
 
 
 def call(name, *args):
-    rc = getattr(load(), name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc != FLM_OK:
         if rc == E_OVERLAP:
             raise ValueError("%s: tensors that are written share memory" % name)
         raise FlmError("%s failed with code %d" % (name, rc))
 
 
+_torch = _current_device = _raw_stream = None
+
+
 def launch(dev, name, *args):
     """call(name, *args, stream) on the current stream of dev, a GPU that need not be the current one."""
-    import torch
-    if torch.cuda.current_device() == dev.index:
-        call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+    global _torch, _current_device, _raw_stream
+    if _torch is None:
+        import torch
+        _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        _torch = torch
+    index = dev.index
+    if _current_device() == index:
+        call(name, *args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+        with _torch.cuda.device(dev):
+            call(name, *args, _raw_stream(index))
 
 
 @functools.lru_cache(maxsize=4096)

@@ -7,6 +7,9 @@ from ._lib import ADAPTER_MAX_RANK, GROUPS_MAX, FlmError, launch, size_of
 from .gradients import DTYPES
 
 
+SIZE_MAX = 1 << 20                                          # rows, inputs, outputs
+
+
 class RowGroups:
     """Rows sorted by group: what group_rows returns and the adapter calls take.  One int32 buffer; n rows, n_groups."""
 
@@ -40,7 +43,7 @@ def group_rows(ids, n_groups):
     if not 1 <= n_groups <= GROUPS_MAX:
         raise ValueError("n_groups must be 1..%d" % GROUPS_MAX)
     dev, n = ids.device, ids.numel()
-    if dev.type != "cuda":
+    if not ids.is_cuda:
         raise FlmError("ids must live on a GPU: there is no CPU path")
     if n == 0:
         return RowGroups(torch.zeros(n_groups + 1, dtype=torch.int32, device=dev), 0, n_groups)
@@ -58,33 +61,37 @@ def group_rows(ids, n_groups):
 
 def _rows(t, name, width, dev, kind):
     """Row stride of a 2-D operand whose rows are contiguous."""
-    if t.dim() != 2 or t.shape[1] != width:
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width:
         raise ValueError("%s [., %d] expected" % (name, width))
     if t.dtype != kind or t.device != dev:
         raise ValueError("%s differs from x in type or device" % name)
-    if t.stride(1) != 1 and width > 1:
+    across, along = t.stride()
+    if along != 1 and width > 1:
         raise ValueError("the rows of %s must be contiguous" % name)
-    return t.stride(0) if t.shape[0] > 1 else width
+    return across if shape[0] > 1 else width
 
 
 def _weights(x, weight, a, b, groups, scale):
-    if x.dim() != 2 or x.dtype not in DTYPES:
+    kind, dev = x.dtype, x.device
+    if x.dim() != 2 or kind not in DTYPES:
         raise ValueError("x [n, K] of float32, bfloat16 or float16 expected")
     n, k = x.shape
-    dev, kind = x.device, x.dtype
-    if dev.type != "cuda":
+    if not x.is_cuda:
         raise FlmError("x must live on a GPU: there is no CPU path")
-    if a.dim() != 3 or b.dim() != 3 or a.shape[2] != k or b.shape[0] != a.shape[0] or b.shape[2] != a.shape[1] or \
-            not a.is_contiguous() or not b.is_contiguous():
+    if a.dim() != 3 or b.dim() != 3:
+        raise ValueError("contiguous a [E, r, K] and b [E, N, r] expected")
+    e, r, k_a = a.shape
+    e_b, n_out, r_b = b.shape
+    if k_a != k or e_b != e or r_b != r or not a.is_contiguous() or not b.is_contiguous():
         raise ValueError("contiguous a [E, r, K] and b [E, N, r] expected")
     if a.dtype != kind or b.dtype != kind or a.device != dev or b.device != dev:
         raise ValueError("a and b differ from x in type or device")
-    e, r = a.shape[0], a.shape[1]
     if not 1 <= r <= ADAPTER_MAX_RANK:
         raise ValueError("rank must be 1..%d" % ADAPTER_MAX_RANK)
     if groups.n != n or groups.n_groups != e or groups.buf.device != dev:
         raise ValueError("groups of %d rows and %d adapters expected" % (n, e))
-    if max(n, k, b.shape[1]) > 1 << 20 or min(k, b.shape[1]) < 1:
+    if not (n <= SIZE_MAX and 1 <= k <= SIZE_MAX and 1 <= n_out <= SIZE_MAX):
         raise ValueError("rows, inputs and outputs must be at most 2^20")
     if isinstance(scale, torch.Tensor):
         if scale.dtype != torch.float32 or scale.shape != (e,) or scale.device != dev or not scale.is_contiguous():
@@ -92,7 +99,7 @@ def _weights(x, weight, a, b, groups, scale):
         scales = (scale.data_ptr(), 1.0)
     else:
         scales = (None, float(scale))
-    return n, k, b.shape[1], r, e, scales, _rows(x, "x", k, dev, kind), \
+    return n, k, n_out, r, e, scales, _rows(x, "x", k, dev, kind), \
         _rows(weight, "weight", k, dev, kind) if weight is not None else 0
 
 

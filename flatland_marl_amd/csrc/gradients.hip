@@ -169,9 +169,10 @@ __device__ __forceinline__ void grad_chunks(const GradList& list, int first, int
   }
 }
 
-__device__ __forceinline__ double grad_norm_share(const GradList& list, int first, int stride, bool inf_norm, double* red) {
+// tid, threads: who walks a chunk together, the workgroup or a wave; the result is the workgroup's
+__device__ __forceinline__ double grad_norm_share(const GradList& list, int first, int stride, int tid, int threads, bool inf_norm,
+                                                  double* red) {
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
-  const int tid = threadIdx.x, threads = blockDim.x;
   grad_chunks<false>(list, first, stride, [&](const GradItem& it, long off, int n, int lead) {
     if (it.dtype == FLM_F32) grad_norm_chunk((const float*)it.src + off, n, lead, tid, threads, inf_norm, acc);
     else if (it.dtype == FLM_BF16) grad_norm_chunk((const __bf16*)it.src + off, n, lead, tid, threads, inf_norm, acc);
@@ -182,8 +183,7 @@ __device__ __forceinline__ double grad_norm_share(const GradList& list, int firs
 }
 
 template <bool PAST>
-__device__ __forceinline__ void grad_scale_share(const GradList& list, int first, int stride, double coef) {
-  const int tid = threadIdx.x, threads = blockDim.x;
+__device__ __forceinline__ void grad_scale_share(const GradList& list, int first, int stride, int tid, int threads, double coef) {
   grad_chunks<true>(list, first, stride, [&](const GradItem& it, long off, int n, int lead) {
     if (!it.dst || (it.dst == it.src && coef == 1.0)) return;
     if (it.dtype == FLM_F32) grad_scale_chunk<float, PAST>((const float*)it.src + off, (float*)it.dst + off, n, lead, tid, threads, coef);
@@ -201,7 +201,7 @@ __device__ __forceinline__ double grad_factor(double norm, double max_norm) {
 __global__ __launch_bounds__(256) void grad_norm_kernel(GradList list, GradOuter outer, int inf_norm, double* __restrict__ part) {
   __shared__ double red[16];
   const bool inf = inf_norm != 0;
-  double v = grad_norm_share(list, blockIdx.x, gridDim.x, inf, red);
+  double v = grad_norm_share(list, blockIdx.x, gridDim.x, threadIdx.x, 256, inf, red);
   if (outer.r && blockIdx.x == gridDim.x - 1) {          // the implicit part: a product of two short sums
     double sr = 0.0, sg = 0.0;
     auto add = [&](double s, double g) { return inf ? larger(s, __builtin_fabs(g)) : __builtin_fma(g, g, s); };
@@ -225,17 +225,19 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(GradList list, int inf_n
   v = grad_fold(v, inf, red);
   const double norm = inf ? v : __builtin_sqrt(v);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
-  if (list.chunks) grad_scale_share<PAST>(list, blockIdx.x, gridDim.x, grad_factor(norm, max_norm));
+  if (list.chunks) grad_scale_share<PAST>(list, blockIdx.x, gridDim.x, threadIdx.x, 256, grad_factor(norm, max_norm));
 }
 
-// short lists: one workgroup sums, then scales what it has just read
+// Short lists: one workgroup sums, then scales what it has just read; its waves take the chunks in turn, each with its own
+// loads under way.
 __global__ __launch_bounds__(1024) void grad_clip_small_kernel(GradList list, int inf_norm, double max_norm,
                                                                float* __restrict__ norm_out) {
   __shared__ double red[16];
-  const double v = grad_norm_share(list, 0, 1, inf_norm != 0, red);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const double v = grad_norm_share(list, w, 16, lane, 64, inf_norm != 0, red);
   const double norm = inf_norm ? v : __builtin_sqrt(v);
   if (threadIdx.x == 0) *norm_out = (float)norm;
-  grad_scale_share<false>(list, 0, 1, grad_factor(norm, max_norm));
+  grad_scale_share<false>(list, w, 16, lane, 64, grad_factor(norm, max_norm));
 }
 
 // tensors [lo, lo + count) of the caller's arrays as one launch's list
@@ -281,8 +283,10 @@ static int grad_overlap(const void* const* src, void* const* dst, const int64_t*
   return FLM_OK;
 }
 
-// A list that one workgroup handles alone: up to this many elements in all, in up to 4 tensors.
-#define GRAD_SMALL 8192
+// A list that one workgroup handles alone: up to this many chunks of 2048 elements, one a wave.  (Replayed from a graph, one
+// launch / two: 64 elements 3.9 / 5.1 us, 10 tensors of 100 6.7 / 7.1, one of 8192 5.3 / 6.1, 10 of 2048 8.4 / 7.0, 10 of 6000
+// 17 / 7.3; called, the second launch costs 3 us of the host's time more.)
+#define GRAD_SMALL 16
 
 static int grad_clip_run(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count,
                          const GradOuter& outer, double max_norm, int inf_norm, double* workspace, float* norm_out,
@@ -297,7 +301,8 @@ static int grad_clip_run(const void* const* src, void* const* dst, const int64_t
     const int rc = grad_overlap(src, dst, numel, dtype, count);
     if (rc) return rc;
   }
-  if (list.count == count && count <= 4 && total <= GRAD_SMALL && !outer.r) {
+  if (count <= FLM_GRAD_LIST && total <= 2048L * GRAD_SMALL && !outer.r &&
+      grad_list(list, src, dst, numel, dtype, 0, count, 2048) && list.chunks <= GRAD_SMALL) {
     hipLaunchKernelGGL(grad_clip_small_kernel, dim3(1), dim3(1024), 0, stream, list, inf_norm, max_norm, norm_out);
     FLM_CHECK_LAUNCH();
     return FLM_OK;

@@ -24,7 +24,8 @@ def _dense(t):
 
 
 _place, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
-_device, _dtype, _layout, _shape = map(attrgetter, ("device", "dtype", "layout", "shape"))
+_device = torch.Tensor.get_device
+_dtype, _layout, _shape = map(attrgetter, ("dtype", "layout", "shape"))
 
 
 def _address(values):
@@ -46,10 +47,10 @@ def _run(grads, max_norm, norm_type, outs):
     count = len(grads)
     if count > GRAD_MAX_TENSORS:
         raise ValueError("%d gradient tensors, at most %d" % (count, GRAD_MAX_TENSORS))
-    dev = grads[0].device
-    if dev.type != "cuda":
+    dev, index = grads[0].device, grads[0].get_device()
+    if not grads[0].is_cuda:
         raise FlmError("gradients must live on a GPU: there is no CPU norm")
-    if set(map(_device, grads)) != {dev}:
+    if set(map(_device, grads)) != {index}:
         raise ValueError("gradients of several devices")
     if set(map(_layout, grads)) != {torch.strided}:
         raise ValueError("sparse gradients are not taken")
@@ -66,7 +67,7 @@ def _run(grads, max_norm, norm_type, outs):
         dst = src
         if outs is not grads:
             if list(map(_shape, outs)) != list(map(_shape, grads)) or list(map(_dtype, outs)) != types or \
-                    set(map(_device, outs)) != {dev}:
+                    set(map(_device, outs)) != {index}:
                 raise ValueError("an output differs from its gradient in shape, type or device")
             if not (straight and all(map(_contiguous, outs))) and \
                     any(o.stride() != g.stride() for o, g in zip(outs, grads)):
