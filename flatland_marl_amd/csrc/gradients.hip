@@ -23,6 +23,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 #define FLM_GRAD_LIST 112                // tensors per launch: 32 bytes each of the 4 KiB a launch's arguments may take
+#define GRAD_STEPS 12                    // a place in the list is found by halves where there are more tensors than this
 #define GRAD_PARTS FLM_GRAD_WORKSPACE    // partial results at most
 
 struct GradItem {
@@ -152,7 +153,16 @@ __device__ __forceinline__ double grad_fold(double v, bool inf_norm, double* red
 // 16-byte boundary; f(item, offset, count, leading) gets them as `leading` (0..7) elements before `offset`.
 template <bool BACK, typename F>
 __device__ __forceinline__ void grad_chunks(const GradList& list, int first, int stride, F&& f) {
-  int t = BACK ? list.count - 1 : 0;
+  // the tensor of the first chunk: by halves down to a few, from there a step at a time (100 tensors of 1000 elements, replayed:
+  // 18 -> 8.1 us; lists of ten are better off with steps alone)
+  int lo = 0, hi = list.count - 1;
+  const int start = BACK ? list.chunks - 1 - first : first;
+  while (hi - lo > GRAD_STEPS) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (list.item[mid].first <= start) lo = mid;
+    else hi = mid - 1;
+  }
+  int t = BACK ? hi : lo;
   for (int i = first; i < list.chunks; i += stride) {
     const int c = BACK ? list.chunks - 1 - i : i;
     if (BACK) {
