@@ -635,6 +635,56 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
   }
 }
 
+// The same for few rows, one output a thread and one row a workgroup, in fp32 without the matrix cores: a fifth of the code
+// and three loads that wait for each other, which is what a launch of this size takes its time for.  V_e(n, .) contiguous.
+template <typename T>
+__global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs a, RowGroups g) {
+  __shared__ float low[FLM_ADAPTER_MAX_RANK + 8];
+  const int pos = blockIdx.y, n = blockIdx.x * blockDim.x + threadIdx.x, at = min(n, a.N - 1);
+  const int e = g.key[pos], row = g.order[pos];
+  float y = 0.f;
+  const float* p = a.part + (long)row * a.N + at;
+  const long step = (long)a.n * a.N;
+#pragma unroll 1
+  for (int z = 0; z < a.slices; z += 8) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = p[min(z + k, a.slices - 1) * step];
+#pragma unroll
+    for (int k = 0; k < 8; k++) y += z + k < a.slices ? v[k] : 0.f;
+  }
+  if (a.bias) y += (float)((const T*)a.bias)[at];
+  if (e < a.E) {                                             // (the same for the whole workgroup)
+    const float s = adapter_scale(a.scale, a.scale_all, e);
+    for (int j = threadIdx.x; j < a.rp; j += blockDim.x) {
+      const float* q = a.low + (long)pos * a.rp + j;
+      float f = 0.f;
+#pragma unroll 1
+      for (int z = 0; z < a.low_slices; z += 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = q[min(z + k, a.low_slices - 1) * a.low_step];
+#pragma unroll
+        for (int k = 0; k < 8; k++) f += z + k < a.low_slices ? v[k] : 0.f;
+      }
+      low[j] = j < a.r ? f : 0.f;
+    }
+    const T* v = (const T*)a.v + (long)e * a.v_group + (long)at * a.v_row;
+    Vec8<T> b = load8(v, a.r);
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < a.r; j += 8) {
+      const Vec8<T> c = b;
+      if (j + 8 < a.r) b = load8(v + j + 8, a.r - j - 8);
+#pragma unroll
+      for (int u = 0; u < 8; u++) t = __builtin_fmaf((float)c.v[u], low[j + u], t);
+    }
+    y = __builtin_fmaf(s, t, y);
+  }
+  if (n < a.N) ((T*)a.y)[(long)row * a.ldy + n] = (T)y;
+}
+
 // ---- the projection of many rows, 16-bit types -------------------------------------------------------------------------
 // Tiles of BM sorted rows x BN outputs, waves as WM x WN of them, 64 k a stage, two stages in LDS.  A thread fetches its
 // share of the stage after next into registers while the matrix cores work on one stage; it goes to LDS one stage later.
@@ -1351,6 +1401,15 @@ static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st
   return FLM_OK;
 }
 
+// Whether finish_rows_kernel ends a few-row projection: its vectors' way through the caches grows with the product, the
+// matrix cores' form takes a fixed time (replayed, with / without, all kernels of the call, bf16: one row of 13440 x 512, 16
+// ranks 8.2 / 12.3 us, 37 rows of 4096 x 4096 17.0 / 21.4, 16 rows of 128 ranks 24.7 / 30.7, 64 rows of 64 ranks 40.8 / 35.7;
+// fp32: 64 rows of 64 ranks 74 / 80, of 128 ranks, two adapters 58 / 48).
+template <typename T>
+static bool finish_by_rows(const FinishArgs& f) {
+  return (long)f.n * f.N * f.r <= (sizeof(T) == 4 ? 1L << 24 : 1L << 23);
+}
+
 // The narrow product (low_slices = 0: it is there already, as always with W_KN) and y = X * W^T + bias + adapters, any type
 // and size.  W is [N,K], or (W_KN) [K,N].  f.part / b.part: base_part_bytes() of workspace
 template <typename T, bool W_KN, bool V_STRIDED>
@@ -1360,6 +1419,12 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, const ShrinkArgs&
   if constexpr (!W_KN) {
     if (plan.form == BASE_ROWS) {
       if ((rc = launch_few_rows<T>(b, plan.slices, s, low_slices, g, st))) return rc;
+      if (finish_by_rows<T>(f)) {
+        const int threads = (long)f.n * f.N <= 32768 ? 64 : 256;
+        hipLaunchKernelGGL(finish_rows_kernel<T>, dim3((f.N + threads - 1) / threads, f.n), dim3(threads), 0, st, f, g);
+        FLM_CHECK_LAUNCH();
+        return FLM_OK;
+      }
       return launch_finish<T, V_STRIDED>(f, g, st);
     }
   }
