@@ -1237,9 +1237,10 @@ struct BasePlan {
 
 // The time of 128 x 128 tiles for n rows, in units of one round of 256 x 256 tiles (one a CU), and the K slices to take.
 // Measured: a round of 512 tiles of 128 x 128 (two a CU) takes 0.62 of one of 256 tiles of 256 x 256 that do twice its work,
-// half a round 0.4.  Slices are added up by a launch of its own: 5 us and 4 bytes per slice and output at 5 TB/s, against
-// 28.7 ns per k for a round.
-static double tiles_128_time(int n, int K, int N, int* slices, int* kslice) {
+// half a round 0.4.  Slices are added up at 4 bytes per slice and output and 5 TB/s, against 28.7 ns per k for a round, and
+// by a launch of its own: join ns, 5000, or 0 where whole tiles would have to wait for the narrow products' launch and slices
+// do not (250 rows of 512 x 1000 24 -> 14.6 us, 2000 of 2048 x 1024 41 -> 38).
+static double tiles_128_time(int n, int K, int N, double join, int* slices, int* kslice) {
   const double t = (double)((n + 127) / 128) * ((N + 127) / 128), rest = t - 512.0 * (long)(t / 512);
   *slices = 1;
   *kslice = K;
@@ -1247,7 +1248,7 @@ static double tiles_128_time(int n, int K, int N, int* slices, int* kslice) {
   int ks;
   const int s = k_slices((long)t, 512, K, 256, 16, &ks);
   if (s <= 1) return whole;
-  const double cut = 0.62 * t / 512 + (5000.0 + (4.0 * (2 * s) + 2) * n * N / 5000) / (28.7 * K);
+  const double cut = 0.62 * t / 512 + (join + (4.0 * (2 * s) + 2) * n * N / 5000) / (28.7 * K);
   if (cut >= whole) return whole;
   *slices = s;
   *kslice = ks;
@@ -1271,11 +1272,12 @@ static BasePlan base_plan(int n, int K, int N, bool f32, bool w_kn = false) {
   }
   if (f32) {
     b.form = BASE_X3;
-    b.slices = k_slices((long)((n + 127) / 128) * ((N + 127) / 128), 512, K, 512, 16, &b.kslice);
+    // (slices of at least 512 / 256 / 128 k: 100 rows of 512 x 256 39 / 26 / 19 us, 1001 of 700 x 515 51 / 35 / 31)
+    b.slices = k_slices((long)((n + 127) / 128) * ((N + 127) / 128), 512, K, 128, 16, &b.kslice);
     return b;
   }
   b.form = BASE_TILES;
-  double best = tiles_128_time(n, K, N, &b.slices, &b.kslice);
+  double best = tiles_128_time(n, K, N, w_kn ? 5000.0 : 0.0, &b.slices, &b.kslice);
   // all rows in large tiles, or as many row tiles as fill whole rounds and the rest in small ones
   const int rounds = (int)(((long)tm * tn + 255) / 256);
   if (rounds < best) {
@@ -1287,7 +1289,7 @@ static BasePlan base_plan(int n, int K, int N, bool f32, bool w_kn = false) {
   const int full = (int)((rounds - 1) * 256L / tn);
   if (full > 0 && full * 256 < n) {
     int s, ks;
-    const double t = rounds - 1 + tiles_128_time(n - full * 256, K, N, &s, &ks) + 3000.0 / (28.7 * K);
+    const double t = rounds - 1 + tiles_128_time(n - full * 256, K, N, 5000.0, &s, &ks) + 3000.0 / (28.7 * K);
     if (t < best) {
       b.rows = full * 256;
       b.slices = s;
