@@ -388,7 +388,7 @@ struct FinishArgs {
   const float* low;                      // [low_slices][sorted position][rp], low_step floats a slice
   long low_step;
   int low_slices, r, rp;
-  const void* v;                         // V_e(n, j) = v[e*v_group + n*v_row + j*v_j]; without V_STRIDED v_j = 1, r % 8 = 0
+  const void* v;                         // V_e(n, j) = v[e*v_group + n*v_row + j*v_j]; without V_STRIDED v_j = 1, r >= 8
   long v_group, v_row, v_j;
   const float* scale;                    // per adapter, or nullptr: scale_all
   float scale_all;
@@ -401,37 +401,35 @@ __device__ __forceinline__ float adapter_scale(const float* scale, float all, in
 
 // The scaled narrow products of `rows` sorted positions from pos on, as bf16 terms in LDS: lt[(term*rows + row)*stride + j],
 // stride = low_stride(rp).  threads of the workgroup share the work; a barrier follows at the caller.
+// Without V_STRIDED the last piece of eight ranks ends at the last rank, as AddAdapters reads it of V, and holds zeros where
+// it repeats those of the piece before.
 __device__ __forceinline__ int low_stride(int rp) { return rp + 8; }          // (16 bytes more: rows fall into different banks)
-template <int LOW>
+template <int LOW, bool V_STRIDED>
 __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& g, long pos, int rows, __bf16* lt) {
   const int per = a.rp >> 3, stride = low_stride(a.rp);
 #pragma unroll 1
   for (int i = threadIdx.x; i < rows * per; i += blockDim.x) {
-    const int row = i / per, j = (i - row * per) * 8;
+    const int row = i / per, j = (i - row * per) * 8, jr = V_STRIDED ? j : min(j, a.r - 8);
     float f[8];
 #pragma unroll
     for (int u = 0; u < 8; u++) f[u] = 0.f;
     const int e = pos + row < a.n ? g.key[pos + row] : a.E;
     if (e < a.E) {
-      const float* p = a.low + (pos + row) * a.rp + j;
+      const float* p = a.low + (pos + row) * a.rp + jr;
       const long step = a.low_step;
 #pragma unroll 1
       for (int z = 0; z < a.low_slices; z += 8) {                    // eight slices in flight, the last one again behind the end
-        f32x4 v[8][2];
+        Packed8<float> v[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const float* q = p + min(z + k, a.low_slices - 1) * step;
-          v[k][0] = reinterpret_cast<const f32x4*>(q)[0];
-          v[k][1] = reinterpret_cast<const f32x4*>(q)[1];
-        }
+        for (int k = 0; k < 8; k++) v[k] = *reinterpret_cast<const Packed8<float>*>(p + min(z + k, a.low_slices - 1) * step);
 #pragma unroll
         for (int k = 0; k < 8; k++)
 #pragma unroll
-          for (int u = 0; u < 8; u++) f[u] += z + k < a.low_slices ? v[k][u >> 2][u & 3] : 0.f;
+          for (int u = 0; u < 8; u++) f[u] += z + k < a.low_slices ? __uint_as_float(v[k].w[u]) : 0.f;
       }
       const float s = adapter_scale(a.scale, a.scale_all, e);
 #pragma unroll
-      for (int u = 0; u < 8; u++) f[u] = j + u < a.r ? f[u] * s : 0.f;
+      for (int u = 0; u < 8; u++) f[u] = u >= j - jr && jr + u < a.r ? f[u] * s : 0.f;
     }
     bf16x8 t[LOW];
     split_terms<LOW, true>(f, t);
@@ -477,9 +475,10 @@ struct AddAdapters {
     for (int b = 0; b < NB; b++)
 #pragma unroll
       for (int jj = 0; jj < JB; jj++) {
+        if (jj > 0 && j0 + 16 * jj >= a.r) break;              // (the same for all lanes)
         const int j = j0 + 16 * jj + 8 * h;
         const T* p = (const T*)a.v + (long)max(es[b], 0) * a.v_group + (long)n * a.v_row;
-        // (no test around a load: ranks behind the last are read from the last, or the first eight, and cleared)
+        // (no lane's test around a load: ranks behind the last are read from the last, or the last eight, and cleared)
         if (V_STRIDED) {
 #pragma unroll
           for (int i = 0; i < 8; i++) {
@@ -487,11 +486,10 @@ struct AddAdapters {
             v[b][jj].v[i] = j + i < a.r ? x : (T)0.f;
           }
         } else {
-          uint4 x[sizeof(T) / 2];
-          __builtin_memcpy(x, p + (j < a.r ? j : 0), sizeof(x));
+          const int jr = min(j, a.r - 8);
+          v[b][jj] = load8(p + jr, 8);
 #pragma unroll
-          for (int i = 0; i < (int)sizeof(T) / 2; i++) x[i] = j < a.r ? x[i] : make_uint4(0, 0, 0, 0);
-          __builtin_memcpy(&v[b][jj], x, sizeof(x));
+          for (int i = 0; i < 8; i++) v[b][jj].v[i] = i < j - jr ? (T)0.f : v[b][jj].v[i];
         }
       }
   }
@@ -516,7 +514,8 @@ struct AddAdapters {
         if (es[b] >= 0) {
           bf16x8 vt[JB][Terms<T>::own];
 #pragma unroll
-          for (int jj = 0; jj < JB; jj++) own_terms<T>(v[b][jj], vt[jj]);
+          for (int jj = 0; jj < JB; jj++)
+            if (jj == 0 || j0 + 16 * jj < a.r) own_terms<T>(v[b][jj], vt[jj]);
 #pragma unroll
           for (int mi = 0; mi < MI; mi++) {
             const bool mine = key[mi] == es[b];
@@ -599,7 +598,7 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
         if (n < a.N) acc[0][r] += p[z * step + n];
       }
   }
-  stage_low<Terms<T>::low>(a, g, pos, 32, lt);
+  stage_low<Terms<T>::low, V_STRIDED>(a, g, pos, 32, lt);
   for (int o = span; o < 32; o <<= 1)
 #pragma unroll
     for (int r = 0; r < 16; r++) acc[0][r] += __shfl_xor(acc[0][r], o);
@@ -846,7 +845,7 @@ __device__ __forceinline__ void wide_tile(const BaseArgs& b, const FinishArgs& a
       key[mi] = pos < b.n ? g.key[pos] : a.E;
     }
     __bf16* lt = reinterpret_cast<__bf16*>(lds);
-    stage_low<Terms<T>::low>(a, g, m0, BM, lt);
+    stage_low<Terms<T>::low, V_STRIDED>(a, g, m0, BM, lt);
     __syncthreads();
 #pragma unroll
     for (int ni = 0; ni < NI; ni++)
@@ -985,7 +984,7 @@ struct OuterArgs {
   float* part;                           // [chunks][2][r*KQ], laid out as out
   void* out;                             // out[e*r*KQ + j*o_j + q*o_q]
   long o_j, o_q;
-  int across;                            // workgroups over the columns
+  int cols, across;                      // workgroups over the columns, and over columns and blocks of ranks
 };
 
 // CPL neighbouring elements as words
@@ -1021,7 +1020,8 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
   const OuterArgs a = one ? first : second;
   const int block = one ? blockIdx.x : blockIdx.x - groups, chunk = block / a.across;
   const int t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, g.first_tile[a.E]);
-  const int q0 = ((block - chunk * a.across) * 4 + w) * (16 * CPL), q = q0 + c * CPL;
+  const int part_of = block - chunk * a.across, rank0 = part_of / a.cols * (16 * NRJ);
+  const int q0 = (part_of % a.cols * 4 + w) * (16 * CPL), q = q0 + c * CPL;
   if (t0 >= t1) return;
   // whichever axis is contiguous in the result ends up four neighbouring elements a lane: the ranks' (by_rank: a lane holds
   // one rank and 4*CPL neighbouring columns) or the columns' (one column and four neighbouring ranks)
@@ -1073,7 +1073,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
   auto fetch_p = [&](int2 tile) {
 #pragma unroll
     for (int k = 0; k < PI; k++) {
-      const int i = tid + 256 * k, m = i / PER, j = (i - m * PER) * 8;
+      const int i = tid + 256 * k, m = i / PER, j = rank0 + (i - m * PER) * 8;
       const float* p = a.p + (long)p_row[k] * a.pld + (j < a.r ? j : 0);
       Vec8<float> f;
       if (j + 8 <= a.pld || j >= a.r) f = load8(p, min(8, a.pld));
@@ -1115,7 +1115,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
       const int col = q0 + 4 * h * CPL;
 #pragma unroll
       for (int jj = 0; jj < NRJ; jj++) {
-        const int j = jj * 16 + at;
+        const int j = rank0 + jj * 16 + at;
         if (j >= a.r) continue;
 #pragma unroll
         for (int i = 0; i < CPL; i++) {
@@ -1133,7 +1133,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
         if (col >= a.KQ) continue;
 #pragma unroll
         for (int jj = 0; jj < NRJ; jj++) {
-          const int j = jj * 16 + 4 * h;
+          const int j = rank0 + jj * 16 + 4 * h;
           const float v[4] = {acc[jj][u][0], acc[jj][u][1], acc[jj][u][2], acc[jj][u][3]};
           if (whole) store4(out + (long)col * a.o_q + j, v, a.r - j);
           else store4(part + (long)col * a.o_q + j, v, a.r - j);
@@ -1233,32 +1233,49 @@ enum { BASE_ROWS, BASE_X3, BASE_TILES };
 struct BasePlan {
   int form, slices, kslice;              // of the rows behind the first `rows`
   int rows;
+  bool straight;                         // these rows' tiles go straight to the result (one slice); otherwise finish_kernel ends them
 };
+
+// What the adapters cost at the end of tiles of 64 rows a wave and 64 outputs / in finish_kernel, ns: an adapter is 300 ns and
+// 15 (10) per rank, one after the other (204 rows of 50 adapters, 120 ranks: 84 us in the tiles, 6 in finish_kernel).
+static double adapters_64_time(int n, int N, int r, int E) {
+  const long tiles = (long)((n + 127) / 128) * ((N + 127) / 128);
+  const double each = 1.0 + 64.0 * E / n;
+  return (double)((tiles + 511) / 512) * 2 * (each < 64 ? each : 64) * (300 + 15 * r);
+}
+static double adapters_finish_time(int n, int N, int r, int E) {
+  const double tiles = (double)((n + 31) / 32) * ((N + 31) / 32), each = 1.0 + 32.0 * E / n;
+  return (tiles > 1024 ? tiles / 1024 : 1.0) * (each < 32 ? each : 32) * (tiles <= 256 ? 0.25 : 1.0) * (300 + 10 * r);
+}
 
 // The time of 128 x 128 tiles for n rows, in units of one round of 256 x 256 tiles (one a CU), and the K slices to take.
 // Measured: a round of 512 tiles of 128 x 128 (two a CU) takes 0.62 of one of 256 tiles of 256 x 256 that do twice its work,
 // half a round 0.4.  Slices are added up at 4 bytes per slice and output and 5 TB/s, against 28.7 ns per k for a round, and
 // by a launch of its own: join ns, 5000, or 0 where whole tiles would have to wait for the narrow products' launch and slices
 // do not (250 rows of 512 x 1000 24 -> 14.6 us, 2000 of 2048 x 1024 41 -> 38).
-static double tiles_128_time(int n, int K, int N, double join, int* slices, int* kslice) {
+static double tiles_128_time(int n, int K, int N, int r, int E, double join, int* slices, int* kslice, bool* straight) {
   const double t = (double)((n + 127) / 128) * ((N + 127) / 128), rest = t - 512.0 * (long)(t / 512);
   *slices = 1;
   *kslice = K;
-  const double whole = 0.62 * (long)(t / 512) + (rest == 0 ? 0 : (rest <= 256 ? 0.4 : 0.62));
+  *straight = true;
+  const double round = 28.7 * K, last = rest == 0 ? 0 : (rest <= 256 ? 0.4 : 0.62);
+  const double whole = 0.62 * (long)(t / 512) + last + adapters_64_time(n, N, r, E) / round;
   int ks;
   const int s = k_slices((long)t, 512, K, 256, 16, &ks);
-  if (s <= 1) return whole;
-  const double cut = 0.62 * t / 512 + (join + (4.0 * (2 * s) + 2) * n * N / 5000) / (28.7 * K);
+  const double cut = (s > 1 ? 0.62 * t / 512 : 0.62 * (long)(t / 512) + last) +
+                     (join + (4.0 * (2 * s) + 2) * n * N / 5000 + adapters_finish_time(n, N, r, E)) / round;
   if (cut >= whole) return whole;
   *slices = s;
   *kslice = ks;
+  *straight = false;
   return cut;
 }
 
 // w_kn: W is [K,N]: the few-row form is for [N,K] only.
-static BasePlan base_plan(int n, int K, int N, bool f32, bool w_kn = false) {
+static BasePlan base_plan(int n, int K, int N, int r, int E, bool f32, bool w_kn = false) {
   BasePlan b;
   b.rows = 0;
+  b.straight = false;
   b.slices = 1;
   b.kslice = K;
   const int tn = (N + 255) / 256, tm = (n + 255) / 256;
@@ -1277,20 +1294,26 @@ static BasePlan base_plan(int n, int K, int N, bool f32, bool w_kn = false) {
     return b;
   }
   b.form = BASE_TILES;
-  double best = tiles_128_time(n, K, N, w_kn ? 5000.0 : 0.0, &b.slices, &b.kslice);
+  double best = tiles_128_time(n, K, N, r, E, w_kn ? 5000.0 : 0.0, &b.slices, &b.kslice, &b.straight);
   // all rows in large tiles, or as many row tiles as fill whole rounds and the rest in small ones
   const int rounds = (int)(((long)tm * tn + 255) / 256);
-  if (rounds < best) {
-    best = rounds;
+  const double each = 1.0 + 128.0 * E / n, walk = 2 * (each < 128 ? each : 128) * (300 + 15 * r) / (28.7 * K);
+  if (rounds * (1 + walk) < best) {
+    best = rounds * (1 + walk);
     b.rows = n;
     b.slices = 1;
     b.kslice = K;
+    b.straight = true;
   }
   const int full = (int)((rounds - 1) * 256L / tn);
   if (full > 0 && full * 256 < n) {
     int s, ks;
-    const double t = rounds - 1 + tiles_128_time(n - full * 256, K, N, 5000.0, &s, &ks) + 3000.0 / (28.7 * K);
+    bool straight;
+    // (the rows behind use as many adapters a row as all do)
+    const int behind = n - full * 256, e = 1 + (int)((long)E * behind / n);
+    const double t = (rounds - 1) * (1 + walk) + tiles_128_time(behind, K, N, r, e, 5000.0, &s, &ks, &straight) + 3000.0 / (28.7 * K);
     if (t < best) {
+      b.straight = straight;
       b.rows = full * 256;
       b.slices = s;
       b.kslice = ks;
@@ -1300,7 +1323,7 @@ static BasePlan base_plan(int n, int K, int N, bool f32, bool w_kn = false) {
 }
 // bytes of the projection's partial sums (0: it goes straight to the result)
 static long base_part_bytes(const BasePlan& b, int n, int N) {
-  return b.form == BASE_TILES && (b.slices == 1 || b.rows == n) ? 0 : 4L * b.slices * (n - b.rows) * N;
+  return b.form == BASE_TILES && b.straight ? 0 : 4L * b.slices * (n - b.rows) * N;
 }
 struct ShrinkPlan { int slices, kslice; };
 static ShrinkPlan shrink_plan(int n, int K, int E) {
@@ -1436,7 +1459,7 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, const ShrinkArgs&
     else rc = launch_parts<float, false>(b, plan.slices, g, s, low_slices, st);
     if (rc) return rc;
   } else {
-    const bool beside = plan.rows == 0 && plan.slices > 1;           // nothing needs low before it is through
+    const bool beside = plan.rows == 0 && !plan.straight;            // nothing needs low before it is through
     if (!W_KN && low_slices && !beside && (rc = launch_shrink<T, false>(s, g, low_slices, st))) return rc;
     if (plan.rows) {
       BaseArgs large = b;
@@ -1453,29 +1476,35 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, const ShrinkArgs&
     b.n = f.n = b.n - plan.rows;
     f.low += (long)plan.rows * f.rp;
     f.part_sorted = 1;
-    if (plan.slices == 1) return launch_wide<T, 128, 128, 2, 2, W_KN, V_STRIDED>(b, f, rest, st);
+    if (plan.straight) return launch_wide<T, 128, 128, 2, 2, W_KN, V_STRIDED>(b, f, rest, st);
     if ((rc = launch_parts<T, W_KN>(b, plan.slices, rest, s, beside ? low_slices : 0, st))) return rc;
     return launch_finish<T, V_STRIDED>(f, rest, st);
   }
   return launch_finish<T, V_STRIDED>(f, g, st);
 }
 
-// Columns a lane of outer_kernel holds: 16 bytes' worth, half where 128 ranks leave no registers.
-static int outer_cols(int r, bool f32) { return f32 || r > 64 ? 4 : 8; }
+// Columns a lane of outer_kernel holds: 16 bytes' worth, half of 16-bit types where more than 32 ranks leave no registers;
+// ranks go in blocks of 64 (16282 rows, 79 ranks, fp32: 88 us, all ranks in one workgroup 144).
+static int outer_cols(int r, bool f32) { return f32 || r > 32 ? 4 : 8; }
+static int outer_across(int KQ, int r, bool f32) {
+  const int cols = 64 * outer_cols(r, f32);
+  return (KQ + cols - 1) / cols * ((r + 63) / 64);
+}
 
 // both gradients
 template <typename T>
 static int launch_outer(OuterArgs a, OuterArgs b, const RowGroups& g, hipStream_t st) {
   constexpr int CPL = sizeof(T) == 4 ? 4 : 8;
-  const int cols = 64 * outer_cols(a.r, sizeof(T) == 4);
-  a.across = (a.KQ + cols - 1) / cols;
-  b.across = (b.KQ + cols - 1) / cols;
+  const int ranks = (a.r + 63) / 64;
+  a.across = outer_across(a.KQ, a.r, sizeof(T) == 4);
+  b.across = outer_across(b.KQ, b.r, sizeof(T) == 4);
+  a.cols = a.across / ranks;
+  b.cols = b.across / ranks;
   const int groups = a.across * ((g.cap + a.chunk - 1) / a.chunk);
   const dim3 grid(groups + b.across * ((g.cap + b.chunk - 1) / b.chunk));
   if (a.r <= 16) hipLaunchKernelGGL((outer_kernel<T, 1, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
   else if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 2, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
-  else if (a.r <= 64) hipLaunchKernelGGL((outer_kernel<T, 4, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
-  else hipLaunchKernelGGL((outer_kernel<T, 8, 4>), grid, dim3(256), 0, st, a, b, groups, g);
+  else hipLaunchKernelGGL((outer_kernel<T, 4, 4>), grid, dim3(256), 0, st, a, b, groups, g);
   FLM_CHECK_LAUNCH();
   const long most = (long)a.r * (a.KQ > b.KQ ? a.KQ : b.KQ);
   hipLaunchKernelGGL(outer_join_kernel<T>, dim3((unsigned)((most + 1023) / 1024), a.E, 2), dim3(256), 0, st, a, b, g);
@@ -1489,8 +1518,7 @@ static long round16(long bytes) { return (bytes + 255) & ~255L; }
 // spans costs a partial sum, and half as many workgroups are better (4099 rows of 24 adapters, chunks of 2 / 4 tiles: product
 // and join 65 / 54 us; 512 rows of 20, 3 / 7 tiles: 23 / 34 us).
 static int outer_chunk(long tiles, int n, int E, int KQ, int r, bool f32) {
-  const int cols = 64 * outer_cols(r, f32);
-  const long work = tiles * ((KQ + cols - 1) / cols), group = n / (32L * E);
+  const long work = tiles * outer_across(KQ, r, f32), group = n / (32L * E);
   const long c = work / 512, most = work / 256;
   const long wish = group < most ? group : most;
   return (int)(c > wish ? (c < 1 ? 1 : c) : (wish < 1 ? 1 : wish));
@@ -1505,13 +1533,13 @@ static int forward(const void* x, long ldx, const void* w, long ldw, const void*
                    long ldy, float* low, hipStream_t st) {
   const int rp = ranks_padded(r);
   const ShrinkPlan ss = shrink_plan(n, K, E);
-  const BasePlan bs = base_plan(n, K, N, sizeof(T) == 4);
+  const BasePlan bs = base_plan(n, K, N, r, E, sizeof(T) == 4);
   float* low_part = (float*)ws;
   float* part = (float*)(ws + round16(4L * ss.slices * n * rp));
   const ShrinkArgs s{x, a, ldx, (long)r * K, K, 1, K, r, rp, n, ss.kslice, low_part};
   const FinishArgs f{part, bs.slices, 0, bias, low_part, (long)n * rp, ss.slices, r, rp, b, (long)N * r, r, 1, scale, scale_all, n, N, E, y, ldy};
   const BaseArgs base{x, w, ldx, ldw, n, K, N, bs.kslice, part};
-  const int rc = r % 8 == 0 ? launch_projection<T, false, false>(base, bs, s, ss.slices, f, g, st)
+  const int rc = r >= 8 ? launch_projection<T, false, false>(base, bs, s, ss.slices, f, g, st)
                             : launch_projection<T, false, true>(base, bs, s, ss.slices, f, g, st);
   if (rc) return rc;
   if (low) {
@@ -1543,7 +1571,7 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
                             OuterArgs{low, r, 1, dy, lddy, N, r, E, n, cb, scale, scale_all, part_b, db, 1, r, 0}, g, st)))
     return rc;
   if (!dx) return FLM_OK;
-  const BasePlan bs = base_plan(n, N, K, sizeof(T) == 4, true);
+  const BasePlan bs = base_plan(n, N, K, r, E, sizeof(T) == 4, true);
   float* dx_part = (float*)ws;
   const FinishArgs f{dx_part, bs.slices, 0, nullptr, u, (long)n * rp, 1, r, rp, a, (long)r * K, 1, K, scale, scale_all, n, K, E, dx, lddx};
   return launch_projection<T, true, true>(BaseArgs{dy, w, lddy, ldw, n, N, K, bs.kslice, dx_part}, bs, s, 0, f, g, st);
@@ -1574,7 +1602,7 @@ static bool adapter_sizes(int n, int K, int N, int r, int E, int dtype) {
 
 extern "C" long flm_adapter_workspace(int n, int K, int N, int r, int E, int dtype) {
   if (!adapter_sizes(n, K, N, r, E, dtype)) return 0;
-  return round16(4L * shrink_plan(n, K, E).slices * n * ranks_padded(r)) + base_part_bytes(base_plan(n, K, N, dtype == FLM_F32), n, N) +
+  return round16(4L * shrink_plan(n, K, E).slices * n * ranks_padded(r)) + base_part_bytes(base_plan(n, K, N, r, E, dtype == FLM_F32), n, N) +
          256;
 }
 
@@ -1584,7 +1612,7 @@ extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E
   const int ca = outer_chunk(tiles, n, E, K, r, dtype == FLM_F32), cb = outer_chunk(tiles, n, E, N, r, dtype == FLM_F32);
   long rest = 4L * r * (outer_part(tiles, ca) * K + outer_part(tiles, cb) * N);
   if (need_dx) {
-    const long base = base_part_bytes(base_plan(n, N, K, dtype == FLM_F32, true), n, K);
+    const long base = base_part_bytes(base_plan(n, N, K, r, E, dtype == FLM_F32, true), n, K);
     if (base > rest) rest = base;
   }
   return round16(4L * shrink_plan(n, N, E).slices * n * ranks_padded(r)) + rest + 256;
