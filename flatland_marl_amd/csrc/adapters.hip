@@ -15,10 +15,6 @@
 
 namespace flm {
 
-// C[slice][M,N] = A[M,K] * B over K slices with the fp32 product of the dense layers (dqn.hip); B is [N,K] (b_kc) or [K,N]
-int gemm_x3_slices(const float* A, long lda, const float* B, long ldb, bool b_kc, float* C, int M, int N, int K, int slices,
-                   int kslice, hipStream_t stream);
-
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -925,13 +921,13 @@ __global__ __launch_bounds__(256, 2) void parts_kernel(BaseArgs b, ShrinkArgs s,
 }
 
 // the same for fp32: the first gx * gy * gz workgroups are the dense layers' product over K slices
-template <int NR>
+template <int NR, bool W_KN>
 __global__ __launch_bounds__(512, 4) void x3_parts_kernel(GemmArgs p, unsigned gx, unsigned gy, unsigned gz, ShrinkArgs s, RowGroups g,
                                                           int low_slices) {
   extern __shared__ __attribute__((aligned(16))) unsigned x3_lds[];
   const int i = (int)blockIdx.x - (int)(gx * gy * gz);
   if (i < 0) {
-    gemm_x3_body<true, true, EPI_PLAIN>(p, blockIdx.x, gx, gy, gz, x3_lds);
+    gemm_x3_body<true, !W_KN, EPI_PLAIN, 0, true>(p, blockIdx.x, gx, gy, gz, x3_lds);
   } else {
     const int rest = i / g.cap;
     shrink_tile<float, 2, NR, 1, 8, false>(s, g, i - rest * g.cap, rest % low_slices, rest / low_slices * 16 * NR,
@@ -1388,9 +1384,9 @@ static int launch_parts_ranks(const BaseArgs& b, int slices, const RowGroups& g,
     p.M = b.n; p.N = b.N; p.K = b.K; p.lda = b.ldx; p.ldb = b.ldw; p.ldc = b.N;
     p.ksplit = slices > 1 ? b.kslice : 0; p.c_zs = (long)b.n * b.N;
     const unsigned gx = (b.N + GBN - 1) / GBN, gy = (b.n + GBM - 1) / GBM;
-    FLM_RAISE_LDS_ONCE(x3_parts_kernel<NR>);
-    hipLaunchKernelGGL(x3_parts_kernel<NR>, dim3(gx * gy * slices + low), dim3(512), X3_LDS_BYTES, st, p, gx, gy, (unsigned)slices, s, g,
-                       low_slices);
+    FLM_RAISE_LDS_ONCE((x3_parts_kernel<NR, W_KN>));
+    hipLaunchKernelGGL((x3_parts_kernel<NR, W_KN>), dim3(gx * gy * slices + low), dim3(512), X3_LDS_BYTES, st, p, gx, gy, (unsigned)slices,
+                       s, g, low_slices);
   } else {
     const int tiles = ((b.n + 127) / 128) * ((b.N + 127) / 128);
     const size_t lds = 128 * (128 * 4 + 16);                         // (the stages take 64 KiB, the result a little more)
@@ -1454,10 +1450,7 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, const ShrinkArgs&
     }
   }
   if constexpr (sizeof(T) == 4) {
-    if constexpr (W_KN) rc = gemm_x3_slices((const float*)b.x, b.ldx, (const float*)b.w, b.ldw, false, b.part, b.n, b.N, b.K, plan.slices,
-                                            b.kslice, st);
-    else rc = launch_parts<float, false>(b, plan.slices, g, s, low_slices, st);
-    if (rc) return rc;
+    if ((rc = launch_parts<float, W_KN>(b, plan.slices, g, s, low_slices, st))) return rc;
   } else {
     const bool beside = plan.rows == 0 && !plan.straight;            // nothing needs low before it is through
     if (!W_KN && low_slices && !beside && (rc = launch_shrink<T, false>(s, g, low_slices, st))) return rc;

@@ -49,17 +49,6 @@ static int launch_gemm(const GemmArgs& g, int nz, hipStream_t stream) {
   return FLM_OK;
 }
 
-// the product for other files (flm_adapter_linear): C[slice][M,N] = A[M,K] * B over K slices of kslice; B is [N,K] (b_kc)
-// or [K,N]
-int gemm_x3_slices(const float* A, long lda, const float* B, long ldb, bool b_kc, float* C, int M, int N, int K, int slices,
-                   int kslice, hipStream_t stream) {
-  GemmArgs g{};
-  g.A = A; g.B = B; g.C = C;
-  g.M = M; g.N = N; g.K = K; g.lda = lda; g.ldb = ldb; g.ldc = N;
-  g.ksplit = slices > 1 ? kslice : 0; g.c_zs = (long)M * N;
-  return b_kc ? launch_gemm<true, true, EPI_PLAIN>(g, slices, stream) : launch_gemm<true, false, EPI_PLAIN>(g, slices, stream);
-}
-
 // out[n] = sum over z of part[z*n_elem + n]  (deterministic reduction: 16 waves take every 16th slice each, their
 // sums meet in LDS in wave order)
 __global__ __launch_bounds__(1024) void reduce_partials_kernel(const float* __restrict__ part, int nz, long n_elem,

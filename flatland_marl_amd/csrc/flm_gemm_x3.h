@@ -82,8 +82,10 @@ __device__ __forceinline__ void split3(float x, unsigned& h, unsigned& m, unsign
 // FAST: the slice lies inside the matrix and its rows are 16-byte aligned: no test around any load.
 // SEG: the operand's contiguous axis (k when KC, the rows otherwise) is mapped through segments (GemmArgs::b_seg_*);
 // the 16-byte loads are then only 4-byte aligned, which global memory allows.
+// EDGE (with FAST): rows at any float, and the slice may pass the last row, whose place the rows behind are then read from
+// (their results are not stored); without KC the number of rows is a multiple of four.
 struct __attribute__((aligned(4))) F4U { float v[4]; };
-template <bool KC, bool FAST, bool SEG = false>
+template <bool KC, bool FAST, bool SEG = false, bool EDGE = false>
 __device__ __forceinline__ void fetch_x3(const float* __restrict__ P, long ld, int r0, int rmax, int k0, int kmax, bool vec,
                                          int tid, float (&v)[2][4], int break_k = 0, long break_off = 0, int seg_len = 0,
                                          int seg_stride = 0, unsigned seg_magic = 0) {
@@ -94,6 +96,7 @@ __device__ __forceinline__ void fetch_x3(const float* __restrict__ P, long ld, i
     bool ok;
     if (KC) {
       r = r0 + (tid >> 2);
+      if (EDGE && FAST) r = min(r, rmax - 1);
       k = k0 + 16 * half + 4 * (tid & 3);
       if (SEG) {
         const unsigned sg = __umulhi((unsigned)k, seg_magic);
@@ -104,6 +107,7 @@ __device__ __forceinline__ void fetch_x3(const float* __restrict__ P, long ld, i
       ok = r < rmax && k + 3 < kmax;
     } else {
       r = r0 + 4 * (tid >> 4);
+      if (EDGE && FAST) r = min(r, rmax - 4);
       k = k0 + 16 * half + (tid & 15);
       long rr = r;
       if (SEG) {                      // the rows of this operand are the mapped axis (four consecutive ones stay together)
@@ -113,7 +117,7 @@ __device__ __forceinline__ void fetch_x3(const float* __restrict__ P, long ld, i
       p = P + (long)k * ld + rr + ((break_k > 0 && k >= break_k) ? break_off : 0);
       ok = k < kmax && r + 3 < rmax;
     }
-    if (SEG && (FAST || (vec && ok))) {
+    if ((SEG && (FAST || (vec && ok))) || (EDGE && FAST)) {
       const F4U t = *reinterpret_cast<const F4U*>(p);
       v[half][0] = t.v[0]; v[half][1] = t.v[1]; v[half][2] = t.v[2]; v[half][3] = t.v[3];
     } else if (FAST || (vec && ok)) {
@@ -186,8 +190,9 @@ __device__ __forceinline__ void stage_schedule() {
 }
 
 // One workgroup (512 threads) of the product; li: its launch index among gx * gy * gz, x3_lds: X3_LDS_BYTES of LDS,
-// [stage][A, B][split][row][XROW].
-template <bool A_KC, bool B_KC, int EPI, int SEG = 0>
+// [stage][A, B][split][row][XROW].  EDGE: operands at any float and matrices that end inside a tile keep the loads without
+// tests (fetch_x3).
+template <bool A_KC, bool B_KC, int EPI, int SEG = 0, bool EDGE = false>
 __device__ __forceinline__ void gemm_x3_body(const GemmArgs& g, unsigned li, unsigned gx, unsigned gy, unsigned gz,
                                              unsigned* x3_lds) {
   constexpr bool B_SEG = SEG == 1 || SEG == 2;
@@ -254,15 +259,15 @@ __device__ __forceinline__ void gemm_x3_body(const GemmArgs& g, unsigned li, uns
       acc[i] = c;
     }
   };
-  auto run = [&](auto fast_tag) {
+  auto run = [&](auto fast_tag, int k_begin, int k_end) {
     constexpr bool FAST = decltype(fast_tag)::value;
     const int nf = (k_end - k_begin + XBK - 1) / XBK;          // fetches of 32 k; stages 2f and 2f+1 hold fetch f
     float a0[2][4], b0[2][4], a1[2][4], b1[2][4];
     auto fetch = [&](int f, float (&ra)[2][4], float (&rb)[2][4]) {
       // past the end the last slice is fetched again (FAST has no tests) and never placed
       const int k0 = k_begin + (FAST ? min(f, nf - 1) : f) * XBK;
-      fetch_x3<A_KC, FAST>(A, g.lda, m0, g.M, k0, k_end, a_vec, tid, ra);
-      fetch_x3<B_KC, FAST, B_SEG>(B, g.ldb, n0, g.N, k0, k_end, b_vec, tid, rb, g.b_break_k, g.b_break_off, g.b_seg_len,
+      fetch_x3<A_KC, FAST, false, EDGE>(A, g.lda, m0, g.M, k0, k_end, a_vec, tid, ra);
+      fetch_x3<B_KC, FAST, B_SEG, EDGE>(B, g.ldb, n0, g.N, k0, k_end, b_vec, tid, rb, g.b_break_k, g.b_break_off, g.b_seg_len,
                                   g.b_seg_stride, g.b_seg_magic);
     };
     auto place = [&](int stage, int half, const float (&ra)[2][4], const float (&rb)[2][4]) {
@@ -311,9 +316,20 @@ __device__ __forceinline__ void gemm_x3_body(const GemmArgs& g, unsigned li, uns
       products();
     }
   };
-  const bool full = a_vec && b_vec && m0 + GBM <= g.M && n0 + GBN <= g.N && ((k_end - k_begin) & (XBK - 1)) == 0;
-  if (full) run(std::true_type{});
-  else run(std::false_type{});
+  if constexpr (EDGE) {
+    static_assert(A_KC && !B_SEG, "");
+    // whole fetches without tests, what is left of k with them
+    const int whole = B_KC || (g.N & 3) == 0 ? k_begin + (k_end - k_begin) / XBK * XBK : k_begin;
+    if (whole > k_begin) run(std::true_type{}, k_begin, whole);
+    if (whole < k_end) {
+      __syncthreads();
+      run(std::false_type{}, whole, k_end);
+    }
+  } else {
+    const bool full = a_vec && b_vec && m0 + GBM <= g.M && n0 + GBN <= g.N && ((k_end - k_begin) & (XBK - 1)) == 0;
+    if (full) run(std::true_type{}, k_begin, k_end);
+    else run(std::false_type{}, k_begin, k_end);
+  }
   {
     const int n = n0 + wn * 32 + (lane & 31);
     if (n < g.N) {
