@@ -261,7 +261,8 @@ struct ShrinkArgs {
   float* out;                            // [slice][sorted position][rp]; what lies behind r is not meant to be read
 };
 
-// low (or u) of row tile t: its 16*MR rows times ranks rank .. rank + 16*NR - 1 of their adapter, over one K slice.
+// low (or u) of row tile t, read once from memory, the adapter's vectors from the L2 (16384 rows of 4096 bf16, 64 ranks: 55-60
+// us, 134 MB of rows; 4099 rows, 32 ranks: 13 us, 2.5 TB/s): its 16*MR rows times ranks rank .. rank + 16*NR - 1 of their adapter, over one K slice.
 // A workgroup of PARTS waves; red: PARTS * MR * NR * 64 of LDS
 template <typename T, int MR, int NR, int S, int PARTS, bool V_STRIDED>
 __device__ __forceinline__ void shrink_tile(const ShrinkArgs& a, const RowGroups& g, int t, int slice, int rank, f32x4* red) {
@@ -347,7 +348,9 @@ struct BaseArgs {
 
 // Up to 64 rows: the projection (16*MR rows x 16*NR outputs a workgroup) and the narrow products (32 rows x 16 ranks) in one
 // launch.  The first base_groups workgroups are (output block, K slice) pairs of the projection, the others (tile, K slice,
-// rank block) of the narrow product: at these sizes both are streams of weights with little else to do.
+// rank block) of the narrow product: at these sizes both are streams of weights with little else to do.  One row of 13440 x 512
+// fp32: 8.3 us, 29 MB at 3.4 TB/s; 37 rows of 4096 x 4096 bf16, 24 adapters: 13.5 us, 37 MB at 2.7 TB/s: the loads' latency
+// twice over and the way through the CUs (48 rows of X pass every workgroup) rather than the memory.
 template <typename T, int MRS, int MR, int NR>
 __global__ __launch_bounds__(256) void few_rows_kernel(BaseArgs a, ShrinkArgs s, RowGroups g, int base_groups, int low_slices) {
   __shared__ f32x4 red[4 * (MR * NR > MRS ? MR * NR : MRS) * 64];
@@ -540,7 +543,8 @@ struct AddAdapters {
 };
 
 // y = sum of the K slices + bias + adapters: 32 sorted rows and 32 outputs a wave, or (SHARED) a workgroup of four waves
-// that take the K slices and the adapters in turn and meet in LDS.
+// that take the K slices and the adapters in turn and meet in LDS.  Bound by its chain of dependent loads where tiles are few, by
+// the slices' way from the caches where they are many (512 x 512 outputs, 16 slices, fp32: 9.5 us; 1001 x 515: 8.4).
 template <typename T, bool V_STRIDED, bool SHARED>
 __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) {
   extern __shared__ __attribute__((aligned(16))) __bf16 lt[];
@@ -638,7 +642,8 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a, RowGroups g) 
 }
 
 // The same for few rows, one output a thread and one row a workgroup, in fp32 without the matrix cores: a fifth of the code
-// and three loads that wait for each other, which is what a launch of this size takes its time for.  V_e(n, .) contiguous.
+// and three loads that wait for each other, which is what a launch of this size takes its time for (one row of 512 outputs 3.3
+// us, finish_kernel 7.9; 37 of 4096 4.2, 7.5).  V_e(n, .) contiguous.
 template <typename T>
 __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs a, RowGroups g) {
   __shared__ float low[FLM_ADAPTER_MAX_RANK + 8];
@@ -694,6 +699,9 @@ __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs a, RowGroup
 // reads at once fall into different banks.  The weight is the instruction's first operand: a lane then holds one row's
 // outputs, four consecutive ones at a time.
 // FUSED: with bias and adapters, straight to y.  Otherwise one K slice to part[slice][position][N].
+// 16384 rows of 4096 x 4096 bf16, 48 adapters of 64 ranks: 560-610 us, 1.0 PFLOP/s; 1.17 in the loop (LDS and the matrix cores
+// are both busy nine tenths of it), 12 us a round of tiles for the adapters and the stores.  Four waves of 128 x 128 with half
+// the LDS reads: a fifth slower (nothing hides a wave's own fetches).  W_KN, 4096 rows of 4096 x 4096: 155 us.
 // li: the workgroup's index among the tiles; lds: wide_lds_bytes()
 #define WIDE_K 64
 // W_KN: W is [K,N] with contiguous outputs (the gradient of the inputs).  A thread then fetches eight outputs of four
@@ -912,7 +920,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void base_wide_kernel(BaseArgs b, 
 }
 
 // K slices of the projection, and beside them the narrow products (ranks in blocks of 16*NR), in one launch: the products of
-// the first `tiles` * slices workgroups keep the matrix cores busy, the others mostly wait for memory.
+// the first `tiles` * slices workgroups keep the matrix cores busy, the others mostly wait for memory (1001 rows of 1003 x 515
+// fp16: 14 us, rows at odd addresses).
 template <typename T, int NR, bool W_KN>
 __global__ __launch_bounds__(256, 2) void parts_kernel(BaseArgs b, ShrinkArgs s, RowGroups g, int tiles, int slices, int low_slices) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -927,7 +936,8 @@ __global__ __launch_bounds__(256, 2) void parts_kernel(BaseArgs b, ShrinkArgs s,
   }
 }
 
-// the same for fp32: the first gx * gy * gz workgroups are the dense layers' product over K slices
+// the same for fp32: the first gx * gy * gz workgroups are the dense layers' product over K slices (512 rows of 13440 x 512: 48
+// us, 42 GFLOP of bf16 products at 0.88 PFLOP/s)
 template <int NR, bool W_KN>
 __global__ __launch_bounds__(512, 4) void x3_parts_kernel(GemmArgs p, unsigned gx, unsigned gy, unsigned gz, ShrinkArgs s, RowGroups g,
                                                           int low_slices) {
@@ -975,7 +985,8 @@ __global__ __launch_bounds__(256) void low_rows_kernel(const float* __restrict__
 // and P one.
 // A group that lies inside one chunk is written at once; a longer one leaves a partial sum per chunk (at most two a chunk: the
 // group it begins in and the one it ends in), added up in order by a second launch, which also clears the groups without
-// rows.
+// rows.  512 rows of 13440 and 512 columns, 20 adapters of 16 ranks, fp32: 18 us and 5 for the join, 46 MB at 2.6 TB/s; 4099 rows
+// of twice 4096, 24 adapters of 32 ranks, bf16: 41 and 12 us: P's terms are turned through LDS for 512 columns at a time.
 struct OuterArgs {
   const float* p;                        // [.][pld]: by sorted position, or (p_gather) by row
   int pld, p_gather;
@@ -1240,7 +1251,7 @@ struct BasePlan {
 };
 
 // What the adapters cost at the end of tiles of 64 rows a wave and 64 outputs / in finish_kernel, ns: an adapter is 300 ns and
-// 15 (10) per rank, one after the other (204 rows of 50 adapters, 120 ranks: 84 us in the tiles, 6 in finish_kernel).
+// 15 (10) per rank, one after the other (204 rows of 50 adapters, 120 ranks: 84 us in the tiles, 22 in finish_kernel).
 static double adapters_64_time(int n, int N, int r, int E) {
   const long tiles = (long)((n + 127) / 128) * ((N + 127) / 128);
   const double each = 1.0 + 64.0 * E / n;
@@ -1416,7 +1427,7 @@ static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st
   const long tiles = (long)((a.N + 31) / 32) * ((a.n + 31) / 32);
   const size_t lds = (size_t)Terms<T>::low * 32 * (a.rp + 8) * 2;
   const unsigned down = (a.n + 31) / 32;
-  // Up to a tile a CU, four waves share each (37 rows of 24 adapters, 4096 outputs: 11.4 -> 8.0 us); up to 1024 a wave each,
+  // Up to a tile a CU, four waves share each (64 rows of 64 adapters, 128 ranks: 83 -> 55 us a call); up to 1024 a wave each,
   // spread over the CUs (1001 rows, 515 outputs: 8.7 us, shared 11.9); beyond that four a workgroup
   if (tiles <= 256) {
     hipLaunchKernelGGL((finish_kernel<T, V_STRIDED, true>), dim3((a.N + 31) / 32, down), dim3(256), lds, st, a, g);

