@@ -10,6 +10,8 @@
 // cores as three bf16 terms each (rounded to nearest: the six products that are kept leave out less than 2^-25 of the
 // largest); the narrow products low and u stay fp32 in memory and enter the next product as two bf16 terms beside bf16 or
 // fp16 operands (2^-17 of the value, far below the rounding of the result).
+#include <initializer_list>
+
 #include "flm_adapters.h"
 #include "flm_gemm_x3.h"
 
@@ -702,7 +704,7 @@ __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs a, RowGroup
 // 16384 rows of 4096 x 4096 bf16, 48 adapters of 64 ranks: 560-610 us, 1.0 PFLOP/s; 1.17 in the loop (LDS and the matrix cores
 // are both busy nine tenths of it), 12 us a round of tiles for the adapters and the stores.  Four waves of 128 x 128 with half
 // the LDS reads: a fifth slower (nothing hides a wave's own fetches).  W_KN, 4096 rows of 4096 x 4096: 155 us.
-// li: the workgroup's index among the tiles; lds: wide_lds_bytes()
+// li: the workgroup's index among the tiles; lds: two stages, then the terms of low, then the result
 #define WIDE_K 64
 // W_KN: W is [K,N] with contiguous outputs (the gradient of the inputs).  A thread then fetches eight outputs of four
 // consecutive k and turns them in registers; lanes of a wave take the sixteen groups of k first, so that they write whole
@@ -1606,6 +1608,12 @@ static bool spans_meet(const Span& a, const Span& b, int size) {
   return d < a.width * size || d + b.width * size > ld;
 }
 
+static bool misplaced(int bytes, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if ((uintptr_t)p & (bytes - 1)) return true;
+  return false;
+}
+
 static bool adapter_sizes(int n, int K, int N, int r, int E, int dtype) {
   return n > 0 && n <= (1 << 20) && K > 0 && N > 0 && K <= (1 << 20) && N <= (1 << 20) && r > 0 && r <= FLM_ADAPTER_MAX_RANK && E > 0 &&
          E <= FLM_GROUPS_MAX && dtype >= FLM_F32 && dtype <= FLM_F16;
@@ -1636,6 +1644,7 @@ extern "C" int flm_adapter_linear(const void* x, long ldx, const void* w, long l
       ((uintptr_t)workspace & 15))
     return FLM_E_ARG;
   const int size = dtype == FLM_F32 ? 4 : 2;
+  if (misplaced(size, {x, w, bias, a, b, y}) || misplaced(4, {scale, low}) || misplaced(16, {groups})) return FLM_E_ARG;
   const Span out{y, ldy, n, N};
   for (const Span& in : {Span{x, ldx, n, K}, Span{w, ldw, N, K}, Span{bias, 0, 1, N}, Span{a, 0, 1, (long)E * r * K}, Span{b, 0, 1, (long)E * N * r}})
     if (spans_meet(out, in, size)) return FLM_E_OVERLAP;
@@ -1654,6 +1663,7 @@ extern "C" int flm_adapter_linear_backward(const void* dy, long lddy, const void
       ldx < 0 || (dx && (!w || !a || ldw < 0 || lddx < K)) || ((uintptr_t)workspace & 15))
     return FLM_E_ARG;
   const int size = dtype == FLM_F32 ? 4 : 2;
+  if (misplaced(size, {dy, x, w, a, b, dx, da, db}) || misplaced(4, {scale, low}) || misplaced(16, {groups})) return FLM_E_ARG;
   const long na = (long)E * r * K, nb = (long)E * N * r;
   const Span in[] = {{dy, lddy, n, N}, {x, ldx, n, K}, {dx ? w : nullptr, ldw, N, K}, {dx ? a : nullptr, 0, 1, na}, {b, 0, 1, nb},
                      {low, 0, 1, (long)n * r * (4 / size)}};

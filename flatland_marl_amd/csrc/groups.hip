@@ -318,6 +318,7 @@ extern "C" long flm_group_rows_workspace(int n, int n_groups) {
 
 extern "C" int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* groups, int32_t* workspace, void* stream) {
   if (!ids || !groups || n <= 0 || n > (1 << 30) || n_groups <= 0 || n_groups > FLM_GROUPS_MAX) return FLM_E_ARG;
+  if (((uintptr_t)groups & 15) || ((uintptr_t)ids & (ids64 ? 7 : 3)) || ((uintptr_t)workspace & 3)) return FLM_E_ARG;
   const int E = n_groups, E1 = E + 1;
   const RowGroups g = row_groups(groups, n, E);
   int* order = const_cast<int*>(g.order);

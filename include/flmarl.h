@@ -643,7 +643,7 @@ int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* gro
 /* A shared projection with low-rank adapters: y_i = W x_i + bias + s_e B_e (A_e x_i) for the adapter e of row i, the
  * projection alone for rows without one.
  *   x [n,K], w [N,K], bias [N] (or NULL), y [n,N]: rows ldx / ldw / ldy elements apart, each row contiguous;
- *   a [E,r,K], b [E,N,r] contiguous; all of type dtype (FLM_F32 / FLM_BF16 / FLM_F16)
+ *   a [E,r,K], b [E,N,r] contiguous; all of type dtype (FLM_F32 / FLM_BF16 / FLM_F16), at any element's address
  *   groups: flm_group_rows(ids, ., n, E, ...); scale [E] float or NULL (then scale_all for every adapter)
  *   low [n,r] float out (or NULL): A_e x_i, not scaled, zeros for rows without an adapter: what the backward pass takes
  *   workspace: flm_adapter_workspace(n, K, N, r, E, dtype) bytes, 16-byte aligned; one per call in flight

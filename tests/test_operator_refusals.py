@@ -34,6 +34,11 @@ def test_group_rows_entry():
         args[i] = bad
         assert lib.flm_group_rows(*args) == -1, i
     assert lib.flm_group_rows(P, 0, 8193, 3, P, None, None) == -1              # needs a workspace
+    for i, at in ((0, 4098), (4, 4104)):                                       # an int, sixteen bytes
+        args = list(ok)
+        args[i] = ctypes.c_void_p(at)
+        assert lib.flm_group_rows(*args) == -1, i
+    assert lib.flm_group_rows(ctypes.c_void_p(4100), 1, 10, 3, P, None, None) == -1
 
 
 def test_adapter_entries():
@@ -51,6 +56,19 @@ def test_adapter_entries():
         args = list(ok)
         args[i] = bad
         assert lib.flm_adapter_linear_backward(*args) == -1, i
+
+
+def test_adapter_operands_between_elements():
+    lib = _lib.load()
+    fwd = [P, 64, P, 64, P, P, P, P, P, 1.0, 8, 64, 32, 4, 2, 1, P, P, 32, P, None]
+    bwd = [P, 32, P, 64, P, 64, P, P, P, P, 1.0, P, 8, 64, 32, 4, 2, 1, P, P, 64, P, P, None]
+    for call, ok, places in ((lib.flm_adapter_linear, fwd, ((0, 1), (2, 1), (4, 1), (5, 1), (6, 1), (7, 8), (8, 2), (17, 1), (19, 2))),
+                             (lib.flm_adapter_linear_backward, bwd, ((0, 1), (2, 1), (4, 1), (6, 1), (7, 1), (8, 8), (9, 2), (11, 2),
+                                                                     (19, 1), (21, 1), (22, 1)))):
+        for i, off in places:
+            args = list(ok)
+            args[i] = ctypes.c_void_p(4096 + off)
+            assert call(*args) == -1, i
 
 
 def test_adapter_results_that_share_memory():
