@@ -988,7 +988,7 @@ __global__ __launch_bounds__(256) void low_rows_kernel(const float* __restrict__
 // A group that lies inside one chunk is written at once; a longer one leaves a partial sum per chunk (at most two a chunk: the
 // group it begins in and the one it ends in), added up in order by a second launch, which also clears the groups without
 // rows.  512 rows of 13440 and 512 columns, 20 adapters of 16 ranks, fp32: 18 us and 5 for the join, 46 MB at 2.6 TB/s; 4099 rows
-// of twice 4096, 24 adapters of 32 ranks, bf16: 41 and 12 us: P's terms are turned through LDS for 512 columns at a time.
+// of twice 4096, 24 adapters of 32 ranks, bf16: 33 and 9 us: P's terms are turned through LDS for 512 columns at a time.
 struct OuterArgs {
   const float* p;                        // [.][pld]: by sorted position, or (p_gather) by row
   int pld, p_gather;
@@ -1527,14 +1527,14 @@ static int launch_outer(OuterArgs a, OuterArgs b, const RowGroups& g, hipStream_
 
 static long round16(long bytes) { return (bytes + 255) & ~255L; }
 
-// Tiles a workgroup of outer_kernel takes.  Enough workgroups (512) come first; where groups are long, each chunk that one
-// spans costs a partial sum, and half as many workgroups are better (4099 rows of 24 adapters, chunks of 2 / 4 tiles: product
-// and join 65 / 54 us; 512 rows of 20, 3 / 7 tiles: 23 / 34 us).
-static int outer_chunk(long tiles, int n, int E, int KQ, int r, bool f32) {
-  const long work = tiles * outer_across(KQ, r, f32), group = n / (32L * E);
-  const long c = work / 512, most = work / 256;
+// Tiles a workgroup of outer_kernel takes.  Both gradients' workgroups in one round of 512 (4099 rows of 24 adapters, chunks of
+// 4 / 5 / 6 / 8 tiles: 259 / 251 / 253 / 251 us for the whole pass; 512 rows of 20, 3 / 7: 23 / 34 for product and join); where
+// groups are long, each chunk that one spans costs a partial sum, and half as many workgroups are better (4099 rows, 2 / 4: 65 / 54).
+static int outer_chunk(long tiles, int n, int E, int K, int N, int r, bool f32) {
+  const long work = tiles * (outer_across(K, r, f32) + outer_across(N, r, f32)), group = n / (32L * E);
+  const long least = work < 512 ? 1 : work / 512, most = work / 256;
   const long wish = group < most ? group : most;
-  return (int)(c > wish ? (c < 1 ? 1 : c) : (wish < 1 ? 1 : wish));
+  return (int)(least > wish ? least : wish);
 }
 
 // partial sums of outer_kernel: two a chunk
@@ -1578,10 +1578,10 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
     hipLaunchKernelGGL(sum_slices_kernel, dim3((unsigned)(((long)n * rp / 4 + 255) / 256)), dim3(256), 0, st, u, ss.slices, (long)n * rp / 4);
     FLM_CHECK_LAUNCH();
   }
-  const int ca = outer_chunk(g.cap, n, E, K, r, sizeof(T) == 4), cb = outer_chunk(g.cap, n, E, N, r, sizeof(T) == 4);
-  float *part_a = (float*)ws, *part_b = part_a + outer_part(g.cap, ca) * r * K;
-  if ((rc = launch_outer<T>(OuterArgs{u, rp, 0, x, ldx, K, r, E, n, ca, scale, scale_all, part_a, da, K, 1, 0},
-                            OuterArgs{low, r, 1, dy, lddy, N, r, E, n, cb, scale, scale_all, part_b, db, 1, r, 0}, g, st)))
+  const int chunk = outer_chunk(g.cap, n, E, K, N, r, sizeof(T) == 4);
+  float *part_a = (float*)ws, *part_b = part_a + outer_part(g.cap, chunk) * r * K;
+  if ((rc = launch_outer<T>(OuterArgs{u, rp, 0, x, ldx, K, r, E, n, chunk, scale, scale_all, part_a, da, K, 1, 0},
+                            OuterArgs{low, r, 1, dy, lddy, N, r, E, n, chunk, scale, scale_all, part_b, db, 1, r, 0}, g, st)))
     return rc;
   if (!dx) return FLM_OK;
   const BasePlan bs = base_plan(n, N, K, r, E, sizeof(T) == 4, true);
@@ -1628,8 +1628,7 @@ extern "C" long flm_adapter_workspace(int n, int K, int N, int r, int E, int dty
 extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E, int dtype, int need_dx) {
   if (!adapter_sizes(n, K, N, r, E, dtype)) return 0;
   const long tiles = row_tiles_cap(n, E);
-  const int ca = outer_chunk(tiles, n, E, K, r, dtype == FLM_F32), cb = outer_chunk(tiles, n, E, N, r, dtype == FLM_F32);
-  long rest = 4L * r * (outer_part(tiles, ca) * K + outer_part(tiles, cb) * N);
+  long rest = 4L * r * outer_part(tiles, outer_chunk(tiles, n, E, K, N, r, dtype == FLM_F32)) * ((long)K + N);
   if (need_dx) {
     const long base = base_part_bytes(base_plan(n, N, K, r, E, dtype == FLM_F32, true), n, K);
     if (base > rest) rest = base;
