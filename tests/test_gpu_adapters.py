@@ -243,6 +243,28 @@ def test_no_rows():
 
 
 @pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("n,r", [(5, 13), (100, 13), (100, 8), (700, 67)])
+def test_operands_at_any_element(n, r, kind):
+    """Every operand begins one element behind a 16-byte boundary: the same bits as where it begins on one."""
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    d = ref.to_gpu(ref.case(n + r, n, 136, 200, r, 6, kind))
+
+    def shifted(t):
+        flat = torch.full((t.numel() + 9,), float("nan"), dtype=t.dtype, device="cuda")
+        flat[1:t.numel() + 1] = t.reshape(-1)
+        return flat[1:t.numel() + 1].view(t.shape)
+
+    s = {name: shifted(t) if name != "ids" else t for name, t in d.items()}
+    g = group_rows(d["ids"], 6)
+    results = []
+    for t in (d, s):
+        y, low = adapter_linear(t["x"], t["weight"], t["bias"], t["a"], t["b"], g, scale=t["scale"], keep_low=True)
+        results.append((y, low) + adapter_linear_backward(t["dy"], t["x"], t["weight"], t["a"], t["b"], g, low, scale=t["scale"]))
+    for want, got in zip(*results):
+        assert torch.equal(want, got)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
 def test_results_beside_their_inputs(kind):
     """Columns of one matrix may be input and result of a call; results that meet an input are refused."""
     from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
