@@ -1051,12 +1051,15 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
 #pragma unroll
     for (int i = 0; i < 8; i++) rows_of[i] = 8 * h + i < rows ? g.order[tile.x + 8 * h + i] : -1;
   };
+  // A lane whose columns pass the last one reads the last CPL instead and stores those that are its own: no load is tested
+  // (12638 rows, 274 and 1036 columns, 113 ranks: 150 -> 83 us; 9115 rows, 6345 and 54, 10: 116 -> 47).
   const bool inside = q0 + 16 * CPL <= a.KQ;
+  const int qc = min(q, a.KQ - CPL);
   auto fetch_q = [&]() {
-    if (inside) {
+    if (a.KQ >= CPL) {
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        qv[i] = *reinterpret_cast<const ColWords<T, CPL>*>((const T*)a.q + (long)max(rows_of[i], 0) * a.ldq + q);
+        qv[i] = *reinterpret_cast<const ColWords<T, CPL>*>((const T*)a.q + (long)max(rows_of[i], 0) * a.ldq + qc);
 #pragma unroll
       for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -1127,7 +1130,25 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
     // (the places are worked out here, not kept in registers over the whole walk: hundreds of them)
     int at = c;
     asm volatile("" : "+v"(at));
-    if (by_rank) {
+    const int shift = a.KQ >= CPL ? a.KQ - CPL : q0 + 16 * CPL;          // columns of a lane begin here at the latest
+    if (by_rank && !inside) {
+#pragma unroll
+      for (int jj = 0; jj < NRJ; jj++) {
+        const int j = rank0 + jj * 16 + at;
+        if (j >= a.r) continue;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const int own = q0 + (4 * h + x) * CPL, from = min(own, shift);
+#pragma unroll
+          for (int u = 0; u < CPL; u++) {
+            const int col = from + u;
+            if (col < own || col >= a.KQ) continue;
+            if (whole) out[(long)j * a.o_j + col] = (T)acc[jj][u][x];
+            else part[(long)j * a.o_j + col] = acc[jj][u][x];
+          }
+        }
+      }
+    } else if (by_rank) {
       const int col = q0 + 4 * h * CPL;
 #pragma unroll
       for (int jj = 0; jj < NRJ; jj++) {
@@ -1145,8 +1166,8 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
     } else {
 #pragma unroll
       for (int u = 0; u < CPL; u++) {
-        const int col = q0 + at * CPL + u;
-        if (col >= a.KQ) continue;
+        const int own = q0 + at * CPL, col = min(own, shift) + u;
+        if (col < own || col >= a.KQ) continue;
 #pragma unroll
         for (int jj = 0; jj < NRJ; jj++) {
           const int j = rank0 + jj * 16 + 4 * h;
@@ -1496,11 +1517,12 @@ static int launch_projection(BaseArgs b, const BasePlan& plan, const ShrinkArgs&
   return launch_finish<T, V_STRIDED>(f, g, st);
 }
 
-// Columns a lane of outer_kernel holds: 16 bytes' worth, half of 16-bit types where more than 32 ranks leave no registers;
-// ranks go in blocks of 64 (16282 rows, 79 ranks, fp32: 88 us, all ranks in one workgroup 144).
-static int outer_cols(int r, bool f32) { return f32 || r > 32 ? 4 : 8; }
-static int outer_across(int KQ, int r, bool f32) {
-  const int cols = 64 * outer_cols(r, f32);
+// Columns a lane of outer_kernel holds: 16 bytes' worth, half of 16-bit types where more ranks leave no registers (bf16 33, fp16
+// with its two terms 17); ranks go in blocks of 64 (16282 rows, 79 ranks, fp32: 88 us, all ranks in one workgroup 144).
+// terms: Terms<T>::own
+static int outer_cols(int r, int terms) { return terms == 3 || r > (terms == 1 ? 32 : 16) ? 4 : 8; }
+static int outer_across(int KQ, int r, int terms) {
+  const int cols = 64 * outer_cols(r, terms);
   return (KQ + cols - 1) / cols * ((r + 63) / 64);
 }
 
@@ -1509,14 +1531,14 @@ template <typename T>
 static int launch_outer(OuterArgs a, OuterArgs b, const RowGroups& g, hipStream_t st) {
   constexpr int CPL = sizeof(T) == 4 ? 4 : 8;
   const int ranks = (a.r + 63) / 64;
-  a.across = outer_across(a.KQ, a.r, sizeof(T) == 4);
-  b.across = outer_across(b.KQ, b.r, sizeof(T) == 4);
+  a.across = outer_across(a.KQ, a.r, Terms<T>::own);
+  b.across = outer_across(b.KQ, b.r, Terms<T>::own);
   a.cols = a.across / ranks;
   b.cols = b.across / ranks;
   const int groups = a.across * ((g.cap + a.chunk - 1) / a.chunk);
   const dim3 grid(groups + b.across * ((g.cap + b.chunk - 1) / b.chunk));
   if (a.r <= 16) hipLaunchKernelGGL((outer_kernel<T, 1, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
-  else if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 2, CPL>), grid, dim3(256), 0, st, a, b, groups, g);
+  else if (a.r <= 32) hipLaunchKernelGGL((outer_kernel<T, 2, Terms<T>::own == 2 ? 4 : CPL>), grid, dim3(256), 0, st, a, b, groups, g);
   else hipLaunchKernelGGL((outer_kernel<T, 4, 4>), grid, dim3(256), 0, st, a, b, groups, g);
   FLM_CHECK_LAUNCH();
   const long most = (long)a.r * (a.KQ > b.KQ ? a.KQ : b.KQ);
@@ -1530,8 +1552,8 @@ static long round16(long bytes) { return (bytes + 255) & ~255L; }
 // Tiles a workgroup of outer_kernel takes.  Both gradients' workgroups in one round of 512 (4099 rows of 24 adapters, chunks of
 // 4 / 5 / 6 / 8 tiles: 259 / 251 / 253 / 251 us for the whole pass; 512 rows of 20, 3 / 7: 23 / 34 for product and join); where
 // groups are long, each chunk that one spans costs a partial sum, and half as many workgroups are better (4099 rows, 2 / 4: 65 / 54).
-static int outer_chunk(long tiles, int n, int E, int K, int N, int r, bool f32) {
-  const long work = tiles * (outer_across(K, r, f32) + outer_across(N, r, f32)), group = n / (32L * E);
+static int outer_chunk(long tiles, int n, int E, int K, int N, int r, int terms) {
+  const long work = tiles * (outer_across(K, r, terms) + outer_across(N, r, terms)), group = n / (32L * E);
   const long least = work < 512 ? 1 : work / 512, most = work / 256;
   const long wish = group < most ? group : most;
   return (int)(least > wish ? least : wish);
@@ -1578,7 +1600,7 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
     hipLaunchKernelGGL(sum_slices_kernel, dim3((unsigned)(((long)n * rp / 4 + 255) / 256)), dim3(256), 0, st, u, ss.slices, (long)n * rp / 4);
     FLM_CHECK_LAUNCH();
   }
-  const int chunk = outer_chunk(g.cap, n, E, K, N, r, sizeof(T) == 4);
+  const int chunk = outer_chunk(g.cap, n, E, K, N, r, Terms<T>::own);
   float *part_a = (float*)ws, *part_b = part_a + outer_part(g.cap, chunk) * r * K;
   if ((rc = launch_outer<T>(OuterArgs{u, rp, 0, x, ldx, K, r, E, n, chunk, scale, scale_all, part_a, da, K, 1, 0},
                             OuterArgs{low, r, 1, dy, lddy, N, r, E, n, chunk, scale, scale_all, part_b, db, 1, r, 0}, g, st)))
@@ -1628,7 +1650,7 @@ extern "C" long flm_adapter_workspace(int n, int K, int N, int r, int E, int dty
 extern "C" long flm_adapter_backward_workspace(int n, int K, int N, int r, int E, int dtype, int need_dx) {
   if (!adapter_sizes(n, K, N, r, E, dtype)) return 0;
   const long tiles = row_tiles_cap(n, E);
-  long rest = 4L * r * outer_part(tiles, outer_chunk(tiles, n, E, K, N, r, dtype == FLM_F32)) * ((long)K + N);
+  long rest = 4L * r * outer_part(tiles, outer_chunk(tiles, n, E, K, N, r, dtype == FLM_F32 ? 3 : (dtype == FLM_BF16 ? 1 : 2))) * ((long)K + N);
   if (need_dx) {
     const long base = base_part_bytes(base_plan(n, N, K, r, E, dtype == FLM_F32, true), n, K);
     if (base > rest) rest = base;
