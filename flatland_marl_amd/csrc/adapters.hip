@@ -399,6 +399,10 @@ struct FinishArgs {
 };
 
 __device__ __forceinline__ float adapter_scale(const float* scale, float all, int e) { return scale ? scale[e] : all; }
+// Where s_e is applied: a factor of at most one to the narrow product, a larger one to the sums behind it.  Neither can then
+// pass fp32's range where the narrow product and the result do not.
+__device__ __forceinline__ float scale_before(float s) { return __builtin_fabsf(s) > 1.f ? 1.f : s; }
+__device__ __forceinline__ float scale_after(float s) { return __builtin_fabsf(s) > 1.f ? s : 1.f; }
 
 // The scaled narrow products of `rows` sorted positions from pos on, as bf16 terms in LDS: lt[(term*rows + row)*stride + j],
 // stride = low_stride(rp).  threads of the workgroup share the work; a barrier follows at the caller.
@@ -428,7 +432,7 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
 #pragma unroll
           for (int u = 0; u < 8; u++) f[u] += z + k < a.low_slices ? __uint_as_float(v[k].w[u]) : 0.f;
       }
-      const float s = adapter_scale(a.scale, a.scale_all, e);
+      const float s = scale_before(adapter_scale(a.scale, a.scale_all, e));
 #pragma unroll
       for (int u = 0; u < 8; u++) f[u] = u >= j - jr && jr + u < a.r ? f[u] * s : 0.f;
     }
@@ -439,7 +443,7 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
   }
 }
 
-// Adds s_e * low_i . V_e(n, .) to acc[mi]: lane (c, h) holds row lds_row0 + 32*mi + c of the staged tile of lds_rows rows,
+// Adds s_e * low_i . V_e(n, .) to acc[mi] (staged with scale_before, scale_after here): lane (c, h) holds row lds_row0 + 32*mi + c of the staged tile of lds_rows rows,
 // outputs n0 + 8*(r >> 2) + 4*h + (r & 3).  The rows may use several adapters: each adapter's product is formed apart and
 // added to its own rows only, so that no value of one adapter (an infinity, a NaN) can reach the rows of another.
 // key[mi]: the lane's adapter (E: none), ascending over the rows.  V comes straight from memory (the L2): NB adapters and
@@ -449,6 +453,7 @@ template <typename T, bool V_STRIDED, int MI, int JB, int NB>
 struct AddAdapters {
   int es[NB], j0, seen;
   unsigned todo[MI];
+  float after[NB];                         // scale_after
   Vec8<T> v[NB][JB];
   int turn = 0, share = 1;                 // this wave takes the adapters whose number in the tile is turn modulo share
 
@@ -472,6 +477,8 @@ struct AddAdapters {
         seen++;
       } while (es[b] >= 0 && share > 1 && (seen & (share - 1)) != turn);
     }
+#pragma unroll
+    for (int b = 0; b < NB; b++) after[b] = scale_after(adapter_scale(a.scale, a.scale_all, max(es[b], 0)));
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -534,7 +541,7 @@ struct AddAdapters {
                   t = mul_terms32<Terms<T>::own, Terms<T>::low>(vt[jj], l, t);
                 }
 #pragma unroll
-              for (int r = 0; r < 16; r++) acc[mi][r] = mine ? acc[mi][r] + t[r] : acc[mi][r];
+              for (int r = 0; r < 16; r++) acc[mi][r] = mine ? __builtin_fmaf(after[b], t[r], acc[mi][r]) : acc[mi][r];
             }
           }
         }
@@ -676,7 +683,7 @@ __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs a, RowGroup
 #pragma unroll
         for (int k = 0; k < 8; k++) f += z + k < a.low_slices ? v[k] : 0.f;
       }
-      low[j] = j < a.r ? f : 0.f;
+      low[j] = j < a.r ? f * scale_before(s) : 0.f;
     }
     const T* v = (const T*)a.v + (long)e * a.v_group + (long)at * a.v_row;
     Vec8<T> b = load8(v, a.r);
@@ -689,7 +696,7 @@ __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs a, RowGroup
 #pragma unroll
       for (int u = 0; u < 8; u++) t = __builtin_fmaf((float)c.v[u], low[j + u], t);
     }
-    y = __builtin_fmaf(s, t, y);
+    y = __builtin_fmaf(scale_after(s), t, y);
   }
   if (n < a.N) ((T*)a.y)[(long)row * a.ldy + n] = (T)y;
 }
@@ -1123,6 +1130,13 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
       for (int u = 0; u < CPL; u++) acc[jj][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
   auto flush = [&](int e) {
+    const float after = scale_after(adapter_scale(a.scale, a.scale_all, e));
+#pragma unroll
+    for (int jj = 0; jj < NRJ; jj++)
+#pragma unroll
+      for (int u = 0; u < CPL; u++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) acc[jj][u][x] *= after;
     const int head = g.first_tile[e], last = g.first_tile[e + 1] - 1;
     const bool whole = head >= t0 && last < t0 + a.chunk;
     float* part = a.part + ((long)chunk * 2 + (head < t0 ? 0 : 1)) * a.r * a.KQ;
@@ -1189,7 +1203,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
     bf16x8 qt[CPL][Terms<T>::own];
     if (t >= t0) {
       __syncthreads();                     // (the products of the tile before have read pt)
-      place_p(adapter_scale(a.scale, a.scale_all, e), tile.y >> 16);
+      place_p(scale_before(adapter_scale(a.scale, a.scale_all, e)), tile.y >> 16);
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < CPL; u++) own_terms<T>(column<T, CPL>(qv, u), qt[u]);
@@ -1591,7 +1605,7 @@ static int backward(const void* dy, long lddy, const void* x, long ldx, const vo
                     char* ws, void* dx, long lddx, void* da, void* db, hipStream_t st) {
   const int rp = ranks_padded(r);
   const ShrinkPlan ss = shrink_plan(n, N, E);
-  float* u = (float*)ws;                                             // s_e is applied where u is used
+  float* u = (float*)ws;                                             // s_e is applied where u is used (scale_before, scale_after)
   ws += round16(4L * ss.slices * n * rp);
   const ShrinkArgs s{dy, b, lddy, (long)N * r, 1, r, N, r, rp, n, ss.kslice, u};
   int rc = launch_shrink<T, true>(s, g, ss.slices, st);

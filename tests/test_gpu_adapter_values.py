@@ -1,0 +1,69 @@
+"""The adapter operators on values at the ends of their types, against plain 64-bit forms.  Needs an MI355X."""
+import pytest
+import torch
+
+from tests import adapter_ref as ref
+
+pytestmark = pytest.mark.gpu
+ROWS = [1, 24, 64, 65, 150]                                  # few-row form, its last size, tiles
+
+
+def _check(got, exact, absolute, terms, kind):
+    assert torch.isfinite(got).all()
+    err = (got.cpu().double() - exact).abs()
+    worst = (err / ref.bound(exact, absolute, terms, kind)).max().item()
+    assert worst <= 1.0, worst
+
+
+def _small(n, k, n_out, r, e, kind, seed):
+    """A case whose operands are all around 2^-6, with every row on adapter 0 or 1."""
+    c = ref.case(seed, n, k, n_out, r, e, kind, bare=0.0)
+    for name in ("x", "weight", "bias", "a", "b", "dy"):
+        c[name] = (c[name].double() / c[name].double().abs().max() * 2.0 ** -6).to(kind)
+    c["ids"] = torch.arange(n, dtype=torch.int32) % 2
+    return c
+
+
+def _both_passes(c, low=None):
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    n, k = c["x"].shape
+    n_out, r = c["b"].shape[1:]
+    kind = c["x"].dtype
+    d = ref.to_gpu(c)
+    g = group_rows(d["ids"], c["a"].shape[0])
+    y, kept = adapter_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], g, scale=d["scale"], keep_low=True)
+    # (what errors are relative to: the sum of the products' absolute values, so the factor's absolute value as well)
+    whole = dict(c, scale=c["scale"].abs())
+    (want, want_low), (size, size_low) = ref.forward(c), ref.forward(whole, absolute=True)
+    _check(kept, want_low, size_low, k, torch.float32)
+    _check(y, want, size, k + r, kind)
+    low = want_low.float() if low is None else low
+    got = adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low.cuda(), scale=d["scale"])
+    for t, w, s, terms in zip(got, ref.backward(c, low), ref.backward(whole, low, absolute=True), (n_out + r, n_out + n, n)):
+        _check(t, w, s, terms, kind)
+
+
+@pytest.mark.parametrize("scale", [3.0, -200.0, 2.0 ** -20])
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("n", ROWS)
+def test_scaled_narrow_products_outside_the_range(n, kind, scale):
+    """low or u of 1.5e38: the factor takes them, or a sum without the factor is, beyond fp32; no result is."""
+    big = 2.0 ** 126 * 1.75
+    met = 2.0 ** -16 if abs(scale) > 1 else 4.0              # what the large one is multiplied with
+    for large in ("x", "dy"):
+        c = _small(n, 40, 56, 9, 2, kind, 11)
+        c["scale"].fill_(scale)
+        for name in ("a", "b", "x", "dy"):
+            c[name] = (c[name].double() * 2.0 ** -10).to(kind)
+        c[large][:, 0] = big
+        if large == "x":                                     # low[:, 0] = x[:, 0], the other ranks do not see it
+            c["a"][:, :, 0], c["a"][:, 0, 1:], c["a"][:, 0, 0] = 0.0, 0.0, 1.0
+            c["weight"][:, 0] = 0.0
+            c["b"][:, :, 0] = met
+            c["dy"][:, 0] = met
+        else:                                                # u[:, 0] = scale * dy[:, 0]
+            c["b"][:, 0], c["b"][:, 1:, 0], c["b"][:, 0, 0] = 0.0, 0.0, 1.0
+            c["weight"][0] = 0.0
+            c["a"][:, 0] = met
+            c["x"][:, 0] = met
+        _both_passes(c)
