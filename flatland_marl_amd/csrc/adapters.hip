@@ -65,10 +65,15 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], long avail) {
 }
 
 // ---- operands as bf16 terms ---------------------------------------------------------------------------------------
-// x = t[0] + t[1] + ... with every term rounded to nearest.  KEEP_INF: a value that is infinite in bf16 keeps zero in its
-// further terms (its difference from itself is NaN); without, an infinity becomes NaN, which saves a third of the work.
-template <int N, bool KEEP_INF>
+// x = t[0] + t[1] + ... with every term rounded to nearest.
+// WIDE (values of fp32's range, which ends above the largest bf16): the first term is rounded no further than to that
+// largest one, whose difference from a finite x the other terms hold; rounded to infinity, a finite x above 3.396e38 would
+// become NaN.  An infinity's difference from it stays one, and a NaN's a NaN.
+// KEEP_INF: an infinite value is an infinity and zeros from that term on (its difference from itself would be NaN); without,
+// it becomes NaN, which saves two instructions a term.
+template <int N, bool KEEP_INF, bool WIDE>
 __device__ __forceinline__ void split_terms(const float (&x)[8], bf16x8 (&t)[N]) {
+  constexpr float TOP = 0x1.fep127f;                       // the largest bf16
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     f32x2 r;
@@ -76,13 +81,19 @@ __device__ __forceinline__ void split_terms(const float (&x)[8], bf16x8 (&t)[N])
     r[1] = x[2 * i + 1];
 #pragma unroll
     for (int s = 0; s < N; s++) {
-      const bf16x2 h = __builtin_convertvector(r, bf16x2);
+      f32x2 near = r;
+      if (WIDE && s == 0 && N > 1) {
+        near[0] = __builtin_amdgcn_fmed3f(r[0], -TOP, TOP);
+        near[1] = __builtin_amdgcn_fmed3f(r[1], -TOP, TOP);
+      }
+      const bf16x2 h = __builtin_convertvector(near, bf16x2);
       t[s][2 * i] = h[0];
       t[s][2 * i + 1] = h[1];
       if (s + 1 < N) {
         const f32x2 f = __builtin_convertvector(h, f32x2);
-        r[0] = !KEEP_INF || __builtin_fabsf(f[0]) < __builtin_inff() ? r[0] - f[0] : 0.f;
-        r[1] = !KEEP_INF || __builtin_fabsf(f[1]) < __builtin_inff() ? r[1] - f[1] : 0.f;
+        const bool finite = !KEEP_INF || (WIDE && s == 0);
+        r[0] = finite || __builtin_fabsf(f[0]) < __builtin_inff() ? r[0] - f[0] : 0.f;
+        r[1] = finite || __builtin_fabsf(f[1]) < __builtin_inff() ? r[1] - f[1] : 0.f;
       }
     }
   }
@@ -103,7 +114,7 @@ __device__ __forceinline__ void own_terms(const Vec8<T>& v, bf16x8 (&t)[Terms<T>
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) f[j] = (float)v.v[j];
-    split_terms<Terms<T>::own, sizeof(T) != 4>(f, t);
+    split_terms<Terms<T>::own, sizeof(T) != 4, sizeof(T) == 4>(f, t);
   }
 }
 
@@ -146,7 +157,7 @@ __device__ __forceinline__ Wide<_Float16> wide(const Vec8<_Float16>& v) {
 }
 __device__ __forceinline__ Wide<float> wide(const Vec8<float>& v) {
   Wide<float> w;
-  split_terms<3, false>(v.v, w.t);
+  split_terms<3, false, true>(v.v, w.t);
   return w;
 }
 __device__ __forceinline__ f32x4 mul16(const Wide<__bf16>& a, const Wide<__bf16>& b, f32x4 c) {
@@ -437,7 +448,7 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
       for (int u = 0; u < 8; u++) f[u] = u >= j - jr && jr + u < a.r ? f[u] * s : 0.f;
     }
     bf16x8 t[LOW];
-    split_terms<LOW, true>(f, t);
+    split_terms<LOW, true, true>(f, t);
 #pragma unroll
     for (int k = 0; k < LOW; k++) *reinterpret_cast<bf16x8*>(lt + (k * rows + row) * stride + j) = t[k];
   }
@@ -1116,7 +1127,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
 #pragma unroll
       for (int u = 0; u < 8; u++) pv[k][u] = m < rows ? pv[k][u] * s : 0.f;
       bf16x8 t[LOW];
-      split_terms<LOW, true>(pv[k], t);
+      split_terms<LOW, true, true>(pv[k], t);
 #pragma unroll
       for (int o = 0; o < LOW; o++)
 #pragma unroll

@@ -6,6 +6,7 @@ from tests import adapter_ref as ref
 
 pytestmark = pytest.mark.gpu
 ROWS = [1, 24, 64, 65, 150]                                  # few-row form, its last size, tiles
+TOP = torch.finfo(torch.float32).max
 
 
 def _check(got, exact, absolute, terms, kind):
@@ -41,6 +42,57 @@ def _both_passes(c, low=None):
     got = adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low.cuda(), scale=d["scale"])
     for t, w, s, terms in zip(got, ref.backward(c, low), ref.backward(whole, low, absolute=True), (n_out + r, n_out + n, n)):
         _check(t, w, s, terms, kind)
+
+
+@pytest.mark.parametrize("r", [5, 16])
+@pytest.mark.parametrize("where", ["x", "weight", "a", "b", "dy"])
+@pytest.mark.parametrize("n", ROWS)
+def test_largest_finite_values(n, where, r):
+    """The largest and the lowest value that fp32 has, in one operand at a time: no result is infinite by the formula."""
+    c = _small(n, 72, 56, r, 2, torch.float32, 3)
+    t = c[where]
+    flat = t.view(-1)
+    flat[::37] = TOP
+    flat[5::41] = -TOP
+    # (sums of a few products of 5e36 each stay below 3.4e38; so do those that pass through a second operand of 2^-6)
+    _both_passes(c)
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("n", ROWS)
+def test_narrow_products_above_the_largest_bf16(n, kind):
+    """low = A x between the largest bf16 and the largest fp32; u = s B^T dy as well."""
+    c = _small(n, 40, 56, 9, 2, kind, 7)
+    top = torch.finfo(torch.bfloat16).max
+    c["scale"].fill_(1.0)
+    for wide, narrow in (("x", "a"), ("dy", "b")):
+        c[wide][:, :2] = torch.tensor([top, 2.0 ** 119 * 1.875], dtype=torch.float64).to(kind)
+        if wide == "x":
+            c[narrow][:, 0] = 0.0
+            c[narrow][:, 0, :2] = 1.0
+        else:
+            c[narrow][:, :, 0] = 0.0
+            c[narrow][:, :2, 0] = 1.0
+        c["weight"][:, :2] = 0.0
+        c["weight"][:2] = 0.0
+        low = ref.forward(c)[1]
+        if wide == "x":
+            assert (low[:, 0] > top).all() and (low[:, 0] <= TOP).all()
+            c["b"][:, :, 0] = 2.0 ** -7
+            _both_passes(c)
+        else:
+            c["x"] = c["x"].double().clamp(-2.0 ** -6, 2.0 ** -6).to(kind)
+            c["a"][:, 0] = 2.0 ** -7
+            # dA: sums over up to n / 2 + 1 rows of u x
+            c["x"] = (c["x"].double() / n).to(kind)
+            _both_passes(c)
+    # low as the caller hands it over
+    c = _small(n, 40, 56, 9, 2, kind, 8)
+    low = ref.forward(c)[1].float()
+    low[::5, 3] = TOP
+    low[1::7, 8] = -TOP
+    c["dy"] = (c["dy"].double() / n).to(kind)
+    _both_passes(c, low)
 
 
 @pytest.mark.parametrize("scale", [3.0, -200.0, 2.0 ** -20])
