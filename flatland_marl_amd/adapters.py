@@ -108,7 +108,8 @@ def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False, out
     without an adapter get the projection alone.  x [n, K], weight [N, K], bias [N] or None, a [E, r, K], b [E, N, r], all
     of one type (float32, bfloat16, float16); scale: a number or float32 [E].  keep_low: returns (y, low) with low [n, r]
     float32 = a[e] x[i], which the backward pass takes.  out: a tensor [n, N] with contiguous rows that receives y (it may
-    share no element with an input).  Runs on the current stream; no autograd."""
+    share no element with an input).  A result is finite where the formula's is; an infinite one may be NaN instead.  Runs on
+    the current stream; no autograd."""
     n, k, n_out, r, e, scales, ldx, ldw = _weights(x, weight, a, b, groups, scale)
     if weight.shape[0] != n_out:
         raise ValueError("weight [%d, %d] expected" % (n_out, k))

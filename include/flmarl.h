@@ -647,8 +647,11 @@ int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* gro
  *   groups: flm_group_rows(ids, ., n, E, ...); scale [E] float or NULL (then scale_all for every adapter)
  *   low [n,r] float out (or NULL): A_e x_i, not scaled, zeros for rows without an adapter: what the backward pass takes
  *   workspace: flm_adapter_workspace(n, K, N, r, E, dtype) bytes, 16-byte aligned; one per call in flight
- * Sums are fp32, rounded once.  fp32 operands are multiplied as three bf16 terms each (fp32 accuracy; a row that meets an
- * infinity or NaN becomes NaN, other rows do not).  An adapter's values reach the rows of that adapter only.
+ * Sums are fp32, rounded once.  fp32 operands are multiplied as three bf16 terms each (fp32 accuracy); beside bf16 and fp16
+ * operands A_e x_i is held to 2^-17 of its value where it meets B.  Infinities and NaN, in every type and size: a result is
+ * finite exactly where the formula's is; where that is infinite it may be NaN instead (which of the two depends on type and
+ * sizes), where that is NaN it is NaN (a sum beyond fp32's range and a result beyond its type's are infinite).  An adapter's
+ * values reach the rows of that adapter only.
  * n, K, N <= 2^20, r <= FLM_ADAPTER_MAX_RANK, E <= FLM_GROUPS_MAX.  y shares no element with an input (FLM_E_OVERLAP). */
 long flm_adapter_workspace(int n, int K, int N, int r, int E, int dtype);
 int flm_adapter_linear(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* a, const void* b,
@@ -658,7 +661,8 @@ int flm_adapter_linear(const void* x, long ldx, const void* w, long ldw, const v
 /* Its backward pass for the gradient dy [n,N] of y; the projection itself (w, bias) is held fixed.
  *   u_i = s_e B_e^T dy_i;  da_e = sum_{i of e} u_i x_i^T [E,r,K];  db_e = s_e sum_{i of e} dy_i low_i^T [E,N,r];
  *   dx_i = W^T dy_i + A_e^T u_i [n,K] (dx = NULL: not computed, w and a may then be NULL)
- * da and db are written whole: zeros for adapters without rows.  Sums have a fixed order.  No result shares an element
+ * da and db are written whole: zeros for adapters without rows.  Sums have a fixed order.  Accuracy, infinities and NaN as in
+ * the forward pass (u_i and low_i are held to 2^-17 where they meet 16-bit operands).  No result shares an element
  * with an input or another result (FLM_E_OVERLAP).
  * workspace: flm_adapter_backward_workspace(n, K, N, r, E, dtype, dx != NULL) bytes, 16-byte aligned. */
 long flm_adapter_backward_workspace(int n, int K, int N, int r, int E, int dtype, int need_dx);

@@ -119,3 +119,42 @@ def test_scaled_narrow_products_outside_the_range(n, kind, scale):
             c["a"][:, 0] = met
             c["x"][:, 0] = met
         _both_passes(c)
+
+
+def _same_places(got, exact, absolute, terms, kind):
+    """Not finite exactly where the formula is not; NaN or that infinity there, and within the bound elsewhere."""
+    got = got.cpu().double()
+    bad = ~torch.isfinite(exact)
+    assert torch.equal(~torch.isfinite(got), bad)
+    infinite = torch.isinf(got)
+    assert torch.equal(got[infinite], exact[infinite])
+    tol = ref.bound(exact, absolute, terms, kind)
+    assert ((got - exact).abs() <= tol)[~bad].all()
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("where", ["x", "weight", "bias", "a", "b", "dy", "low"])
+@pytest.mark.parametrize("n", ROWS)
+def test_infinities_are_not_lost_and_reach_no_other_sum(n, where, kind):
+    """An infinity of either sign and a NaN in one operand at a time, among operands some of whose bf16 terms are zero."""
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    k, n_out, r, e = 72, 56, 9, 4
+    c = ref.case(17, n, k, n_out, r, e, kind, bare=0.0)
+    c["ids"] = torch.arange(n, dtype=torch.int32) % e
+    c["a"][2], c["b"][3] = (c[m][i].double().mul(8).round().div(8).to(kind) for m, i in (("a", 2), ("b", 3)))
+    low = ref.forward(c)[1].float()
+    t = low if where == "low" else c[where]
+    flat = t.view(-1)
+    for i, bad in enumerate((float("inf"), -float("inf"), float("nan"))):
+        flat[(i * 31 + 5) % flat.numel()] = bad
+    d = ref.to_gpu(c)
+    g = group_rows(d["ids"], e)
+    y, kept = adapter_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], g, scale=d["scale"], keep_low=True)
+    got = adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low.cuda(), scale=d["scale"])
+    finite = {name: t.double().nan_to_num(0.0, 0.0, 0.0) if t.is_floating_point() else t for name, t in c.items()}
+    (want, want_low), (size, size_low) = ref.forward(c), ref.forward(finite, absolute=True)
+    _same_places(kept, want_low, size_low, k, torch.float32)
+    _same_places(y, want, size, k + r, kind)
+    sizes = ref.backward(finite, low.double().nan_to_num(0.0, 0.0, 0.0), absolute=True)
+    for t, w, s, terms in zip(got, ref.backward(c, low), sizes, (n_out + r, n_out + n, n)):
+        _same_places(t, w, s, terms, kind)
