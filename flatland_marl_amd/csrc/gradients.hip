@@ -42,8 +42,8 @@ struct GradList {
 // What the gradient holds beside the listed tensors: `times` copies of the outer products g_i (x) r, r [64], over the
 // 512 + 512 values of two vectors (the first dense layer's gradient under empty rows, formed by the optimizer pass).
 struct GradOuter {
-  const float *r, *g0, *g1;
-  double times;
+  const float *r, *g0, *g1;              // r == nullptr: nothing
+  double times;                          // at least one
 };
 
 template <typename T> struct Pack8;
@@ -389,6 +389,7 @@ extern "C" int flm_dqn_grad_clip(float* grads, int Rp, int T1, int NA, int rails
   const void* src[3] = {piece[0], piece[1], piece[2]};
   void* dst[3] = {piece[0], piece[1], piece[2]};
   const int32_t dtype[3] = {FLM_F32, FLM_F32, FLM_F32};
-  const flm::GradOuter outer{rcb, grads + a1_w + block, grads + v1_w + block, 3.0 * (Rp - rails4)};
+  flm::GradOuter outer{};
+  if (rails4 < Rp) outer = {rcb, grads + a1_w + block, grads + v1_w + block, 3.0 * (Rp - rails4)};     // (else: no empty rows)
   return flm::grad_clip_run(src, dst, numel, dtype, 3, outer, max_norm, inf_norm, workspace, norm_out, (hipStream_t)stream);
 }

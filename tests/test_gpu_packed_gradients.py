@@ -1,0 +1,78 @@
+"""Clipping of the network's gradient in the packed form (flm_dqn_grad_clip), piece by piece against 64-bit forms.  Needs an
+MI355X."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _pieces(Rp, T1, n, rails4):
+    """(first, end) of what the packed form holds: the convolution with the advantage stream's packed weights, its biases with
+    the value stream's packed weights, the value stream's biases with the output layers."""
+    a1_w, block, used = 64 * T1 + 64, 512 * 64 * 3 * Rp, 512 * 64 * 3 * rails4
+    a1_b = a1_w + block
+    v1_w = a1_b + 512
+    return [(0, a1_w + used), (a1_b, v1_w + used), (v1_w + block, n)]
+
+
+def _clipped(g, factor):
+    """What a clipped element may be: the 64-bit product rounded once to fp32."""
+    want = g.double() * factor
+    return want, 2.0 ** -24 * want.abs() * (1 + 2.0 ** -20) + 2.0 ** -149
+
+
+@pytest.mark.parametrize("inf_norm", [0, 1])
+@pytest.mark.parametrize("limit", [0.3, 3.0])
+@pytest.mark.parametrize("Rp,rails4", [(9, 4), (5, 4), (8, 8), (12, 12), (4, 4)])
+def test_every_piece_is_counted_and_scaled(Rp, rails4, limit, inf_norm):
+    """rails4 == Rp: there are no empty rows, and nothing but the pieces counts, whatever rcb holds."""
+    from flatland_marl_amd import _lib
+    T1, NA = 13, 2
+    n = _lib.query("flm_dqn_param_count", 3 * Rp, T1, NA)
+    gen = torch.Generator().manual_seed(Rp * 16 + rails4)
+    g = torch.randn(n, generator=gen)
+    pieces = _pieces(Rp, T1, n, rails4)
+    (_, _), (a1_b, _), (v1_b, _) = pieces
+    keep = torch.zeros(n, dtype=torch.bool)
+    for lo, hi in pieces:
+        keep[lo:hi] = True
+    rcb = torch.rand(64, generator=gen) * 5                  # (large: a product that should not count would show)
+    bias = torch.cat([g[a1_b:a1_b + 512], g[v1_b:v1_b + 512]]).double()
+    empty = (bias[:, None] * rcb.double()).flatten().repeat(3 * (Rp - rails4))
+    every = torch.cat([g[keep].double(), empty])
+    norm = every.abs().max().item() if inf_norm else math.sqrt(math.fsum((every * every).tolist()))
+    limit *= norm
+    buf = torch.where(keep, g, torch.tensor(float("nan"))).cuda()
+    r = rcb.cuda()
+    work = torch.empty(_lib.GRAD_WORKSPACE, dtype=torch.float64, device="cuda")
+    out = torch.full((), -1.0, device="cuda")
+    _lib.launch(buf.device, "flm_dqn_grad_clip", buf.data_ptr(), Rp, T1, NA, rails4, 1, r.data_ptr(), limit, inf_norm, work.data_ptr(),
+                out.data_ptr())
+    assert abs(out.item() - norm) <= 2.0 ** -23 * norm
+    got = buf.cpu()
+    assert torch.isnan(got[~keep]).all()                     # what lies between the pieces is not touched
+    want, tol = _clipped(g, min(1.0, limit / (norm + 1e-6)))
+    # (the factor's 64-bit norm may differ in its last bits: far below half a step of fp32)
+    assert ((got.double() - want).abs() <= tol)[keep].all()
+    assert torch.equal(r.cpu(), rcb)
+
+
+@pytest.mark.parametrize("inf_norm", [0, 1])
+def test_an_infinite_norm_without_empty_rows(inf_norm):
+    """An infinite bias gradient and no empty rows: the finite elements become zero, none of them NaN."""
+    from flatland_marl_amd import _lib
+    Rp, T1, NA = 4, 13, 2
+    n = _lib.query("flm_dqn_param_count", 3 * Rp, T1, NA)
+    g = torch.ones(n)
+    a1_b = _pieces(Rp, T1, n, Rp)[1][0]
+    g[a1_b + 3] = float("inf")
+    buf, r = g.cuda(), torch.zeros(64).cuda()
+    work = torch.empty(_lib.GRAD_WORKSPACE, dtype=torch.float64, device="cuda")
+    out = torch.empty((), device="cuda")
+    _lib.launch(buf.device, "flm_dqn_grad_clip", buf.data_ptr(), Rp, T1, NA, Rp, 1, r.data_ptr(), 1.0, inf_norm, work.data_ptr(),
+                out.data_ptr())
+    assert math.isinf(out.item())
+    got = buf.cpu()
+    assert torch.isnan(got[a1_b + 3]) and int(torch.isnan(got).sum()) == 1 and got.nan_to_num().abs().max() == 0
