@@ -13,7 +13,6 @@
 // kept or refreshed by the caller.
 #include <algorithm>
 #include <new>
-#include <utility>
 #include <vector>
 
 #include "flm_common.h"
@@ -260,6 +259,8 @@ static bool grad_list(GradList& list, const void* const* src, void* const* dst, 
   for (int i = lo; i < lo + count; i++) {
     if (numel[i] < 0 || (numel[i] > 0 && !src[i]) || dtype[i] < FLM_F32 || dtype[i] > FLM_F16) return false;
     if (numel[i] == 0) continue;
+    const uintptr_t between = dtype[i] == FLM_F32 ? 3 : 1;
+    if (((uintptr_t)src[i] | (uintptr_t)(dst ? dst[i] : nullptr)) & between) return false;
     GradItem& it = list.item[list.count++];
     it.src = src[i];
     it.dst = dst ? dst[i] : nullptr;
@@ -273,21 +274,32 @@ static bool grad_list(GradList& list, const void* const* src, void* const* dst, 
   return true;
 }
 
-// Whether a place would be written twice, or written as one tensor's and read as another's: sorted by address, two
-// neighbouring spans must not overlap (a destination that is its own source counts once).
+// Whether a place would be written twice, written as one tensor's and read as another's, or clipped as two tensors' (into
+// places elsewhere): spans in the order of their addresses, each against the ends of those before it.  Tensors that only count
+// in the norm may overlap each other.
 static int grad_overlap(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count) {
+  enum { COUNTED, CLIPPED, WRITTEN };
+  struct Span {
+    uintptr_t begin, end;
+    int kind;
+    bool operator<(const Span& o) const { return begin < o.begin; }
+  };
   try {
-    std::vector<std::pair<uintptr_t, uintptr_t>> span;
+    std::vector<Span> span;
     span.reserve(2 * (size_t)count);
     for (int i = 0; i < count; i++) {
-      if (numel[i] == 0 || !dst[i]) continue;
-      const uintptr_t bytes = (uintptr_t)numel[i] * (dtype[i] == FLM_F32 ? 4 : 2);
-      span.emplace_back((uintptr_t)src[i], (uintptr_t)src[i] + bytes);
-      if (dst[i] != src[i]) span.emplace_back((uintptr_t)dst[i], (uintptr_t)dst[i] + bytes);
+      if (numel[i] == 0) continue;
+      const uintptr_t bytes = (uintptr_t)numel[i] * (dtype[i] == FLM_F32 ? 4 : 2), s = (uintptr_t)src[i], d = (uintptr_t)dst[i];
+      span.push_back({s, s + bytes, !d ? COUNTED : (d == s ? WRITTEN : CLIPPED)});
+      if (d && d != s) span.push_back({d, d + bytes, WRITTEN});
     }
     if (!std::is_sorted(span.begin(), span.end())) std::sort(span.begin(), span.end());
-    for (size_t i = 1; i < span.size(); i++)
-      if (span[i].first < span[i - 1].second) return FLM_E_OVERLAP;
+    uintptr_t end[3] = {0, 0, 0};
+    for (const Span& s : span) {
+      if (s.begin < end[WRITTEN] || (s.kind != COUNTED && s.begin < end[CLIPPED]) || (s.kind == WRITTEN && s.begin < end[COUNTED]))
+        return FLM_E_OVERLAP;
+      end[s.kind] = std::max(end[s.kind], s.end);
+    }
   } catch (const std::bad_alloc&) {
     return FLM_E_CAPACITY;
   }
@@ -359,7 +371,7 @@ static int grad_clip_run(const void* const* src, void* const* dst, const int64_t
 extern "C" int flm_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count,
                              double max_norm, int inf_norm, double* workspace, float* norm_out, void* stream) {
   if (!src || !numel || !dtype || count <= 0 || count > FLM_GRAD_MAX_TENSORS || !workspace || !norm_out ||
-      !(max_norm >= 0.0))
+      !(max_norm >= 0.0) || ((uintptr_t)workspace & 7) || ((uintptr_t)norm_out & 3))
     return FLM_E_ARG;
   return flm::grad_clip_run(src, dst, numel, dtype, count, flm::GradOuter{}, max_norm, inf_norm, workspace, norm_out,
                             (hipStream_t)stream);
@@ -368,7 +380,8 @@ extern "C" int flm_grad_clip(const void* const* src, void* const* dst, const int
 extern "C" int flm_dqn_grad_clip(float* grads, int Rp, int T1, int NA, int rails4, int packed, const float* rcb,
                                  double max_norm, int inf_norm, double* workspace, float* norm_out, void* stream) {
   if (!grads || Rp <= 0 || T1 <= 0 || rails4 < 0 || rails4 > Rp || (rails4 > 0 && !rcb) || (packed && rails4 <= 0) ||
-      !workspace || !norm_out || !(max_norm >= 0.0))
+      !workspace || !norm_out || !(max_norm >= 0.0) || (((uintptr_t)grads | (uintptr_t)rcb | (uintptr_t)norm_out) & 3) ||
+      ((uintptr_t)workspace & 7))
     return FLM_E_ARG;
   const long n = flm_dqn_param_count(3 * Rp, T1, NA);
   if (n <= 0) return FLM_E_ARG;

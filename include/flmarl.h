@@ -691,7 +691,8 @@ int flm_dqn_hidden_grads(const float* params, const float* hidden, const float* 
  * absolute value), dst = src * min(1, max_norm / (norm + 1e-6)).
  *   src, dst, numel, dtype: HOST arrays of count device pointers, element counts and FLM_F32 / FLM_BF16 / FLM_F16;
  *   dst[i] == src[i] clips in place, dst[i] == NULL only counts in the norm, dst == NULL: the norm alone.  A dst overlaps no
- *   src but its own, and no other dst, and two src that are clipped do not overlap (FLM_E_OVERLAP)
+ *   src but its own (which it is or does not meet), and no other dst, and two src that are clipped do not overlap
+ *   (FLM_E_OVERLAP); those that only count may.  Pointers lie at whole elements (FLM_E_ARG)
  *   workspace [FLM_GRAD_WORKSPACE] double; norm_out [1] float
  * Sums are kept in 64 bits and have a fixed order.  A NaN norm makes every gradient NaN, an infinite one makes the finite
  * ones zero, as the formula does.  count <= FLM_GRAD_MAX_TENSORS, max_norm >= 0. */
