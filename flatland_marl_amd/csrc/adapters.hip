@@ -1693,9 +1693,14 @@ extern "C" int flm_adapter_linear(const void* x, long ldx, const void* w, long l
     return FLM_E_ARG;
   const int size = dtype == FLM_F32 ? 4 : 2;
   if (misplaced(size, {x, w, bias, a, b, y}) || misplaced(4, {scale, low}) || misplaced(16, {groups})) return FLM_E_ARG;
-  const Span out{y, ldy, n, N};
-  for (const Span& in : {Span{x, ldx, n, K}, Span{w, ldw, N, K}, Span{bias, 0, 1, N}, Span{a, 0, 1, (long)E * r * K}, Span{b, 0, 1, (long)E * N * r}})
-    if (spans_meet(out, in, size)) return FLM_E_OVERLAP;
+  const long words = 4 / size;                             // elements of the call's type in a float or an int
+  const Span in[] = {{x, ldx, n, K}, {w, ldw, N, K}, {bias, 0, 1, N}, {a, 0, 1, (long)E * r * K}, {b, 0, 1, (long)E * N * r},
+                     {scale, 0, 1, E * words}, {groups, 0, 1, row_groups_ints(n, E) * words}};
+  const Span out[] = {{y, ldy, n, N}, {low, 0, 1, (long)n * r * words}};
+  if (spans_meet(out[0], out[1], size)) return FLM_E_OVERLAP;
+  for (const Span& o : out)
+    for (const Span& i : in)
+      if (spans_meet(o, i, size)) return FLM_E_OVERLAP;
   const RowGroups g = row_groups(groups, n, E);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == FLM_F32) return forward<float>(x, ldx, w, ldw, bias, a, b, g, scale, scale_all, n, K, N, r, E, (char*)workspace, y, ldy, low, st);
@@ -1712,9 +1717,9 @@ extern "C" int flm_adapter_linear_backward(const void* dy, long lddy, const void
     return FLM_E_ARG;
   const int size = dtype == FLM_F32 ? 4 : 2;
   if (misplaced(size, {dy, x, w, a, b, dx, da, db}) || misplaced(4, {scale, low}) || misplaced(16, {groups})) return FLM_E_ARG;
-  const long na = (long)E * r * K, nb = (long)E * N * r;
+  const long na = (long)E * r * K, nb = (long)E * N * r, words = 4 / size;
   const Span in[] = {{dy, lddy, n, N}, {x, ldx, n, K}, {dx ? w : nullptr, ldw, N, K}, {dx ? a : nullptr, 0, 1, na}, {b, 0, 1, nb},
-                     {low, 0, 1, (long)n * r * (4 / size)}};
+                     {low, 0, 1, (long)n * r * words}, {scale, 0, 1, E * words}, {groups, 0, 1, row_groups_ints(n, E) * words}};
   const Span out[] = {{da, 0, 1, na}, {db, 0, 1, nb}, {dx, lddx, n, K}};
   for (int i = 0; i < 3; i++) {
     for (const Span& s : in)

@@ -652,7 +652,8 @@ int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* gro
  * finite exactly where the formula's is; where that is infinite it may be NaN instead (which of the two depends on type and
  * sizes), where that is NaN it is NaN (a sum beyond fp32's range and a result beyond its type's are infinite).  An adapter's
  * values reach the rows of that adapter only.
- * n, K, N <= 2^20, r <= FLM_ADAPTER_MAX_RANK, E <= FLM_GROUPS_MAX.  y shares no element with an input (FLM_E_OVERLAP). */
+ * n, K, N <= 2^20, r <= FLM_ADAPTER_MAX_RANK, E <= FLM_GROUPS_MAX.  Neither y nor low shares an element with an input (scale and
+ * groups among them) or with the other (FLM_E_OVERLAP). */
 long flm_adapter_workspace(int n, int K, int N, int r, int E, int dtype);
 int flm_adapter_linear(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* a, const void* b,
                        const int32_t* groups, const float* scale, float scale_all, int n, int K, int N, int r, int E,
