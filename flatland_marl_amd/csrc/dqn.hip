@@ -367,16 +367,22 @@ __global__ __launch_bounds__(256) void fc1_padding_bias_kernel(PaddingBiasJob j0
   const float* W = o < 512 ? Wa + (long)o * K1 : Wv + (long)(o - 512) * K1;
   const int L = Rp - R4;
   // a wave takes every fourth filter, its lanes the consecutive weights of a segment: 48 independent loads per lane
-  // and pass (16 filters x 3 planes); the lanes' sums of a filter meet in LDS and are added in lane order
+  // and pass (16 filters x 3 planes), all on their way before the first addition (80 of 100 rails, two networks 26 us, a pair
+  // of loads at a time 51); the lanes' sums of a filter meet in LDS and are added in lane order
   float a[16];
 #pragma unroll
   for (int j = 0; j < 16; j++) a[j] = 0.f;
   for (int i = lane; i < L; i += 64) {
+    float v[16][3];
 #pragma unroll
     for (int j = 0; j < 16; j++) {
       const float* p = W + (long)(w + 4 * j) * H3 + R4 + i;
-      a[j] += (p[0] + p[Rp]) + p[2 * Rp];
+#pragma unroll
+      for (int pl = 0; pl < 3; pl++) v[j][pl] = p[pl * Rp];
     }
+    __builtin_amdgcn_sched_barrier(0);         // (the additions are not moved in between: each would wait for its loads)
+#pragma unroll
+    for (int j = 0; j < 16; j++) a[j] += (v[j][0] + v[j][1]) + v[j][2];
   }
 #pragma unroll
   for (int j = 0; j < 16; j++) lane_sum[w + 4 * j][lane] = a[j];
