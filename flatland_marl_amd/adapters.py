@@ -109,7 +109,12 @@ def adapter_linear(x, weight, bias, a, b, groups, scale=1.0, keep_low=False, out
     of one type (float32, bfloat16, float16); scale: a number or float32 [E].  keep_low: returns (y, low) with low [n, r]
     float32 = a[e] x[i], which the backward pass takes.  out: a tensor [n, N] with contiguous rows that receives y (it may
     share no element with an input).  A result is finite where the formula's is; an infinite one may be NaN instead.  Runs on
-    the current stream; no autograd."""
+    the current stream.  No autograd: where gradients are recorded, operands that require one are refused (torch.no_grad(), or
+    detached operands, and adapter_linear_backward)."""
+    if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
+        raise ValueError("adapter_linear records no graph: call it under torch.no_grad(), or with detached operands, and "
+                         "adapter_linear_backward for the gradients")
     n, k, n_out, r, e, scales, ldx, ldw = _weights(x, weight, a, b, groups, scale)
     if weight.shape[0] != n_out:
         raise ValueError("weight [%d, %d] expected" % (n_out, k))
