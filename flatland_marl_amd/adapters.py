@@ -208,10 +208,14 @@ class NetworkAdapters:
     def state_dict(self):
         return {name: getattr(self, name).clone() for name in self.PARTS}
 
-    def load_state_dict(self, state):
+    def check_state_dict(self, state):
+        """Whether load_state_dict() takes this; raises if not."""
         for name in self.PARTS:
             if tuple(state[name].shape) != tuple(getattr(self, name).shape):
                 raise ValueError("%s %s expected" % (name, tuple(getattr(self, name).shape)))
+
+    def load_state_dict(self, state):
+        self.check_state_dict(state)
         for name in self.PARTS:
             getattr(self, name).copy_(state[name])
 
@@ -272,6 +276,21 @@ class AdapterAdam:
         self.adapters, self.lr, self.betas, self.eps = adapters, lr, betas, eps
         self.m, self.v, self.grads = (torch.zeros_like(adapters.flat) for _ in range(3))
         self.step_count = 0
+
+    def state_dict(self):
+        return {"m": self.m.clone(), "v": self.v.clone(), "step_count": self.step_count}
+
+    def check_state_dict(self, state):
+        """Whether load_state_dict() takes this; raises if not."""
+        if state is not None and (not state["m"].shape == state["v"].shape == self.m.shape or int(state["step_count"]) < 0):
+            raise ValueError("moments of %d adapter parameters expected" % self.m.numel())
+
+    def load_state_dict(self, state):
+        """None: as before the first step."""
+        self.check_state_dict(state)
+        for name in ("m", "v"):
+            getattr(self, name).zero_() if state is None else getattr(self, name).copy_(state[name])
+        self.step_count = 0 if state is None else int(state["step_count"])
 
     def step(self, target=None, tau=None):
         """One step with self.grads; with target (the target's NetworkAdapters) and tau its soft update in the same pass."""

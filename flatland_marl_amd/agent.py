@@ -170,17 +170,27 @@ class DQNAgent:
         torch.save(self.qnetwork_local.state_dict(), filename + ".local")
         torch.save(self.qnetwork_target.state_dict(), filename + ".target")
         if self.adapters is not None:
-            torch.save({"local": self.adapters.state_dict(), "target": self.adapters_target.state_dict()}, filename + ".adapters")
+            torch.save({"local": self.adapters.state_dict(), "target": self.adapters_target.state_dict(), "scale": self.adapters.scale,
+                        "optimizer": self.adapter_optimizer.state_dict()}, filename + ".adapters")
 
     def load(self, filename):
+        """What save() wrote.  Attached adapters come back with the scale they were trained with and their optimizer's state (a
+        file that holds neither: the present scale, an optimizer that has not stepped); adapters of other sizes are refused
+        before anything is changed."""
+        adapters = None
+        if self.adapters is not None and os.path.exists(filename + ".adapters"):
+            adapters = torch.load(filename + ".adapters", weights_only=True, map_location=self.adapters.device)
+            for bank, name in ((self.adapters, "local"), (self.adapters_target, "target"), (self.adapter_optimizer, "optimizer")):
+                bank.check_state_dict(adapters.get(name) if name == "optimizer" else adapters[name])
         if os.path.exists(filename + ".local"):
             self.qnetwork_local.load_state_dict(torch.load(filename + ".local", weights_only=True))
         if os.path.exists(filename + ".target"):
             self.qnetwork_target.load_state_dict(torch.load(filename + ".target", weights_only=True))
-        if self.adapters is not None and os.path.exists(filename + ".adapters"):
-            state = torch.load(filename + ".adapters", weights_only=True)
-            self.adapters.load_state_dict(state["local"])
-            self.adapters_target.load_state_dict(state["target"])
+        if adapters is not None:
+            self.adapters.load_state_dict(adapters["local"])
+            self.adapters_target.load_state_dict(adapters["target"])
+            self.adapters.scale = self.adapters_target.scale = float(adapters.get("scale", self.adapters.scale))
+            self.adapter_optimizer.load_state_dict(adapters.get("optimizer"))
 
     def attach_adapters(self, n_adapters, rank, alpha=None, lr=None):
         """Low-rank adapters beside the networks' first dense layers: from now on learn_adapters() trains them (Adam, lr or

@@ -1,0 +1,71 @@
+"""The agent's adapters over their whole life: saved and loaded, without rows, beside other buffers.  Needs an MI355X."""
+import pytest
+import torch
+
+from tests.test_gpu_adapter_training import _agent, _batch, _with_adapters
+
+pytestmark = pytest.mark.gpu
+Rp, T1, PS, B, E, R = 8, 17, 144, 24, 3, 4
+
+
+def _learn(agent, seed):
+    dev, _ = _batch(B, Rp, T1, PS, 6, seed)
+    ids = torch.randint(-1, E, (B,), generator=torch.Generator().manual_seed(seed)).cuda()
+    agent.learn_adapters(dev, ids, 0.9, PS)
+
+
+def test_training_goes_on_where_it_was_saved(tmp_path):
+    """Values, target values, scale, moments and step count: two further steps give the same bits as without a break."""
+    agent = _agent(Rp, T1)
+    _with_adapters(agent, E, R)
+    for seed in (1, 2):
+        _learn(agent, seed)
+    agent.save(str(tmp_path / "net"))
+    other = _agent(Rp, T1, seed=9)
+    other.attach_adapters(E, R, alpha=1.0)                    # (another scale)
+    for seed in (5, 6, 7):                                   # moments and a step count of its own
+        _learn(other, seed)
+    other.load(str(tmp_path / "net"))
+    assert other.adapters.scale == other.adapters_target.scale == agent.adapters.scale
+    for seed in (3, 4):
+        _learn(agent, seed)
+        _learn(other, seed)
+    for a, b in ((agent.adapters.flat, other.adapters.flat), (agent.adapters_target.flat, other.adapters_target.flat),
+                 (agent.adapter_optimizer.m, other.adapter_optimizer.m), (agent.adapter_optimizer.v, other.adapter_optimizer.v)):
+        assert torch.equal(a, b)
+    assert agent.adapter_optimizer.step_count == other.adapter_optimizer.step_count == 4
+
+
+def test_files_without_scale_and_optimizer(tmp_path):
+    agent = _agent(Rp, T1)
+    ad = _with_adapters(agent, E, R)
+    name = str(tmp_path / "net")
+    agent.save(name)
+    torch.save({"local": ad.state_dict(), "target": agent.adapters_target.state_dict()}, name + ".adapters")
+    kept, scale = ad.flat.clone(), ad.scale
+    _learn(agent, 1)
+    agent.load(name)
+    assert torch.equal(ad.flat, kept) and ad.scale == scale and agent.adapter_optimizer.step_count == 0
+    assert not agent.adapter_optimizer.m.any() and not agent.adapter_optimizer.v.any()
+
+
+def test_a_refused_file_changes_nothing(tmp_path):
+    agent = _agent(Rp, T1)
+    _with_adapters(agent, E, R)
+    name = str(tmp_path / "net")
+    for change in ("rank", "target", "moments"):
+        writer = _agent(Rp, T1, seed=4)
+        _with_adapters(writer, E, R + 1 if change == "rank" else R)
+        writer.save(name)
+        state = torch.load(name + ".adapters", weights_only=True)
+        if change == "target":
+            state["target"]["b_val"] = state["target"]["b_val"][:1]
+        elif change == "moments":
+            state["optimizer"]["v"] = state["optimizer"]["v"][:-1]
+        torch.save(state, name + ".adapters")
+        before = [t.clone() for t in (agent.qnetwork_local.flat_params(), agent.qnetwork_target.flat_params(), agent.adapters.flat,
+                                      agent.adapters_target.flat)]
+        with pytest.raises(ValueError):
+            agent.load(name)
+        after = (agent.qnetwork_local.flat_params(), agent.qnetwork_target.flat_params(), agent.adapters.flat, agent.adapters_target.flat)
+        assert all(torch.equal(a, b) for a, b in zip(before, after)), change
