@@ -193,9 +193,11 @@ class DQNAgent:
             self.adapter_optimizer.load_state_dict(adapters.get("optimizer"))
 
     def attach_adapters(self, n_adapters, rank, alpha=None, lr=None):
-        """Low-rank adapters beside the networks' first dense layers: from now on learn_adapters() trains them (Adam, lr or
-        the agent's) and the networks stay as they are.  Returns the local network's NetworkAdapters.  (Several ranks draw the
-        same start if they are seeded alike, as for the network itself.)"""
+        """Low-rank adapters beside the networks' first dense layers.  learn_adapters() trains them (Adam, lr or the agent's) and
+        leaves the networks as they are; DQNPolicy and BatchedTrainer use them where they are given adapter_of_env.  Everything
+        else is the shared network's as before: act() answers without adapters, step(), learn() and learn_obs() train the
+        network under them.  Returns the local network's NetworkAdapters.  (Several ranks draw the same start if they are seeded
+        alike, as for the network itself.)"""
         self.adapters = NetworkAdapters(self.qnetwork_local, n_adapters, rank, alpha)
         self.adapters_target = self.adapters.copy_for(self.qnetwork_target)
         self.adapter_optimizer = AdapterAdam(self.adapters, self.args.lr if lr is None else lr)
@@ -246,7 +248,8 @@ class DQNAgent:
                     self.learn(experiences, self.args.gamma)
 
     def act(self, state, eps=0.):
-        """Q-values [action_space] (device tensor) of one observation [3*max_rails, depth+1]."""
+        """Q-values [action_space] (device tensor) of one observation [3*max_rails, depth+1], by the network alone: an
+        observation by itself names no adapter."""
         state = torch.from_numpy(np.ascontiguousarray(state)).float().unsqueeze(0).unsqueeze(0).to(device)
         self.qnetwork_local.eval()
         with torch.no_grad():

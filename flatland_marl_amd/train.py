@@ -206,7 +206,8 @@ class BatchedTrainer:
                  eps_decay=0.998, crash_penalty=False, switch2switch=False, max_learns_per_step=None, seed=0,
                  strict=False, adapter_of_env=None):
         """adapter_of_env [E] (integers): decisions are taken with the agent's adapter of each environment (-1: none) and the
-        learn steps train the adapters alone (DQNAgent.attach_adapters, learn_adapters), in the default feeding mode."""
+        learn steps train the adapters alone (DQNAgent.attach_adapters, learn_adapters), in the default feeding mode.  None: the
+        network acts and is trained, adapters that the agent has are left out."""
         self.ro = rollout
         self.agent = agent
         b = rollout.b

@@ -69,3 +69,19 @@ def test_a_refused_file_changes_nothing(tmp_path):
             agent.load(name)
         after = (agent.qnetwork_local.flat_params(), agent.qnetwork_target.flat_params(), agent.adapters.flat, agent.adapters_target.flat)
         assert all(torch.equal(a, b) for a, b in zip(before, after)), change
+
+
+def test_what_stays_the_shared_networks():
+    """act() and learn() with adapters attached: the network's values and training, the adapters untouched."""
+    with_ad, without = _agent(Rp, T1), _agent(Rp, T1)
+    _with_adapters(with_ad, E, R)
+    dev, (s, a, r, n, d) = _batch(B, Rp, T1, PS, 6, 2)
+    kept, kept_t = with_ad.adapters.flat.clone(), with_ad.adapters_target.flat.clone()
+    state = s[0, 0].float().numpy()
+    assert torch.equal(with_ad.act(state), without.act(state))
+    batch = tuple(t.float().cuda() if t.is_floating_point() else t.cuda() for t in (s, a, r, n, d))
+    for agent in (with_ad, without):
+        agent.learn(batch, 0.9)
+        agent.learn_obs(dev, 0.9, PS)
+    assert torch.equal(with_ad.qnetwork_local.flat_params(), without.qnetwork_local.flat_params())
+    assert torch.equal(with_ad.adapters.flat, kept) and torch.equal(with_ad.adapters_target.flat, kept_t)
