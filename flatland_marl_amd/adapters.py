@@ -183,15 +183,16 @@ class NetworkAdapters:
         n_adapters, rank = int(n_adapters), int(rank)
         if not 1 <= n_adapters <= GROUPS_MAX or not 1 <= rank <= ADAPTER_MAX_RANK:
             raise ValueError("1..%d adapters of rank 1..%d" % (GROUPS_MAX, ADAPTER_MAX_RANK))
-        self.n_adapters, self.rank = n_adapters, rank
+        self._allocate(network, n_adapters, rank, 1.0 if alpha is None else float(alpha) / rank)
+        for a in (self.a_adv, self.a_val):
+            a.uniform_(-self.inputs ** -0.5, self.inputs ** -0.5)
+
+    def _allocate(self, network, n_adapters, rank, scale):
+        self.n_adapters, self.rank, self.scale = n_adapters, rank, scale
         self.inputs, self.outputs = network.fc1_adv.in_features, network.fc1_adv.out_features
-        self.scale = 1.0 if alpha is None else float(alpha) / rank
         self.device = network.flat_params().device
         self.flat = torch.zeros(sum(n for _, n in self._layout()), dtype=torch.float32, device=self.device)
-        views = self.views(self.flat)
-        for name in ("a_adv", "a_val"):
-            views[name].uniform_(-self.inputs ** -0.5, self.inputs ** -0.5)
-        self.__dict__.update(views)
+        self.__dict__.update(self.views(self.flat))
 
     def _layout(self):
         e, r, k, n = self.n_adapters, self.rank, self.inputs, self.outputs
@@ -221,7 +222,8 @@ class NetworkAdapters:
 
     def copy_for(self, network):
         """The same adapters, values and scale, beside another network of the same shape (the target network)."""
-        other = NetworkAdapters(network, self.n_adapters, self.rank, self.scale * self.rank)
+        other = object.__new__(type(self))
+        other._allocate(network, self.n_adapters, self.rank, self.scale)
         other.flat.copy_(self.flat)
         return other
 

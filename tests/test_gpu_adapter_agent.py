@@ -85,3 +85,16 @@ def test_what_stays_the_shared_networks():
         agent.learn_obs(dev, 0.9, PS)
     assert torch.equal(with_ad.qnetwork_local.flat_params(), without.qnetwork_local.flat_params())
     assert torch.equal(with_ad.adapters.flat, kept) and torch.equal(with_ad.adapters_target.flat, kept_t)
+
+
+def test_a_copy_has_the_same_scale_and_draws_nothing():
+    from flatland_marl_amd.adapters import NetworkAdapters
+    agent = _agent(Rp, T1)
+    for rank, alpha in ((49, 1.0), (3, 1.3), (107, 0.7), (R, None)):
+        torch.manual_seed(3)
+        ad = NetworkAdapters(agent.qnetwork_local, 2, rank, alpha)
+        state = torch.cuda.get_rng_state()
+        other = ad.copy_for(agent.qnetwork_target)
+        assert torch.equal(torch.cuda.get_rng_state(), state)
+        assert other.scale == ad.scale and torch.equal(other.flat, ad.flat) and other.flat.data_ptr() != ad.flat.data_ptr()
+        assert other.a_adv.data_ptr() == other.flat.data_ptr()
