@@ -88,17 +88,19 @@ class FlatAdam:
         nothing waited for).  rails: as for step(), when the learn step left the packed form; the gradient under the empty
         rows, which step() forms itself, counts in the norm and is scaled with the bias gradient it is formed from."""
         self._ensure()
-        net, dev = self.network, self.grads.device
+        if rails is None:
+            return clip_grad_norm_(self.grads, max_norm)
+        Rp, T1, NA, rails4, rcb, packed = rails
+        if not packed:
+            raise ValueError("the used rails' gradient lies among rows that were not written: only the packed form can be clipped")
+        if not max_norm >= 0:
+            raise ValueError("max_norm must not be negative")
+        dev = self.grads.device
         norm = torch.empty((), dtype=torch.float32, device=dev)
         work = torch.empty(GRAD_WORKSPACE, dtype=torch.float64, device=dev)
-        if rails is not None:
-            Rp, T1, NA, rails4, rcb, packed = rails
-            if not packed:
-                raise ValueError("the used rails' gradient lies among rows that were not written: only the packed form can be clipped")
-            launch(dev, "flm_dqn_grad_clip", ptr(self.grads), int(Rp), int(T1), int(NA), int(rails4), 1, ptr(rcb), float(max_norm), 0,
-                   ptr(work), norm.data_ptr())
-            return norm
-        return clip_grad_norm_(self.grads, max_norm)
+        launch(dev, "flm_dqn_grad_clip", ptr(self.grads), int(Rp), int(T1), int(NA), int(rails4), 1, ptr(rcb), float(max_norm), 0,
+               ptr(work), norm.data_ptr())
+        return norm
 
     def step(self, target=None, tau=None, rails=None):
         """One Adam step; with target (the target network's flat parameters) and tau also its soft update with

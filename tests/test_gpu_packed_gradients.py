@@ -108,3 +108,11 @@ def test_a_learn_step_clips_every_piece():
     # (the norm is known here as its fp32 rounding: half a step of the factor)
     want, tol = _clipped(g, min(1.0, bound.max_grad_norm / (norm + 1e-6)))
     assert ((got.double() - want).abs() <= tol + 2.0 ** -23 * want.abs())[keep].all()
+
+
+def test_a_bad_bound_is_the_same_error_in_either_form():
+    agent = _agent(8, 17)
+    for rails in (None, (8, 17, 2, 4, torch.zeros(64).cuda(), True)):
+        for bad in (-1.0, float("nan")):
+            with pytest.raises(ValueError):
+                agent.optimizer.clip_grad_norm_(bad, rails=rails)
