@@ -247,13 +247,14 @@ class NetworkAdapters:
         x = torch.empty(n * self.inputs, dtype=torch.float32, device=flat.device) if features is None else features
         x = x[:n * self.inputs].view(n, self.inputs)
         hidden = torch.empty((n, 2 * self.outputs), dtype=torch.float32, device=flat.device)
+        half = self.outputs
         if n:
             launch(flat.device, "flm_dqn_features_u8", flat.data_ptr(), obs_u8.data_ptr(), n, network.height // 3, network.width,
                    int(plane_stride), network.action_space, x.data_ptr())
-            half = self.outputs
-            res = [adapter_linear(x, layer.weight.data, layer.bias.data, a, b, groups, scale=self.scale, keep_low=keep, out=y)
-                   for layer, a, b, y in ((network.fc1_adv, self.a_adv, self.b_adv, hidden[:, :half]),
-                                          (network.fc1_val, self.a_val, self.b_val, hidden[:, half:]))]
+        res = [adapter_linear(x, layer.weight.data, layer.bias.data, a, b, groups, scale=self.scale, keep_low=keep, out=y)
+               for layer, a, b, y in ((network.fc1_adv, self.a_adv, self.b_adv, hidden[:, :half]),
+                                      (network.fc1_val, self.a_val, self.b_val, hidden[:, half:]))]
+        if n:
             launch(flat.device, "flm_dqn_heads", flat.data_ptr(), hidden.data_ptr(), n, network.height, network.width,
                    network.action_space, q.data_ptr())
         if not keep:

@@ -98,3 +98,15 @@ def test_a_copy_has_the_same_scale_and_draws_nothing():
         assert torch.equal(torch.cuda.get_rng_state(), state)
         assert other.scale == ad.scale and torch.equal(other.flat, ad.flat) and other.flat.data_ptr() != ad.flat.data_ptr()
         assert other.a_adv.data_ptr() == other.flat.data_ptr()
+
+
+def test_no_observations_keep_what_their_gradients_take():
+    from flatland_marl_amd.adapters import group_rows
+    agent = _agent(Rp, T1)
+    ad = _with_adapters(agent, E, R)
+    dev, _ = _batch(4, Rp, T1, PS, 6, 1)
+    q, kept = ad.q_values(agent.qnetwork_local, dev[0][:0], PS, group_rows(torch.zeros(0, dtype=torch.int32).cuda(), E), keep=True)
+    assert q.shape == (0, 2)
+    grads = torch.full_like(ad.flat, float("nan"))
+    ad.gradients(kept, torch.empty((0, 2 * ad.outputs), device="cuda"), grads)
+    assert (grads == 0).all()
