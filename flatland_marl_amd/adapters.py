@@ -230,7 +230,8 @@ class NetworkAdapters:
     def q_values(self, network, obs_u8, plane_stride, groups, out=None, features=None, keep=False):
         """Q-values [n, actions] of uint8 observations [n, 3, plane_stride] with the adapters of groups = group_rows(ids,
         n_adapters), ids the adapter of each observation; observations without one get the network's own values.  All rails
-        are computed.  out: a float32 buffer of at least n rows; features: one of n * inputs floats (both optional).
+        are computed.  out: a float32 buffer of at least n * actions floats, whose first the result is; features: one of n * inputs
+        floats (both optional, of any shape).
         keep: returns (q, what gradients() takes)."""
         if network.height % 3:
             raise ValueError("observations have three planes: the network height must be 3*max_rails")
@@ -243,8 +244,9 @@ class NetworkAdapters:
         for name, t, want in (("out", out, n * network.action_space), ("features", features, n * self.inputs)):
             if t is not None and (t.dtype != torch.float32 or t.device != flat.device or not t.is_contiguous() or t.numel() < want):
                 raise ValueError("%s: a contiguous float32 buffer of at least %d elements on the network's device expected" % (name, want))
-        q = torch.empty((n, network.action_space), dtype=torch.float32, device=flat.device) if out is None else out[:n]
-        x = torch.empty(n * self.inputs, dtype=torch.float32, device=flat.device) if features is None else features
+        q = torch.empty((n, network.action_space), dtype=torch.float32, device=flat.device) if out is None else \
+            out.view(-1)[:n * network.action_space].view(n, network.action_space)
+        x = torch.empty(n * self.inputs, dtype=torch.float32, device=flat.device) if features is None else features.view(-1)
         x = x[:n * self.inputs].view(n, self.inputs)
         hidden = torch.empty((n, 2 * self.outputs), dtype=torch.float32, device=flat.device)
         half = self.outputs

@@ -110,3 +110,18 @@ def test_no_observations_keep_what_their_gradients_take():
     grads = torch.full_like(ad.flat, float("nan"))
     ad.gradients(kept, torch.empty((0, 2 * ad.outputs), device="cuda"), grads)
     assert (grads == 0).all()
+
+
+def test_buffers_of_any_shape_receive_the_q_values():
+    from flatland_marl_amd.adapters import group_rows
+    agent = _agent(Rp, T1)
+    ad = _with_adapters(agent, E, R)
+    dev, _ = _batch(5, Rp, T1, PS, 6, 1)
+    groups = group_rows(torch.tensor([0, 1, 2, -1, 0], dtype=torch.int32).cuda(), E)
+    args = (agent.qnetwork_local, dev[0], PS, groups)
+    want = ad.q_values(*args)
+    for shape, rows in (((10,), (5 * ad.inputs + 3,)), ((7, 2), (5, ad.inputs)), ((2, 11), (9, ad.inputs)), ((3, 2, 2), (1, 5, ad.inputs))):
+        out, features = torch.full(shape, -5.0).cuda(), torch.empty(rows).cuda()
+        got = ad.q_values(*args, out=out, features=features)
+        assert got.shape == (5, 2) and torch.equal(got, want) and got.data_ptr() == out.data_ptr()
+        assert (out.view(-1)[10:] == -5.0).all()
