@@ -33,6 +33,7 @@ class DeviceReplay:
         self.draws = 0
         self.group = None                                  # per transition, if the caller tells some apart (keep_groups)
         self._out = None
+        self._groups = None                                # of the last sample()'s transitions
 
     def __len__(self):
         return self.size
@@ -46,10 +47,13 @@ class DeviceReplay:
             torch.cuda.current_stream(self.device).synchronize()       # (steps may be stored on another stream)
 
     def sampled_groups(self):
-        """The groups [batch] of the last sample()'s transitions."""
+        """The groups [batch] of the last sample()'s transitions, as they were when it drew them (what is stored since then may
+        have taken their places)."""
         if self.group is None or self._out is None:
             raise ValueError("keep_groups() and sample() first")
-        return self.group.index_select(0, self._out[5].long())
+        if self._groups is None:                           # (drawn before keep_groups(): none had a group)
+            self._groups = torch.full_like(self._out[5], -1)
+        return self._groups.clone()
 
     def add(self, state, action, reward, next_state, done, groups=None):
         """Append n transitions (oldest entries are overwritten, as with deque(maxlen))."""
@@ -193,4 +197,5 @@ class DeviceReplay:
              ptr(self.done), self.size, self.seed, self.draws & 0xFFFFFFFF, B, self.row_bytes, *shape, ptr(s), ptr(sn),
              ptr(a), ptr(r), ptr(d), ptr(idx), st)
         self.draws += 1
+        self._groups = None if self.group is None else self.group.index_select(0, idx)
         return s, a, r, sn, d
