@@ -97,12 +97,25 @@ def grad_norm(grads, norm_type=2.0):
 def clip_grad_norm_(grads, max_norm, norm_type=2.0, out=None):
     """Scales all tensors by min(1, max_norm / (norm + 1e-6)) in place and returns the norm they had, as grad_norm does.
     grads: gradient tensors (float32, bfloat16, float16, mixed at will; any size, no element twice), None entries are
-    skipped.  out: a tensor for each gradient that receives the clipped values instead; the gradients stay as they are.
-    A NaN norm makes every gradient NaN, an infinite one the finite ones zero."""
+    skipped.  out: a tensor for each gradient that receives the clipped values instead; the gradients stay as they are (an entry
+    for every entry of grads, those of None entries are left alone, or one for every gradient).  A NaN norm makes every gradient
+    NaN, an infinite one the finite ones zero (as the formula does: with an infinite max_norm as well it is NaN)."""
     outs = None
-    listed = _listed(grads)
-    if out is not None:
-        outs = [out] if isinstance(out, torch.Tensor) else [o for o in out if o is not None]
+    if out is None or isinstance(grads, torch.Tensor):
+        listed = _listed(grads)
+        if out is not None:
+            outs = _listed(out)
+    else:
+        grads, outs = list(grads), [out] if isinstance(out, torch.Tensor) else list(out)
+        listed = _listed(grads)
+        if len(outs) == len(grads):                         # one for one: what belongs to a None entry is left alone
+            outs = [o for g, o in zip(grads, outs) if g is not None]
+            if any(o is None for o in outs):
+                raise ValueError("a gradient without an output")
+        else:
+            outs = [o for o in outs if o is not None]
+        if len(outs) != len(listed):
+            raise ValueError("%d outputs for %d gradients" % (len(outs), len(listed)))
     if not listed:
         _inf_norm(norm_type)
         return torch.zeros(())

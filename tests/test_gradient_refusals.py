@@ -51,3 +51,20 @@ def test_pointers_between_elements(kind, off):
         args = list(ok)
         args[i] = ctypes.c_void_p(at)
         assert _lib.load().flm_dqn_grad_clip(*args) == -1, i
+
+
+def test_outputs_stay_with_their_gradients():
+    """A None among the gradients and one among the outputs are not dropped apart from each other."""
+    import torch
+    from flatland_marl_amd import FlmError
+    from flatland_marl_amd.gradients import clip_grad_norm_
+    g, o = torch.ones(4), torch.zeros(4)
+    with pytest.raises(ValueError):
+        clip_grad_norm_([None, g], 1.0, out=[o, None])
+    with pytest.raises(ValueError):
+        clip_grad_norm_([g, g.clone()], 1.0, out=[o])
+    for grads, out in (([None, g], [o, o]), ([None, g], [None, o]), ([None, g], [o]), (g, o), (iter([None, g]), iter([None, o])),
+                       ([g], o)):
+        with pytest.raises(FlmError):                       # (as far as the missing GPU)
+            clip_grad_norm_(grads, 1.0, out=out)
+    assert clip_grad_norm_([None], 1.0, out=[o]).item() == 0 and (o == 0).all()
