@@ -106,14 +106,14 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, out=None):
         if out is not None:
             outs = _listed(out)
     else:
-        grads, outs = list(grads), [out] if isinstance(out, torch.Tensor) else list(out)
+        if not isinstance(grads, (list, tuple)):
+            grads = list(grads)
+        if not isinstance(out, (list, tuple)):
+            out = [out] if isinstance(out, torch.Tensor) else list(out)
         listed = _listed(grads)
-        if len(outs) == len(grads):                         # one for one: what belongs to a None entry is left alone
-            outs = [o for g, o in zip(grads, outs) if g is not None]
-            if any(o is None for o in outs):
-                raise ValueError("a gradient without an output")
-        else:
-            outs = [o for o in outs if o is not None]
+        if len(out) == len(grads) != len(listed):           # one for one: what belongs to a None entry is left alone
+            out = [o for g, o in zip(grads, out) if g is not None]
+        outs = _listed(out)
         if len(outs) != len(listed):
             raise ValueError("%d outputs for %d gradients" % (len(outs), len(listed)))
     if not listed:
