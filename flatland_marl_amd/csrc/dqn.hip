@@ -2360,15 +2360,22 @@ extern "C" int flm_dqn_learn_grads_u8_rails(const float* local, const float* tar
                           H3, T1, NA, ws, grads, loss_out, (hipStream_t)stream, phase, R4, fill_padding);
 }
 
+// The element-wise passes go over at most this many elements a launch: one of 2^32 threads and more is not taken (the adapters'
+// parameters may be more than the network's).
+#define ELEMENTWISE_MAX (1L << 30)
+
 extern "C" int flm_dqn_adam(float* params, const float* grads, float* m, float* v, long n, double lr, double beta1,
                             double beta2, double eps, int step, void* stream) {
   if (!params || !grads || !m || !v || n <= 0 || step <= 0) return FLM_E_ARG;
   const double bc1 = 1.0 - pow(beta1, (double)step);
   const double bc2 = 1.0 - pow(beta2, (double)step);
-  hipLaunchKernelGGL(flm::adam_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, params, grads, m,
-                     v, n, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(lr / bc1),
-                     (float)sqrt(bc2));
-  if (hipGetLastError() != hipSuccess) return FLM_E_LAUNCH;
+  for (long lo = 0; lo < n; lo += ELEMENTWISE_MAX) {
+    const long part = std::min(ELEMENTWISE_MAX, n - lo);
+    hipLaunchKernelGGL(flm::adam_kernel, dim3((unsigned)((part + 255) / 256)), dim3(256), 0, (hipStream_t)stream, params + lo,
+                       grads + lo, m + lo, v + lo, part, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
+                       (float)(lr / bc1), (float)sqrt(bc2));
+    if (hipGetLastError() != hipSuccess) return FLM_E_LAUNCH;
+  }
   return FLM_OK;
 }
 
@@ -2378,10 +2385,13 @@ extern "C" int flm_dqn_adam_soft_update(float* params, const float* grads, float
   if (!params || !grads || !m || !v || !target || n <= 0 || step <= 0) return FLM_E_ARG;
   const double bc1 = 1.0 - pow(beta1, (double)step);
   const double bc2 = 1.0 - pow(beta2, (double)step);
-  hipLaunchKernelGGL(flm::adam_soft_update_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
-                     params, grads, m, v, target, n, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
-                     (float)(lr / bc1), (float)sqrt(bc2), (float)tau, (float)(1.0 - tau));
-  if (hipGetLastError() != hipSuccess) return FLM_E_LAUNCH;
+  for (long lo = 0; lo < n; lo += ELEMENTWISE_MAX) {
+    const long part = std::min(ELEMENTWISE_MAX, n - lo);
+    hipLaunchKernelGGL(flm::adam_soft_update_kernel, dim3((unsigned)((part + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                       params + lo, grads + lo, m + lo, v + lo, target + lo, part, (float)(1.0 - beta1), (float)beta2,
+                       (float)(1.0 - beta2), (float)eps, (float)(lr / bc1), (float)sqrt(bc2), (float)tau, (float)(1.0 - tau));
+    if (hipGetLastError() != hipSuccess) return FLM_E_LAUNCH;
+  }
   return FLM_OK;
 }
 
@@ -2443,8 +2453,11 @@ extern "C" int flm_dqn_adam_moments(float* m, float* v, long n, int Rp, int T1, 
 
 extern "C" int flm_dqn_soft_update(float* target, const float* local, long n, double tau, void* stream) {
   if (!target || !local || n <= 0) return FLM_E_ARG;
-  hipLaunchKernelGGL(flm::soft_update_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, target,
-                     local, n, (float)tau, (float)(1.0 - tau));
-  if (hipGetLastError() != hipSuccess) return FLM_E_LAUNCH;
+  for (long lo = 0; lo < n; lo += ELEMENTWISE_MAX) {
+    const long part = std::min(ELEMENTWISE_MAX, n - lo);
+    hipLaunchKernelGGL(flm::soft_update_kernel, dim3((unsigned)((part + 255) / 256)), dim3(256), 0, (hipStream_t)stream, target + lo,
+                       local + lo, part, (float)tau, (float)(1.0 - tau));
+    if (hipGetLastError() != hipSuccess) return FLM_E_LAUNCH;
+  }
   return FLM_OK;
 }
