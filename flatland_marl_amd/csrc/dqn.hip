@@ -2360,7 +2360,8 @@ extern "C" int flm_dqn_learn_grads_u8_rails(const float* local, const float* tar
                           H3, T1, NA, ws, grads, loss_out, (hipStream_t)stream, phase, R4, fill_padding);
 }
 
-// The element-wise passes go over at most this many elements a launch: one of 2^32 threads and more is not taken (the adapters'
+// The element-wise passes go over at most this many elements a launch: of 2^32 threads and more the runtime starts only what is
+// left of them modulo 2^32, without an error (the adapters'
 // parameters may be more than the network's).
 #define ELEMENTWISE_MAX (1L << 30)
 
