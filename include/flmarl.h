@@ -647,8 +647,9 @@ int flm_group_rows(const void* ids, int ids64, int n, int n_groups, int32_t* gro
  *   groups: flm_group_rows(ids, ., n, E, ...); scale [E] float or NULL (then scale_all for every adapter)
  *   low [n,r] float out (or NULL): A_e x_i, not scaled, zeros for rows without an adapter: what the backward pass takes
  *   workspace: flm_adapter_workspace(n, K, N, r, E, dtype) bytes, 16-byte aligned; one per call in flight
- * Sums are fp32, rounded once.  fp32 operands are multiplied as three bf16 terms each (fp32 accuracy); beside bf16 and fp16
- * operands A_e x_i is held to 2^-17 of its value where it meets B.  Infinities and NaN, in every type and size: a result is
+ * Sums are fp32, rounded once.  fp32 operands are multiplied as three bf16 terms each: fp32 accuracy, but no term holds less
+ * than 2^-133, so that values below 2^-110 count to that.  Beside bf16 and fp16 operands A_e x_i is held to 2^-17 of its value
+ * where it meets B.  Infinities and NaN, in every type and size: a result is
  * finite exactly where the formula's is; where that is infinite it may be NaN instead (which of the two depends on type and
  * sizes), where that is NaN it is NaN (a sum beyond fp32's range and a result beyond its type's are infinite).  An adapter's
  * values reach the rows of that adapter only.

@@ -158,3 +158,34 @@ def test_infinities_are_not_lost_and_reach_no_other_sum(n, where, kind):
     sizes = ref.backward(finite, low.double().nan_to_num(0.0, 0.0, 0.0), absolute=True)
     for t, w, s, terms in zip(got, ref.backward(c, low), sizes, (n_out + r, n_out + n, n)):
         _same_places(t, w, s, terms, kind)
+
+
+@pytest.mark.parametrize("power", [-100, -112, -120, -124])
+@pytest.mark.parametrize("n", ROWS)
+def test_small_fp32_values_are_held_to_the_smallest_bf16(n, power):
+    """x and dy of 2^power: each enters its products, and so do low and u, with an error of at most 2^-133 beside fp32's."""
+    from flatland_marl_amd.adapters import adapter_linear, adapter_linear_backward, group_rows
+    k, n_out, r, e = 72, 56, 9, 4
+    c = ref.case(31, n, k, n_out, r, e, torch.float32, bare=0.0)
+    for name in ("x", "dy"):
+        c[name] = (c[name].double() * 2.0 ** power).float()
+    c["bias"].zero_()
+    low = ref.forward(c)[1].float()
+    d = ref.to_gpu(c)
+    g = group_rows(d["ids"], e)
+    y, kept = adapter_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], g, scale=d["scale"], keep_low=True)
+    dx = adapter_linear_backward(d["dy"], d["x"], d["weight"], d["a"], d["b"], g, low.cuda(), scale=d["scale"])[0]
+    # the same sums with every x (dy) of 2^-133, and the narrow product off by as much once more
+    f = {name: t.double().abs() if t.is_floating_point() else t.long() for name, t in c.items()}
+    step, s = 2.0 ** -133, f["scale"][f["ids"]][:, None]
+    a, b = f["a"][f["ids"]], f["b"][f["ids"]]                # [n, r, K], [n, N, r]
+    ones = torch.ones(n, r, 1, dtype=torch.float64)
+    slack_low = step * a.sum(2)
+    slack_y = step * f["weight"].sum(1)[None] + s * torch.bmm(b, slack_low[:, :, None] + step * ones)[:, :, 0]
+    slack_dx = step * f["weight"].sum(0)[None] + s * torch.bmm(a.transpose(1, 2).contiguous(),
+                                                               step * b.sum(1)[:, :, None] + step * ones)[:, :, 0]
+    for got, want, size, terms, slack in ((kept, *(t[1] for t in (ref.forward(c), ref.forward(c, True))), k, slack_low),
+                                          (y, *(t[0] for t in (ref.forward(c), ref.forward(c, True))), k + r, slack_y),
+                                          (dx, *(t[0] for t in (ref.backward(c, low), ref.backward(c, low, True))), n_out + r, slack_dx)):
+        err = (got.cpu().double() - want).abs()
+        assert (err <= ref.bound(want, size, terms, torch.float32) + slack).all()
