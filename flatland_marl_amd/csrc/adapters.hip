@@ -8,7 +8,7 @@
 // Rows are taken in the order of a grouping (flm_group_rows): tiles of rows that share an adapter.  Types: fp32, bf16,
 // fp16 for all tensors of a call; every sum is kept in fp32 and rounded once, at the end.  fp32 operands enter the matrix
 // cores as three bf16 terms each, of whose nine products six are kept.  In the few-row projection, the narrow products and the
-// adapters' gradients the terms are rounded to nearest: what is left out is below 2^-24 of the product.  The projection of more
+// adapters' gradients the first term is cut off and the others are rounded: what is left out is below 2^-22 of the product.  The projection of more
 // than 64 rows and the inputs' gradient run through the dense layers' product, which truncates: below 2^-21 (flm_gemm_x3.h).
 // The narrow products low and u stay fp32 in memory and enter the next product as two bf16 terms beside bf16 or fp16 operands
 // (2^-17 of the value, far below the rounding of the result).
@@ -67,14 +67,17 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], long avail) {
 }
 
 // ---- operands as bf16 terms ---------------------------------------------------------------------------------------
-// x = t[0] + t[1] + ... with every term rounded to nearest.
-// WIDE (values of fp32's range, which ends above the largest bf16): the first term is rounded no further than to that
-// largest one, whose difference from a finite x the other terms hold; rounded to infinity, a finite x above 3.396e38 would
-// become NaN.  An infinity's difference from it stays one, and a NaN's a NaN.
-// KEEP_INF: an infinite value is an infinity and zeros from that term on (its difference from itself would be NaN); without,
-// it becomes NaN, which saves two instructions a term.
-template <int N, bool KEEP_INF, bool WIDE>
+// x = t[0] + t[1] + ..., every term behind the first rounded to nearest.  The first:
+//   ROUND  to nearest, for types whose range ends below bf16's: the most exact.
+//   CLAMP  to nearest, but no further than to the largest bf16, whose difference from a finite x the other terms hold: rounded
+//          to infinity, a finite fp32 x above 3.396e38 would become NaN.  Two instructions a pair of values more.
+//   CUT    towards zero, for the same reason, at no cost: the second term then holds up to 2^-7 of x instead of 2^-8.
+// KEEP_INF: an infinite value is an infinity and zeros from that term on (its difference from itself would be NaN; its difference
+// from the largest bf16 still is one); without, it becomes NaN, which saves two instructions a term.
+enum First { ROUND, CLAMP, CUT };
+template <int N, bool KEEP_INF, First FIRST>
 __device__ __forceinline__ void split_terms(const float (&x)[8], bf16x8 (&t)[N]) {
+  static_assert(FIRST != CUT || !KEEP_INF, "");
   constexpr float TOP = 0x1.fep127f;                       // the largest bf16
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -83,17 +86,25 @@ __device__ __forceinline__ void split_terms(const float (&x)[8], bf16x8 (&t)[N])
     r[1] = x[2 * i + 1];
 #pragma unroll
     for (int s = 0; s < N; s++) {
-      f32x2 near = r;
-      if (WIDE && s == 0 && N > 1) {
-        near[0] = __builtin_amdgcn_fmed3f(r[0], -TOP, TOP);
-        near[1] = __builtin_amdgcn_fmed3f(r[1], -TOP, TOP);
+      bf16x2 h;
+      f32x2 f;
+      if (FIRST == CUT && s == 0) {
+        h = __builtin_bit_cast(bf16x2, pack_hi16(__float_as_uint(r[0]), __float_as_uint(r[1])));
+        f[0] = __uint_as_float(__float_as_uint(r[0]) & 0xffff0000u);
+        f[1] = __uint_as_float(__float_as_uint(r[1]) & 0xffff0000u);
+      } else {
+        f32x2 near = r;
+        if (FIRST == CLAMP && s == 0) {
+          near[0] = __builtin_amdgcn_fmed3f(r[0], -TOP, TOP);
+          near[1] = __builtin_amdgcn_fmed3f(r[1], -TOP, TOP);
+        }
+        h = __builtin_convertvector(near, bf16x2);
+        f = __builtin_convertvector(h, f32x2);
       }
-      const bf16x2 h = __builtin_convertvector(near, bf16x2);
       t[s][2 * i] = h[0];
       t[s][2 * i + 1] = h[1];
       if (s + 1 < N) {
-        const f32x2 f = __builtin_convertvector(h, f32x2);
-        const bool finite = !KEEP_INF || (WIDE && s == 0);
+        const bool finite = !KEEP_INF || (FIRST == CLAMP && s == 0);
         r[0] = finite || __builtin_fabsf(f[0]) < __builtin_inff() ? r[0] - f[0] : 0.f;
         r[1] = finite || __builtin_fabsf(f[1]) < __builtin_inff() ? r[1] - f[1] : 0.f;
       }
@@ -116,7 +127,7 @@ __device__ __forceinline__ void own_terms(const Vec8<T>& v, bf16x8 (&t)[Terms<T>
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) f[j] = (float)v.v[j];
-    split_terms<Terms<T>::own, sizeof(T) != 4, sizeof(T) == 4>(f, t);
+    split_terms<Terms<T>::own, sizeof(T) != 4, sizeof(T) == 4 ? CUT : ROUND>(f, t);
   }
 }
 
@@ -159,7 +170,7 @@ __device__ __forceinline__ Wide<_Float16> wide(const Vec8<_Float16>& v) {
 }
 __device__ __forceinline__ Wide<float> wide(const Vec8<float>& v) {
   Wide<float> w;
-  split_terms<3, false, true>(v.v, w.t);
+  split_terms<3, false, CUT>(v.v, w.t);
   return w;
 }
 __device__ __forceinline__ f32x4 mul16(const Wide<__bf16>& a, const Wide<__bf16>& b, f32x4 c) {
@@ -420,8 +431,9 @@ __device__ __forceinline__ float scale_after(float s) { return __builtin_fabsf(s
 // The scaled narrow products of `rows` sorted positions from pos on, as bf16 terms in LDS: lt[(term*rows + row)*stride + j],
 // stride = low_stride(rp).  threads of the workgroup share the work; a barrier follows at the caller.
 // Without V_STRIDED the last piece of eight ranks ends at the last rank, as AddAdapters reads it of V, and holds zeros where
-// it repeats those of the piece before.
+// it repeats those of the piece before.  Behind the terms: scale_after of every row.
 __device__ __forceinline__ int low_stride(int rp) { return rp + 8; }          // (16 bytes more: rows fall into different banks)
+static size_t staged_low_bytes(int low_terms, int rows, int rp) { return ((size_t)low_terms * (rp + 8) * 2 + 4) * rows; }
 template <int LOW, bool V_STRIDED>
 __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& g, long pos, int rows, __bf16* lt) {
   const int per = a.rp >> 3, stride = low_stride(a.rp);
@@ -432,6 +444,7 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
 #pragma unroll
     for (int u = 0; u < 8; u++) f[u] = 0.f;
     const int e = pos + row < a.n ? g.key[pos + row] : a.E;
+    float after = 1.f;
     if (e < a.E) {
       const float* p = a.low + (pos + row) * a.rp + jr;
       const long step = a.low_step;
@@ -445,18 +458,20 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
 #pragma unroll
           for (int u = 0; u < 8; u++) f[u] += z + k < a.low_slices ? __uint_as_float(v[k].w[u]) : 0.f;
       }
-      const float s = scale_before(adapter_scale(a.scale, a.scale_all, e));
+      const float scale = adapter_scale(a.scale, a.scale_all, e), s = scale_before(scale);
+      after = scale_after(scale);
 #pragma unroll
       for (int u = 0; u < 8; u++) f[u] = u >= j - jr && jr + u < a.r ? f[u] * s : 0.f;
     }
     bf16x8 t[LOW];
-    split_terms<LOW, true, true>(f, t);
+    split_terms<LOW, true, CLAMP>(f, t);
 #pragma unroll
     for (int k = 0; k < LOW; k++) *reinterpret_cast<bf16x8*>(lt + (k * rows + row) * stride + j) = t[k];
+    if (j == 0) reinterpret_cast<float*>(lt + LOW * rows * stride)[row] = after;
   }
 }
 
-// Adds s_e * low_i . V_e(n, .) to acc[mi] (staged with scale_before, scale_after here): lane (c, h) holds row lds_row0 + 32*mi + c of the staged tile of lds_rows rows,
+// Adds s_e * low_i . V_e(n, .) to acc[mi] (staged with scale_before; scale_after here): lane (c, h) holds row lds_row0 + 32*mi + c of the staged tile of lds_rows rows,
 // outputs n0 + 8*(r >> 2) + 4*h + (r & 3).  The rows may use several adapters: each adapter's product is formed apart and
 // added to its own rows only, so that no value of one adapter (an infinity, a NaN) can reach the rows of another.
 // key[mi]: the lane's adapter (E: none), ascending over the rows.  V comes straight from memory (the L2): NB adapters and
@@ -466,7 +481,6 @@ template <typename T, bool V_STRIDED, int MI, int JB, int NB>
 struct AddAdapters {
   int es[NB], j0, seen;
   unsigned todo[MI];
-  float after[NB];                         // scale_after
   Vec8<T> v[NB][JB];
   int turn = 0, share = 1;                 // this wave takes the adapters whose number in the tile is turn modulo share
 
@@ -490,8 +504,6 @@ struct AddAdapters {
         seen++;
       } while (es[b] >= 0 && share > 1 && (seen & (share - 1)) != turn);
     }
-#pragma unroll
-    for (int b = 0; b < NB; b++) after[b] = scale_after(adapter_scale(a.scale, a.scale_all, max(es[b], 0)));
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -522,6 +534,7 @@ struct AddAdapters {
   __device__ __forceinline__ void run(const FinishArgs& a, const __bf16* lt, int lds_rows, int lds_row0, const int (&key)[MI],
                                       int n0, f32x16 (&acc)[MI]) {
     const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, stride = low_stride(a.rp);
+    const float* afters = reinterpret_cast<const float*>(lt + Terms<T>::low * lds_rows * stride);
     while (true) {
       if (es[0] < 0) {                     // the rows are through: the next ranks
         j0 += 16 * JB;
@@ -541,6 +554,7 @@ struct AddAdapters {
           for (int mi = 0; mi < MI; mi++) {
             const bool mine = key[mi] == es[b];
             if (__ballot(mine) != 0) {
+              const float after = afters[lds_row0 + 32 * mi + c];
               f32x16 t;
 #pragma unroll
               for (int r = 0; r < 16; r++) t[r] = 0.f;
@@ -554,7 +568,7 @@ struct AddAdapters {
                   t = mul_terms32<Terms<T>::own, Terms<T>::low>(vt[jj], l, t);
                 }
 #pragma unroll
-              for (int r = 0; r < 16; r++) acc[mi][r] = mine ? __builtin_fmaf(after[b], t[r], acc[mi][r]) : acc[mi][r];
+              for (int r = 0; r < 16; r++) acc[mi][r] = mine ? __builtin_fmaf(after, t[r], acc[mi][r]) : acc[mi][r];
             }
           }
         }
@@ -1129,7 +1143,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
 #pragma unroll
       for (int u = 0; u < 8; u++) pv[k][u] = m < rows ? pv[k][u] * s : 0.f;
       bf16x8 t[LOW];
-      split_terms<LOW, true, true>(pv[k], t);
+      split_terms<LOW, true, CLAMP>(pv[k], t);
 #pragma unroll
       for (int o = 0; o < LOW; o++)
 #pragma unroll
@@ -1142,14 +1156,15 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
 #pragma unroll
       for (int u = 0; u < CPL; u++) acc[jj][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
-  auto flush = [&](int e) {
-    const float after = scale_after(adapter_scale(a.scale, a.scale_all, e));
+  auto flush = [&](int e, float after) {
+    if (after != 1.f) {
 #pragma unroll
-    for (int jj = 0; jj < NRJ; jj++)
+      for (int jj = 0; jj < NRJ; jj++)
 #pragma unroll
-      for (int u = 0; u < CPL; u++)
+        for (int u = 0; u < CPL; u++)
 #pragma unroll
-        for (int x = 0; x < 4; x++) acc[jj][u][x] *= after;
+          for (int x = 0; x < 4; x++) acc[jj][u][x] *= after;
+    }
     const int head = g.first_tile[e], last = g.first_tile[e + 1] - 1;
     const bool whole = head >= t0 && last < t0 + a.chunk;
     float* part = a.part + ((long)chunk * 2 + (head < t0 ? 0 : 1)) * a.r * a.KQ;
@@ -1214,9 +1229,10 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
     // (the step before the first only fetches)
     const int e = tile.y & 0xffff;
     bf16x8 qt[CPL][Terms<T>::own];
+    const float scale = adapter_scale(a.scale, a.scale_all, e);
     if (t >= t0) {
       __syncthreads();                     // (the products of the tile before have read pt)
-      place_p(scale_before(adapter_scale(a.scale, a.scale_all, e)), tile.y >> 16);
+      place_p(scale_before(scale), tile.y >> 16);
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < CPL; u++) own_terms<T>(column<T, CPL>(qv, u), qt[u]);
@@ -1239,7 +1255,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterArgs first, OuterArg
         acc[jj][u] = by_rank ? mul_terms16<Terms<T>::own, LOW>(qt[u], l, acc[jj][u]) : mul_terms16<Terms<T>::own, LOW>(l, qt[u], acc[jj][u]);
     }
     if (t + 1 == t1 || (next.y & 0xffff) != e) {
-      flush(e);
+      flush(e, scale_after(scale));
       clear();
     }
     tile = next;
@@ -1434,7 +1450,7 @@ template <typename T, int BM, int BN, int WM, int WN, bool W_KN, bool V_STRIDED>
 static int launch_wide(const BaseArgs& b, const FinishArgs& f, const RowGroups& g, hipStream_t st) {
   FLM_RAISE_LDS_ONCE((base_wide_kernel<T, BM, BN, WM, WN, W_KN, V_STRIDED>));
   size_t lds = 2 * (BM + BN) * 128;                                  // two stages; the narrow products' terms; the result
-  const size_t tail = (size_t)Terms<T>::low * BM * (f.rp + 8) * 2, out = (size_t)BM * (BN * sizeof(T) + 16);
+  const size_t tail = staged_low_bytes(Terms<T>::low, BM, f.rp), out = (size_t)BM * (BN * sizeof(T) + 16);
   if (tail > lds) lds = tail;
   if (out > lds) lds = out;
   hipLaunchKernelGGL((base_wide_kernel<T, BM, BN, WM, WN, W_KN, V_STRIDED>), dim3(((b.n + BM - 1) / BM) * ((b.N + BN - 1) / BN)),
@@ -1475,7 +1491,7 @@ static int launch_parts(const BaseArgs& b, int slices, const RowGroups& g, const
 template <typename T, bool V_STRIDED>
 static int launch_finish(const FinishArgs& a, const RowGroups& g, hipStream_t st) {
   const long tiles = (long)((a.N + 31) / 32) * ((a.n + 31) / 32);
-  const size_t lds = (size_t)Terms<T>::low * 32 * (a.rp + 8) * 2;
+  const size_t lds = staged_low_bytes(Terms<T>::low, 32, a.rp);
   const unsigned down = (a.n + 31) / 32;
   // Up to a tile a CU, four waves share each (64 rows of 64 adapters, 128 ranks: 83 -> 55 us a call); up to 1024 a wave each,
   // spread over the CUs (1001 rows, 515 outputs: 8.7 us, shared 11.9); beyond that four a workgroup
