@@ -8,10 +8,10 @@
 // Rows are taken in the order of a grouping (flm_group_rows): tiles of rows that share an adapter.  Types: fp32, bf16,
 // fp16 for all tensors of a call; every sum is kept in fp32 and rounded once, at the end.  fp32 operands enter the matrix
 // cores as three bf16 terms each, of whose nine products six are kept.  In the few-row projection, the narrow products and the
-// adapters' gradients the first term is cut off and the others are rounded: what is left out is below 2^-22 of the product.  The projection of more
-// than 64 rows and the inputs' gradient run through the dense layers' product, which truncates: below 2^-21 (flm_gemm_x3.h).
-// The narrow products low and u stay fp32 in memory and enter the next product as two bf16 terms beside bf16 or fp16 operands
-// (2^-17 of the value, far below the rounding of the result).
+// adapters' gradients the first term is cut off and the others are rounded: what is left out is below 2^-22 of the product.
+// The projection of more than 64 rows and the inputs' gradient run through the dense layers' product, which cuts every term
+// off: below 2^-21 (flm_gemm_x3.h).  The narrow products low and u stay fp32 in memory and enter the next product as two bf16
+// terms beside bf16 or fp16 operands (2^-17 of the value, far below the rounding of the result).
 #include <initializer_list>
 
 #include "flm_adapters.h"
