@@ -471,9 +471,10 @@ __device__ __forceinline__ void stage_low(const FinishArgs& a, const RowGroups& 
   }
 }
 
-// Adds s_e * low_i . V_e(n, .) to acc[mi] (staged with scale_before; scale_after here): lane (c, h) holds row lds_row0 + 32*mi + c of the staged tile of lds_rows rows,
-// outputs n0 + 8*(r >> 2) + 4*h + (r & 3).  The rows may use several adapters: each adapter's product is formed apart and
-// added to its own rows only, so that no value of one adapter (an infinity, a NaN) can reach the rows of another.
+// Adds s_e * low_i . V_e(n, .) to acc[mi] (low is staged with scale_before, scale_after is applied here): lane (c, h) holds
+// row lds_row0 + 32*mi + c of the staged tile of lds_rows rows, outputs n0 + 8*(r >> 2) + 4*h + (r & 3).  The rows may use
+// several adapters: each adapter's product is formed apart and added to its own rows only, so that no value of one adapter (an
+// infinity, a NaN) can reach the rows of another.
 // key[mi]: the lane's adapter (E: none), ascending over the rows.  V comes straight from memory (the L2): NB adapters and
 // 16*JB ranks at a time, so that NB*JB loads are in flight; start() fetches the first of them, before the narrow products are
 // staged if the caller likes.  Waves that hold the same tile may share its adapters.  All lanes of the wave take part.

@@ -114,7 +114,7 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, out=None):
         if len(out) == len(grads) != len(listed):           # one for one: what belongs to a None entry is left alone
             out = [o for g, o in zip(grads, out) if g is not None]
         outs = _listed(out)
-        if len(outs) != len(listed):
+        if listed and len(outs) != len(listed):
             raise ValueError("%d outputs for %d gradients" % (len(outs), len(listed)))
     if not listed:
         _inf_norm(norm_type)

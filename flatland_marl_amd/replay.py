@@ -48,12 +48,12 @@ class DeviceReplay:
 
     def sampled_groups(self):
         """The groups [batch] of the last sample()'s transitions, as they were when it drew them (what is stored since then may
-        have taken their places)."""
+        have taken their places): a tensor of its own for every sample."""
         if self.group is None or self._out is None:
             raise ValueError("keep_groups() and sample() first")
         if self._groups is None:                           # (drawn before keep_groups(): none had a group)
             self._groups = torch.full_like(self._out[5], -1)
-        return self._groups.clone()
+        return self._groups
 
     def add(self, state, action, reward, next_state, done, groups=None):
         """Append n transitions (oldest entries are overwritten, as with deque(maxlen))."""

@@ -68,3 +68,4 @@ def test_outputs_stay_with_their_gradients():
         with pytest.raises(FlmError):                       # (as far as the missing GPU)
             clip_grad_norm_(grads, 1.0, out=out)
     assert clip_grad_norm_([None], 1.0, out=[o]).item() == 0 and (o == 0).all()
+    assert clip_grad_norm_([], 1.0, out=[o]).item() == 0 and clip_grad_norm_(iter(()), 1.0, out=iter(())).item() == 0
